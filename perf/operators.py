@@ -186,7 +186,7 @@ def prepare(case, seed):
             b["dlogits"] = torch.zeros(rows, v, device=dev, dtype=dtype)
         b["logp"] = torch.zeros(rows, device=dev)
         if c["op"] == "logprob":
-            b["lse"] = torch.zeros(rows, device=dev)
+            b["stats"] = torch.zeros(rows, 2, device=dev)
             b["dlogp"] = -torch.rand(rows, generator=gen, device=dev) / rows  # of a weighted mean of -logp
         else:
             live = b["target"] >= 0
@@ -283,8 +283,8 @@ def _plain_dropout(c, t):
 
 
 def _plain_logprob(t):
-    """Rows' log-probabilities and log-sums (64 bits: policies look at small differences of them),
-    softmax, the targets' columns and which rows count."""
+    """Rows' log-probabilities (64 bits: policies look at small differences of them), their maxima and
+    the sums of exp(x - maximum), softmax, the targets' columns and which rows count."""
     x, target = t["logits"].float(), t["target"]
     live, at = target >= 0, target.clamp(min=0).long()[:, None]
     top = x.max(1, keepdim=True).values
@@ -293,7 +293,8 @@ def _plain_logprob(t):
     lse = torch.log(total) + top.double()
     zero = torch.zeros((), device=x.device, dtype=torch.float64)
     logp = torch.where(live, (x.gather(1, at).double() - lse)[:, 0], zero)
-    return logp, torch.where(live, lse[:, 0], zero), e.mul_(1.0 / total.float()), at, live
+    stats = torch.where(live[:, None], torch.cat((top, total.float()), 1), torch.zeros((), device=x.device))
+    return logp, stats, e.mul_(1.0 / total.float()), at, live
 
 
 def _plain_dlogits(p, at, live, d, dtype):
@@ -305,8 +306,8 @@ def _plain_dlogits(p, at, live, d, dtype):
 
 
 def _plain_rows(c, t):
-    logp, lse, p, at, live = _plain_logprob(t)
-    out = {"logp": logp.float(), "lse": lse.float()}
+    logp, stats, p, at, live = _plain_logprob(t)
+    out = {"logp": logp.float(), "stats": stats}
     if c["train"]:
         out["dlogits"] = _plain_dlogits(p, at, live, t["dlogp"], t["logits"].dtype)
     return out
@@ -379,12 +380,12 @@ def _own_run(c, t, b):
         T.dropout_seeded_bwd(c["n"], b["dy"], b["dx"], c["rate"], c["key"], c["step"], dtype=c["dtype"])
         return {"y": t["y"], "dx": t["dx"]}
     if c["op"] == "logprob":
-        T.token_logprob_fwd(c["rows"], c["vocab"], b["logits"], b["target"], b["logp"], b["lse"], dtype=c["dtype"])
+        T.token_logprob_fwd(c["rows"], c["vocab"], b["logits"], b["target"], b["logp"], b["stats"], dtype=c["dtype"])
         if not c["train"]:
-            return {"logp": t["logp"], "lse": t["lse"]}
-        T.token_logprob_bwd(c["rows"], c["vocab"], b["logits"], b["target"], b["lse"], b["dlogp"], b["dlogits"],
+            return {"logp": t["logp"], "stats": t["stats"]}
+        T.token_logprob_bwd(c["rows"], c["vocab"], b["logits"], b["target"], b["stats"], b["dlogp"], b["dlogits"],
                             dtype=c["dtype"])
-        return {k: t[k] for k in ("logp", "lse", "dlogits")}
+        return {k: t[k] for k in ("logp", "stats", "dlogits")}
     if c["op"] == "policy":
         T.policy_loss(c["rows"], c["vocab"], b["logits"], b["target"], b["old"], b["ref"], b["advantage"], b["weight"],
                       b["logp"], b["row_loss"], b["loss"], b["dlogits"], clip_low=CLIP_LOW, clip_high=CLIP_HIGH, kl_coef=KL,
@@ -465,7 +466,8 @@ def exact(case, seed):
         return g
 
     if c["op"] == "logprob":
-        out = {"logp": logp, "lse": torch.logsumexp(t["logits"], 1) * count}
+        top = t["logits"].amax(1)
+        out = {"logp": logp, "stats": torch.stack((top, torch.exp(torch.logsumexp(t["logits"], 1) - top)), 1) * count[:, None]}
         return dict(out, dlogits=dlogits(t["dlogp"])) if c["train"] else out
     if c["op"] == "policy":
         r, gap = torch.exp(logp - t["old"]), t["ref"] - logp
