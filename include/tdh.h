@@ -9,7 +9,7 @@
  *
  * Conventions
  *  - Every tensor argument is a DEVICE pointer obtained from tdh_malloc, dense
- *    fp32, [batch][flat] with tiny-dnn's per-sample CHW layout
+ *    fp32 (the operators of language models: the element type they are called with), [batch][flat] with tiny-dnn's per-sample CHW layout
  *    index = (H*c + y)*W + x  (tiny_dnn/util/util.h:168-173). Conv weights are
  *    OIHW, fully-connected weights [in][out] row-major.
  *  - Convolution inputs/gradients are UNPADDED; padding::same is applied
@@ -57,6 +57,14 @@ enum { TDH_OPT_SGD = 0, TDH_OPT_MOMENTUM = 1, TDH_OPT_ADAM = 2, TDH_OPT_ADAGRAD 
 /* layer kinds of a sequential network */
 enum { TDH_L_CONV = 0, TDH_L_FC = 1, TDH_L_MAXPOOL = 2, TDH_L_AVEPOOL = 3, TDH_L_ACT = 4,
        TDH_L_BATCHNORM = 5, TDH_L_DROPOUT = 6 };
+
+/* element types of the operators that take a dtype (the others are fp32) */
+enum { TDH_F32 = 0, TDH_BF16 = 1, TDH_F16 = 2 };
+/* activations of a gated feed-forward block's gate: silu, gelu (erf), gelu (tanh form), sigmoid, relu, identity */
+enum { TDH_GATE_SILU = 0, TDH_GATE_GELU = 1, TDH_GATE_GELU_TANH = 2, TDH_GATE_SIGMOID = 3, TDH_GATE_RELU = 4,
+       TDH_GATE_NONE = 5 };
+/* what a pair's margin m costs in tdh_preference_loss */
+enum { TDH_PREF_SIGMOID = 0, TDH_PREF_SQUARED = 1, TDH_PREF_HINGE = 2 };
 
 /* core::conv_params (tiny_dnn/core/params/conv_params.h:63-90) */
 typedef struct tdh_conv_desc {
@@ -255,6 +263,82 @@ int tdh_loss_grad(int kind, int batch, int len, const float *y, const float *t, 
 /* softmax_layer backward applied to cross_entropy_multiclass::df in one kernel:
  * dz = y * sum(t) - t  (= y - t for one-hot targets) */
 int tdh_softmax_xent_grad(int batch, int len, const float *y, const float *t, float *dz);
+
+/* -------------------------------------------- operators of language models
+ * They have no counterpart in the reference. `dtype` (TDH_F32, TDH_BF16, TDH_F16) is the element type of the
+ * tensors declared void *; those declared float * are fp32 in every type. Sums are held in 32 bits or more, and
+ * results are rounded once, to nearest. Tensors are aligned to their elements; where they lie on 16-byte
+ * boundaries and rows are multiples of 16 bytes apart, they move in words of that size. The same inputs give
+ * the same bits. */
+
+/* Gated feed-forward block: z = x W + b, h = act(z_gate) * z_up. x [batch][in], w [in][2*hidden] with the gate's
+ * columns first, b [2*hidden] (has_bias), h [batch][hidden]. z [batch][2*hidden], fp32, is what the backward pass
+ * reads; NULL where there is none (inference). */
+int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
+                     const void *b, void *h, float *z);
+/* dz = (dh * z_up * act'(z_gate), dh * act(z_gate)), dx = dz W^T, dw = x^T dz, db = the sum of dz over the batch. dx is overwritten;
+ * dw and db (as in tdh_fc_bwd) overwritten, or added to with accumulate != 0. Any of dx, dw, db may be NULL.
+ * In the 16-bit types dz is rounded to that type once, as the operand of the two products. The derivative of relu at zero is 0. */
+int tdh_gated_ff_bwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
+                     const float *z, const void *dh, void *dx, void *dw, void *db, int accumulate);
+
+/* Dropout with the mask drawn on the device and stored nowhere: y = [residual +] (kept ? x / (1 - rate) : 0).
+ * Element i is dropped where word i % 4 of Philox4x32-10 with counter (i / 4, offset) and key seed (low words
+ * first) lies below floor(rate * 2^32): the same (seed, offset) gives the same mask, another offset another one.
+ * A training step counts offset up, with a number of its own for every dropout layer in it. n elements in any layout;
+ * residual may be NULL; y may be x or residual; 0 <= rate < 1. Unlike tdh_dropout_fwd, whose mask and missing
+ * scale on the way back are the reference's, rate is the share that is dropped and the backward pass scales. */
+int tdh_dropout_seeded_fwd(int dtype, size_t n, float rate, uint64_t seed, uint64_t offset, const void *x,
+                           const void *residual, void *y);
+/* dx = kept ? dy / (1 - rate) : 0 (the residual's gradient is dy itself); dx may be dy */
+int tdh_dropout_seeded_bwd(int dtype, size_t n, float rate, uint64_t seed, uint64_t offset, const void *dy, void *dx);
+
+/* Log-probabilities of given tokens: logp[r] = logits[r][target[r]] - m - log(s), m the row's maximum and
+ * s = sum_j exp(logits[r][j] - m). Row r starts ld elements behind row r-1 (ld >= vocab). A row with a negative
+ * target does not count (prompt, padding): its logits are not read, logp and stats are 0. A target of vocab or more
+ * gives NaN. stats [rows][2] receives (m, s), from which the gradient is computed; NULL where there is none. */
+int tdh_token_logprob_fwd(int dtype, int rows, int vocab, const void *logits, size_t ld, const int32_t *target,
+                          float *logp, float *stats);
+/* dlogits[r][j] = dlogp[r] * ((j == target[r]) - exp(logits[r][j] - m) / s), zero in rows that do not count.
+ * Rows of dlogits are ld_d elements apart; it may be logits itself (with ld_d == ld). */
+int tdh_token_logprob_bwd(int dtype, int rows, int vocab, const void *logits, size_t ld, const int32_t *target,
+                          const float *stats, const float *dlogp, void *dlogits, size_t ld_d);
+
+/* Clipped policy loss with a KL term. Of row r, with the token target[r] (negative: the row does not count),
+ *   ratio = exp(logp - old_logp), gap = ref_logp - logp,
+ *   row_loss = weight * (-min(ratio * advantage, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantage)
+ *                        + kl_coef * (exp(gap) - gap - 1)),
+ * loss[0] = the sum of row_loss, and dlogits its gradient. weight NULL: 1 for every row (1 / rows makes a mean);
+ * ref_logp NULL: no KL term. Any of logp, row_loss, loss and dlogits may be NULL; dlogits as in
+ * tdh_token_logprob_bwd. Where the two sides of the minimum are equal the gradient is the first one's. */
+typedef struct tdh_policy_desc {
+  float clip_low, clip_high, kl_coef;
+} tdh_policy_desc;
+int tdh_policy_loss(const tdh_policy_desc *p, int dtype, int rows, int vocab, const void *logits, size_t ld,
+                    const int32_t *target, const float *old_logp, const float *ref_logp, const float *advantage,
+                    const float *weight, float *logp, float *row_loss, float *loss, void *dlogits, size_t ld_d);
+
+/* Preference loss on paired log ratios. Sequence s is rows seq_start[s] .. seq_start[s+1]-1 (2*pairs + 1 ascending
+ * values within 0 .. rows; a sequence may be empty); 2p is pair p's chosen answer, 2p+1 the rejected one. With
+ * seq_logp[s] the sum of logp over the sequence's rows that count and ref_logp[s] the same of the reference
+ * model (NULL: 0),
+ *   margin = beta * ((seq_logp - ref_logp)[2p] - (seq_logp - ref_logp)[2p+1]), and its loss
+ *   TDH_PREF_SIGMOID  (1 - smoothing) * log(1 + exp(-margin)) + smoothing * log(1 + exp(margin))
+ *   TDH_PREF_SQUARED  ((margin - 1/2) / beta)^2
+ *   TDH_PREF_HINGE    max(0, 1 - margin)   (derivative 0 at 1)
+ * loss[0] = the mean over the pairs, dlogits its gradient. Any of logp [rows], seq_logp [2*pairs], margin [pairs],
+ * loss and dlogits may be NULL; dlogits as above. Rows of logp and dlogits outside the sequences keep what they hold. */
+typedef struct tdh_preference_desc {
+  int32_t kind;
+  float beta, smoothing;
+} tdh_preference_desc;
+int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int rows, int vocab, const void *logits, size_t ld,
+                        const int32_t *target, const int32_t *seq_start, const float *ref_logp, float *logp,
+                        float *seq_logp, float *margin, float *loss, void *dlogits, size_t ld_d);
+
+/* n elements from one element type to another, rounded to nearest: fp32 weights to the 16-bit ones that a block
+ * computes with, and its 16-bit gradients to the fp32 ones that tdh_opt_update takes */
+int tdh_cast(int dst_dtype, int src_dtype, size_t n, const void *src, void *dst);
 
 /* -------------------------------------------------------------- optimizers */
 /* layer::update_weight for one tensor (tiny_dnn/layers/layer.h:663-682) followed by

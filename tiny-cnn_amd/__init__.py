@@ -24,6 +24,9 @@ ACT = {"tanh": 0, "relu": 1, "softmax": 2, "sigmoid": 3, "leaky_relu": 4, "elu":
        "softplus": 7, "softsign": 8, "asinh": 9, "tanh_p1m2": 10}
 LOSS = {"mse": 0, "ce_multiclass": 1, "ce": 2}
 OPT = {"sgd": 0, "momentum": 1, "adam": 2, "adagrad": 3, "rmsprop": 4, "adamax": 5, "nesterov": 6}
+DTYPE = {"f32": 0, "bf16": 1, "f16": 2}
+GATE = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4, "none": 5}
+PREFERENCE = {"sigmoid": 0, "squared": 1, "hinge": 2}
 L_CONV, L_FC, L_MAXPOOL, L_AVEPOOL, L_ACT, L_BATCHNORM, L_DROPOUT = range(7)
 NET_FUSE_ACT_GRAD, NET_GRAPH, NET_SAMPLE_STEP, NET_NO_INPUT_GRAD = 1, 2, 4, 8
 
@@ -49,6 +52,14 @@ class PoolDesc(C.Structure):
 class OptDesc(C.Structure):
     _fields_ = [("kind", C.c_int32)] + [(n, C.c_float) for n in (
         "alpha", "lam", "mu", "b1", "b2", "eps", "b1_t", "b2_t")]
+
+
+class PolicyDesc(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("clip_low", "clip_high", "kl_coef")]
+
+
+class PreferenceDesc(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("beta", C.c_float), ("smoothing", C.c_float)]
 
 
 class LayerDesc(C.Structure):
@@ -455,6 +466,66 @@ def loss_grad(kind, batch, length, y, t, dy):
 def softmax_xent_grad(batch, length, y, t, dz):
     check(lib().tdh_softmax_xent_grad(batch, length, _p(y), _p(t), _p(dz)),
           "tdh_softmax_xent_grad")
+
+
+# Operators of language models. dtype names the element type of x, weights, logits and their gradients: "f32",
+# "bf16" or "f16" (buffers of a 16-bit type are uint16 here: numpy has no bf16).
+
+def gated_ff_fwd(n_in, n_hidden, has_bias, batch, x, w, b, h, z=None, act="silu", dtype="f32"):
+    """h = act(gate) * up of z = x w + b, w [n_in][2*n_hidden] with the gate's columns first; z (fp32) is kept
+    for gated_ff_bwd where it is given."""
+    check(lib().tdh_gated_ff_fwd(DTYPE[dtype], GATE[act], n_in, n_hidden, int(has_bias), batch, _p(x), _p(w), _p(b),
+                                 _p(h), _p(z)), "tdh_gated_ff_fwd")
+
+
+def gated_ff_bwd(n_in, n_hidden, has_bias, batch, x, w, z, dh, dx, dw, db, act="silu", dtype="f32", accumulate=False):
+    check(lib().tdh_gated_ff_bwd(DTYPE[dtype], GATE[act], n_in, n_hidden, int(has_bias), batch, _p(x), _p(w), _p(z),
+                                 _p(dh), _p(dx), _p(dw), _p(db), int(accumulate)), "tdh_gated_ff_bwd")
+
+
+def dropout_seeded_fwd(n, x, y, rate, seed, offset=0, residual=None, dtype="f32"):
+    """y = [residual +] dropout(x), the mask drawn from (seed, offset) and stored nowhere"""
+    check(lib().tdh_dropout_seeded_fwd(DTYPE[dtype], C.c_size_t(n), C.c_float(rate), C.c_uint64(seed), C.c_uint64(offset),
+                                       _p(x), _p(residual), _p(y)), "tdh_dropout_seeded_fwd")
+
+
+def dropout_seeded_bwd(n, dy, dx, rate, seed, offset=0, dtype="f32"):
+    check(lib().tdh_dropout_seeded_bwd(DTYPE[dtype], C.c_size_t(n), C.c_float(rate), C.c_uint64(seed), C.c_uint64(offset),
+                                       _p(dy), _p(dx)), "tdh_dropout_seeded_bwd")
+
+
+def token_logprob_fwd(rows, vocab, logits, target, logp, stats=None, dtype="f32", ld=None):
+    """logp[r] of token target[r] (int32; negative: the row does not count) under logits[r]; stats [rows][2], the
+    rows' maxima and sums of exp(x - maximum), is what token_logprob_bwd reads"""
+    check(lib().tdh_token_logprob_fwd(DTYPE[dtype], rows, vocab, _p(logits), C.c_size_t(ld or vocab), _p(target), _p(logp),
+                                      _p(stats)), "tdh_token_logprob_fwd")
+
+
+def token_logprob_bwd(rows, vocab, logits, target, stats, dlogp, dlogits, dtype="f32", ld=None, ld_d=None):
+    check(lib().tdh_token_logprob_bwd(DTYPE[dtype], rows, vocab, _p(logits), C.c_size_t(ld or vocab), _p(target), _p(stats),
+                                      _p(dlogp), _p(dlogits), C.c_size_t(ld_d or vocab)), "tdh_token_logprob_bwd")
+
+
+def policy_loss(rows, vocab, logits, target, old_logp, ref_logp, advantage, weight=None, logp=None, row_loss=None,
+                loss=None, dlogits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, dtype="f32", ld=None, ld_d=None):
+    """The clipped policy loss with a KL term and its gradient, from logits"""
+    p = PolicyDesc(clip_low, clip_high, kl_coef)
+    check(lib().tdh_policy_loss(C.byref(p), DTYPE[dtype], rows, vocab, _p(logits), C.c_size_t(ld or vocab), _p(target),
+                                _p(old_logp), _p(ref_logp), _p(advantage), _p(weight), _p(logp), _p(row_loss), _p(loss),
+                                _p(dlogits), C.c_size_t(ld_d or vocab)), "tdh_policy_loss")
+
+
+def preference_loss(pairs, rows, vocab, logits, target, seq_start, ref_logp=None, logp=None, seq_logp=None, margin=None,
+                    loss=None, dlogits=None, beta=0.1, smoothing=0.0, kind="sigmoid", dtype="f32", ld=None, ld_d=None):
+    """The preference loss of pairs of packed sequences and its gradient, from logits"""
+    p = PreferenceDesc(PREFERENCE[kind], beta, smoothing)
+    check(lib().tdh_preference_loss(C.byref(p), DTYPE[dtype], pairs, rows, vocab, _p(logits), C.c_size_t(ld or vocab),
+                                    _p(target), _p(seq_start), _p(ref_logp), _p(logp), _p(seq_logp), _p(margin), _p(loss),
+                                    _p(dlogits), C.c_size_t(ld_d or vocab)), "tdh_preference_loss")
+
+
+def cast(n, src, dst, src_dtype, dst_dtype):
+    check(lib().tdh_cast(DTYPE[dst_dtype], DTYPE[src_dtype], C.c_size_t(n), _p(src), _p(dst)), "tdh_cast")
 
 
 def opt_update(o, n, merged_grad, w, s0=None, s1=None, grad_scale=1.0):

@@ -1,0 +1,69 @@
+// lm_types.h — element types of the language-model operators: what tdh_dtype names, as device types with
+// their conversions to and from fp32 (to nearest, ties to even), and 16-byte words of them.
+#pragma once
+#include "common.h"
+
+namespace tdh {
+
+struct bf16 {
+  uint16_t bits;
+};
+struct f16 {
+  _Float16 v;
+};
+
+__device__ __forceinline__ float to_f32(const float v) { return v; }
+__device__ __forceinline__ float to_f32(const bf16 v) { return __uint_as_float(static_cast<uint32_t>(v.bits) << 16); }
+__device__ __forceinline__ float to_f32(const f16 v) { return static_cast<float>(v.v); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(const float v) { return v; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(const float v) {
+  return bf16{__builtin_bit_cast(uint16_t, static_cast<__bf16>(v))};
+}
+template <>
+__device__ __forceinline__ f16 from_f32<f16>(const float v) { return f16{static_cast<_Float16>(v)}; }
+
+// Sixteen bytes of T: element e of the word, and words put together from fp32 values.
+template <class T>
+struct Word {
+  static constexpr int N = 16 / static_cast<int>(sizeof(T));
+  uint4 raw;
+  __device__ __forceinline__ float operator[](const int e) const {
+    const uint32_t w = (&raw.x)[e * static_cast<int>(sizeof(T)) / 4];
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w);
+    else
+      return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(e & 1 ? w >> 16 : w)));
+  }
+  __device__ __forceinline__ static Word from(const float (&v)[N]) {
+    Word o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4)
+        (&o.raw.x)[i] = __float_as_uint(v[i]);
+      else
+        (&o.raw.x)[i] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * i]))) |
+                        static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * i + 1]))) << 16;
+    }
+    return o;
+  }
+};
+
+inline bool dtype_known(int dtype) { return dtype == TDH_F32 || dtype == TDH_BF16 || dtype == TDH_F16; }
+inline size_t dtype_size(int dtype) { return dtype == TDH_F32 ? 4 : 2; }
+
+// Calls f with a value of the device type that `dtype` names.
+template <class F>
+inline int with_dtype(int dtype, const F &f) {
+  switch (dtype) {
+    case TDH_F32: return f(float());
+    case TDH_BF16: return f(bf16());
+    default: return f(f16());
+  }
+}
+
+}  // namespace tdh
