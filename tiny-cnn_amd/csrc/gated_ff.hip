@@ -1,7 +1,7 @@
 // gated_ff.hip — the gated feed-forward block: z = x W + b with W = [in][2 hidden], gate columns first, and
 // h = act(z_gate) * z_up; on the way back dz = (dh * z_up * act'(z_gate), dh * act(z_gate)),
 // dx = dz W^T, dW = x^T dz, db = the column sums of dz.
-#include "lm_types.h"
+#include "gemm16.h"
 
 namespace tdh {
 
@@ -63,20 +63,20 @@ gate_bwd_kernel(const float *__restrict__ z, const T *__restrict__ dh, float *__
   dz[row * 2 * hidden + hidden + c] = d * a;
 }
 
-// dst (+)= src in another type
-template <class D, class S, bool ADD>
+// dst = src in another type
+template <class D, class S>
 __global__ void __launch_bounds__(GF_NT)
 cast_kernel(const S *__restrict__ src, D *__restrict__ dst, const size_t n) {
   const size_t stride = static_cast<size_t>(gridDim.x) * GF_NT;
   for (size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x; i < n; i += stride)
-    dst[i] = from_f32<D>(to_f32(src[i]) + (ADD ? to_f32(dst[i]) : 0.0f));
+    dst[i] = from_f32<D>(to_f32(src[i]));
 }
 
-template <class D, class S, bool ADD = false>
+template <class D, class S>
 int launch_cast(const S *src, D *dst, size_t n) {
   if (!n) return TDH_OK;
   ProfScope prof("cast", static_cast<double>(n) * (sizeof(D) + sizeof(S)), WORK_BYTE);
-  TDH_LAUNCH((cast_kernel<D, S, ADD>), dim3(static_cast<unsigned>(std::min<size_t>(ceil_div_sz(n, GF_NT), GRID_X_MAX))),
+  TDH_LAUNCH((cast_kernel<D, S>), dim3(static_cast<unsigned>(std::min<size_t>(ceil_div_sz(n, GF_NT), GRID_X_MAX))),
              dim3(GF_NT), 0, ctx().stream, src, dst, n);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
@@ -90,72 +90,350 @@ int take(size_t n, T **out) {
   return TDH_OK;
 }
 
-template <class T>
-int ff_fwd(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
-  const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * hidden, nz = static_cast<size_t>(batch) * 2 * hidden;
-  constexpr bool cast = sizeof(T) == 2;
-  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + (z ? 0 : ws_align(4 * nz)) +
-                   (cast ? ws_align(4 * nx) + ws_align(4 * nw) + ws_align(8 * hidden) : 0)));
-  const float *xf = reinterpret_cast<const float *>(x), *wf = reinterpret_cast<const float *>(w), *bf = reinterpret_cast<const float *>(b);
+// ------------------------------------------------------------------- fp32
+int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *b, float *h, float *z) {
+  const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
+  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + (z ? 0 : ws_align(4 * nz))));
   if (!z) TDH_TRY(take(nz, &z));
-  if (cast) {
-    float *p;
-    TDH_TRY(take(nx, &p));
-    TDH_TRY((launch_cast<float, T>(x, p, nx)));
-    xf = p;
-    TDH_TRY(take(nw, &p));
-    TDH_TRY((launch_cast<float, T>(w, p, nw)));
-    wf = p;
-    if (b) {
-      TDH_TRY(take(2 * static_cast<size_t>(hidden), &p));
-      TDH_TRY((launch_cast<float, T>(b, p, 2 * static_cast<size_t>(hidden))));
-      bf = p;
-    }
-  }
-  TDH_TRY(fc_fwd(in, 2 * hidden, b != nullptr, batch, xf, wf, bf, z));
+  TDH_TRY(fc_fwd(in, 2 * hidden, b != nullptr, batch, x, w, b, z));
   const size_t total = nz / 2;
-  ProfScope prof("gate_fwd", (8.0 + sizeof(T)) * total, WORK_BYTE);
-  TDH_LAUNCH((gate_fwd_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h,
+  ProfScope prof("gate_fwd", 12.0 * total, WORK_BYTE);
+  TDH_LAUNCH((gate_fwd_kernel<float>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h,
              hidden, total, act);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
-
-template <class T>
-int ff_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
-           int accumulate) {
-  const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * hidden, nz = static_cast<size_t>(batch) * 2 * hidden,
-               nb = 2 * static_cast<size_t>(hidden);
-  constexpr bool cast = sizeof(T) == 2;
-  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + ws_align(4 * nz) +
-                   (cast ? 2 * ws_align(4 * nx) + 2 * ws_align(4 * nw) + ws_align(4 * nb) : 0)));
+int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *z, const float *dh, float *dx,
+               float *dw, float *db, int accumulate) {
+  const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
+  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + ws_align(4 * nz)));
   float *dz;
   TDH_TRY(take(nz, &dz));
   const size_t total = nz / 2;
   {
-    ProfScope prof("gate_bwd", (16.0 + sizeof(T)) * total, WORK_BYTE);
-    TDH_LAUNCH((gate_bwd_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, dh,
+    ProfScope prof("gate_bwd", 20.0 * total, WORK_BYTE);
+    TDH_LAUNCH((gate_bwd_kernel<float>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, dh,
                dz, hidden, total, act);
     TDH_LAUNCH_CHECK();
   }
-  if constexpr (!cast) {
-    return fc_bwd(in, 2 * hidden, db != nullptr, batch, reinterpret_cast<const float *>(x), reinterpret_cast<const float *>(w), dz,
-                  reinterpret_cast<float *>(dx), reinterpret_cast<float *>(dw), reinterpret_cast<float *>(db), accumulate, ActGrad());
-  } else {
-    float *xf, *wf, *dxf, *dwf, *dbf;
-    TDH_TRY(take(nx, &xf));
-    TDH_TRY(take(nw, &wf));
-    TDH_TRY(take(nx, &dxf));
-    TDH_TRY(take(nw, &dwf));
-    TDH_TRY(take(nb, &dbf));
-    TDH_TRY((launch_cast<float, T>(x, xf, nx)));
-    TDH_TRY((launch_cast<float, T>(w, wf, nw)));
-    TDH_TRY(fc_bwd(in, 2 * hidden, db != nullptr, batch, xf, wf, dz, dx ? dxf : nullptr, dw ? dwf : nullptr, db ? dbf : nullptr, 0, ActGrad()));
-    if (dx) TDH_TRY((launch_cast<T, float>(dxf, dx, nx)));
-    if (dw) TDH_TRY(accumulate ? (launch_cast<T, float, true>(dwf, dw, nw)) : (launch_cast<T, float>(dwf, dw, nw)));
-    if (db) TDH_TRY(accumulate ? (launch_cast<T, float, true>(dbf, db, nb)) : (launch_cast<T, float>(dbf, db, nb)));
-    return TDH_OK;
+  return fc_bwd(in, 2 * hidden, db != nullptr, batch, x, w, dz, dx, dw, db, accumulate, ActGrad());
+}
+
+// ------------------------------------------------------------ 16-bit types
+// What leaves the products. Columns of z, w and dz come in two halves of `half` columns, of which the first `hidden`
+// are in use (half is hidden rounded up to a multiple of 8 where a packed copy is read).
+
+// forward: h, and z where it is kept
+template <class T>
+struct EpiGate {
+  T *h;
+  float *z;            // or null
+  const T *bias;       // or null
+  float *partial;      // slices of z instead, [split][rows][2 half]
+  int rows, hidden, half, act;
+  __device__ __forceinline__ void one(const size_t m, const int n, float g, float u) const {
+    if (bias) {
+      g += to_f32(bias[n]);
+      u += to_f32(bias[hidden + n]);
+    }
+    if (z) {
+      z[m * 2 * hidden + n]          = g;
+      z[m * 2 * hidden + hidden + n] = u;
+    }
+    float slope;
+    h[m * hidden + n] = from_f32<T>(gate_act(act, g, &slope) * u);
   }
+  template <int TM, int TN>
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split) const {
+#pragma unroll
+    for (int j = 0; j < TN / 2; ++j) {
+      const int n = n0 + 32 * j + (lane & 31);
+      if (n >= hidden) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          if (m >= rows) continue;
+          if (partial) {
+            float *p = partial + (static_cast<size_t>(split) * rows + m) * 2 * half;
+            p[n]        = acc[i][2 * j][r];
+            p[half + n] = acc[i][2 * j + 1][r];
+          } else {
+            one(m, n, acc[i][2 * j][r], acc[i][2 * j + 1][r]);
+          }
+        }
+    }
+  }
+};
+
+// a gradient: out (+)= C
+template <class T>
+struct EpiGrad {
+  T *out;
+  float *partial;      // slices instead, [split][rows][cols]
+  int rows, cols;      // of C
+  int hidden, half;    // two halves of columns, as above (one: both are cols)
+  int accumulate;
+  __device__ __forceinline__ void one(const size_t m, int n, float v) const {
+    if (n >= hidden) {
+      if (n < half || n - half >= hidden) return;
+      n += hidden - half;
+    }
+    T *p = out + m * (cols > half ? 2 * hidden : hidden) + n;
+    if (accumulate) v += to_f32(*p);
+    *p = from_f32<T>(v);
+  }
+  template <int TM, int TN>
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split) const {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + 32 * j + (lane & 31);
+      if (n >= cols) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          if (m >= rows) continue;
+          if (partial)
+            partial[(static_cast<size_t>(split) * rows + m) * cols + n] = acc[i][j][r];
+          else
+            one(m, n, acc[i][j][r]);
+        }
+    }
+  }
+};
+
+// slices added up, in their order
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+gate_reduce_kernel(const EpiGate<T> epi, const int splits) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
+  if (i >= static_cast<size_t>(epi.rows) * epi.hidden) return;
+  const size_t m = i / epi.hidden, slice = static_cast<size_t>(epi.rows) * 2 * epi.half;
+  const int n = static_cast<int>(i - m * epi.hidden);
+  const float *p = epi.partial + m * 2 * epi.half + n;
+  float g = 0.0f, u = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    g += p[s * slice];
+    u += p[s * slice + epi.half];
+  }
+  epi.one(m, n, g, u);
+}
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+grad_reduce_kernel(const EpiGrad<T> epi, const int splits) {
+  const size_t total = static_cast<size_t>(epi.rows) * epi.cols, i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
+  if (i >= total) return;
+  const size_t m = i / epi.cols;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += epi.partial[s * total + i];
+  epi.one(m, static_cast<int>(i - m * epi.cols), v);
+}
+
+// A matrix copied to a padded one: columns in one or two halves of `used` values, `half` apart in the copy; what is
+// behind a half is zero.
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+pack_kernel(const T *__restrict__ src, T *__restrict__ dst, const size_t total, const int used, const int half, const int halves) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
+  if (i >= total) return;
+  const size_t row = i / (halves * half);
+  const int c = static_cast<int>(i - row * (halves * half)), h = c >= half ? 1 : 0, n = c - h * half;
+  dst[i] = n < used ? src[(row * halves + h) * used + n] : T{};
+}
+
+// dz in the operand's type, [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
+// workgroup's band (in fp32, before the rounding)
+constexpr int DZ_ROWS = 32;
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restrict__ dz, float *__restrict__ bias_part,
+               const int rows, const int hidden, const int half, const int act, const int blocks_n) {
+  const int n = blockIdx.x % blocks_n * GF_NT + threadIdx.x, band = blockIdx.x / blocks_n;
+  if (n >= half) return;
+  float sg = 0.0f, su = 0.0f;
+  const int end = min(rows, (band + 1) * DZ_ROWS);
+  for (int m = band * DZ_ROWS; m < end; ++m) {
+    float dg = 0.0f, du = 0.0f;
+    if (n < hidden) {
+      const float *zr = z + static_cast<size_t>(m) * 2 * hidden + n;
+      float slope;
+      const float a = gate_act(act, zr[0], &slope), d = to_f32(dh[static_cast<size_t>(m) * hidden + n]);
+      dg = d * zr[hidden] * slope;
+      du = d * a;
+    }
+    if (dz) {
+      dz[static_cast<size_t>(m) * 2 * half + n]        = from_f32<T>(dg);
+      dz[static_cast<size_t>(m) * 2 * half + half + n] = from_f32<T>(du);
+    }
+    sg += dg;
+    su += du;
+  }
+  if (bias_part && n < hidden) {
+    bias_part[static_cast<size_t>(band) * 2 * hidden + n]          = sg;
+    bias_part[static_cast<size_t>(band) * 2 * hidden + hidden + n] = su;
+  }
+}
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+bias_sum_kernel(const float *__restrict__ part, T *__restrict__ db, const int bands, const int cols, const int accumulate) {
+  const int n = blockIdx.x * GF_NT + threadIdx.x;
+  if (n >= cols) return;
+  float s = 0.0f;
+  for (int b = 0; b < bands; ++b) s += part[static_cast<size_t>(b) * cols + n];
+  if (accumulate) s += to_f32(db[n]);
+  db[n] = from_f32<T>(s);
+}
+
+// ---- plans
+struct FfPlan {
+  int cfg;       // index into the tile shapes of ff_gemm
+  int splits, k_per_split;
+};
+struct FfTile {
+  int bm, bn, per_cu;
+  double us;     // of one tile of 64 reduction indices, per workgroup, with per_cu of them on a compute unit
+};
+constexpr FfTile FF_TILES[] = {{256, 256, 1, 1.7}, {128, 128, 2, 1.0}, {32, 256, 2, 0.6}};
+
+FfPlan ff_plan(int M, int N, int K) {
+  const int cus = ctx().compute_units > 0 ? ctx().compute_units : 256, ktiles = std::max(1, ceil_div(K, G16_BK));
+  FfPlan best{0, 1, ktiles * G16_BK};
+  double best_us = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    const FfTile &t = FF_TILES[c];
+    const long tiles = static_cast<long>(ceil_div(M, t.bm)) * ceil_div(N, t.bn);
+    for (int want = 1; want <= 32 && want <= ktiles; want *= 2) {
+      const int per = ceil_div(ktiles, want), splits = ceil_div(ktiles, per);
+      const long groups = tiles * splits, slots = static_cast<long>(cus) * t.per_cu;
+      double us = static_cast<double>((groups + slots - 1) / slots) * (per * t.us + 3.0);
+      if (splits > 1) us += 3.0 + (2.0 * splits) * M * N * 4 / 4e6;
+      if (us < best_us) {
+        best_us = us;
+        best    = FfPlan{c, splits, per * G16_BK};
+      }
+    }
+  }
+  return best;
+}
+size_t ff_partial_bytes(const FfPlan &p, size_t elements) { return p.splits > 1 ? ws_align(4 * p.splits * elements) : 0; }
+
+// N: the columns of B in use (PAIR: both halves)
+template <class T, bool A_KC, bool B_KC, bool PAIR, class Epi>
+int ff_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const Epi &epi, int M, int N, int K, const char *tag) {
+  ProfScope prof(tag, M, N, K);
+  const FfTile &t   = FF_TILES[p.cfg];
+  const int tiles_m = ceil_div(M, t.bm), tiles_n = PAIR ? ceil_div(N / 2, t.bn / 2) : ceil_div(N, t.bn);
+  const dim3 grid(static_cast<unsigned>(tiles_m) * tiles_n * p.splits);
+  auto go = [&](auto kernel, int threads) {
+    TDH_LAUNCH(kernel, grid, dim3(threads), 0, ctx().stream, A, B, epi, tiles_m, tiles_n, K, p.k_per_split);
+    TDH_LAUNCH_CHECK();
+    return static_cast<int>(TDH_OK);
+  };
+  switch (p.cfg) {
+    case 0: return go(gemm16_kernel<T, 2, 4, 4, 2, A_KC, B_KC, PAIR, Epi>, 512);
+    case 1: return go(gemm16_kernel<T, 2, 2, 2, 2, A_KC, B_KC, PAIR, Epi>, 256);
+    default: return go(gemm16_kernel<T, 1, 4, 1, 2, A_KC, B_KC, PAIR, Epi>, 256);
+  }
+}
+
+// `src` as the products read it: itself where it lies on 16-byte boundaries, else a padded copy out of the scratch
+int padded(int n) { return (n + 7) & ~7; }
+template <class T>
+bool fits(const T *p, int cols) { return cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+template <class T>
+size_t pack_bytes(const T *p, int rows, int used, int halves) {
+  return fits(p, used) ? 0 : ws_align(static_cast<size_t>(rows) * halves * padded(used) * sizeof(T));
+}
+template <class T>
+int pack(const T *src, int rows, int used, int halves, G16Matrix *out) {
+  const int half = padded(used);
+  *out = G16Matrix{src, static_cast<long>(halves) * half, rows, halves * half};
+  if (fits(src, used)) return TDH_OK;
+  T *copy;
+  const size_t total = static_cast<size_t>(rows) * halves * half;
+  TDH_TRY(take(total, &copy));
+  ProfScope prof("ff_pack", 2.0 * sizeof(T) * total, WORK_BYTE);
+  TDH_LAUNCH((pack_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, src, copy, total,
+             used, half, halves);
+  TDH_LAUNCH_CHECK();
+  out->p = copy;
+  return TDH_OK;
+}
+
+template <class T>
+int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
+  const int half    = padded(hidden);
+  const FfPlan plan = ff_plan(batch, 2 * half, in);
+  const size_t part = static_cast<size_t>(batch) * 2 * half;
+  TDH_TRY(ws_begin(pack_bytes(x, batch, in, 1) + pack_bytes(w, in, hidden, 2) + ff_partial_bytes(plan, part)));
+  G16Matrix A, B;
+  TDH_TRY(pack(x, batch, in, 1, &A));
+  TDH_TRY(pack(w, in, hidden, 2, &B));
+  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act};
+  if (plan.splits > 1) TDH_TRY(take(plan.splits * part, &epi.partial));
+  TDH_TRY((ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd")));
+  if (plan.splits > 1) {
+    const size_t total = static_cast<size_t>(batch) * hidden;
+    ProfScope prof("gated_ff_fwd_reduce", 8.0 * plan.splits * total, WORK_BYTE);
+    TDH_LAUNCH((gate_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, plan.splits);
+    TDH_LAUNCH_CHECK();
+  }
+  return TDH_OK;
+}
+
+template <class T, bool A_KC, bool B_KC>
+int ff_grad(const FfPlan &plan, const G16Matrix &A, const G16Matrix &B, EpiGrad<T> epi, int K, const char *tag) {
+  if (plan.splits > 1) TDH_TRY(take(plan.splits * static_cast<size_t>(epi.rows) * epi.cols, &epi.partial));
+  TDH_TRY((ff_gemm<T, A_KC, B_KC, false>(plan, A, B, epi, epi.rows, epi.cols, K, tag)));
+  if (plan.splits > 1) {
+    const size_t total = static_cast<size_t>(epi.rows) * epi.cols;
+    ProfScope prof("gated_ff_bwd_reduce", 4.0 * plan.splits * total, WORK_BYTE);
+    TDH_LAUNCH((grad_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, plan.splits);
+    TDH_LAUNCH_CHECK();
+  }
+  return TDH_OK;
+}
+
+template <class T>
+int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
+              int accumulate) {
+  const int half = padded(hidden), bands = ceil_div(batch, DZ_ROWS);
+  const FfPlan px = ff_plan(batch, in, 2 * half), pw = ff_plan(in, 2 * half, batch);
+  const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
+  TDH_TRY(ws_begin(ws_align(sizeof(T) * batch * 2 * half) + ws_align(4 * static_cast<size_t>(bands) * 2 * hidden) +
+                   (dx ? pack_bytes(w, in, hidden, 2) + ff_partial_bytes(px, nx) : 0) +
+                   (dw ? pack_bytes(x, batch, in, 1) + ff_partial_bytes(pw, nw) : 0)));
+  T *dz = nullptr;
+  float *bias_part = nullptr;
+  if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * 2 * half, &dz));
+  if (db) TDH_TRY(take(static_cast<size_t>(bands) * 2 * hidden, &bias_part));
+  {
+    ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
+    const int blocks_n = ceil_div(half, GF_NT);
+    TDH_LAUNCH((gate_dz_kernel<T>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half, act,
+               blocks_n);
+    TDH_LAUNCH_CHECK();
+  }
+  if (db) {
+    ProfScope prof("gated_ff_db", 8.0 * bands * hidden, WORK_BYTE);
+    TDH_LAUNCH((bias_sum_kernel<T>), dim3(ceil_div(2 * hidden, GF_NT)), dim3(GF_NT), 0, ctx().stream, bias_part, db, bands, 2 * hidden, accumulate);
+    TDH_LAUNCH_CHECK();
+  }
+  const G16Matrix Z{dz, 2L * half, batch, 2 * half};
+  if (dx) {
+    G16Matrix W;   // [in][2 half], rows along m of the product are w's rows
+    TDH_TRY(pack(w, in, hidden, 2, &W));
+    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx")));
+  }
+  if (dw) {
+    G16Matrix X;
+    TDH_TRY(pack(x, batch, in, 1, &X));
+    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw")));
+  }
+  return TDH_OK;
 }
 
 int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch) {
@@ -164,6 +442,8 @@ int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch)
   TDH_CHECK_ARG(in > 0 && hidden > 0 && batch >= 0, "%s: bad shape %d->2*%d batch %d", who, in, hidden, batch);
   TDH_CHECK_ARG(2L * in * hidden < (1L << 31) && static_cast<long>(batch) * in < (1L << 31) && 2L * batch * hidden < (1L << 31),
                 "%s: tensor exceeds 2^31 elements", who);
+  // (offsets within a tile of 256 rows are 32 bits)
+  TDH_CHECK_ARG(dtype == TDH_F32 || (in <= (1 << 21) && hidden <= (1 << 20)), "%s: %d->2*%d is too wide for 16-bit types", who, in, hidden);
   return TDH_OK;
 }
 int check_aligned(const char *who, int dtype, std::initializer_list<const void *> tensors) {
@@ -190,8 +470,11 @@ int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int b
   if (batch == 0) return TDH_OK;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    return ff_fwd<T>(act, in, hidden, batch, static_cast<const T *>(x), static_cast<const T *>(w),
-                     has_bias ? static_cast<const T *>(b) : nullptr, static_cast<T *>(h), z);
+    const T *xt = static_cast<const T *>(x), *wt = static_cast<const T *>(w), *bt = has_bias ? static_cast<const T *>(b) : nullptr;
+    if constexpr (sizeof(T) == 4)
+      return ff_fwd_f32(act, in, hidden, batch, xt, wt, bt, static_cast<T *>(h), z);
+    else
+      return ff_fwd_16<T>(act, in, hidden, batch, xt, wt, bt, static_cast<T *>(h), z);
   });
 }
 
@@ -205,8 +488,12 @@ int tdh_gated_ff_bwd(int dtype, int act, int in, int hidden, int has_bias, int b
   if (batch == 0) return TDH_OK;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    return ff_bwd<T>(act, in, hidden, batch, static_cast<const T *>(x), static_cast<const T *>(w), z, static_cast<const T *>(dh),
-                     static_cast<T *>(dx), static_cast<T *>(dw), has_bias ? static_cast<T *>(db) : nullptr, accumulate);
+    const T *xt = static_cast<const T *>(x), *wt = static_cast<const T *>(w), *dt = static_cast<const T *>(dh);
+    T *dbt = has_bias ? static_cast<T *>(db) : nullptr;
+    if constexpr (sizeof(T) == 4)
+      return ff_bwd_f32(act, in, hidden, batch, xt, wt, z, dt, static_cast<T *>(dx), static_cast<T *>(dw), dbt, accumulate);
+    else
+      return ff_bwd_16<T>(act, in, hidden, batch, xt, wt, z, dt, static_cast<T *>(dx), static_cast<T *>(dw), dbt, accumulate);
   });
 }
 
