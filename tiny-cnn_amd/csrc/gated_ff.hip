@@ -9,58 +9,76 @@ namespace {
 
 constexpr int GF_NT = 256;
 
+// 1 / (1 + exp(-x)); the two instructions are off by an ulp each
+__device__ __forceinline__ float logistic(const float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
 // the gate's activation, and its derivative
-__device__ __forceinline__ float gate_act(const int kind, const float g, float *slope) {
-  switch (kind) {
-    case TDH_GATE_SILU: {
-      const float s = 1.0f / (1.0f + expf(-g));
-      *slope = s * (1.0f + g * (1.0f - s));
-      return g * s;
-    }
-    case TDH_GATE_GELU: {
-      const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-      *slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
-      return g * cdf;
-    }
-    case TDH_GATE_GELU_TANH: {
-      // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3)
-      const float y2 = 1.5957691216057308f * (g + 0.044715f * g * g * g);
-      const float s  = 1.0f / (1.0f + expf(-y2));
-      *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * g * g));
-      return g * s;
-    }
-    case TDH_GATE_SIGMOID: {
-      const float s = 1.0f / (1.0f + expf(-g));
-      *slope = s * (1.0f - s);
-      return s;
-    }
-    case TDH_GATE_RELU: *slope = g > 0.0f ? 1.0f : 0.0f; return g > 0.0f ? g : 0.0f;
-    default: *slope = 1.0f; return g;
+template <int KIND>
+__device__ __forceinline__ float gate_act(const float g, float *slope) {
+  if constexpr (KIND == TDH_GATE_SILU) {
+    const float s = logistic(g);
+    *slope = s * (1.0f + g * (1.0f - s));
+    return g * s;
+  } else if constexpr (KIND == TDH_GATE_GELU) {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    *slope = cdf + g * (0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g));
+    return g * cdf;
+  } else if constexpr (KIND == TDH_GATE_GELU_TANH) {
+    // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3)
+    const float s = logistic(1.5957691216057308f * (g + 0.044715f * g * g * g));
+    *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * g * g));
+    return g * s;
+  } else if constexpr (KIND == TDH_GATE_SIGMOID) {
+    const float s = logistic(g);
+    *slope = s * (1.0f - s);
+    return s;
+  } else if constexpr (KIND == TDH_GATE_RELU) {
+    *slope = g > 0.0f ? 1.0f : 0.0f;
+    return g > 0.0f ? g : g != g ? g : 0.0f;
+  } else {
+    *slope = 1.0f;
+    return g;
+  }
+}
+// f with the kind as a constant: one branch around a loop, not one in every turn
+template <class F>
+__device__ __forceinline__ void with_gate(const int act, const F &f) {
+  switch (act) {
+    case TDH_GATE_SILU: return f(std::integral_constant<int, TDH_GATE_SILU>());
+    case TDH_GATE_GELU: return f(std::integral_constant<int, TDH_GATE_GELU>());
+    case TDH_GATE_GELU_TANH: return f(std::integral_constant<int, TDH_GATE_GELU_TANH>());
+    case TDH_GATE_SIGMOID: return f(std::integral_constant<int, TDH_GATE_SIGMOID>());
+    case TDH_GATE_RELU: return f(std::integral_constant<int, TDH_GATE_RELU>());
+    default: return f(std::integral_constant<int, TDH_GATE_NONE>());
   }
 }
 
-template <class T>
 __global__ void __launch_bounds__(GF_NT)
-gate_fwd_kernel(const float *__restrict__ z, T *__restrict__ h, const int hidden, const size_t total, const int act) {
+gate_fwd_kernel(const float *__restrict__ z, float *__restrict__ h, const int hidden, const size_t total, const int act) {
   const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
   if (i >= total) return;
   const size_t row = i / hidden, c = i - row * hidden;
-  float slope;
-  const float a = gate_act(act, z[row * 2 * hidden + c], &slope);
-  h[i] = from_f32<T>(a * z[row * 2 * hidden + hidden + c]);
+  with_gate(act, [&](auto kind) {
+    float slope;
+    const float a = gate_act<decltype(kind)::value>(z[row * 2 * hidden + c], &slope);
+    h[i] = a * z[row * 2 * hidden + hidden + c];
+  });
 }
 
-template <class T>
 __global__ void __launch_bounds__(GF_NT)
-gate_bwd_kernel(const float *__restrict__ z, const T *__restrict__ dh, float *__restrict__ dz, const int hidden,
+gate_bwd_kernel(const float *__restrict__ z, const float *__restrict__ dh, float *__restrict__ dz, const int hidden,
                 const size_t total, const int act) {
   const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
   if (i >= total) return;
   const size_t row = i / hidden, c = i - row * hidden;
-  float slope;
-  const float a = gate_act(act, z[row * 2 * hidden + c], &slope), d = to_f32(dh[i]);
-  dz[row * 2 * hidden + c]          = d * z[row * 2 * hidden + hidden + c] * slope;
-  dz[row * 2 * hidden + hidden + c] = d * a;
+  with_gate(act, [&](auto kind) {
+    float slope;
+    const float a = gate_act<decltype(kind)::value>(z[row * 2 * hidden + c], &slope), d = dh[i];
+    dz[row * 2 * hidden + c]          = d * z[row * 2 * hidden + hidden + c] * slope;
+    dz[row * 2 * hidden + hidden + c] = d * a;
+  });
 }
 
 // dst = src in another type
@@ -68,8 +86,7 @@ template <class D, class S>
 __global__ void __launch_bounds__(GF_NT)
 cast_kernel(const S *__restrict__ src, D *__restrict__ dst, const size_t n) {
   const size_t stride = static_cast<size_t>(gridDim.x) * GF_NT;
-  for (size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x; i < n; i += stride)
-    dst[i] = from_f32<D>(to_f32(src[i]));
+  for (size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x; i < n; i += stride) dst[i] = from_f32<D>(to_f32(src[i]));
 }
 
 template <class D, class S>
@@ -98,7 +115,7 @@ int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   TDH_TRY(fc_fwd(in, 2 * hidden, b != nullptr, batch, x, w, b, z));
   const size_t total = nz / 2;
   ProfScope prof("gate_fwd", 12.0 * total, WORK_BYTE);
-  TDH_LAUNCH((gate_fwd_kernel<float>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h,
+  TDH_LAUNCH(gate_fwd_kernel, dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h,
              hidden, total, act);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
@@ -112,7 +129,7 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   const size_t total = nz / 2;
   {
     ProfScope prof("gate_bwd", 20.0 * total, WORK_BYTE);
-    TDH_LAUNCH((gate_bwd_kernel<float>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, dh,
+    TDH_LAUNCH(gate_bwd_kernel, dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, dh,
                dz, hidden, total, act);
     TDH_LAUNCH_CHECK();
   }
@@ -131,39 +148,68 @@ struct EpiGate {
   const T *bias;       // or null
   float *partial;      // slices of z instead, [split][rows][2 half]
   int rows, hidden, half, act;
-  __device__ __forceinline__ void one(const size_t m, const int n, float g, float u) const {
-    if (bias) {
-      g += to_f32(bias[n]);
-      u += to_f32(bias[hidden + n]);
-    }
-    if (z) {
-      z[m * 2 * hidden + n]          = g;
-      z[m * 2 * hidden + hidden + n] = u;
+  bool wide;           // h's rows lie on 16-byte boundaries
+  // g and u at (m, n) to h; writes z
+  template <int KIND>
+  __device__ __forceinline__ float one(const size_t m, const int n, const float g, const float u) const {
+    if (z) {   // (read in the backward pass, after much else: past the caches)
+      __builtin_nontemporal_store(g, z + m * 2 * hidden + n);
+      __builtin_nontemporal_store(u, z + m * 2 * hidden + hidden + n);
     }
     float slope;
-    h[m * hidden + n] = from_f32<T>(gate_act(act, g, &slope) * u);
+    return gate_act<KIND>(g, &slope) * u;
   }
   template <int TM, int TN>
-  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split) const {
-#pragma unroll
-    for (int j = 0; j < TN / 2; ++j) {
-      const int n = n0 + 32 * j + (lane & 31);
-      if (n >= hidden) continue;
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split,
+                                       float *lds) const {
+    const int n = n0 + (lane & 31), m = m0 + 4 * (lane >> 5);
+    if (partial) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-          if (m >= rows) continue;
-          if (partial) {
-            float *p = partial + (static_cast<size_t>(split) * rows + m) * 2 * half;
-            p[n]        = acc[i][2 * j][r];
-            p[half + n] = acc[i][2 * j + 1][r];
-          } else {
-            one(m, n, acc[i][2 * j][r], acc[i][2 * j + 1][r]);
-          }
+          const int row = m + 32 * i + 8 * (r >> 2) + (r & 3);
+          float *p = partial + (static_cast<size_t>(split) * rows + row) * 2 * half;
+#pragma unroll
+          for (int j = 0; j < TN / 2; ++j)
+            if (row < rows && n + 32 * j < hidden) {
+              p[n + 32 * j]        = acc[i][2 * j][r];
+              p[half + n + 32 * j] = acc[i][2 * j + 1][r];
+            }
         }
+      return;
     }
+    float bg[TN / 2], bu[TN / 2];
+#pragma unroll
+    for (int j = 0; j < TN / 2; ++j) {
+      const bool in = bias && n + 32 * j < hidden;
+      bg[j] = in ? to_f32(bias[n + 32 * j]) : 0.0f;
+      bu[j] = in ? to_f32(bias[hidden + n + 32 * j]) : 0.0f;
+    }
+    with_gate(act, [&](auto kind) {
+      const G16Turn<16 * TN> turn{lds};
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN / 2; ++j)
+          turn.put(lane, j, [&](int r) {
+            const int row = m + 32 * i + 8 * (r >> 2) + (r & 3);
+            if (row >= rows || n + 32 * j >= hidden) return 0.0f;
+            return one<decltype(kind)::value>(row, n + 32 * j, acc[i][2 * j][r] + bg[j], acc[i][2 * j + 1][r] + bu[j]);
+          });
+        turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
+          if (m0 + 32 * i + row >= rows) return;
+          T *p = h + static_cast<size_t>(m0 + 32 * i + row) * hidden + n0 + col;
+          if (wide) {
+            if (n0 + col < hidden) *reinterpret_cast<uint4 *>(p) = Word<T>::from(v).raw;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n0 + col + e < hidden) p[e] = from_f32<T>(v[e]);
+          }
+        });
+      }
+    });
   }
 };
 
@@ -175,6 +221,7 @@ struct EpiGrad {
   int rows, cols;      // of C
   int hidden, half;    // two halves of columns, as above (one: both are cols)
   int accumulate;
+  bool wide;           // out's rows lie on 16-byte boundaries, and its columns are C's
   __device__ __forceinline__ void one(const size_t m, int n, float v) const {
     if (n >= hidden) {
       if (n < half || n - half >= hidden) return;
@@ -185,22 +232,45 @@ struct EpiGrad {
     *p = from_f32<T>(v);
   }
   template <int TM, int TN>
-  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split) const {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + 32 * j + (lane & 31);
-      if (n >= cols) continue;
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split,
+                                       float *lds) const {
+    if (partial) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int m = m0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-          if (m >= rows) continue;
-          if (partial)
-            partial[(static_cast<size_t>(split) * rows + m) * cols + n] = acc[i][j][r];
-          else
-            one(m, n, acc[i][j][r]);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int n = n0 + 32 * j + (lane & 31);
+            if (m < rows && n < cols) partial[(static_cast<size_t>(split) * rows + m) * cols + n] = acc[i][j][r];
+          }
         }
+      return;
+    }
+    const G16Turn<32 * TN> turn{lds};
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) turn.put(lane, j, [&](int r) { return acc[i][j][r]; });
+      turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
+        const int m = m0 + 32 * i + row, n = n0 + col;
+        if (m >= rows) return;
+        if (wide) {
+          if (n >= cols) return;
+          uint4 *p = reinterpret_cast<uint4 *>(out + static_cast<size_t>(m) * cols + n);
+          float o[8];
+          Word<T> was{};
+          if (accumulate) was.raw = *p;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = accumulate ? v[e] + was[e] : v[e];
+          *p = Word<T>::from(o).raw;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < cols) one(m, n + e, v[e]);
+        }
+      });
     }
   }
 };
@@ -219,7 +289,11 @@ gate_reduce_kernel(const EpiGate<T> epi, const int splits) {
     g += p[s * slice];
     u += p[s * slice + epi.half];
   }
-  epi.one(m, n, g, u);
+  if (epi.bias) {
+    g += to_f32(epi.bias[n]);
+    u += to_f32(epi.bias[epi.hidden + n]);
+  }
+  with_gate(epi.act, [&](auto kind) { epi.h[i] = from_f32<T>(epi.template one<decltype(kind)::value>(m, n, g, u)); });
 }
 template <class T>
 __global__ void __launch_bounds__(GF_NT)
@@ -245,35 +319,70 @@ pack_kernel(const T *__restrict__ src, T *__restrict__ dst, const size_t total, 
 }
 
 // dz in the operand's type, [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
-// workgroup's band (in fp32, before the rounding)
+// workgroup's band (in fp32, before the rounding). A thread takes E columns: eight where every row lies on a 16-byte
+// boundary (wide), else one.
 constexpr int DZ_ROWS = 32;
-template <class T>
+template <class T, int E>
 __global__ void __launch_bounds__(GF_NT)
 gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restrict__ dz, float *__restrict__ bias_part,
                const int rows, const int hidden, const int half, const int act, const int blocks_n) {
-  const int n = blockIdx.x % blocks_n * GF_NT + threadIdx.x, band = blockIdx.x / blocks_n;
+  const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
   if (n >= half) return;
-  float sg = 0.0f, su = 0.0f;
+  float sg[E] = {}, su[E] = {};
   const int end = min(rows, (band + 1) * DZ_ROWS);
-  for (int m = band * DZ_ROWS; m < end; ++m) {
-    float dg = 0.0f, du = 0.0f;
-    if (n < hidden) {
+  with_gate(act, [&](auto kind) {
+#pragma unroll 2
+    for (int m = band * DZ_ROWS; m < end; ++m) {
+      float g[E], u[E], d[E], dg[E], du[E];
       const float *zr = z + static_cast<size_t>(m) * 2 * hidden + n;
-      float slope;
-      const float a = gate_act(act, zr[0], &slope), d = to_f32(dh[static_cast<size_t>(m) * hidden + n]);
-      dg = d * zr[hidden] * slope;
-      du = d * a;
+      const T *dr     = dh + static_cast<size_t>(m) * hidden + n;
+      if constexpr (E == 8) {
+        const float4 g0 = reinterpret_cast<const float4 *>(zr)[0], g1 = reinterpret_cast<const float4 *>(zr)[1];
+        const float4 u0 = reinterpret_cast<const float4 *>(zr + hidden)[0], u1 = reinterpret_cast<const float4 *>(zr + hidden)[1];
+        const Word<T> w{*reinterpret_cast<const uint4 *>(dr)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = (&g0.x)[e];
+          g[4 + e] = (&g1.x)[e];
+          u[e] = (&u0.x)[e];
+          u[4 + e] = (&u1.x)[e];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = w[e];
+      } else {
+        const bool in = n < hidden;
+        g[0] = in ? zr[0] : 0.0f;
+        u[0] = in ? zr[hidden] : 0.0f;
+        d[0] = in ? to_f32(dr[0]) : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float slope;
+        const float a = gate_act<decltype(kind)::value>(g[e], &slope);
+        dg[e] = d[e] * u[e] * slope;
+        du[e] = d[e] * a;
+        sg[e] += dg[e];
+        su[e] += du[e];
+      }
+      if (dz) {
+        T *o = dz + static_cast<size_t>(m) * 2 * half + n;
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint4 *>(o)        = Word<T>::from(dg).raw;
+          *reinterpret_cast<uint4 *>(o + half) = Word<T>::from(du).raw;
+        } else {
+          o[0]    = from_f32<T>(dg[0]);
+          o[half] = from_f32<T>(du[0]);
+        }
+      }
     }
-    if (dz) {
-      dz[static_cast<size_t>(m) * 2 * half + n]        = from_f32<T>(dg);
-      dz[static_cast<size_t>(m) * 2 * half + half + n] = from_f32<T>(du);
-    }
-    sg += dg;
-    su += du;
-  }
+  });
   if (bias_part && n < hidden) {
-    bias_part[static_cast<size_t>(band) * 2 * hidden + n]          = sg;
-    bias_part[static_cast<size_t>(band) * 2 * hidden + hidden + n] = su;
+    float *p = bias_part + static_cast<size_t>(band) * 2 * hidden + n;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      p[e]          = sg[e];
+      p[hidden + e] = su[e];
+    }
   }
 }
 template <class T>
@@ -372,7 +481,7 @@ int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   G16Matrix A, B;
   TDH_TRY(pack(x, batch, in, 1, &A));
   TDH_TRY(pack(w, in, hidden, 2, &B));
-  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act};
+  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act, fits(h, hidden)};
   if (plan.splits > 1) TDH_TRY(take(plan.splits * part, &epi.partial));
   TDH_TRY((ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd")));
   if (plan.splits > 1) {
@@ -412,9 +521,14 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   if (db) TDH_TRY(take(static_cast<size_t>(bands) * 2 * hidden, &bias_part));
   {
     ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
-    const int blocks_n = ceil_div(half, GF_NT);
-    TDH_LAUNCH((gate_dz_kernel<T>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half, act,
-               blocks_n);
+    const bool wide    = hidden % 8 == 0 && ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
+    const int blocks_n = ceil_div(half, wide ? 8 * GF_NT : GF_NT);
+    if (wide)
+      TDH_LAUNCH((gate_dz_kernel<T, 8>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
+                 act, blocks_n);
+    else
+      TDH_LAUNCH((gate_dz_kernel<T, 1>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
+                 act, blocks_n);
     TDH_LAUNCH_CHECK();
   }
   if (db) {
@@ -426,12 +540,12 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   if (dx) {
     G16Matrix W;   // [in][2 half], rows along m of the product are w's rows
     TDH_TRY(pack(w, in, hidden, 2, &W));
-    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx")));
+    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0, fits(dx, in)}, 2 * half, "gated_ff_dx")));
   }
   if (dw) {
     G16Matrix X;
     TDH_TRY(pack(x, batch, in, 1, &X));
-    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw")));
+    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate, fits(dw, hidden)}, batch, "gated_ff_dw")));
   }
   return TDH_OK;
 }

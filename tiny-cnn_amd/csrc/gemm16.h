@@ -146,8 +146,40 @@ __device__ __forceinline__ void g16_tile(int id, const int tiles_m, const int ti
   tn = id / rows;
 }
 
-// Epi: done(acc, m0, n0, lane, split) with the wave's blocks: register r of lane l of block (i, j) is row
-// m0 + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 and column n0 + 32 j + l % 32 (PAIR: of the tile's column order).
+// 32 rows of COLS fp32 values that a wave turns in LDS, so that a lane has eight neighbours of one row: put() takes
+// block j in the matrix cores' layout, rows() hands out (row, column of the first, values).
+template <int COLS>
+struct G16Turn {
+  static constexpr int STRIDE = COLS + 4, BYTES = 32 * STRIDE * 4;
+  float *at;
+  template <class F>
+  __device__ __forceinline__ void put(const int lane, const int j, const F &value) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) at[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * STRIDE + 32 * j + (lane & 31)] = value(r);
+  }
+  template <class F>
+  __device__ __forceinline__ void rows(const int lane, const F &take) const {
+    constexpr int PER = COLS / 8, ROWS = 64 / PER;   // lanes a row, rows at a time
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 32 / ROWS; ++k) {
+      const int row = k * ROWS + lane / PER, col = lane % PER * 8;
+      const float4 *p = reinterpret_cast<const float4 *>(at + row * STRIDE + col);
+      const float4 lo = p[0], hi = p[1];
+      const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      take(row, col, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (before the next put)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+};
+
+// Epi: done(acc, m0, n0, lane, split, lds) with the wave's blocks: register r of lane l of block (i, j) is row
+// m0 + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 and column n0 + 32 j + l % 32 (PAIR: of the tile's column order); lds:
+// G16Turn<32 TN>::BYTES of the wave's own.
 template <class T, int WM, int WN, int TM, int TN, bool A_KC, bool B_KC, bool PAIR, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN)
 gemm16_kernel(const G16Matrix A, const G16Matrix B, const Epi epi, const int tiles_m, const int tiles_n, const int K,
@@ -208,7 +240,10 @@ gemm16_kernel(const G16Matrix A, const G16Matrix B, const Epi epi, const int til
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma16(T(), a[i], b[j], acc[i][j]);
     }
   }
-  epi.template done<TM, TN>(acc, m0 + 32 * TM * wm, n0 + (PAIR ? 16 * TN * wn : 32 * TN * wn), lane, split);
+  static_assert(sizeof(lds) >= WM * WN * G16Turn<32 * TN>::BYTES, "");
+  __syncthreads();
+  epi.template done<TM, TN>(acc, m0 + 32 * TM * wm, n0 + (PAIR ? 16 * TN * wn : 32 * TN * wn), lane, split,
+                            reinterpret_cast<float *>(lds[0] + wave * G16Turn<32 * TN>::BYTES));
 }
 
 }  // namespace
