@@ -105,7 +105,7 @@ def test_dropout_in_place_rate_zero_and_exceptional_values(T, dtype):
 # ------------------------------------------------------- gated feed-forward
 
 ACTS = ["silu", "gelu", "gelu_tanh", "sigmoid", "relu", "none"]
-SHAPES = [(1, 1, 1), (1, 64, 32), (1, 257, 100), (2, 8, 8), (3, 7, 33), (5, 100, 1), (7, 1, 64), (16, 64, 64), (17, 40, 24),
+SHAPES = [(1, 1, 1), (1, 9000, 24), (2, 5000, 40), (3, 520, 1100), (4, 300, 70), (6, 64, 520), (8, 2100, 36), (9, 65, 40), (1, 64, 32), (1, 257, 100), (2, 8, 8), (3, 7, 33), (5, 100, 1), (7, 1, 64), (16, 64, 64), (17, 40, 24),
           (33, 128, 200), (64, 96, 128), (65, 257, 130), (130, 72, 72), (200, 320, 264)]
 
 
@@ -177,6 +177,20 @@ def test_gated_ff_gradients_left_out(T, dtype):
         T.gated_ff_bwd(d, f, True, n, x, w, z, dh, one if k == "dx" else None, one if k == "dw" else None,
                        one if k == "db" else None, act="silu", dtype=dtype)
         L.within(one.read(), *want[k], k + " alone")
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+def test_gated_ff_without_rows(T, dtype):
+    """The weight gradients of no samples are zero, or with accumulate what they were."""
+    d, f = 9, 7
+    x, w, h = (Buf(T, np.ones(s), dtype) for s in ((1, d), (d, 2 * f), (1, f)))
+    z = Buf(T, np.ones((1, 2 * f)))
+    dw, db = out(T, (d, 2 * f), dtype), out(T, 2 * f, dtype)
+    T.gated_ff_fwd(d, f, False, 0, x, w, None, h, z, dtype=dtype)
+    T.gated_ff_bwd(d, f, True, 0, x, w, z, h, x, dw, db, dtype=dtype, accumulate=True)
+    assert (dw.read() == 3.25).all() and (db.read() == 3.25).all()
+    T.gated_ff_bwd(d, f, True, 0, x, w, z, h, x, dw, db, dtype=dtype)
+    assert (dw.read() == 0).all() and (db.read() == 0).all() and (h.read() == 1).all() and (x.read() == 1).all()
 
 
 @pytest.mark.parametrize("dtype", L.DTYPES)

@@ -159,6 +159,14 @@ struct EpiGate {
     float slope;
     return gate_act<KIND>(g, &slope) * u;
   }
+  // the whole sums of (m, n), without the bias
+  __device__ __forceinline__ void finish(const size_t m, const int n, float g, float u) const {
+    if (bias) {
+      g += to_f32(bias[n]);
+      u += to_f32(bias[hidden + n]);
+    }
+    with_gate(act, [&](auto kind) { h[m * hidden + n] = from_f32<T>(one<decltype(kind)::value>(m, n, g, u)); });
+  }
   template <int TM, int TN>
   __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split,
                                        float *lds) const {
@@ -279,21 +287,27 @@ struct EpiGrad {
 template <class T>
 __global__ void __launch_bounds__(GF_NT)
 gate_reduce_kernel(const EpiGate<T> epi, const int splits) {
-  const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
+  const size_t i = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= static_cast<size_t>(epi.rows) * epi.hidden) return;
   const size_t m = i / epi.hidden, slice = static_cast<size_t>(epi.rows) * 2 * epi.half;
   const int n = static_cast<int>(i - m * epi.hidden);
   const float *p = epi.partial + m * 2 * epi.half + n;
   float g = 0.0f, u = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
     g += p[s * slice];
     u += p[s * slice + epi.half];
   }
-  if (epi.bias) {
-    g += to_f32(epi.bias[n]);
-    u += to_f32(epi.bias[epi.hidden + n]);
-  }
-  with_gate(epi.act, [&](auto kind) { epi.h[i] = from_f32<T>(epi.template one<decltype(kind)::value>(m, n, g, u)); });
+  epi.finish(m, n, g, u);
+}
+template <class T>
+int launch_gate_reduce(const EpiGate<T> &epi, int splits) {
+  const size_t total = static_cast<size_t>(epi.rows) * epi.hidden;
+  const int threads  = total < 32768 ? 64 : GF_NT;
+  ProfScope prof("gated_ff_fwd_reduce", 8.0 * splits * total, WORK_BYTE);
+  TDH_LAUNCH((gate_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, threads))), dim3(threads), 0, ctx().stream, epi, splits);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
 }
 template <class T>
 __global__ void __launch_bounds__(GF_NT)
@@ -302,51 +316,69 @@ grad_reduce_kernel(const EpiGrad<T> epi, const int splits) {
   if (i >= total) return;
   const size_t m = i / epi.cols;
   float v = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) v += epi.partial[s * total + i];
   epi.one(m, static_cast<int>(i - m * epi.cols), v);
 }
 
-// A matrix copied to a padded one: columns in one or two halves of `used` values, `half` apart in the copy; what is
-// behind a half is zero.
+// Matrices copied to padded ones: columns in one or two halves of `used` values, `half` (a multiple of 8) apart in the copy;
+// what is behind a half is zero. A thread writes eight values as a word.
+template <class T>
+struct PackJobs {
+  struct Job {
+    const T *src;
+    T *dst;
+    int used, half, halves;
+    unsigned blocks;
+    size_t words;
+  } job[2];
+};
 template <class T>
 __global__ void __launch_bounds__(GF_NT)
-pack_kernel(const T *__restrict__ src, T *__restrict__ dst, const size_t total, const int used, const int half, const int halves) {
-  const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
-  if (i >= total) return;
-  const size_t row = i / (halves * half);
-  const int c = static_cast<int>(i - row * (halves * half)), h = c >= half ? 1 : 0, n = c - h * half;
-  dst[i] = n < used ? src[(row * halves + h) * used + n] : T{};
+pack_kernel(const PackJobs<T> jobs) {
+  const bool second = blockIdx.x >= jobs.job[0].blocks;
+  const typename PackJobs<T>::Job &j = jobs.job[second];
+  const size_t i = static_cast<size_t>(blockIdx.x - (second ? jobs.job[0].blocks : 0)) * GF_NT + threadIdx.x;
+  if (i >= j.words) return;
+  const int per = j.half / 8;   // words of a half
+  const size_t row = i / (per * j.halves);
+  int c = static_cast<int>(i - row * (per * j.halves)), h = c >= per ? 1 : 0;
+  c = (c - h * per) * 8;
+  const T *p = j.src + (row * j.halves + h) * j.used + c;
+  T v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = c + e < j.used ? p[e] : T{};
+  *reinterpret_cast<uint4 *>(j.dst + i * 8) = *reinterpret_cast<const uint4 *>(v);
 }
 
 // dz in the operand's type, [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
-// workgroup's band (in fp32, before the rounding). A thread takes E columns: eight where every row lies on a 16-byte
-// boundary (wide), else one.
-constexpr int DZ_ROWS = 32;
+// workgroup's band (in fp32, before the rounding). A thread takes E columns: a 16-byte word where every row lies on a 16-byte
+// boundary, else one.
 template <class T, int E>
 __global__ void __launch_bounds__(GF_NT)
 gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restrict__ dz, float *__restrict__ bias_part,
-               const int rows, const int hidden, const int half, const int act, const int blocks_n) {
+               const int rows, const int hidden, const int half, const int act, const int blocks_n, const int band_rows) {
   const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
   if (n >= half) return;
   float sg[E] = {}, su[E] = {};
-  const int end = min(rows, (band + 1) * DZ_ROWS);
+  const int end = min(rows, (band + 1) * band_rows);
   with_gate(act, [&](auto kind) {
 #pragma unroll 2
-    for (int m = band * DZ_ROWS; m < end; ++m) {
+    for (int m = band * band_rows; m < end; ++m) {
       float g[E], u[E], d[E], dg[E], du[E];
       const float *zr = z + static_cast<size_t>(m) * 2 * hidden + n;
       const T *dr     = dh + static_cast<size_t>(m) * hidden + n;
-      if constexpr (E == 8) {
-        const float4 g0 = reinterpret_cast<const float4 *>(zr)[0], g1 = reinterpret_cast<const float4 *>(zr)[1];
-        const float4 u0 = reinterpret_cast<const float4 *>(zr + hidden)[0], u1 = reinterpret_cast<const float4 *>(zr + hidden)[1];
-        const Word<T> w{*reinterpret_cast<const uint4 *>(dr)};
+      if constexpr (E > 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = (&g0.x)[e];
-          g[4 + e] = (&g1.x)[e];
-          u[e] = (&u0.x)[e];
-          u[4 + e] = (&u1.x)[e];
+        for (int q = 0; q < E / 4; ++q) {
+          const float4 gq = reinterpret_cast<const float4 *>(zr)[q], uq = reinterpret_cast<const float4 *>(zr + hidden)[q];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            g[4 * q + e] = (&gq.x)[e];
+            u[4 * q + e] = (&uq.x)[e];
+          }
         }
+        const Word<T> w{*reinterpret_cast<const uint4 *>(dr)};
 #pragma unroll
         for (int e = 0; e < E; ++e) d[e] = w[e];
       } else {
@@ -366,7 +398,7 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restr
       }
       if (dz) {
         T *o = dz + static_cast<size_t>(m) * 2 * half + n;
-        if constexpr (E == 8) {
+        if constexpr (E > 1) {
           *reinterpret_cast<uint4 *>(o)        = Word<T>::from(dg).raw;
           *reinterpret_cast<uint4 *>(o + half) = Word<T>::from(du).raw;
         } else {
@@ -385,40 +417,365 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restr
     }
   }
 }
+// rows of a band: 32, or as few as it takes for four workgroups a compute unit (bias sums: no more than 128 bands up to 4096 samples)
+struct DzPlan {
+  bool wide;
+  int blocks_n, band_rows, bands;
+};
+template <class T>
+DzPlan dz_plan(int hidden, int half, int batch, const float *z, const T *dh, bool sums) {
+  constexpr int E = Word<T>::N;
+  DzPlan p;
+  p.wide      = hidden % E == 0 && ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
+  p.blocks_n  = ceil_div(half, p.wide ? E * GF_NT : GF_NT);
+  p.band_rows = std::max(1, std::min<int>(32, static_cast<long>(batch) * p.blocks_n / 1024));
+  if (sums) p.band_rows = std::max(p.band_rows, std::min(32, ceil_div(batch, 128)));
+  p.bands = ceil_div(batch, p.band_rows);
+  return p;
+}
+template <class T>
+int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, T *dz, float *bias_part) {
+  ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
+  auto go = [&](auto kernel) {
+    TDH_LAUNCH(kernel, dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half, act,
+               p.blocks_n, p.band_rows);
+    TDH_LAUNCH_CHECK();
+    return static_cast<int>(TDH_OK);
+  };
+  return p.wide ? go(gate_dz_kernel<T, Word<T>::N>) : go(gate_dz_kernel<T, 1>);
+}
+// db (+)= the bands' sums: 32 columns a workgroup, eight groups of bands, their sums in order
 template <class T>
 __global__ void __launch_bounds__(GF_NT)
 bias_sum_kernel(const float *__restrict__ part, T *__restrict__ db, const int bands, const int cols, const int accumulate) {
-  const int n = blockIdx.x * GF_NT + threadIdx.x;
-  if (n >= cols) return;
+  __shared__ float lds[8][32];
+  const int c = threadIdx.x & 31, group = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
   float s = 0.0f;
-  for (int b = 0; b < bands; ++b) s += part[static_cast<size_t>(b) * cols + n];
+  if (n < cols) {
+#pragma unroll 4
+    for (int b = group; b < bands; b += 8) s += part[static_cast<size_t>(b) * cols + n];
+  }
+  lds[group][c] = s;
+  __syncthreads();
+  if (group || n >= cols) return;
+#pragma unroll
+  for (int g = 1; g < 8; ++g) s += lds[g][c];
   if (accumulate) s += to_f32(db[n]);
   db[n] = from_f32<T>(s);
+}
+template <class T>
+int launch_db(const float *part, T *db, int bands, int hidden, int accumulate) {
+  ProfScope prof("gated_ff_db", 8.0 * bands * hidden, WORK_BYTE);
+  TDH_LAUNCH((bias_sum_kernel<T>), dim3(ceil_div(2 * hidden, 32)), dim3(GF_NT), 0, ctx().stream, part, db, bands, 2 * hidden, accumulate);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
+}
+
+// ------------------------------------------------------------ a few rows, any type
+// Up to FEW_ROWS samples: the weights are read once, in words, straight into the vector units; bound by that read (and
+// the write of dW).
+constexpr int FEW_ROWS = 4, FEW_NT = 512;
+
+// Forward. A unit of work is a strip of LANES words along the columns and `rows` of the k; its threads are LANES lanes along
+// the columns times 512 / LANES along k, x lies in LDS in slices, and the sums of the waves meet in LDS at the end. Long
+// rows matter more than anything: 1 KB of a row at a time reaches 6.4 TB/s, 128 bytes of many rows 4.1 to 4.4. So
+// large matrices are split along k, gate and up columns apart, and their slices added up by a launch of its own (BOTH =
+// false); where a strip is small a workgroup takes the gate's columns and the up columns that belong to them, and
+// finishes (BOTH = true). E = 1: columns one by one, for rows that do not lie on 16-byte boundaries. 4096 -> 2 x 12288
+// in bf16, one row: 31.5 us and 2.5 for the sum of 16 slices; through the caches 35.6.
+constexpr int FEW_X = 8192;   // values of x in LDS
+template <class T, int E, int M, int LANES, bool BOTH, bool ONCE>
+__global__ void __launch_bounds__(FEW_NT)
+few_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const EpiGate<T> epi, const int in, const int strips, const int split_rows) {
+  constexpr int COLS = LANES * E, KG = FEW_NT / LANES, H = BOTH ? 2 : 1;
+  constexpr int SLICE = FEW_X / M, SUMS = FEW_NT / 64 * H * COLS;
+  __shared__ float lds[FEW_X > SUMS ? FEW_X : SUMS];
+  const int tid = threadIdx.x, lc = tid % LANES, kg = tid / LANES, hidden = epi.hidden;
+  const int id    = xcd_compact_id(blockIdx.x, gridDim.x);
+  const int strip = id % strips, split = BOTH ? 0 : id / strips / 2, half = BOTH ? 0 : id / strips % 2;
+  const int first = strip * COLS, n = first + lc * E;
+  const int kend = min(in, (split + 1) * split_rows);
+  const size_t ld = 2 * static_cast<size_t>(hidden);
+  float acc[M][H][E] = {};
+  for (int k0 = split * split_rows; k0 < kend; k0 += SLICE) {
+    const int len = min(SLICE, kend - k0);
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      for (int k = tid; k < len; k += FEW_NT) lds[m * SLICE + k] = m < epi.rows ? to_f32(x[static_cast<size_t>(m) * in + k0 + k]) : 0.0f;
+    __syncthreads();
+    if (n < hidden) {
+      const T *wp = w + static_cast<size_t>(k0 + kg) * ld + half * hidden + n;
+#pragma unroll 8
+      for (int k = kg; k < len; k += KG, wp += KG * ld) {
+        float v[H][E];
+#pragma unroll
+        for (int s = 0; s < H; ++s) {
+          if constexpr (E > 1) {
+            const Word<T> word = load_word<T, ONCE>(wp + s * hidden);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[s][e] = word[e];
+          } else {
+            v[s][0] = to_f32(wp[s * hidden]);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const float xv = lds[m * SLICE + k];
+#pragma unroll
+          for (int s = 0; s < H; ++s)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[m][s][e] = __builtin_fmaf(xv, v[s][e], acc[m][s][e]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = LANES; o < 64; o <<= 1)
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int s = 0; s < H; ++s)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[m][s][e] += __shfl_xor(acc[m][s][e], o);
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    if (m >= epi.rows) break;
+    __syncthreads();
+    if ((tid & 63) < LANES) {
+#pragma unroll
+      for (int s = 0; s < H; ++s)
+#pragma unroll
+        for (int e = 0; e < E; ++e) lds[(tid / 64 * H + s) * COLS + lc * E + e] = acc[m][s][e];
+    }
+    __syncthreads();
+    for (int c = tid; c < COLS; c += FEW_NT) {
+      const int col = first + c;
+      if (col >= hidden) break;
+      float v[H] = {};
+#pragma unroll
+      for (int q = 0; q < FEW_NT / 64; ++q)
+#pragma unroll
+        for (int s = 0; s < H; ++s) v[s] += lds[(q * H + s) * COLS + c];
+      if constexpr (BOTH)
+        epi.finish(m, col, v[0], v[1]);
+      else
+        epi.partial[(static_cast<size_t>(split) * epi.rows + m) * 2 * hidden + half * hidden + col] = v[0];
+    }
+  }
+}
+
+// Backward: dx[m][i] = sum_c dz[m][c] w[i][c] and dw[i][c] (+)= sum_m x[m][i] dz[m][c] in one pass over c: a workgroup has
+// FEW_I rows of w and dw, its four waves take turns along c. dx null: only dw, and w is not read; dw null: only dx.
+constexpr int FEW_I = 4;
+template <class T, int E, int M, bool ONCE>
+__global__ void __launch_bounds__(256)
+few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ dz, T *__restrict__ dx, T *__restrict__ dw,
+               const int in, const int cols, const int batch, const int accumulate) {
+  __shared__ float sums[4][M * FEW_I];
+  const int tid = threadIdx.x, lane = tid & 63, i0 = blockIdx.x * FEW_I;
+  float xv[M][FEW_I], acc[M][FEW_I] = {};
+  size_t row[FEW_I];   // (rows past the end: the last one again, and nothing of it is kept)
+#pragma unroll
+  for (int i = 0; i < FEW_I; ++i) {
+    row[i] = static_cast<size_t>(min(i0 + i, in - 1));
+#pragma unroll
+    for (int m = 0; m < M; ++m) xv[m][i] = dw && m < batch ? to_f32(x[m * static_cast<size_t>(in) + row[i]]) : 0.0f;
+  }
+#pragma unroll 2
+  for (int c = tid * E; c < cols; c += 256 * E) {
+    float d[M][E];
+    Word<T> wv[FEW_I];
+    T w1[FEW_I];
+#pragma unroll
+    for (int i = 0; i < FEW_I; ++i) {
+      if (!dx) break;
+      if constexpr (E > 1)
+        wv[i] = load_word<T, ONCE>(w + row[i] * cols + c);
+      else
+        w1[i] = w[row[i] * cols + c];
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const T *p = dz + static_cast<size_t>(m < batch ? m : 0) * cols + c;
+      if constexpr (E > 1) {
+        const Word<T> v{*reinterpret_cast<const uint4 *>(p)};
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[m][e] = m < batch ? v[e] : 0.0f;
+      } else {
+        d[m][0] = m < batch ? to_f32(p[0]) : 0.0f;
+      }
+    }
+    if (dx) {
+#pragma unroll
+      for (int i = 0; i < FEW_I; ++i)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            float v;
+            if constexpr (E > 1) v = wv[i][e]; else v = to_f32(w1[i]);
+            acc[m][i] = __builtin_fmaf(d[m][e], v, acc[m][i]);
+          }
+    }
+    if (dw) {
+#pragma unroll
+      for (int i = 0; i < FEW_I; ++i) {
+        if (i0 + i >= in) break;
+        T *p = dw + row[i] * cols + c;
+        float o[E] = {};
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = m < batch ? __builtin_fmaf(xv[m][i], d[m][e], o[e]) : o[e];
+        if constexpr (E > 1) {
+          if (accumulate) {
+            const Word<T> was = load_word<T, ONCE>(p);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += was[e];
+          }
+          store_word16<ONCE>(p, Word<T>::from(o).raw);
+        } else {
+          *p = from_f32<T>(accumulate ? o[0] + to_f32(*p) : o[0]);
+        }
+      }
+    }
+  }
+  if (!dx) return;
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int i = 0; i < FEW_I; ++i) {
+      float v = acc[m][i];
+#pragma unroll
+      for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+      if (lane == 0) sums[tid >> 6][m * FEW_I + i] = v;
+    }
+  __syncthreads();
+  if (tid < M * FEW_I) {
+    const int m = tid / FEW_I, i = tid % FEW_I;
+    if (m < batch && i0 + i < in)
+      dx[static_cast<size_t>(m) * in + i0 + i] = from_f32<T>(sums[0][tid] + sums[1][tid] + sums[2][tid] + sums[3][tid]);
+  }
+}
+
+// f with the rows rounded up to a power of two as a constant
+template <class F>
+int with_rows(int batch, const F &f) {
+  if (batch <= 1) return f(std::integral_constant<int, 1>());
+  if (batch <= 2) return f(std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, 4>());
+}
+template <class T>
+bool in_words(std::initializer_list<const void *> tensors, int cols) {
+  uintptr_t all = 0;
+  for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15) == 0 && cols % Word<T>::N == 0;
+}
+
+// matrices that the L2 caches (8 x 4 MB) do not hold are read past them
+constexpr size_t FEW_ONCE_BYTES = 32u << 20;
+
+template <class T>
+int few_fwd(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
+  const bool words = in_words<T>({w}, hidden), wide = hidden >= 256;
+  const size_t bytes = sizeof(T) * static_cast<size_t>(in) * 2 * hidden;
+  const int cols = (wide ? 64 : 16) * (words ? Word<T>::N : 1), strips = ceil_div(hidden, cols);
+  // a workgroup reads 256 KB at most, or an equal part of one of 768
+  const long want  = std::min<long>(768, static_cast<long>(bytes >> 17));
+  const bool both  = bytes / strips <= (256u << 10);
+  const int most   = std::max(1, in / 32), splits = both ? 1 : static_cast<int>(std::min<long>(most, std::max(1L, (want + 2 * strips - 1) / (2 * strips))));
+  const int rows_s = ceil_div(in, splits), used = ceil_div(in, rows_s);
+  const size_t part = static_cast<size_t>(batch) * 2 * hidden;
+  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, hidden, act, false};
+  if (!both) {
+    TDH_TRY(ws_begin(ws_align(4 * part * used)));
+    TDH_TRY(take(part * used, &epi.partial));
+  }
+  const bool once = bytes > FEW_ONCE_BYTES;
+  TDH_TRY(with_rows(batch, [&](auto rows) {
+    constexpr int M = decltype(rows)::value, E = Word<T>::N;
+    ProfScope prof("gated_ff_few_fwd", static_cast<double>(bytes), WORK_BYTE);
+    auto go = [&](auto kernel) {
+      TDH_LAUNCH(kernel, dim3(both ? strips : 2 * strips * used), dim3(FEW_NT), 0, ctx().stream, x, w, epi, in, strips, rows_s);
+      TDH_LAUNCH_CHECK();
+      return static_cast<int>(TDH_OK);
+    };
+    if (words && wide)
+      return both ? go(few_fwd_kernel<T, E, M, 64, true, false>)
+             : once ? go(few_fwd_kernel<T, E, M, 64, false, true>) : go(few_fwd_kernel<T, E, M, 64, false, false>);
+    if (words) return both ? go(few_fwd_kernel<T, E, M, 16, true, false>) : go(few_fwd_kernel<T, E, M, 16, false, false>);
+    if (wide) return both ? go(few_fwd_kernel<T, 1, M, 64, true, false>) : go(few_fwd_kernel<T, 1, M, 64, false, false>);
+    return both ? go(few_fwd_kernel<T, 1, M, 16, true, false>) : go(few_fwd_kernel<T, 1, M, 16, false, false>);
+  }));
+  return both ? static_cast<int>(TDH_OK) : launch_gate_reduce(epi, used);
+}
+
+template <class T>
+int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
+            int accumulate) {
+  const int cols = 2 * hidden;
+  const DzPlan pz = dz_plan(hidden, hidden, batch, z, dh, db != nullptr);
+  TDH_TRY(ws_begin(ws_align(sizeof(T) * batch * cols) + ws_align(4 * static_cast<size_t>(pz.bands) * cols)));
+  T *dz = nullptr;
+  float *bias_part = nullptr;
+  if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * cols, &dz));
+  if (db) TDH_TRY(take(static_cast<size_t>(pz.bands) * cols, &bias_part));
+  TDH_TRY(launch_dz(pz, act, hidden, hidden, batch, z, dh, dz, bias_part));
+  if (db) TDH_TRY(launch_db(bias_part, db, pz.bands, hidden, accumulate));
+  if (!dx && !dw) return TDH_OK;
+  ProfScope prof("gated_ff_few_bwd", sizeof(T) * static_cast<double>(in) * cols * ((dx ? 1 : 0) + (dw ? 1 : 0)), WORK_BYTE);
+  return with_rows(batch, [&](auto rows) {
+    constexpr int M = decltype(rows)::value;
+    auto go = [&](auto kernel) {
+      TDH_LAUNCH(kernel, dim3(ceil_div(in, FEW_I)), dim3(256), 0, ctx().stream, x, w, dz, dx, dw, in, cols, batch, accumulate);
+      TDH_LAUNCH_CHECK();
+      return static_cast<int>(TDH_OK);
+    };
+    if (!in_words<T>({w, dw}, cols)) return go(few_bwd_kernel<T, 1, M, false>);
+    return sizeof(T) * static_cast<size_t>(in) * cols > FEW_ONCE_BYTES ? go(few_bwd_kernel<T, Word<T>::N, M, true>)
+                                                                       : go(few_bwd_kernel<T, Word<T>::N, M, false>);
+  });
 }
 
 // ---- plans
 struct FfPlan {
-  int cfg;       // index into the tile shapes of ff_gemm
+  int cfg;       // index into FF_TILES
   int splits, k_per_split;
 };
+// A tile shape: the workgroups that a compute unit holds, us of a tile of 64 reduction indices with one, two, ... of them on a
+// compute unit (all of them take that long), us of a round of workgroups beside that, and of the launch. Measured on
+// products of 256 to 1024 tiles with k of 64, 1024 and 2048; 256 x 256 reaches 1140 TFLOP/s there, 128 x 128 890, 64 x 128 780,
+// 64 x 64 620, 32 x 256 590.
 struct FfTile {
   int bm, bn, per_cu;
-  double us;     // of one tile of 64 reduction indices, per workgroup, with per_cu of them on a compute unit
+  double us[4], round_us, launch_us;
 };
-constexpr FfTile FF_TILES[] = {{256, 256, 1, 1.7}, {128, 128, 2, 1.0}, {32, 256, 2, 0.6}};
+constexpr FfTile FF_TILES[] = {{256, 256, 1, {1.6}, 5.0, 5.0},
+                               {128, 128, 2, {0.82, 0.97}, 3.0, 3.0},
+                               {64, 128, 3, {0.47, 0.68, 0.87}, 2.0, 2.5},
+                               {64, 64, 4, {0.30, 0.46, 0.62, 0.80}, 1.2, 2.5},
+                               {32, 256, 2, {0.80, 0.85}, 2.0, 2.5}};
 
+// The tile shape and the split along k that take the least by these figures. A split writes and reads its slices (4 TB/s), and its
+// sum is another launch.
 FfPlan ff_plan(int M, int N, int K) {
-  const int cus = ctx().compute_units > 0 ? ctx().compute_units : 256, ktiles = std::max(1, ceil_div(K, G16_BK));
+  const long cus = ctx().compute_units > 0 ? ctx().compute_units : 256;
+  const int ktiles = std::max(1, ceil_div(K, G16_BK));
   FfPlan best{0, 1, ktiles * G16_BK};
   double best_us = 1e30;
-  for (int c = 0; c < 3; ++c) {
-    const FfTile &t = FF_TILES[c];
+  for (int c = 0; c < 5; ++c) {
+    const FfTile &t  = FF_TILES[c];
     const long tiles = static_cast<long>(ceil_div(M, t.bm)) * ceil_div(N, t.bn);
-    for (int want = 1; want <= 32 && want <= ktiles; want *= 2) {
+    int last = 0;
+    for (int want = 1; want <= 64 && want <= ktiles; want += want < 4 ? 1 : want / 4) {
       const int per = ceil_div(ktiles, want), splits = ceil_div(ktiles, per);
-      const long groups = tiles * splits, slots = static_cast<long>(cus) * t.per_cu;
-      double us = static_cast<double>((groups + slots - 1) / slots) * (per * t.us + 3.0);
-      if (splits > 1) us += 3.0 + (2.0 * splits) * M * N * 4 / 4e6;
+      if (splits == last) continue;
+      last = splits;
+      const long groups = tiles * splits, full = groups / (cus * t.per_cu), rest = groups - full * cus * t.per_cu;
+      double us = t.launch_us + full * (per * t.us[t.per_cu - 1] + t.round_us);
+      if (rest) us += per * t.us[(rest - 1) / cus] + t.round_us;
+      if (splits > 1) us += 3.0 + 8.0 * splits * M * N / 4e6;
       if (us < best_us) {
         best_us = us;
         best    = FfPlan{c, splits, per * G16_BK};
@@ -444,6 +801,8 @@ int ff_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const Epi &
   switch (p.cfg) {
     case 0: return go(gemm16_kernel<T, 2, 4, 4, 2, A_KC, B_KC, PAIR, Epi>, 512);
     case 1: return go(gemm16_kernel<T, 2, 2, 2, 2, A_KC, B_KC, PAIR, Epi>, 256);
+    case 2: return go(gemm16_kernel<T, 2, 2, 1, 2, A_KC, B_KC, PAIR, Epi>, 256);
+    case 3: return go(gemm16_kernel<T, 2, 1, 1, 2, A_KC, B_KC, PAIR, Epi>, 128);
     default: return go(gemm16_kernel<T, 1, 4, 1, 2, A_KC, B_KC, PAIR, Epi>, 256);
   }
 }
@@ -457,20 +816,30 @@ size_t pack_bytes(const T *p, int rows, int used, int halves) {
   return fits(p, used) ? 0 : ws_align(static_cast<size_t>(rows) * halves * padded(used) * sizeof(T));
 }
 template <class T>
-int pack(const T *src, int rows, int used, int halves, G16Matrix *out) {
-  const int half = padded(used);
-  *out = G16Matrix{src, static_cast<long>(halves) * half, rows, halves * half};
-  if (fits(src, used)) return TDH_OK;
-  T *copy;
-  const size_t total = static_cast<size_t>(rows) * halves * half;
-  TDH_TRY(take(total, &copy));
-  ProfScope prof("ff_pack", 2.0 * sizeof(T) * total, WORK_BYTE);
-  TDH_LAUNCH((pack_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, src, copy, total,
-             used, half, halves);
-  TDH_LAUNCH_CHECK();
-  out->p = copy;
-  return TDH_OK;
-}
+struct Packer {
+  PackJobs<T> jobs{};
+  int n = 0;
+  // notes the copy, if one is needed; run() makes them all
+  int add(const T *src, int rows, int used, int halves, G16Matrix *out) {
+    const int half = padded(used);
+    *out = G16Matrix{src, static_cast<long>(halves) * half, rows, halves * half};
+    if (fits(src, used)) return TDH_OK;
+    typename PackJobs<T>::Job &j = jobs.job[n++];
+    j = {src, nullptr, used, half, halves, 0, static_cast<size_t>(rows) * halves * half / 8};
+    j.blocks = static_cast<unsigned>(ceil_div_sz(j.words, GF_NT));
+    TDH_TRY(take(j.words * 8, &j.dst));
+    out->p = j.dst;
+    return TDH_OK;
+  }
+  int run() {
+    if (!n) return TDH_OK;
+    const size_t words = jobs.job[0].words + jobs.job[1].words;
+    ProfScope prof("ff_pack", 32.0 * words, WORK_BYTE);
+    TDH_LAUNCH((pack_kernel<T>), dim3(jobs.job[0].blocks + jobs.job[1].blocks), dim3(GF_NT), 0, ctx().stream, jobs);
+    TDH_LAUNCH_CHECK();
+    return TDH_OK;
+  }
+};
 
 template <class T>
 int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
@@ -479,18 +848,14 @@ int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   const size_t part = static_cast<size_t>(batch) * 2 * half;
   TDH_TRY(ws_begin(pack_bytes(x, batch, in, 1) + pack_bytes(w, in, hidden, 2) + ff_partial_bytes(plan, part)));
   G16Matrix A, B;
-  TDH_TRY(pack(x, batch, in, 1, &A));
-  TDH_TRY(pack(w, in, hidden, 2, &B));
+  Packer<T> packer;
+  TDH_TRY(packer.add(x, batch, in, 1, &A));
+  TDH_TRY(packer.add(w, in, hidden, 2, &B));
+  TDH_TRY(packer.run());
   EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act, fits(h, hidden)};
   if (plan.splits > 1) TDH_TRY(take(plan.splits * part, &epi.partial));
   TDH_TRY((ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd")));
-  if (plan.splits > 1) {
-    const size_t total = static_cast<size_t>(batch) * hidden;
-    ProfScope prof("gated_ff_fwd_reduce", 8.0 * plan.splits * total, WORK_BYTE);
-    TDH_LAUNCH((gate_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, plan.splits);
-    TDH_LAUNCH_CHECK();
-  }
-  return TDH_OK;
+  return plan.splits > 1 ? launch_gate_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
 }
 
 template <class T, bool A_KC, bool B_KC>
@@ -509,7 +874,9 @@ int ff_grad(const FfPlan &plan, const G16Matrix &A, const G16Matrix &B, EpiGrad<
 template <class T>
 int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
               int accumulate) {
-  const int half = padded(hidden), bands = ceil_div(batch, DZ_ROWS);
+  const int half = padded(hidden);
+  const DzPlan pz = dz_plan(hidden, half, batch, z, dh, db != nullptr);
+  const int bands = pz.bands;
   const FfPlan px = ff_plan(batch, in, 2 * half), pw = ff_plan(in, 2 * half, batch);
   const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
   TDH_TRY(ws_begin(ws_align(sizeof(T) * batch * 2 * half) + ws_align(4 * static_cast<size_t>(bands) * 2 * hidden) +
@@ -519,35 +886,33 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   float *bias_part = nullptr;
   if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * 2 * half, &dz));
   if (db) TDH_TRY(take(static_cast<size_t>(bands) * 2 * hidden, &bias_part));
-  {
-    ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
-    const bool wide    = hidden % 8 == 0 && ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
-    const int blocks_n = ceil_div(half, wide ? 8 * GF_NT : GF_NT);
-    if (wide)
-      TDH_LAUNCH((gate_dz_kernel<T, 8>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
-                 act, blocks_n);
-    else
-      TDH_LAUNCH((gate_dz_kernel<T, 1>), dim3(blocks_n * bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
-                 act, blocks_n);
-    TDH_LAUNCH_CHECK();
-  }
-  if (db) {
-    ProfScope prof("gated_ff_db", 8.0 * bands * hidden, WORK_BYTE);
-    TDH_LAUNCH((bias_sum_kernel<T>), dim3(ceil_div(2 * hidden, GF_NT)), dim3(GF_NT), 0, ctx().stream, bias_part, db, bands, 2 * hidden, accumulate);
-    TDH_LAUNCH_CHECK();
-  }
+  TDH_TRY(launch_dz(pz, act, hidden, half, batch, z, dh, dz, bias_part));
+  if (db) TDH_TRY(launch_db(bias_part, db, bands, hidden, accumulate));
   const G16Matrix Z{dz, 2L * half, batch, 2 * half};
+  G16Matrix W, X;   // w: [in][2 half], of which the rows are the product's columns
+  Packer<T> packer;
+  if (dx) TDH_TRY(packer.add(w, in, hidden, 2, &W));
+  if (dw) TDH_TRY(packer.add(x, batch, in, 1, &X));
+  TDH_TRY(packer.run());
   if (dx) {
-    G16Matrix W;   // [in][2 half], rows along m of the product are w's rows
-    TDH_TRY(pack(w, in, hidden, 2, &W));
     TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0, fits(dx, in)}, 2 * half, "gated_ff_dx")));
   }
   if (dw) {
-    G16Matrix X;
-    TDH_TRY(pack(x, batch, in, 1, &X));
     TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate, fits(dw, hidden)}, batch, "gated_ff_dw")));
   }
   return TDH_OK;
+}
+
+// the gradients of no samples
+template <class T>
+int no_rows(int in, int hidden, T *dw, T *db) {
+  const size_t total = static_cast<size_t>(in) * 2 * hidden;
+  if (dw) {
+    const EpiGrad<T> epi{dw, nullptr, in, 2 * hidden, hidden, hidden, 0, false};
+    TDH_LAUNCH((grad_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, 0);
+    TDH_LAUNCH_CHECK();
+  }
+  return db ? launch_db<T>(nullptr, db, 0, hidden, 0) : static_cast<int>(TDH_OK);
 }
 
 int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch) {
@@ -585,6 +950,7 @@ int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int b
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const T *xt = static_cast<const T *>(x), *wt = static_cast<const T *>(w), *bt = has_bias ? static_cast<const T *>(b) : nullptr;
+    if (batch <= FEW_ROWS) return few_fwd<T>(act, in, hidden, batch, xt, wt, bt, static_cast<T *>(h), z);
     if constexpr (sizeof(T) == 4)
       return ff_fwd_f32(act, in, hidden, batch, xt, wt, bt, static_cast<T *>(h), z);
     else
@@ -599,11 +965,13 @@ int tdh_gated_ff_bwd(int dtype, int act, int in, int hidden, int has_bias, int b
   TDH_TRY(check_aligned("tdh_gated_ff_bwd", dtype, {x, w, dh, dx, dw, db}));
   TDH_TRY(check_aligned("tdh_gated_ff_bwd", TDH_F32, {z}));
   TDH_REQUIRE_INIT();
-  if (batch == 0) return TDH_OK;
+  if (batch == 0 && accumulate) return TDH_OK;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const T *xt = static_cast<const T *>(x), *wt = static_cast<const T *>(w), *dt = static_cast<const T *>(dh);
     T *dbt = has_bias ? static_cast<T *>(db) : nullptr;
+    if (batch == 0) return no_rows<T>(in, hidden, static_cast<T *>(dw), dbt);
+    if (batch <= FEW_ROWS) return few_bwd<T>(act, in, hidden, batch, xt, wt, z, dt, static_cast<T *>(dx), static_cast<T *>(dw), dbt, accumulate);
     if constexpr (sizeof(T) == 4)
       return ff_bwd_f32(act, in, hidden, batch, xt, wt, z, dt, static_cast<T *>(dx), static_cast<T *>(dw), dbt, accumulate);
     else

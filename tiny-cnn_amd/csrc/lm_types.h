@@ -53,6 +53,25 @@ struct Word {
   }
 };
 
+// A word from memory; ONCE: past the caches (data larger than they are, read once).
+template <class T, bool ONCE>
+__device__ __forceinline__ Word<T> load_word(const T *p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (ONCE)
+    return Word<T>{__builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)))};
+  else
+    return Word<T>{*reinterpret_cast<const uint4 *>(p)};
+}
+
+template <bool ONCE>
+__device__ __forceinline__ void store_word16(void *p, const uint4 v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4 *>(p));
+  else
+    *static_cast<uint4 *>(p) = v;
+}
+
 inline bool dtype_known(int dtype) { return dtype == TDH_F32 || dtype == TDH_BF16 || dtype == TDH_F16; }
 inline size_t dtype_size(int dtype) { return dtype == TDH_F32 ? 4 : 2; }
 
