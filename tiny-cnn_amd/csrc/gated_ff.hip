@@ -22,8 +22,13 @@ __device__ __forceinline__ float gate_act(const float g, float *slope) {
     *slope = s * (1.0f + g * (1.0f - s));
     return g * s;
   } else if constexpr (KIND == TDH_GATE_GELU) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-    *slope = cdf + g * (0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g));
+    // erfc(x) for x >= 0 as a polynomial in 1 / (1 + p x) times exp(-x^2), off by 1.5e-7 at most (Abramowitz and
+    // Stegun, Handbook of Mathematical Functions, 7.1.26)
+    const float x = 0.70710678118654752f * __builtin_fabsf(g), e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float cdf  = g < 0.0f ? tail : 1.0f - tail;   // (NaN stays)
+    *slope = cdf + g * (0.39894228040143268f * e);
     return g * cdf;
   } else if constexpr (KIND == TDH_GATE_GELU_TANH) {
     // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3)
@@ -146,7 +151,7 @@ struct EpiGate {
   T *h;
   float *z;            // or null
   const T *bias;       // or null
-  float *partial;      // slices of z instead, [split][rows][2 half]
+  float *partial;      // slices of z, [split][rows][2 half], that a sum of them reads
   int rows, hidden, half, act;
   bool wide;           // h's rows lie on 16-byte boundaries
   // g and u at (m, n) to h; writes z
@@ -168,25 +173,9 @@ struct EpiGate {
     with_gate(act, [&](auto kind) { h[m * hidden + n] = from_f32<T>(one<decltype(kind)::value>(m, n, g, u)); });
   }
   template <int TM, int TN>
-  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split,
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int,
                                        float *lds) const {
     const int n = n0 + (lane & 31), m = m0 + 4 * (lane >> 5);
-    if (partial) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = m + 32 * i + 8 * (r >> 2) + (r & 3);
-          float *p = partial + (static_cast<size_t>(split) * rows + row) * 2 * half;
-#pragma unroll
-          for (int j = 0; j < TN / 2; ++j)
-            if (row < rows && n + 32 * j < hidden) {
-              p[n + 32 * j]        = acc[i][2 * j][r];
-              p[half + n + 32 * j] = acc[i][2 * j + 1][r];
-            }
-        }
-      return;
-    }
     float bg[TN / 2], bu[TN / 2];
 #pragma unroll
     for (int j = 0; j < TN / 2; ++j) {
@@ -745,37 +734,47 @@ struct FfPlan {
 };
 // A tile shape: the workgroups that a compute unit holds, us of a tile of 64 reduction indices with one, two, ... of them on a
 // compute unit (all of them take that long), us of a round of workgroups beside that, and of the launch. Measured on
-// products of 256 to 1024 tiles with k of 64, 1024 and 2048; 256 x 256 reaches 1140 TFLOP/s there, 128 x 128 890, 64 x 128 780,
-// 64 x 64 620, 32 x 256 590.
+// products of 256 to 1024 tiles with k of 64 to 2048; 256 x 256 reaches 1100 TFLOP/s there, 128 x 128 990, 64 x 128 760,
+// 64 x 64 650, 32 x 256 620.
 struct FfTile {
-  int bm, bn, per_cu;
+  int bm, bn, bufs, per_cu;
   double us[4], round_us, launch_us;
 };
-constexpr FfTile FF_TILES[] = {{256, 256, 1, {1.6}, 5.0, 5.0},
-                               {128, 128, 2, {0.82, 0.97}, 3.0, 3.0},
-                               {64, 128, 3, {0.47, 0.68, 0.87}, 2.0, 2.5},
-                               {64, 64, 4, {0.30, 0.46, 0.62, 0.80}, 1.2, 2.5},
-                               {32, 256, 2, {0.80, 0.85}, 2.0, 2.5}};
+constexpr FfTile FF_TILES[] = {{256, 256, 2, 1, {1.65}, 5.0, 5.0},
+                               {128, 128, 2, 2, {0.77, 0.92}, 3.0, 3.0},
+                               {64, 128, 3, 2, {0.39, 0.64}, 1.7, 2.5},
+                               {64, 64, 2, 4, {0.37, 0.45, 0.60, 0.78}, 1.0, 2.7},
+                               {32, 256, 2, 2, {0.80, 0.78}, 2.0, 2.5}};
 
-// The tile shape and the split along k that take the least by these figures. A split writes and reads its slices (4 TB/s), and its
-// sum is another launch.
-FfPlan ff_plan(int M, int N, int K) {
-  const long cus = ctx().compute_units > 0 ? ctx().compute_units : 256;
-  const int ktiles = std::max(1, ceil_div(K, G16_BK));
+// The tile shape and the split along k that take the least by these figures, round of workgroups by round. What a round reads
+// comes no faster than the bytes in flight allow: 3.3 TB/s with 3.5 MB of them, 4.5 with 7, 5.4 with 14 and more
+// (a product of 32 rows with 200 MB of weights, 32 x 256: 78 us unsplit, 39 in 5 slices that are just resident, 50 in
+// 11), and of rows of 64 or 128 bytes 0.4 or 0.6 of that (pair: an unsplit tile takes half of its columns from either half of
+// the matrix; the product above, 64 x 128: 64 us, 39 if its columns lie together). A split's slices are written and
+// read once and its sum is another launch.
+FfPlan ff_plan(int M, int N, int K, bool pair = false) {
+  const long cus    = ctx().compute_units > 0 ? ctx().compute_units : 256;
+  const int ktiles  = std::max(1, ceil_div(K, G16_BK));
+  const double read = 2.0 * (static_cast<double>(M) + N) * K;
   FfPlan best{0, 1, ktiles * G16_BK};
   double best_us = 1e30;
   for (int c = 0; c < 5; ++c) {
     const FfTile &t  = FF_TILES[c];
-    const long tiles = static_cast<long>(ceil_div(M, t.bm)) * ceil_div(N, t.bn);
+    const long tiles = static_cast<long>(ceil_div(M, t.bm)) * ceil_div(N, t.bn), slots = cus * t.per_cu;
     int last = 0;
-    for (int want = 1; want <= 64 && want <= ktiles; want += want < 4 ? 1 : want / 4) {
+    for (int want = 1; want <= 64 && want <= ktiles; want += want < 8 ? 1 : want / 4) {
       const int per = ceil_div(ktiles, want), splits = ceil_div(ktiles, per);
       if (splits == last) continue;
       last = splits;
-      const long groups = tiles * splits, full = groups / (cus * t.per_cu), rest = groups - full * cus * t.per_cu;
-      double us = t.launch_us + full * (per * t.us[t.per_cu - 1] + t.round_us);
-      if (rest) us += per * t.us[(rest - 1) / cus] + t.round_us;
-      if (splits > 1) us += 3.0 + 8.0 * splits * M * N / 4e6;
+      const long groups = tiles * splits;
+      auto round = [&](long n) {
+        const double flight = n * (t.bufs - 1) * (t.bm + t.bn) * 128.0, scatter = !pair || splits > 1 || t.bn >= 256 ? 1.0 : t.bn == 128 ? 0.6 : 0.4,
+                     speed = scatter * std::min(5.4e6, 7.0e6 * flight / (flight + 4e6));
+        return std::max(per * t.us[(n - 1) / cus], read * n / groups / speed) + t.round_us;
+      };
+      double us = t.launch_us + (groups / slots) * round(slots);
+      if (groups % slots) us += round(groups % slots);
+      if (splits > 1) us += 3.0 + 8.0 * splits * M * N / 8e6;
       if (us < best_us) {
         best_us = us;
         best    = FfPlan{c, splits, per * G16_BK};
@@ -799,11 +798,11 @@ int ff_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const Epi &
     return static_cast<int>(TDH_OK);
   };
   switch (p.cfg) {
-    case 0: return go(gemm16_kernel<T, 2, 4, 4, 2, A_KC, B_KC, PAIR, Epi>, 512);
-    case 1: return go(gemm16_kernel<T, 2, 2, 2, 2, A_KC, B_KC, PAIR, Epi>, 256);
-    case 2: return go(gemm16_kernel<T, 2, 2, 1, 2, A_KC, B_KC, PAIR, Epi>, 256);
-    case 3: return go(gemm16_kernel<T, 2, 1, 1, 2, A_KC, B_KC, PAIR, Epi>, 128);
-    default: return go(gemm16_kernel<T, 1, 4, 1, 2, A_KC, B_KC, PAIR, Epi>, 256);
+    case 0: return go(gemm16_kernel<T, 2, 4, 4, 2, 2, A_KC, B_KC, PAIR, Epi>, 512);
+    case 1: return go(gemm16_kernel<T, 2, 2, 2, 2, 2, A_KC, B_KC, PAIR, Epi>, 256);
+    case 2: return go(gemm16_kernel<T, 2, 2, 1, 2, 3, A_KC, B_KC, PAIR, Epi>, 256);
+    case 3: return go(gemm16_kernel<T, 2, 1, 1, 2, 2, A_KC, B_KC, PAIR, Epi>, 128);
+    default: return go(gemm16_kernel<T, 1, 4, 1, 2, 2, A_KC, B_KC, PAIR, Epi>, 256);
   }
 }
 
@@ -844,7 +843,7 @@ struct Packer {
 template <class T>
 int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
   const int half    = padded(hidden);
-  const FfPlan plan = ff_plan(batch, 2 * half, in);
+  const FfPlan plan = ff_plan(batch, 2 * half, in, /*pair=*/true);
   const size_t part = static_cast<size_t>(batch) * 2 * half;
   TDH_TRY(ws_begin(pack_bytes(x, batch, in, 1) + pack_bytes(w, in, hidden, 2) + ff_partial_bytes(plan, part)));
   G16Matrix A, B;
@@ -853,9 +852,11 @@ int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   TDH_TRY(packer.add(w, in, hidden, 2, &B));
   TDH_TRY(packer.run());
   EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act, fits(h, hidden)};
-  if (plan.splits > 1) TDH_TRY(take(plan.splits * part, &epi.partial));
-  TDH_TRY((ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd")));
-  return plan.splits > 1 ? launch_gate_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
+  if (plan.splits == 1) return ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd");
+  TDH_TRY(take(plan.splits * part, &epi.partial));
+  const EpiGrad<T> slices{nullptr, epi.partial, batch, 2 * half, hidden, half, 0, false};
+  TDH_TRY((ff_gemm<T, true, false, false>(plan, A, B, slices, batch, 2 * half, in, "gated_ff_fwd")));
+  return launch_gate_reduce(epi, plan.splits);
 }
 
 template <class T, bool A_KC, bool B_KC>
