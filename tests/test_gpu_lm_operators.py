@@ -334,6 +334,9 @@ def policy_case(T, dtype, rows, vocab, ld, skew, use_ref, use_weight, in_place):
     old, ref = L.rounded(now + 0.3 * rng.randn(rows), "f32"), L.rounded(now + 0.5 * rng.randn(rows), "f32")
     adv, weight = L.rounded(rng.randn(rows), "f32"), L.rounded(rng.rand(rows), "f32")
     low, high, kl = (float(np.float32(v)) for v in (low, high, kl))
+    # (no row so near a clipping bound that rounding decides on which side of it it falls)
+    near = (np.abs(np.exp(now - old)[:, None] - [1 - low, 1 + high]) < 1e-3).any(1)
+    old = L.rounded(np.where(near, old + 0.01, old), "f32")
     bx, bt = Buf(T, padded(x, ld), dtype, skew), Buf(T, target, "i32")
     g = bx if in_place else Buf(T, padded(np.zeros((rows, vocab)), ld), dtype, skew)
     logp, row, total = out(T, rows), out(T, rows), out(T, 1)
@@ -366,7 +369,15 @@ def test_policy_loss(T, dtype, vocab):
     policy_case(T, dtype, 5, vocab, vocab + 5, 1, False, False, True)
 
 
-@pytest.mark.parametrize("rows", [1, 4, 5, 100, 1500])
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("vocab", [33, 700, 3000, 9000, 20000])
+def test_losses_of_more_rows_than_compute_units(T, dtype, vocab):
+    """(where a row has fewer waves)"""
+    policy_case(T, dtype, 260, vocab, vocab, 0, True, True, False)
+    preference_case(T, dtype, [130, 133], vocab, "sigmoid", 0.1, vocab, 0, True)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 5, 100, 1024, 1025, 1500])
 def test_policy_loss_rows(T, rows):
     policy_case(T, "f32", rows, 10, 10, 0, True, True, False)
     policy_case(T, "bf16", rows, 37, 40, 0, True, False, False)

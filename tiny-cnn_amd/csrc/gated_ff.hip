@@ -340,12 +340,12 @@ pack_kernel(const PackJobs<T> jobs) {
   *reinterpret_cast<uint4 *>(j.dst + i * 8) = *reinterpret_cast<const uint4 *>(v);
 }
 
-// dz in the operand's type, [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
+// dz as the products read it (type Z), [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
 // workgroup's band (in fp32, before the rounding). A thread takes E columns: a 16-byte word where every row lies on a 16-byte
 // boundary, else one.
-template <class T, int E>
+template <class T, class Z, int E>
 __global__ void __launch_bounds__(GF_NT)
-gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restrict__ dz, float *__restrict__ bias_part,
+gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restrict__ dz, float *__restrict__ bias_part,
                const int rows, const int hidden, const int half, const int act, const int blocks_n, const int band_rows) {
   const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
   if (n >= half) return;
@@ -386,13 +386,19 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, T *__restr
         su[e] += du[e];
       }
       if (dz) {
-        T *o = dz + static_cast<size_t>(m) * 2 * half + n;
-        if constexpr (E > 1) {
-          *reinterpret_cast<uint4 *>(o)        = Word<T>::from(dg).raw;
-          *reinterpret_cast<uint4 *>(o + half) = Word<T>::from(du).raw;
+        Z *o = dz + static_cast<size_t>(m) * 2 * half + n;
+        if constexpr (E > 1 && sizeof(Z) == 2) {
+          *reinterpret_cast<uint4 *>(o)        = Word<Z>::from(dg).raw;
+          *reinterpret_cast<uint4 *>(o + half) = Word<Z>::from(du).raw;
+        } else if constexpr (E > 1) {
+#pragma unroll
+          for (int q = 0; q < E / 4; ++q) {
+            reinterpret_cast<float4 *>(o)[q]        = make_float4(dg[4 * q], dg[4 * q + 1], dg[4 * q + 2], dg[4 * q + 3]);
+            reinterpret_cast<float4 *>(o + half)[q] = make_float4(du[4 * q], du[4 * q + 1], du[4 * q + 2], du[4 * q + 3]);
+          }
         } else {
-          o[0]    = from_f32<T>(dg[0]);
-          o[half] = from_f32<T>(du[0]);
+          o[0]    = from_f32<Z>(dg[0]);
+          o[half] = from_f32<Z>(du[0]);
         }
       }
     }
@@ -422,8 +428,8 @@ DzPlan dz_plan(int hidden, int half, int batch, const float *z, const T *dh, boo
   p.bands = ceil_div(batch, p.band_rows);
   return p;
 }
-template <class T>
-int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, T *dz, float *bias_part) {
+template <class T, class Z>
+int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, Z *dz, float *bias_part) {
   ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
   auto go = [&](auto kernel) {
     TDH_LAUNCH(kernel, dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half, act,
@@ -431,7 +437,7 @@ int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const f
     TDH_LAUNCH_CHECK();
     return static_cast<int>(TDH_OK);
   };
-  return p.wide ? go(gate_dz_kernel<T, Word<T>::N>) : go(gate_dz_kernel<T, 1>);
+  return p.wide ? go(gate_dz_kernel<T, Z, Word<T>::N>) : go(gate_dz_kernel<T, Z, 1>);
 }
 // db (+)= the bands' sums: 32 columns a workgroup, eight groups of bands, their sums in order
 template <class T>
@@ -555,11 +561,11 @@ few_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const EpiGate<T
 }
 
 // Backward: dx[m][i] = sum_c dz[m][c] w[i][c] and dw[i][c] (+)= sum_m x[m][i] dz[m][c] in one pass over c: a workgroup has
-// FEW_I rows of w and dw, its four waves take turns along c. dx null: only dw, and w is not read; dw null: only dx.
+// FEW_I rows of w and dw, its four waves take turns along c. dz is in fp32 (there is little of it). dx null: only dw, and w is not read; dw null: only dx.
 constexpr int FEW_I = 4;
 template <class T, int E, int M, bool ONCE>
 __global__ void __launch_bounds__(256)
-few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ dz, T *__restrict__ dx, T *__restrict__ dw,
+few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const float *__restrict__ dz, T *__restrict__ dx, T *__restrict__ dw,
                const int in, const int cols, const int batch, const int accumulate) {
   __shared__ float sums[4][M * FEW_I];
   const int tid = threadIdx.x, lane = tid & 63, i0 = blockIdx.x * FEW_I;
@@ -586,13 +592,16 @@ few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__rest
     }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const T *p = dz + static_cast<size_t>(m < batch ? m : 0) * cols + c;
+      const float *p = dz + static_cast<size_t>(m < batch ? m : 0) * cols + c;
       if constexpr (E > 1) {
-        const Word<T> v{*reinterpret_cast<const uint4 *>(p)};
 #pragma unroll
-        for (int e = 0; e < E; ++e) d[m][e] = m < batch ? v[e] : 0.0f;
+        for (int q = 0; q < E / 4; ++q) {
+          const float4 v = reinterpret_cast<const float4 *>(p)[q];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[m][4 * q + e] = m < batch ? (&v.x)[e] : 0.0f;
+        }
       } else {
-        d[m][0] = m < batch ? to_f32(p[0]) : 0.0f;
+        d[m][0] = m < batch ? p[0] : 0.0f;
       }
     }
     if (dx) {
@@ -705,9 +714,8 @@ int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, cons
             int accumulate) {
   const int cols = 2 * hidden;
   const DzPlan pz = dz_plan(hidden, hidden, batch, z, dh, db != nullptr);
-  TDH_TRY(ws_begin(ws_align(sizeof(T) * batch * cols) + ws_align(4 * static_cast<size_t>(pz.bands) * cols)));
-  T *dz = nullptr;
-  float *bias_part = nullptr;
+  TDH_TRY(ws_begin(ws_align(sizeof(float) * batch * cols) + ws_align(4 * static_cast<size_t>(pz.bands) * cols)));
+  float *dz = nullptr, *bias_part = nullptr;
   if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * cols, &dz));
   if (db) TDH_TRY(take(static_cast<size_t>(pz.bands) * cols, &bias_part));
   TDH_TRY(launch_dz(pz, act, hidden, hidden, batch, z, dh, dz, bias_part));

@@ -34,9 +34,10 @@ struct Row {
   }
   __device__ __forceinline__ bool whole(const int k) const { return k * N >= shift && k * N + N <= shift + len; }
   // elements outside the row read as -inf
+  template <bool ONCE>
   __device__ __forceinline__ Word<T> load(const int k) const {
     const T *at = p + (static_cast<long>(k) * N - shift);
-    if (whole(k)) return Word<T>{*reinterpret_cast<const uint4 *>(at)};
+    if (whole(k)) return load_word<T, ONCE>(at);
     float v[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -52,7 +53,7 @@ template <class T>
 __device__ __forceinline__ void store_word(const Row<T> &r, T *out, const int k, const float (&v)[Word<T>::N]) {
   T *at = out + (static_cast<long>(k) * Word<T>::N - r.shift);
   if (r.whole(k) && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-    *reinterpret_cast<uint4 *>(at) = Word<T>::from(v).raw;
+    store_word16<true>(at, Word<T>::from(v).raw);
     return;
   }
 #pragma unroll
@@ -60,6 +61,12 @@ __device__ __forceinline__ void store_word(const Row<T> &r, T *out, const int k,
     const int i = k * Word<T>::N - r.shift + e;
     if (i >= 0 && i < r.len) at[e] = from_f32<T>(v[e]);
   }
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
 }
 
 // (m, s) of a part of a row: its maximum and the sum of exp(x - m)
@@ -90,7 +97,9 @@ __device__ __forceinline__ float word_sum(const Word<T> &w, const float m, float
   return s;
 }
 
-// What is made of a row: MODE
+// What is made of a row: MODE. A row that is read once goes past the caches where nothing reads it again soon: 8192 x
+// 65536 logits in bf16, log-probabilities alone 167 us without that and 159 with it; with the gradient's pass behind them
+// 476 and 488.
 enum { ROW_LOGP, ROW_POLICY };
 struct RowArgs {
   const void *logits;
@@ -126,8 +135,39 @@ __device__ __forceinline__ double policy_row(const RowArgs &a, const int row, co
   return w * d;
 }
 
-// WAVES waves a row; W 16-byte words a thread in registers, or W = 0: any number, read once more for the gradient
-template <class T, int MODE, int WAVES, int W>
+// What one thread makes of its row, whose maximum and sum it has: d and d / s of the policy loss's gradient
+template <class T, int MODE>
+__device__ __forceinline__ void finish_row(const RowArgs &a, const int row, const T *x, const int t, const Part p, float *d, float *scale) {
+  const bool in = t < a.vocab;
+  // (x_t - m first: m + log s would lose the logarithm beside a large m)
+  const double lp = in ? static_cast<double>(to_f32(x[in ? t : 0])) - static_cast<double>(p.m) - log(p.s) : __builtin_nan("");
+  if (a.logp) a.logp[row] = static_cast<float>(lp);
+  if (a.logp64) a.logp64[row] = lp;
+  if (a.stats) {
+    const bool none = p.s == 0.0;   // nothing but -inf: exp(x - m) is exp(-inf + inf)
+    a.stats[2 * static_cast<size_t>(row)]     = none ? -INFINITY : p.m;
+    a.stats[2 * static_cast<size_t>(row) + 1] = none ? __builtin_nanf("") : static_cast<float>(p.s);
+  }
+  if constexpr (MODE == ROW_POLICY) {
+    double loss, dd = policy_row(a, row, lp, &loss);
+    if (a.row_loss) a.row_loss[row] = static_cast<float>(loss);
+    *d     = static_cast<float>(dd);
+    *scale = static_cast<float>(dd / p.s);
+  }
+}
+// ... of a row that does not count
+template <int MODE>
+__device__ __forceinline__ void skip_row(const RowArgs &a, const int row) {
+  if (a.logp) a.logp[row] = 0.0f;
+  if (a.stats) a.stats[2 * static_cast<size_t>(row)] = a.stats[2 * static_cast<size_t>(row) + 1] = 0.0f;
+  if (a.logp64) a.logp64[row] = 0.0;
+  if (MODE == ROW_POLICY && a.row_loss) a.row_loss[row] = 0.0f;
+}
+
+// WAVES waves a row; W 16-byte words a thread in registers, or W = 0: any number, read once more for the gradient. Rows in
+// registers of few waves are fastest as long as several workgroups fit a compute unit (policy loss of 8192 x 32000 in
+// bf16: 4 waves 198 us, 8 waves 208, 16 waves 258, read twice 214).
+template <class T, int MODE, int WAVES, int W, bool ONCE>
 __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256)
 row_kernel(const RowArgs a) {
   constexpr int NT = 64 * WAVES, ROWS = WAVES >= 4 ? 1 : 4 / WAVES;   // threads and rows of a workgroup
@@ -143,12 +183,7 @@ row_kernel(const RowArgs a) {
   const Row<T> r(x, a.vocab);
   const int t = a.target[row];
   if (t < 0) {   // not counted, and not read
-    if (tid == 0) {
-      if (a.logp) a.logp[row] = 0.0f;
-      if (a.stats) a.stats[2 * static_cast<size_t>(row)] = a.stats[2 * static_cast<size_t>(row) + 1] = 0.0f;
-      if (a.logp64) a.logp64[row] = 0.0;
-      if (MODE == ROW_POLICY && a.row_loss) a.row_loss[row] = 0.0f;
-    }
+    if (tid == 0) skip_row<MODE>(a, row);
     if (dx) {
       const float zero[N] = {};
       for (int k = tid; k < r.words; k += NT) store_word(r, dx, k, zero);
@@ -162,7 +197,7 @@ row_kernel(const RowArgs a) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const int k = tid + i * NT;
-      if (k < r.words) held[i] = r.load(k);
+      if (k < r.words) held[i] = r.template load<MODE == ROW_POLICY || ONCE>(k);
     }
     p.m = LOWEST;
 #pragma unroll
@@ -176,7 +211,7 @@ row_kernel(const RowArgs a) {
   } else {
     p = Part{LOWEST, 0.0};
     for (int k = tid; k < r.words; k += NT) {
-      const Word<T> w = r.load(k);
+      const Word<T> w = r.template load<MODE == ROW_LOGP && ONCE>(k);
       const float m   = word_max(w, p.m);
       p.s = p.s * static_cast<double>(exp_base2((p.m - m) * LOG2E)) + static_cast<double>(word_sum(w, m, 0.0f));
       p.m = m;
@@ -184,24 +219,7 @@ row_kernel(const RowArgs a) {
   }
   p = wave_join(p);
   float scale = 0.0f, d = 0.0f;   // d / s and d
-  auto finish = [&]() {           // one thread of the row
-    const bool in = t < a.vocab;
-    // (x_t - m first: m + log s would lose the logarithm beside a large m)
-    const double lp = in ? static_cast<double>(to_f32(x[in ? t : 0])) - static_cast<double>(p.m) - log(p.s) : __builtin_nan("");
-    if (a.logp) a.logp[row] = static_cast<float>(lp);
-    if (a.logp64) a.logp64[row] = lp;
-    if (a.stats) {
-      const bool none = p.s == 0.0;   // nothing but -inf: exp(x - m) is exp(-inf + inf)
-      a.stats[2 * static_cast<size_t>(row)]     = none ? -INFINITY : p.m;
-      a.stats[2 * static_cast<size_t>(row) + 1] = none ? __builtin_nanf("") : static_cast<float>(p.s);
-    }
-    if constexpr (MODE == ROW_POLICY) {
-      double loss, dd = policy_row(a, row, lp, &loss);
-      if (a.row_loss) a.row_loss[row] = static_cast<float>(loss);
-      d     = static_cast<float>(dd);
-      scale = static_cast<float>(dd / p.s);
-    }
-  };
+  auto finish = [&]() { finish_row<T, MODE>(a, row, x, t, p, &d, &scale); };
   if constexpr (WAVES == 1) {
     if (tid == 0) finish();
     if (MODE != ROW_POLICY || !dx) return;
@@ -247,8 +265,50 @@ row_kernel(const RowArgs a) {
       for (int i = 0; i < W; ++i)
         if (tid + i * NT < r.words) grad(held[i], tid + i * NT);
     } else {
-      for (int k = tid; k < r.words; k += NT) grad(r.load(k), k);
+      for (int k = tid; k < r.words; k += NT) grad(r.template load<true>(k), k);
     }
+  }
+}
+
+// Rows of a few logits (small policy nets), a thread each. With `loss` one workgroup has all of them, and adds up the
+// losses as well.
+constexpr int SHORT_ROW = 32, SHORT_NT = 1024;
+template <class T, int MODE>
+__global__ void __launch_bounds__(SHORT_NT)
+short_row_kernel(const RowArgs a, float *__restrict__ loss) {
+  __shared__ double part[SHORT_NT / 64];
+  const int row = blockIdx.x * blockDim.x + threadIdx.x;
+  const bool in = row < a.rows && !(a.seq_start && (row < a.seq_start[0] || row >= a.seq_start[a.sequences]));
+  if (in) {
+    const T *x  = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
+    T *dx       = MODE == ROW_POLICY && a.dlogits ? static_cast<T *>(a.dlogits) + static_cast<size_t>(row) * a.ld_d : nullptr;
+    const int t = a.target[row];
+    if (t < 0) {
+      skip_row<MODE>(a, row);
+      if (dx)
+        for (int j = 0; j < a.vocab; ++j) dx[j] = T{};
+    } else {
+      Part p{LOWEST, 0.0};
+      for (int j = 0; j < a.vocab; ++j) p.m = fmaxf(p.m, to_f32(x[j]));
+      for (int j = 0; j < a.vocab; ++j) p.s += static_cast<double>(exp_base2((to_f32(x[j]) - p.m) * LOG2E));
+      float d = 0.0f, scale = 0.0f;
+      finish_row<T, MODE>(a, row, x, t, p, &d, &scale);
+      if (dx)
+        for (int j = 0; j < a.vocab; ++j) {
+          const float g = -scale * exp_base2((to_f32(x[j]) - p.m) * LOG2E);
+          dx[j] = from_f32<T>(j == t ? g + d : g);
+        }
+    }
+  }
+  if (!loss) return;
+  double s = in && a.row_loss ? a.row_loss[row] : 0.0;   // (what this thread has just written)
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int w = 0; w < static_cast<int>(blockDim.x / 64); ++w) sum += part[w];
+    loss[0] = static_cast<float>(sum);
   }
 }
 
@@ -265,11 +325,33 @@ struct GradArgs {
   int sequences;
   void *dlogits;
   size_t ld_d;
+  // the mean of these, which a workgroup behind the others computes (null: none)
+  const float *pair_loss;
+  float *loss;
 };
+// out[0] = scale * (v[0] + ... + v[n-1]), by one workgroup, in an order that n and its size set
+template <int NT>
+__device__ __forceinline__ void sum_of(const float *v, const int n, const double scale, float *out) {
+  __shared__ double part[NT / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += NT) s += v[i];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int w = 0; w < NT / 64; ++w) sum += part[w];
+    out[0] = static_cast<float>(scale * sum);
+  }
+}
 template <class T>
 __global__ void __launch_bounds__(GRAD_NT)
 dlogits_kernel(const GradArgs a) {
   constexpr int N = Word<T>::N;
+  if (a.loss && blockIdx.x == gridDim.x - 1) {
+    sum_of<GRAD_NT>(a.pair_loss, a.sequences / 2, 2.0 / a.sequences, a.loss);
+    return;
+  }
   const int row = blockIdx.x / a.blocks_per_row, part = blockIdx.x % a.blocks_per_row, tid = threadIdx.x;
   float d = 0.0f;
   if (a.seq_start) {
@@ -300,7 +382,7 @@ dlogits_kernel(const GradArgs a) {
   Word<T> w[GRAD_WORDS];
 #pragma unroll
   for (int i = 0; i < GRAD_WORDS; ++i)
-    if (k0 + i * GRAD_NT < r.words) w[i] = r.load(k0 + i * GRAD_NT);
+    if (k0 + i * GRAD_NT < r.words) w[i] = r.template load<true>(k0 + i * GRAD_NT);
 #pragma unroll
   for (int i = 0; i < GRAD_WORDS; ++i) {
     const int k = k0 + i * GRAD_NT;
@@ -317,26 +399,10 @@ dlogits_kernel(const GradArgs a) {
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// out[0] = scale * (v[0] + ... + v[n-1]), one workgroup, in an order that n alone sets
 constexpr int SUM_NT = 1024;
 __global__ void __launch_bounds__(SUM_NT)
 sum_kernel(const float *__restrict__ v, const int n, const double scale, float *__restrict__ out) {
-  __shared__ double part[SUM_NT / 64];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += SUM_NT) s += v[i];
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    s = wave_sum(threadIdx.x < SUM_NT / 64 ? part[threadIdx.x] : 0.0);
-    if (threadIdx.x == 0) out[0] = static_cast<float>(scale * s);
-  }
+  sum_of<SUM_NT>(v, n, scale, out);
 }
 
 // One workgroup a pair: the sums over its two sequences, its margin, its loss and the factors of its gradient.
@@ -395,8 +461,9 @@ pair_kernel(const PairArgs a) {
   a.d[2 * pair + 1]   = -d;
 }
 
+// `again`: the logits are read again soon
 template <class T, int MODE>
-int launch_rows(const RowArgs &a) {
+int launch_rows(const RowArgs &a, bool again) {
   const int words = static_cast<int>((static_cast<long>(a.vocab) * sizeof(T) + 15 + 15) / 16);   // at any alignment
   auto go = [&](auto kernel, int waves) {
     const int rows_per = waves >= 4 ? 1 : 4 / waves;
@@ -404,13 +471,28 @@ int launch_rows(const RowArgs &a) {
     TDH_LAUNCH_CHECK();
     return static_cast<int>(TDH_OK);
   };
-  if (words <= 64) return go(row_kernel<T, MODE, 1, 1>, 1);
-  if (words <= 256) return go(row_kernel<T, MODE, 1, 4>, 1);
-  if (words <= 1024) return go(row_kernel<T, MODE, 4, 4>, 4);
-  if (words <= 2048) return go(row_kernel<T, MODE, 4, 8>, 4);
-  if (words <= 4096) return go(row_kernel<T, MODE, 16, 4>, 16);
-  if (words <= 8192) return go(row_kernel<T, MODE, 16, 8>, 16);
-  return go(row_kernel<T, MODE, 16, 0>, 16);
+  if (a.vocab <= SHORT_ROW) {
+    TDH_LAUNCH((short_row_kernel<T, MODE>), dim3(ceil_div(a.rows, 256)), dim3(256), 0, ctx().stream, a, static_cast<float *>(nullptr));
+    TDH_LAUNCH_CHECK();
+    return TDH_OK;
+  }
+  if (words <= 64) return go(row_kernel<T, MODE, 1, 1, false>, 1);
+  if (words <= 128) return go(row_kernel<T, MODE, 1, 2, false>, 1);
+  if (words <= 256) return go(row_kernel<T, MODE, 1, 4, false>, 1);
+  // fewer rows than compute units: all the waves there are for each
+  if (a.rows > 256) {
+    if (words <= 512) return go(row_kernel<T, MODE, 1, 8, false>, 1);
+    if (words <= 1024) return go(row_kernel<T, MODE, 4, 4, false>, 4);
+    if (words <= 2048) return go(row_kernel<T, MODE, 4, 8, false>, 4);
+    if (words <= 4096) return go(row_kernel<T, MODE, 4, 16, false>, 4);
+    if (MODE == ROW_LOGP) return again ? go(row_kernel<T, MODE, 8, 0, false>, 8) : go(row_kernel<T, MODE, 8, 0, true>, 8);
+  }
+  if (words <= 1024) return go(row_kernel<T, MODE, 16, 1, false>, 16);
+  if (words <= 4096) return go(row_kernel<T, MODE, 16, 4, false>, 16);
+  if (MODE == ROW_LOGP) return go(row_kernel<T, MODE, 16, 0, false>, 16);
+  if (words <= 8192) return go(row_kernel<T, MODE, 16, 8, false>, 16);
+  if (words <= 16384) return go(row_kernel<T, MODE, 16, 16, false>, 16);
+  return go(row_kernel<T, MODE, 16, 0, false>, 16);
 }
 
 // workgroups of a row at any alignment
@@ -418,7 +500,7 @@ int grad_blocks(int vocab, size_t size) { return ceil_div(static_cast<int>((voca
 template <class T>
 int launch_dlogits(GradArgs a) {
   a.blocks_per_row = grad_blocks(a.vocab, sizeof(T));
-  TDH_LAUNCH((dlogits_kernel<T>), dim3(a.rows * a.blocks_per_row), dim3(GRAD_NT), 0, ctx().stream, a);
+  TDH_LAUNCH((dlogits_kernel<T>), dim3(a.rows * a.blocks_per_row + (a.loss ? 1 : 0)), dim3(GRAD_NT), 0, ctx().stream, a);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
@@ -448,7 +530,7 @@ int check_dlogits(const char *who, int dtype, int rows, int vocab, const void *l
   TDH_CHECK_ARG(ld_d >= static_cast<size_t>(vocab) && ld_d <= (static_cast<size_t>(1) << 40),
                 "%s: rows of %d gradients %zu elements apart", who, vocab, ld_d);
   TDH_CHECK_ARG((reinterpret_cast<uintptr_t>(dlogits) & (dtype_size(dtype) - 1)) == 0, "%s: gradient not aligned to its elements", who);
-  TDH_CHECK_ARG(static_cast<long>(rows) * grad_blocks(vocab, dtype_size(dtype)) <= GRID_X_MAX, "%s: %d rows of %d logits are too many", who, rows, vocab);
+  TDH_CHECK_ARG(static_cast<long>(rows) * grad_blocks(vocab, dtype_size(dtype)) < GRID_X_MAX, "%s: %d rows of %d logits are too many", who, rows, vocab);
   if (rows == 0 || (dlogits == logits && ld_d == ld)) return TDH_OK;
   const uintptr_t x = reinterpret_cast<uintptr_t>(logits), g = reinterpret_cast<uintptr_t>(dlogits), size = dtype_size(dtype);
   TDH_CHECK_ARG(x + size * ((rows - 1) * ld + vocab) <= g || g + size * ((rows - 1) * ld_d + vocab) <= x,
@@ -473,7 +555,7 @@ int tdh_token_logprob_fwd(int dtype, int rows, int vocab, const void *logits, si
   a.logits = logits; a.ld = ld; a.target = target; a.rows = rows; a.vocab = vocab;
   a.logp = logp; a.stats = stats;
   ProfScope prof("token_logprob_fwd", logits_bytes(dtype, rows, vocab, 1), WORK_BYTE);
-  return with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_LOGP>(a); });
+  return with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_LOGP>(a, stats != nullptr); });
 }
 
 int tdh_token_logprob_bwd(int dtype, int rows, int vocab, const void *logits, size_t ld, const int32_t *target,
@@ -516,7 +598,13 @@ int tdh_policy_loss(const tdh_policy_desc *p, int dtype, int rows, int vocab, co
   a.row_loss = row_loss; a.dlogits = dlogits; a.ld_d = ld_d;
   {
     ProfScope prof("policy_loss", logits_bytes(dtype, rows, vocab, dlogits ? 2 : 1), WORK_BYTE);
-    TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_POLICY>(a); }));
+    if (vocab <= SHORT_ROW && rows <= SHORT_NT && loss)   // one workgroup does it all
+      return with_dtype(dtype, [&](auto t) {
+        TDH_LAUNCH((short_row_kernel<decltype(t), ROW_POLICY>), dim3(1), dim3((rows + 63) / 64 * 64), 0, ctx().stream, a, loss);
+        TDH_LAUNCH_CHECK();
+        return static_cast<int>(TDH_OK);
+      });
+    TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_POLICY>(a, false); }));
   }
   return loss ? launch_sum(row_loss, rows, 1.0, loss) : static_cast<int>(TDH_OK);
 }
@@ -549,7 +637,7 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
     a.stats = static_cast<float *>(stats);
     a.seq_start = seq_start; a.sequences = 2 * pairs;
     ProfScope prof("preference_logprob", logits_bytes(dtype, rows, vocab, 1), WORK_BYTE);
-    TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_LOGP>(a); }));
+    TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_LOGP>(a, dlogits != nullptr); }));
   }
   {
     PairArgs a{};
@@ -565,8 +653,9 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
     g.logits = logits; g.ld = ld; g.target = target; g.rows = rows; g.vocab = vocab;
     g.stats = static_cast<const float *>(stats); g.d = static_cast<const float *>(d);
     g.seq_start = seq_start; g.sequences = 2 * pairs; g.dlogits = dlogits; g.ld_d = ld_d;
+    g.pair_loss = static_cast<const float *>(pair_loss); g.loss = loss;
     ProfScope prof("preference_grad", logits_bytes(dtype, rows, vocab, 2), WORK_BYTE);
-    TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_dlogits<decltype(t)>(g); }));
+    return with_dtype(dtype, [&](auto t) { return launch_dlogits<decltype(t)>(g); });
   }
   return loss ? launch_sum(static_cast<const float *>(pair_loss), pairs, 1.0 / pairs, loss) : static_cast<int>(TDH_OK);
 }
