@@ -152,6 +152,41 @@ def test_gated_ff(T, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("shape", [(1001, 1024, 1000), (130, 2808, 2800), (700, 1336, 1200), (3000, 264, 1400), (300, 520, 392)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ff_of_many_samples(T, dtype, shape):
+    """(the largest tiles, products in three parts, sums split along k, last tiles that are shorter and narrower)"""
+    ff_case(T, shape, "silu", dtype, bias=True)
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+def test_gated_ff_of_many_samples_unaligned_and_accumulating(T, dtype):
+    ff_case(T, (1001, 1024, 1000), "gelu", dtype, bias=True, skew=1, accumulate=True)
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+def test_gated_ff_of_many_samples_with_infinities(T, dtype):
+    """An infinite or NaN value reaches the sums that it is part of, which are what fp32 arithmetic gives, and no others."""
+    n, d, f = 1001, 1024, 1000
+    rng = np.random.RandomState(12)
+    x, w, dh = rng.randn(n, d), rng.randn(d, 2 * f) / 32, rng.randn(n, f)
+    x[3, 17], x[900, 5], x[1000, 1023] = np.inf, np.nan, -np.inf
+    w[40, 7] = np.inf
+    x, w, dh = (L.rounded(v, dtype) for v in (x, w, dh))
+    bx, bw, bdh = (Buf(T, v, dtype) for v in (x, w, dh))
+    h, z, dx, dw = out(T, (n, f), dtype), out(T, (n, 2 * f)), out(T, (n, d), dtype), out(T, (d, 2 * f), dtype)
+    T.gated_ff_fwd(d, f, False, n, bx, bw, None, h, z, act="none", dtype=dtype)
+    T.gated_ff_bwd(d, f, False, n, bx, bw, z, bdh, dx, dw, None, act="none", dtype=dtype)
+    with np.errstate(all="ignore"):
+        want = x @ w
+        got = z.read()
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want))
+        dz = L.rounded(np.concatenate([dh * got[:, f:], dh * got[:, :f]], 1), dtype)
+        for g, v in ((dx.read(), dz @ w.T), (dw.read(), x.T @ dz)):
+            assert np.array_equal(np.isfinite(g), np.isfinite(v)) and np.array_equal(np.isnan(g), np.isnan(v))
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 def test_gated_ff_activations(T, dtype, act):
     ff_case(T, (9, 48, 56), act, dtype, bias=True, scale=3.0)

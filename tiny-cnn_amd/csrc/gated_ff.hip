@@ -2,6 +2,7 @@
 // h = act(z_gate) * z_up; on the way back dz = (dh * z_up * act'(z_gate), dh * act(z_gate)),
 // dx = dz W^T, dW = x^T dz, db = the column sums of dz.
 #include "gemm16.h"
+#include "gemm_x3.h"
 
 namespace tdh {
 
@@ -72,20 +73,6 @@ gate_fwd_kernel(const float *__restrict__ z, float *__restrict__ h, const int hi
   });
 }
 
-__global__ void __launch_bounds__(GF_NT)
-gate_bwd_kernel(const float *__restrict__ z, const float *__restrict__ dh, float *__restrict__ dz, const int hidden,
-                const size_t total, const int act) {
-  const size_t i = static_cast<size_t>(blockIdx.x) * GF_NT + threadIdx.x;
-  if (i >= total) return;
-  const size_t row = i / hidden, c = i - row * hidden;
-  with_gate(act, [&](auto kind) {
-    float slope;
-    const float a = gate_act<decltype(kind)::value>(z[row * 2 * hidden + c], &slope), d = dh[i];
-    dz[row * 2 * hidden + c]          = d * z[row * 2 * hidden + hidden + c] * slope;
-    dz[row * 2 * hidden + hidden + c] = d * a;
-  });
-}
-
 // dst = src in another type
 template <class D, class S>
 __global__ void __launch_bounds__(GF_NT)
@@ -110,35 +97,6 @@ int take(size_t n, T **out) {
   TDH_TRY(ws_take(n * sizeof(T), &p));
   *out = static_cast<T *>(p);
   return TDH_OK;
-}
-
-// ------------------------------------------------------------------- fp32
-int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *b, float *h, float *z) {
-  const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
-  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + (z ? 0 : ws_align(4 * nz))));
-  if (!z) TDH_TRY(take(nz, &z));
-  TDH_TRY(fc_fwd(in, 2 * hidden, b != nullptr, batch, x, w, b, z));
-  const size_t total = nz / 2;
-  ProfScope prof("gate_fwd", 12.0 * total, WORK_BYTE);
-  TDH_LAUNCH(gate_fwd_kernel, dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h,
-             hidden, total, act);
-  TDH_LAUNCH_CHECK();
-  return TDH_OK;
-}
-int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *z, const float *dh, float *dx,
-               float *dw, float *db, int accumulate) {
-  const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
-  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + ws_align(4 * nz)));
-  float *dz;
-  TDH_TRY(take(nz, &dz));
-  const size_t total = nz / 2;
-  {
-    ProfScope prof("gate_bwd", 20.0 * total, WORK_BYTE);
-    TDH_LAUNCH(gate_bwd_kernel, dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, dh,
-               dz, hidden, total, act);
-    TDH_LAUNCH_CHECK();
-  }
-  return fc_bwd(in, 2 * hidden, db != nullptr, batch, x, w, dz, dx, dw, db, accumulate, ActGrad());
 }
 
 // ------------------------------------------------------------ 16-bit types
@@ -198,7 +156,7 @@ struct EpiGate {
           if (m0 + 32 * i + row >= rows) return;
           T *p = h + static_cast<size_t>(m0 + 32 * i + row) * hidden + n0 + col;
           if (wide) {
-            if (n0 + col < hidden) *reinterpret_cast<uint4 *>(p) = Word<T>::from(v).raw;
+            if (n0 + col < hidden) store8(p, v);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -255,13 +213,13 @@ struct EpiGrad {
         if (m >= rows) return;
         if (wide) {
           if (n >= cols) return;
-          uint4 *p = reinterpret_cast<uint4 *>(out + static_cast<size_t>(m) * cols + n);
+          T *p = out + static_cast<size_t>(m) * cols + n;
+          if (!accumulate) return store8(p, v);
           float o[8];
-          Word<T> was{};
-          if (accumulate) was.raw = *p;
+          load8(p, o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = accumulate ? v[e] + was[e] : v[e];
-          *p = Word<T>::from(o).raw;
+          for (int e = 0; e < 8; ++e) o[e] += v[e];
+          store8(p, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -308,6 +266,15 @@ grad_reduce_kernel(const EpiGrad<T> epi, const int splits) {
 #pragma unroll 8
   for (int s = 0; s < splits; ++s) v += epi.partial[s * total + i];
   epi.one(m, static_cast<int>(i - m * epi.cols), v);
+}
+
+template <class T>
+int launch_grad_reduce(const EpiGrad<T> &epi, int splits) {
+  const size_t total = static_cast<size_t>(epi.rows) * epi.cols;
+  ProfScope prof("gated_ff_bwd_reduce", 4.0 * splits * total, WORK_BYTE);
+  TDH_LAUNCH((grad_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, splits);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
 }
 
 // Matrices copied to padded ones: columns in one or two halves of `used` values, `half` (a multiple of 8) apart in the copy;
@@ -871,13 +838,7 @@ template <class T, bool A_KC, bool B_KC>
 int ff_grad(const FfPlan &plan, const G16Matrix &A, const G16Matrix &B, EpiGrad<T> epi, int K, const char *tag) {
   if (plan.splits > 1) TDH_TRY(take(plan.splits * static_cast<size_t>(epi.rows) * epi.cols, &epi.partial));
   TDH_TRY((ff_gemm<T, A_KC, B_KC, false>(plan, A, B, epi, epi.rows, epi.cols, K, tag)));
-  if (plan.splits > 1) {
-    const size_t total = static_cast<size_t>(epi.rows) * epi.cols;
-    ProfScope prof("gated_ff_bwd_reduce", 4.0 * plan.splits * total, WORK_BYTE);
-    TDH_LAUNCH((grad_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, plan.splits);
-    TDH_LAUNCH_CHECK();
-  }
-  return TDH_OK;
+  return plan.splits > 1 ? launch_grad_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
 }
 
 template <class T>
@@ -912,15 +873,185 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   return TDH_OK;
 }
 
+// ------------------------------------------------------------------- fp32
+// Products of many samples on operands that are split in three parts by a pass of their own (gemm_x3.h); the others are the
+// fully-connected layer's.
+
+// fp32 matrices to their three planes, a thread eight neighbours. sign: 1 turns every other group of 32 rows, 2 of columns.
+struct SplitJobs {
+  struct Job {
+    const float *src;
+    uint16_t *dst;   // planes, rows * cols elements each
+    int cols, sign;
+    unsigned blocks;
+    size_t words;    // of eight elements
+  } job[2];
+};
+__global__ void __launch_bounds__(GF_NT)
+split_kernel(const SplitJobs jobs) {
+  const bool second = blockIdx.x >= jobs.job[0].blocks;
+  const SplitJobs::Job &j = jobs.job[second];
+  const size_t i = static_cast<size_t>(blockIdx.x - (second ? jobs.job[0].blocks : 0)) * GF_NT + threadIdx.x;
+  if (i >= j.words) return;
+  const size_t row = i / (j.cols / 8);
+  const int col    = static_cast<int>(i - row * (j.cols / 8)) * 8;
+  const bool turn  = j.sign == 1 ? (row / X3P_BK) & 1 : j.sign == 2 ? (col / X3P_BK) & 1 : false;
+  const float scale = turn ? -X3_SCALE : X3_SCALE;
+  float v[8];
+  if ((reinterpret_cast<uintptr_t>(j.src) & 15) == 0) {
+    load8(j.src + i * 8, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = j.src[i * 8 + e];
+  }
+  uint4 out[X3_PARTS];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t part[X3_PARTS];
+    split_pair(scale * v[2 * c], scale * v[2 * c + 1], part);
+#pragma unroll
+    for (int p = 0; p < X3_PARTS; ++p) (&out[p].x)[c] = part[p];
+  }
+#pragma unroll
+  for (int p = 0; p < X3_PARTS; ++p) reinterpret_cast<uint4 *>(j.dst)[p * j.words + i] = out[p];
+}
+struct Splitter {
+  SplitJobs jobs{};
+  int n = 0;
+  static size_t bytes(size_t rows, int cols) { return ws_align(6 * rows * cols); }
+  int add(const float *src, int rows, int cols, int sign, G16Matrix *out) {
+    SplitJobs::Job &j = jobs.job[n++];
+    j = {src, nullptr, cols, sign, 0, static_cast<size_t>(rows) * cols / 8};
+    j.blocks = static_cast<unsigned>(ceil_div_sz(j.words, GF_NT));
+    TDH_TRY(take(j.words * 24, &j.dst));
+    *out = G16Matrix{j.dst, cols, rows, cols};
+    return TDH_OK;
+  }
+  int run() {
+    const size_t words = jobs.job[0].words + jobs.job[1].words;
+    ProfScope prof("ff_split", 80.0 * words, WORK_BYTE);
+    TDH_LAUNCH(split_kernel, dim3(jobs.job[0].blocks + jobs.job[1].blocks), dim3(GF_NT), 0, ctx().stream, jobs);
+    TDH_LAUNCH_CHECK();
+    return TDH_OK;
+  }
+};
+
+// Tiles of 256 x 128, split along k where they do not fill the compute units.
+constexpr int X3P_BM = 256, X3P_BN = 128;
+FfPlan x3_plan(int M, int N, int K) {
+  const long cus   = ctx().compute_units > 0 ? ctx().compute_units : 256, tiles = static_cast<long>(ceil_div(M, X3P_BM)) * ceil_div(N, X3P_BN);
+  const int ktiles = std::max(1, ceil_div(K, X3P_BK));
+  FfPlan best{0, 1, ktiles * X3P_BK};
+  double best_us = 1e30;
+  for (int want = 1; want <= 16 && want <= ktiles; ++want) {
+    const int per = ceil_div(ktiles, want), splits = ceil_div(ktiles, per);
+    double us = static_cast<double>(ceil_div_sz(tiles * splits, cus)) * (per * 1.7 + 8.0);
+    if (splits > 1) us += 3.0 + 8.0 * splits * M * N / 8e6;
+    if (us < best_us) {
+      best_us = us;
+      best    = FfPlan{0, splits, per * X3P_BK};
+    }
+  }
+  return best;
+}
+template <bool A_KC, bool B_KC, bool PAIR, class Epi>
+int x3_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const X3Source &src, const Epi &epi, int K, const char *tag) {
+  ProfScope prof(tag, src.rows, src.cols, K);
+  const int tiles_m = ceil_div(src.rows, X3P_BM), tiles_n = PAIR ? ceil_div(src.cols / 2, X3P_BN / 2) : ceil_div(src.cols, X3P_BN);
+  TDH_LAUNCH((gemm_x3_kernel<4, 2, A_KC, B_KC, PAIR, Epi>), dim3(static_cast<unsigned>(tiles_m) * tiles_n * p.splits), dim3(512), 0,
+             ctx().stream, A, B, static_cast<long>(A.rows) * A.cols, static_cast<long>(B.rows) * B.cols, src, epi, tiles_m, tiles_n, K,
+             p.k_per_split);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
+}
+template <bool A_KC, bool B_KC>
+int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad<float> epi, int K, const char *tag) {
+  const FfPlan plan  = x3_plan(src.rows, src.cols, K);
+  const size_t total = static_cast<size_t>(src.rows) * src.cols;
+  if (plan.splits > 1) TDH_TRY(take(plan.splits * total, &epi.partial));
+  TDH_TRY((x3_gemm<A_KC, B_KC, false>(plan, A, B, src, epi, K, tag)));
+  return plan.splits > 1 ? launch_grad_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
+}
+
+// Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do.
+bool x3_fits(int in, int hidden) { return in % 8 == 0 && hidden % 8 == 0; }
+constexpr int X3P_BATCH = 768, X3P_DW_BATCH = 128;
+constexpr double X3P_FLOP = 4e9;   // below that the products are short
+bool x3_weights(int in, int hidden, int batch) {
+  return x3_fits(in, hidden) && batch >= X3P_BATCH && 4.0 * batch * in * hidden >= X3P_FLOP;
+}
+bool x3_dw(int in, int hidden, int batch) { return x3_fits(in, hidden) && batch >= X3P_DW_BATCH && 4.0 * batch * in * hidden >= X3P_FLOP; }
+
+int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *b, float *h, float *z) {
+  const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
+  if (x3_weights(in, hidden, batch)) {
+    const FfPlan plan = x3_plan(batch, 2 * hidden, in);
+    TDH_TRY(ws_begin(Splitter::bytes(batch, in) + Splitter::bytes(in, 2 * hidden) + ff_partial_bytes(plan, nz)));
+    Splitter split;
+    G16Matrix X, W;
+    TDH_TRY(split.add(x, batch, in, 2, &X));
+    TDH_TRY(split.add(w, in, 2 * hidden, 0, &W));
+    TDH_TRY(split.run());
+    const X3Source src{x, w, in, 1, 2L * hidden, 1, batch, 2 * hidden};
+    EpiGate<float> epi{h, z, b, nullptr, batch, hidden, hidden, act, fits(h, hidden)};
+    if (plan.splits == 1) return x3_gemm<true, false, true>(plan, X, W, src, epi, in, "gated_ff_fwd_x3");
+    TDH_TRY(take(plan.splits * nz, &epi.partial));
+    const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * hidden, hidden, hidden, 0, false};
+    TDH_TRY((x3_gemm<true, false, false>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
+    return launch_gate_reduce(epi, plan.splits);
+  }
+  TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + (z ? 0 : ws_align(4 * nz))));
+  if (!z) TDH_TRY(take(nz, &z));
+  TDH_TRY(fc_fwd(in, 2 * hidden, b != nullptr, batch, x, w, b, z));
+  const size_t total = nz / 2;
+  ProfScope prof("gate_fwd", 12.0 * total, WORK_BYTE);
+  TDH_LAUNCH(gate_fwd_kernel, dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, z, h, hidden, total, act);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
+}
+int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *z, const float *dh, float *dx,
+               float *dw, float *db, int accumulate) {
+  const int cols = 2 * hidden;
+  const bool planes_x = dx && x3_weights(in, hidden, batch), planes_w = dw && x3_dw(in, hidden, batch);
+  const bool own_db   = db && planes_w;   // (else the sums ride along with dw's launch)
+  const DzPlan pz     = dz_plan(hidden, hidden, batch, z, dh, own_db);
+  const size_t nz = static_cast<size_t>(batch) * cols, nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * cols;
+  TDH_TRY(ws_begin(ws_align(4 * nz) + (own_db ? ws_align(4 * static_cast<size_t>(pz.bands) * cols) : 0) +
+                   (planes_x || planes_w ? Splitter::bytes(batch, cols) : 0) +
+                   (planes_x ? Splitter::bytes(in, cols) + ff_partial_bytes(x3_plan(batch, in, cols), nx) : 0) +
+                   (planes_w ? Splitter::bytes(batch, in) + ff_partial_bytes(x3_plan(in, cols, batch), nw) : 0) +
+                   (planes_x && planes_w ? 0 : fc_workspace_bytes(in, cols, batch))));
+  float *dz = nullptr, *bias_part = nullptr;
+  TDH_TRY(take(nz, &dz));
+  if (own_db) TDH_TRY(take(static_cast<size_t>(pz.bands) * cols, &bias_part));
+  TDH_TRY(launch_dz(pz, act, hidden, hidden, batch, z, dh, dz, bias_part));
+  if (own_db) TDH_TRY(launch_db(bias_part, db, pz.bands, hidden, accumulate));
+  if (!planes_x && !planes_w)
+    return fc_bwd(in, cols, db != nullptr, batch, x, w, dz, dx, dw, db, accumulate, ActGrad());
+  G16Matrix Z, X, W;
+  Splitter split, weights;
+  TDH_TRY(split.add(dz, batch, cols, 0, &Z));
+  if (planes_w) TDH_TRY(split.add(x, batch, in, 1, &X));
+  TDH_TRY(split.run());
+  if (planes_w)
+    TDH_TRY((x3_grad<false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, cols},
+                                   EpiGrad<float>{dw, nullptr, in, cols, hidden, hidden, accumulate, fits(dw, hidden)}, batch, "gated_ff_dw_x3")));
+  if (planes_x) {
+    TDH_TRY(weights.add(w, in, cols, 2, &W));
+    TDH_TRY(weights.run());
+    TDH_TRY((x3_grad<true, true>(Z, W, X3Source{dz, w, cols, 1, 1, cols, batch, in},
+                                 EpiGrad<float>{dx, nullptr, batch, in, in, in, 0, fits(dx, in)}, cols, "gated_ff_dx_x3")));
+  }
+  if ((dx && !planes_x) || (dw && !planes_w) || (db && !own_db))
+    return fc_bwd(in, cols, db && !own_db, batch, x, w, dz, planes_x ? nullptr : dx, planes_w ? nullptr : dw, own_db ? nullptr : db,
+                  accumulate, ActGrad());
+  return TDH_OK;
+}
+
 // the gradients of no samples
 template <class T>
 int no_rows(int in, int hidden, T *dw, T *db) {
-  const size_t total = static_cast<size_t>(in) * 2 * hidden;
-  if (dw) {
-    const EpiGrad<T> epi{dw, nullptr, in, 2 * hidden, hidden, hidden, 0, false};
-    TDH_LAUNCH((grad_reduce_kernel<T>), dim3(static_cast<unsigned>(ceil_div_sz(total, GF_NT))), dim3(GF_NT), 0, ctx().stream, epi, 0);
-    TDH_LAUNCH_CHECK();
-  }
+  if (dw) TDH_TRY(launch_grad_reduce(EpiGrad<T>{dw, nullptr, in, 2 * hidden, hidden, hidden, 0, false}, 0));
   return db ? launch_db<T>(nullptr, db, 0, hidden, 0) : static_cast<int>(TDH_OK);
 }
 

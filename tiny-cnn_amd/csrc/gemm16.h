@@ -10,8 +10,8 @@
 // them in turns: the next one is on its way while this one is multiplied, one barrier a tile. LDS holds a tile as it
 // lies in memory, its 16-byte chunks permuted within each row so that the reads hit different banks (the lanes fetch
 // permuted chunks: the way into LDS is linear in the lane):
-//   along k      rows of 64 k (128 bytes), chunk c of row r at c ^ (r mod 8); a lane's operand, 8 k of its row, is one
-//                16-byte read;
+//   along k      rows of 64 k (128 bytes), chunk c of row r at c ^ (r mod 8) (rows of 32 k: at c ^ (r/2 mod 4)); a lane's
+//                operand, 8 k of its row, is one 16-byte read;
 //   along m, n   rows of one k each, 64-byte segments permuted by k mod 4; ds_read_b64_tr_b16 hands every lane 4 k of
 //                its column out of 4 rows.
 #pragma once
@@ -49,23 +49,25 @@ struct G16Matrix {
   int rows, cols;   // both in use; cols is a multiple of 8
 };
 
-// One operand's tile of ROWS rows (along m or n) x 64 k. KC: the matrix has k as its fast index.
+// One operand's tile of ROWS rows (along m or n) x BK k. KC: the matrix has k as its fast index.
 // PAIR (not KC): the ROWS columns are 32 of the first half of the matrix' columns, 32 of the second half, 32 of
 // the first, ...
-template <int ROWS, bool KC, bool PAIR, int NT>
+template <int ROWS, bool KC, bool PAIR, int NT, int BK = G16_BK>
 struct G16Side {
-  static constexpr int BYTES = ROWS * G16_BK * 2;
+  static constexpr int BYTES = ROWS * BK * 2;
   static constexpr int PER   = BYTES / (NT * 16);   // 16-byte loads a thread
   static_assert(BYTES % (NT * 16) == 0, "");
   const char *base;   // of the tile's k = 0
   unsigned off[PER];  // bytes from there, by load
+  // chunk c of row r lies at c ^ turn(r) (KC): the eight lanes that read at a time hit different banks
+  __device__ __forceinline__ static int turn(const int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
   __device__ __forceinline__ static int swizzle(const int k) { return ROWS >= 128 ? (k & 3) * 4 : ROWS == 64 ? ((k >> 1) & 1) * 4 : 0; }
   // where thread tid's load i lies: row of the tile and 16-byte chunk (of memory) in it
   __device__ __forceinline__ static void place(const int tid, const int i, int &row, int &chunk) {
     const int p = (i * NT + tid) * 16;
     if (KC) {
-      row   = p >> 7;
-      chunk = ((p >> 4) & 7) ^ (row & 7);
+      row   = p / (BK * 2);
+      chunk = ((p >> 4) & (BK / 8 - 1)) ^ turn(row);
     } else {
       row   = p / (ROWS * 2);                        // k
       chunk = ((p / 16) % (ROWS / 8)) ^ swizzle(row);
@@ -96,7 +98,7 @@ struct G16Side {
   // g16_arrived() returns (the compiler would wait for it before any read of LDS, so it is not told).
   __device__ __forceinline__ void fetch(const G16Matrix &mat, char *lds, const int k0, const int left, const int tid) const {
     const char *at = base + (KC ? 2L * k0 : 2L * k0 * mat.ld);
-    if (left >= G16_BK) {
+    if (left >= BK) {
       const uint64_t where = reinterpret_cast<uint64_t>(at);
       const g16_u32x4 desc = {static_cast<uint32_t>(where), static_cast<uint32_t>(where >> 32), 0xffffffffu, 0x00027000u};
       // (a wave's 64 lanes fill 1024 bytes of LDS from an address that is the same for all of them)
@@ -121,14 +123,14 @@ struct G16Side {
   // The operand of 32 rows from `row0` (a multiple of 32) and the 16 k of step s: lane l has row l % 32 and k
   // 8 (l / 32) .. + 7. `lane_off` is what lane_offset() gives for row0's 32 rows.
   __device__ __forceinline__ static int lane_offset(const int lane, const int row0) {
-    if (KC) return (row0 + (lane & 31)) * 128;
+    if (KC) return (row0 + (lane & 31)) * BK * 2;
     const int j = lane & 15, g = lane >> 4;
     const int k = 8 * (g >> 1) + (j >> 2), col = row0 + 16 * (g & 1) + 4 * (j & 3);
     return k * ROWS * 2 + (((col >> 3) ^ swizzle(k)) << 4) + (col & 7) * 2;
   }
   __device__ __forceinline__ static g16_s16x8 read(const char *lds, const int lane_off, const int lane, const int s) {
     if constexpr (KC) {
-      const int chunk = (2 * s + (lane >> 5)) ^ (lane & 7);
+      const int chunk = (2 * s + (lane >> 5)) ^ turn(lane & 31);
       return *reinterpret_cast<const g16_s16x8 *>(lds + lane_off + chunk * 16);
     } else {
       typedef __attribute__((address_space(3))) g16_s16x4 lds_vec;

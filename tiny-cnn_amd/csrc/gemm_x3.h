@@ -1,0 +1,131 @@
+// gemm_x3.h — the products of gemm16.h for fp32 matrices, in three bf16 parts (split_bf16.h) that lie split in memory.
+//
+// fc_x3.hip splits its operands on the way into LDS, once for every tile that reads them, which costs more vector
+// instructions than there are matrix instructions to hide them behind. Here every element is split once, by a pass of
+// its own that writes three planes (10 bytes moved an element), and tiles of 32 reduction indices of all three planes
+// go straight into LDS. Worth its pass where an operand is read by many tiles. One operand's planes carry the sign
+// of their step (split_bf16.h: steps take turns between the product and its negative).
+#pragma once
+#include "gemm16.h"
+#include "split_bf16.h"
+
+namespace tdh {
+namespace {
+
+constexpr int X3P_BK = 32;
+
+// The fp32 matrices themselves, for sums that come out infinite or NaN: element (m, k) at a[m am + k ak], (k, n) at
+// b[k bk + n bn]; rows and cols of C.
+struct X3Source {
+  const float *a, *b;
+  long am, ak, bk, bn;
+  int rows, cols;
+};
+
+template <int WM, int WN, bool A_KC, bool B_KC, bool PAIR, class Epi>
+__global__ void __launch_bounds__(64 * WM * WN)
+gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const X3Source src, const Epi epi,
+               const int tiles_m, const int tiles_n, const int K, const int k_per_split) {
+  constexpr int TM = 2, TN = 2, NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
+  using SideA = G16Side<BM, A_KC, false, NT, X3P_BK>;
+  using SideB = G16Side<BN, B_KC, PAIR, NT, X3P_BK>;
+  constexpr int STAGE = X3_PARTS * (SideA::BYTES + SideB::BYTES);
+  __shared__ __align__(1024) char lds[2][STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
+  const int tiles = tiles_m * tiles_n;
+  int id = xcd_compact_id(blockIdx.x, gridDim.x);
+  const int split = id / tiles;
+  id -= split * tiles;
+  int tm, tn;
+  g16_tile(id, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * BM, n0 = tn * (PAIR ? BN / 2 : BN);
+  const int kbeg = split * k_per_split, kend = min(K, kbeg + k_per_split);
+
+  SideA sa;
+  SideB sb;
+  sa.plan(A, m0, tid);
+  sb.plan(B, n0, tid);
+  floatx16_x3 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx16_x3{};
+  int oa[TM], ob[TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) oa[i] = SideA::lane_offset(lane, 32 * (wm * TM + i));
+#pragma unroll
+  for (int j = 0; j < TN; ++j) ob[j] = X3_PARTS * SideA::BYTES + SideB::lane_offset(lane, 32 * (wn * TN + j));
+  auto fetch = [&](int buf, int k0) {
+#pragma unroll
+    for (int p = 0; p < X3_PARTS; ++p) {
+      SideA a = sa;
+      SideB b = sb;
+      a.base += 2 * p * a_plane;
+      b.base += 2 * p * b_plane;
+      a.fetch(A, lds[buf] + p * SideA::BYTES, k0, kend - k0, tid);
+      b.fetch(B, lds[buf] + X3_PARTS * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
+    }
+  };
+  if (kbeg < kend) fetch(0, kbeg);
+  int buf = 0;
+#pragma unroll 1
+  for (int k0 = kbeg; k0 < kend; k0 += X3P_BK, buf ^= 1) {
+    g16_arrived<0>();
+    __syncthreads();   // this tile has arrived, and everyone has read the one before
+    if (k0 + X3P_BK < kend) fetch(buf ^ 1, k0 + X3P_BK);
+    bf16x8 a[2][TM][X3_PARTS], b[2][TN][X3_PARTS];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int p = 0; p < X3_PARTS; ++p) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          a[s][i][p] = __builtin_bit_cast(bf16x8, SideA::read(lds[buf] + p * SideA::BYTES, oa[i], lane, s));
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          b[s][j][p] = __builtin_bit_cast(bf16x8, SideB::read(lds[buf] + p * SideB::BYTES, ob[j], lane, s));
+      }
+    mfma_x3<TM, TN, 2>(acc, a, b, k0 / X3P_BK & 1 ? -1.0f : 1.0f);
+  }
+  const int mw = m0 + 32 * TM * wm, nw = n0 + (PAIR ? 16 * TN * wn : 32 * TN * wn);
+  const int half = lane >> 5, l32 = lane & 31;
+  // the infinite and NaN sums once more in fp32: lane l brings row and column l % 32 of the blocks at index k + l / 32
+  {
+    int col[TN];   // (PAIR: of either half)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int hidden = src.cols >> 1, n = PAIR ? nw + 32 * (j >> 1) + l32 : nw + 32 * j + l32;
+      col[j] = n < (PAIR ? hidden : src.cols) ? n + (PAIR ? (j & 1) * hidden : 0) : -1;
+    }
+    x3_redo(reinterpret_cast<floatx16_x3(&)[TM * TN]>(acc), [&](int b, int r) {
+      return mw + 32 * (b / TN) + 8 * (r >> 2) + 4 * half + (r & 3) < src.rows && col[b % TN] >= 0;
+    }, [&](floatx16_x3 (&sum)[TM * TN]) {
+#pragma unroll 1
+      for (int k0 = kbeg; k0 < kend; k0 += 8) {
+        float av[4][TM], bv[4][TN];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int k = k0 + 2 * s + half;
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const int m = mw + 32 * i + l32;
+            av[s][i] = k < kend && m < src.rows ? src.a[m * src.am + k * src.ak] : 0.0f;
+          }
+#pragma unroll
+          for (int j = 0; j < TN; ++j) bv[s][j] = k < kend && col[j] >= 0 ? src.b[k * src.bk + col[j] * src.bn] : 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int b = 0; b < TM * TN; ++b) sum[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[s][b / TN], bv[s][b % TN], sum[b], 0, 0, 0);
+        if (x3_all_nan(sum)) return;
+      }
+    });
+  }
+  static_assert(sizeof(lds) >= WM * WN * G16Turn<32 * TN>::BYTES, "");
+  __syncthreads();
+  epi.template done<TM, TN>(acc, mw, nw, lane, split, reinterpret_cast<float *>(lds[0] + wave * G16Turn<32 * TN>::BYTES));
+}
+
+}  // namespace
+}  // namespace tdh

@@ -72,6 +72,27 @@ __device__ __forceinline__ void store_word16(void *p, const uint4 v) {
     *static_cast<uint4 *>(p) = v;
 }
 
+// Eight neighbours on a 16-byte boundary.
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8 / Word<T>::N; ++q) {
+    const Word<T> w{reinterpret_cast<const uint4 *>(p)[q]};
+#pragma unroll
+    for (int e = 0; e < Word<T>::N; ++e) v[q * Word<T>::N + e] = w[e];
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8 / Word<T>::N; ++q) {
+    float w[Word<T>::N];
+#pragma unroll
+    for (int e = 0; e < Word<T>::N; ++e) w[e] = v[q * Word<T>::N + e];
+    reinterpret_cast<uint4 *>(p)[q] = Word<T>::from(w).raw;
+  }
+}
+
 inline bool dtype_known(int dtype) { return dtype == TDH_F32 || dtype == TDH_BF16 || dtype == TDH_F16; }
 inline size_t dtype_size(int dtype) { return dtype == TDH_F32 ? 4 : 2; }
 
