@@ -936,16 +936,19 @@ struct Splitter {
   }
 };
 
-// Tiles of 256 x 128, split along k where they do not fill the compute units.
-constexpr int X3P_BM = 256, X3P_BN = 128;
+// Tiles of 128 x 128, split along k where they do not fill the compute units: 2.55 us a tile of 32 indices with two workgroups a
+// compute unit, 2.3 with one (whose loads nothing covers), and 5 a round.
+constexpr int X3P_TILE = 128;
 FfPlan x3_plan(int M, int N, int K) {
-  const long cus   = ctx().compute_units > 0 ? ctx().compute_units : 256, tiles = static_cast<long>(ceil_div(M, X3P_BM)) * ceil_div(N, X3P_BN);
+  const long cus   = ctx().compute_units > 0 ? ctx().compute_units : 256, tiles = static_cast<long>(ceil_div(M, X3P_TILE)) * ceil_div(N, X3P_TILE);
   const int ktiles = std::max(1, ceil_div(K, X3P_BK));
   FfPlan best{0, 1, ktiles * X3P_BK};
   double best_us = 1e30;
   for (int want = 1; want <= 16 && want <= ktiles; ++want) {
     const int per = ceil_div(ktiles, want), splits = ceil_div(ktiles, per);
-    double us = static_cast<double>(ceil_div_sz(tiles * splits, cus)) * (per * 1.7 + 8.0);
+    const long groups = tiles * splits, rest = groups % (2 * cus);
+    double us = static_cast<double>(groups / (2 * cus)) * (per * 2.55 + 5.0);
+    if (rest) us += per * (rest > cus ? 2.55 : 2.3) + 5.0;
     if (splits > 1) us += 3.0 + 8.0 * splits * M * N / 8e6;
     if (us < best_us) {
       best_us = us;
@@ -957,8 +960,8 @@ FfPlan x3_plan(int M, int N, int K) {
 template <bool A_KC, bool B_KC, bool PAIR, class Epi>
 int x3_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const X3Source &src, const Epi &epi, int K, const char *tag) {
   ProfScope prof(tag, src.rows, src.cols, K);
-  const int tiles_m = ceil_div(src.rows, X3P_BM), tiles_n = PAIR ? ceil_div(src.cols / 2, X3P_BN / 2) : ceil_div(src.cols, X3P_BN);
-  TDH_LAUNCH((gemm_x3_kernel<4, 2, A_KC, B_KC, PAIR, Epi>), dim3(static_cast<unsigned>(tiles_m) * tiles_n * p.splits), dim3(512), 0,
+  const int tiles_m = ceil_div(src.rows, X3P_TILE), tiles_n = PAIR ? ceil_div(src.cols / 2, X3P_TILE / 2) : ceil_div(src.cols, X3P_TILE);
+  TDH_LAUNCH((gemm_x3_kernel<A_KC, B_KC, PAIR, Epi>), dim3(static_cast<unsigned>(tiles_m) * tiles_n * p.splits), dim3(256), 0,
              ctx().stream, A, B, static_cast<long>(A.rows) * A.cols, static_cast<long>(B.rows) * B.cols, src, epi, tiles_m, tiles_n, K,
              p.k_per_split);
   TDH_LAUNCH_CHECK();
@@ -973,12 +976,15 @@ int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad
   return plan.splits > 1 ? launch_grad_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
 }
 
-// Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do.
+// Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do. us of a
+// training step on them and on the fully-connected layer's products: 1024 -> 2 x 2048, 1200 samples 271 / 272, 2400 463 / 473; 1344
+// -> 2 x 2640, 800 samples 307 / 305, 2000 633 / 681; numbers of samples that are no multiple of four, for which that
+// layer's three-part products do not apply: 801 208 / 255, 1601 330 / 447.
 bool x3_fits(int in, int hidden) { return in % 8 == 0 && hidden % 8 == 0; }
-constexpr int X3P_BATCH = 768, X3P_DW_BATCH = 128;
+constexpr int X3P_BATCH = 1000, X3P_BATCH_ODD = 320, X3P_DW_BATCH = 128;
 constexpr double X3P_FLOP = 4e9;   // below that the products are short
 bool x3_weights(int in, int hidden, int batch) {
-  return x3_fits(in, hidden) && batch >= X3P_BATCH && 4.0 * batch * in * hidden >= X3P_FLOP;
+  return x3_fits(in, hidden) && batch >= (batch % 4 ? X3P_BATCH_ODD : X3P_BATCH) && 4.0 * batch * in * hidden >= X3P_FLOP;
 }
 bool x3_dw(int in, int hidden, int batch) { return x3_fits(in, hidden) && batch >= X3P_DW_BATCH && 4.0 * batch * in * hidden >= X3P_FLOP; }
 

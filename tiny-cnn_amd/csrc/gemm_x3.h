@@ -5,6 +5,12 @@
 // its own that writes three planes (10 bytes moved an element), and tiles of 32 reduction indices of all three planes
 // go straight into LDS. Worth its pass where an operand is read by many tiles. One operand's planes carry the sign
 // of their step (split_bf16.h: steps take turns between the product and its negative).
+//
+// Tiles of 128 x 128 on four waves, one of them in LDS at a time (48 KB), two workgroups a compute unit that cover each
+// other's loads and epilogues: 4096 x 8192 with k of 256 in 102 us, 4096 x 4096 with k of 2048 in 314 (m, n), 351 (k, k)
+// and 336 us (k, n), 196 to 219 TFLOP/s. 256 x 128 on eight waves with the next tile on its way in a second buffer,
+// one workgroup a compute unit: 128, 339, 359, 346; operands of 16 indices at a time and three workgroups: 99, 347, 382, 367.
+// Bound by the matrix cores at the power limit, and in short sums by what a round of workgroups writes.
 #pragma once
 #include "gemm16.h"
 #include "split_bf16.h"
@@ -22,15 +28,15 @@ struct X3Source {
   int rows, cols;
 };
 
-template <int WM, int WN, bool A_KC, bool B_KC, bool PAIR, class Epi>
-__global__ void __launch_bounds__(64 * WM * WN)
+template <bool A_KC, bool B_KC, bool PAIR, class Epi>
+__global__ void __launch_bounds__(256, 2)
 gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const X3Source src, const Epi epi,
                const int tiles_m, const int tiles_n, const int K, const int k_per_split) {
-  constexpr int TM = 2, TN = 2, NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
+  constexpr int WM = 2, WN = 2, TM = 2, TN = 2, NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
   using SideA = G16Side<BM, A_KC, false, NT, X3P_BK>;
   using SideB = G16Side<BN, B_KC, PAIR, NT, X3P_BK>;
   constexpr int STAGE = X3_PARTS * (SideA::BYTES + SideB::BYTES);
-  __shared__ __align__(1024) char lds[2][STAGE];
+  __shared__ __align__(1024) char lds[STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
   const int tiles = tiles_m * tiles_n;
   int id = xcd_compact_id(blockIdx.x, gridDim.x);
@@ -55,24 +61,23 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
   for (int i = 0; i < TM; ++i) oa[i] = SideA::lane_offset(lane, 32 * (wm * TM + i));
 #pragma unroll
   for (int j = 0; j < TN; ++j) ob[j] = X3_PARTS * SideA::BYTES + SideB::lane_offset(lane, 32 * (wn * TN + j));
-  auto fetch = [&](int buf, int k0) {
+  auto fetch = [&](int k0) {
 #pragma unroll
     for (int p = 0; p < X3_PARTS; ++p) {
       SideA a = sa;
       SideB b = sb;
       a.base += 2 * p * a_plane;
       b.base += 2 * p * b_plane;
-      a.fetch(A, lds[buf] + p * SideA::BYTES, k0, kend - k0, tid);
-      b.fetch(B, lds[buf] + X3_PARTS * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
+      a.fetch(A, lds + p * SideA::BYTES, k0, kend - k0, tid);
+      b.fetch(B, lds + X3_PARTS * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
     }
   };
-  if (kbeg < kend) fetch(0, kbeg);
-  int buf = 0;
 #pragma unroll 1
-  for (int k0 = kbeg; k0 < kend; k0 += X3P_BK, buf ^= 1) {
+  for (int k0 = kbeg; k0 < kend; k0 += X3P_BK) {
+    __syncthreads();   // everyone has read the tile before
+    fetch(k0);
     g16_arrived<0>();
-    __syncthreads();   // this tile has arrived, and everyone has read the one before
-    if (k0 + X3P_BK < kend) fetch(buf ^ 1, k0 + X3P_BK);
+    __syncthreads();
     bf16x8 a[2][TM][X3_PARTS], b[2][TN][X3_PARTS];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -80,10 +85,10 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
       for (int p = 0; p < X3_PARTS; ++p) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
-          a[s][i][p] = __builtin_bit_cast(bf16x8, SideA::read(lds[buf] + p * SideA::BYTES, oa[i], lane, s));
+          a[s][i][p] = __builtin_bit_cast(bf16x8, SideA::read(lds + p * SideA::BYTES, oa[i], lane, s));
 #pragma unroll
         for (int j = 0; j < TN; ++j)
-          b[s][j][p] = __builtin_bit_cast(bf16x8, SideB::read(lds[buf] + p * SideB::BYTES, ob[j], lane, s));
+          b[s][j][p] = __builtin_bit_cast(bf16x8, SideB::read(lds + p * SideB::BYTES, ob[j], lane, s));
       }
     mfma_x3<TM, TN, 2>(acc, a, b, k0 / X3P_BK & 1 ? -1.0f : 1.0f);
   }
@@ -124,7 +129,7 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
   }
   static_assert(sizeof(lds) >= WM * WN * G16Turn<32 * TN>::BYTES, "");
   __syncthreads();
-  epi.template done<TM, TN>(acc, mw, nw, lane, split, reinterpret_cast<float *>(lds[0] + wave * G16Turn<32 * TN>::BYTES));
+  epi.template done<TM, TN>(acc, mw, nw, lane, split, reinterpret_cast<float *>(lds + wave * G16Turn<32 * TN>::BYTES));
 }
 
 }  // namespace
