@@ -407,6 +407,13 @@ int tdh_net_set_phase(tdh_net *net, int train);
  * sample after sample, tiny_dnn/layers/dropout_layer.h:99-102), once per train step. The copy
  * is queued on the library stream, behind the kernels of the step before. */
 int tdh_net_set_dropout_mask(tdh_net *net, int layer, int batch, const uint8_t *host_mask);
+/* From now on dropout layer `layer` draws its masks itself, on the device (until tdh_net_set_dropout_mask hands it one
+ * again): pass number p behind this call, counting train steps and forward passes in the train phase, does what
+ * tdh_dropout_seeded_fwd and tdh_dropout_seeded_bwd do with (seed, offset + p), so the layer drops a share dropout_rate and scales
+ * both ways. Nothing is uploaded between the steps, a captured step draws another mask at every replay, and
+ * tdh_net_train_steps takes such a net. Layers of one net get seeds of their own, or offsets far apart. It has no
+ * counterpart in the reference. */
+int tdh_net_set_dropout_generator(tdh_net *net, int layer, uint64_t seed, uint64_t offset);
 /* nodes::update_weights (tiny_dnn/nodes.h:103-107): layer::update_weight of every layer, front
  * to back, weight before bias, on the gradients accumulated since the last update, which are
  * then cleared (tiny_dnn/layers/layer.h:663-682). What tdh_net_train_step does with
@@ -447,8 +454,8 @@ int tdh_net_train_step(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, con
  * batches are on the device already. The results are those of n_steps calls of
  * tdh_net_train_step; with TDH_NET_GRAPH the steps are captured into one graph, so a replay
  * starts once for all of them (a few microseconds each time, which is a tenth of a LeNet-5
- * step). A net with a dropout layer in the train phase is refused: its masks change between
- * the steps (tdh_net_set_dropout_mask). */
+ * step). A net with a dropout layer in the train phase is refused, unless that layer draws
+ * its masks itself (tdh_net_set_dropout_generator): handed-over masks change between the steps. */
 int tdh_net_train_steps(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, int n_steps,
                         const float *const *x, const float *const *t);
 

@@ -622,3 +622,113 @@ def test_training_step_of_the_operators_together(T, dtype):
         e = np.zeros_like(w1)
         e[i] = 1e-6
         assert abs((loss_of(x, w1 + e, b1) - loss_of(x, w1 - e, b1)) / 2e-6 - ddw[i]) < 1e-5 * (1 + abs(ddw[i]))
+
+
+# --------------------------------------- dropout layers that draw for themselves
+
+def dropout_net(T, flags, batch, rng):
+    """fc - tanh - dropout - fc - dropout - fc under mse, with set weights"""
+    net = T.Net([T.L_fc(12, 37), T.L_act("tanh"), T.L_dropout(0.3), T.L_fc(37, 21), T.L_dropout(0.6), T.L_fc(21, 5)], batch, flags)
+    for i, which, n in net.params():
+        net.set_param(i, which, (rng.randn(n) / 4).astype(np.float32))
+    return net
+
+
+def check_dropout_step(net, batch, seeds, p):
+    """Both dropout layers of the last step against the masks of pass p, forward and backward."""
+    for layer, rate in ((2, 0.3), (4, 0.6)):
+        n = batch * net.layer_out_size(layer)
+        keep = L.kept(n, rate, *[seeds[layer][0], seeds[layer][1] + p]).reshape(batch, -1)
+        scale = 1 / (1 - np.float64(np.float32(rate)))
+        x, y = net.layer_out(layer - 1, batch), net.layer_out(layer, batch)
+        L.within(y, x.astype(np.float64) * keep * scale, 2.0 ** -22 * np.abs(x) * scale, f"layer {layer}, pass {p}")
+        dy, dx = net.layer_dx(layer + 1, batch), net.layer_dx(layer, batch)
+        L.within(dx, dy.astype(np.float64) * keep * scale, 2.0 ** -22 * np.abs(dy) * scale, f"layer {layer}, pass {p}, backward")
+
+
+@pytest.mark.parametrize("flags", [0, 1, 2, 3, 7])
+def test_net_draws_its_dropout_masks(T, flags):
+    """Another mask every pass, with and without a captured step (each of them replayed, with other work between the
+    replays); several steps a call are the single steps; the test phase is the identity and draws nothing; a mask
+    that is handed over takes the generator's place until the next one is set."""
+    batch, rng = 9, np.random.RandomState(3)
+    x, t = T.to_device(rng.randn(batch, 12)), T.to_device(rng.randn(batch, 5))
+    seeds = {2: (77, 1000), 4: (1 << 63, 0)}
+    net, twin = dropout_net(T, flags, batch, np.random.RandomState(4)), dropout_net(T, 0, batch, np.random.RandomState(4))
+    opt, topt = T.opt_desc("momentum"), T.opt_desc("momentum")
+    with pytest.raises(T.TdhError, match="one step a call"):
+        net.train_steps(opt, "mse", batch, [x, x], [t, t])
+    for n in (net, twin):
+        for layer, (seed, offset) in seeds.items():
+            n.set_dropout_generator(layer, seed, offset)
+    for p in range(5):
+        net.train_step(opt, "mse", batch, x, t)
+        check_dropout_step(net, batch, seeds, p)
+        T.sync()
+        T.fill_zero(T.DevBuf(1000))
+    net.forward(batch, x)                      # pass 5
+    keep = L.kept(batch * 37, 0.3, 77, 1005).reshape(batch, -1)
+    assert np.array_equal(net.layer_out(2, batch) != 0, keep)
+    net.set_phase(False)
+    net.forward(batch, x)
+    assert np.array_equal(net.layer_out(2, batch), net.layer_out(1, batch))
+    net.set_phase(True)
+    net.train_steps(opt, "mse", batch, [x] * 4, [t] * 4)   # passes 6 to 9
+    check_dropout_step(net, batch, seeds, 9)
+    net.train_steps(opt, "mse", batch, [x] * 4, [t] * 4)   # and 10 to 13, the same graph again
+    check_dropout_step(net, batch, seeds, 13)
+    for p in range(14):
+        if p == 5:
+            twin.forward(batch, x)
+        else:
+            twin.train_step(topt, "mse", batch, x, t)
+    for i, which, _ in net.params():
+        L.within(net.get_param(i, which), twin.get_param(i, which), 2e-6 if flags else 0.0, f"parameter {i}.{which}")
+    mask = np.ones((batch, 37), np.uint8)
+    net.set_dropout_mask(2, mask)
+    net.train_step(opt, "mse", batch, x, t)
+    a, b = net.layer_out(1, batch), net.layer_out(2, batch)
+    L.within(b, a / (1 - 0.3), 2.0 ** -21 * np.abs(a), "a mask that was handed over")
+    with pytest.raises(T.TdhError, match="one step a call"):
+        net.train_steps(opt, "mse", batch, [x, x], [t, t])
+    net.set_dropout_generator(2, 77, 0)
+    net.train_step(opt, "mse", batch, x, t)
+    assert np.array_equal(net.layer_out(2, batch) != 0, L.kept(batch * 37, 0.3, 77, 0).reshape(batch, -1))
+    with pytest.raises(T.TdhError):
+        net.set_dropout_generator(1, 77)       # not a dropout layer
+    with pytest.raises(T.TdhError):
+        net.set_dropout_generator(6, 77)
+    net.close()
+    twin.close()
+
+
+def test_gradient_of_a_net_that_draws_its_dropout_masks(T):
+    """Against differences of its own loss, the mask held by setting the same offset again."""
+    batch, rng = 6, np.random.RandomState(8)
+    x, t = T.to_device(rng.randn(batch, 12)), rng.randn(batch, 5)
+    net = dropout_net(T, 0, batch, np.random.RandomState(9))
+
+    def again():
+        net.set_dropout_generator(2, 5, 50)
+        net.set_dropout_generator(4, 6, 60)
+
+    def loss():
+        again()
+        net.forward(batch, x)
+        return np.sum((net.layer_out(5, batch).astype(np.float64) - t) ** 2) / 5   # mse::df is 2 (y - t) / n
+
+    again()
+    net.train_step(None, "mse", batch, x, T.to_device(t), do_update=False)
+    for i, which, n in net.params():
+        grad, w = net.layer_grad(i, which), net.get_param(i, which)
+        for k in (0, n // 2, n - 1):
+            e = np.zeros(n, np.float32)
+            e[k] = 2.0 ** -6
+            net.set_param(i, which, w + e)
+            up = loss()
+            net.set_param(i, which, w - e)
+            down = loss()
+            net.set_param(i, which, w)
+            # third derivatives times (2^-6)^2 / 6, and fp32 outputs of order 1
+            assert abs((up - down) * 32 - grad[k]) < 2e-3 * (1 + abs(grad[k])), (i, which, k)
+    net.close()

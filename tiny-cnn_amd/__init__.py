@@ -685,6 +685,11 @@ class Net:
         check(lib().tdh_net_set_dropout_mask(self.h, i, mask.shape[0], mask.ctypes.data_as(C.c_void_p)),
               "tdh_net_set_dropout_mask")
 
+    def set_dropout_generator(self, i, seed, offset=0):
+        """Dropout layer i draws its masks on the device: pass p behind this call those of (seed, offset + p)"""
+        check(lib().tdh_net_set_dropout_generator(self.h, i, C.c_uint64(seed), C.c_uint64(offset)),
+              "tdh_net_set_dropout_generator")
+
     def update_weights(self, opt):
         check(lib().tdh_net_update_weights(self.h, C.byref(opt)), "tdh_net_update_weights")
 

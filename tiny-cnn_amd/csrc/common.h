@@ -328,6 +328,11 @@ int dropout_fwd(size_t total, int train, float scale, const uint8_t *mask, const
 int dropout_bwd(size_t total, const uint8_t *mask, const float *dy, float *dx);
 // act: tanh, relu or sigmoid, with outputs y
 int dropout_act_bwd(size_t total, const uint8_t *mask, const float *dy, float *dx, int act, const float *y, float *act_dx);
+// seeded_dropout.hip: y = [residual +] dropout(x) with the mask of (seed, offset), or of state[0], state[1] (device memory,
+// so that a captured launch draws another mask at every replay); and the offsets of n states counted up by one
+int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offset, const uint64_t *state, const void *x,
+                   const void *residual, void *y, const char *tag);
+int seeded_dropout_advance(uint64_t *state, int n);
 size_t rowsum_workspace_bytes(int outer, int rows, int cols);
 // out[c] (+)= sum_s src[s*cols + c]
 int launch_colsum(const float *src, int rows, int cols, float *out, int accumulate);

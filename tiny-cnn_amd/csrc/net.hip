@@ -37,6 +37,8 @@ struct tdh_net {
     float *bn_mean = nullptr, *bn_var = nullptr, *bn_mean_cur = nullptr, *bn_var_cur = nullptr,
           *bn_stddev = nullptr;
     uint8_t *mask = nullptr;  // [max_batch][out_size]
+    uint64_t *generator = nullptr;   // dropout: {seed, offset} of its own generator, in device memory
+    bool generates = false;          // ... which draws its masks
   };
   std::vector<Layer> layers;
   int max_batch  = 0;
@@ -70,6 +72,7 @@ struct tdh_net {
     int n_steps = 1;
     const float *x[kMaxSteps] = {}, *t[kMaxSteps] = {};
     const void *scratch = nullptr;      // the library scratch buffer the captured kernels use
+    uint64_t mask_sources = 0;
     tdh_opt hyper = {};                 // hyper-parameters only (powers zeroed)
   };
   // Captured steps are kept, so that rotating input buffers or batch sizes (the short last batch
@@ -84,6 +87,9 @@ struct tdh_net {
     std::vector<uint8_t> dx_unwritten, out_unwritten;  // what the captured step leaves in the net's fields of those names
   } graphs[kGraphSlots];
   uint64_t graph_clock = 0;
+  uint64_t *generators = nullptr;   // of all dropout layers, one behind the other
+  int n_generators     = 0;
+  uint64_t mask_sources = 0;        // counts up when a dropout layer's masks come from elsewhere than before
   // per layer: the last step kept the gradient with respect to this layer's input in registers
   // or read it through a pool (tdh_net_layer_dx has nothing to show)
   std::vector<uint8_t> dx_unwritten;
@@ -744,6 +750,11 @@ int forward(tdh_net *net, int batch, const float *x, const float *xent_t = nullp
                               L.out));
       } break;
       case TDH_L_DROPOUT:      // dropout_layer.h:84-117
+        if (L.generates && !net->test_phase) {
+          TDH_TRY(seeded_dropout(TDH_F32, L.out_size * static_cast<size_t>(batch), s.dropout_rate, 0, 0, L.generator, in, nullptr, L.out,
+                                 "dropout_seeded_fwd"));
+          break;
+        }
         TDH_TRY(dropout_fwd(L.out_size * static_cast<size_t>(batch), !net->test_phase,
                             1.0f / (1.0f - s.dropout_rate), L.mask, in, L.out));
         break;
@@ -833,6 +844,7 @@ int tdh_net_create(const tdh_layer *layers, int n_layers, int max_batch, int fla
       float *p = nullptr;
       if ((rc = net_alloc(net, ceil_div_sz(act, sizeof(float)), &p, true))) break;
       L.mask = reinterpret_cast<uint8_t *>(p);
+      ++net->n_generators;
     }
     if (L.spec.kind == TDH_L_CONV && L.spec.conv.w_stride == 1 && L.spec.conv.h_stride == 1) {
       // (one buffer: an allocation takes the host some 100 us)
@@ -951,6 +963,17 @@ int tdh_net_create(const tdh_layer *layers, int n_layers, int max_batch, int fla
         net->events.push_back(e);
     }
   }
+  if (rc == TDH_OK && net->n_generators) {
+    float *p = nullptr;
+    rc = net_alloc(net, 4 * static_cast<size_t>(net->n_generators), &p, true);
+    net->generators = reinterpret_cast<uint64_t *>(p);
+    uint64_t *at    = net->generators;
+    for (tdh_net::Layer &L : net->layers)
+      if (rc == TDH_OK && L.spec.kind == TDH_L_DROPOUT) {
+        L.generator = at;
+        at += 2;
+      }
+  }
   if (rc == TDH_OK) rc = build_tiny_plan(net);
   // reserve the scratch every layer may need, so that no op ever has to grow it
   if (rc == TDH_OK) rc = ws_begin(net->scratch);
@@ -1051,7 +1074,26 @@ int tdh_net_set_dropout_mask(tdh_net *net, int layer, int batch, const uint8_t *
                   net->layers[layer].spec.kind == TDH_L_DROPOUT && batch > 0 && batch <= net->max_batch,
                 "tdh_net_set_dropout_mask: bad argument");
   tdh_net::Layer &L = net->layers[layer];
+  if (L.generates) ++net->mask_sources;
+  L.generates = false;
   return tdh_memcpy_h2d(L.mask, host_mask, L.out_size * static_cast<size_t>(batch));
+}
+int tdh_net_set_dropout_generator(tdh_net *net, int layer, uint64_t seed, uint64_t offset) {
+  TDH_REQUIRE_INIT();
+  TDH_CHECK_ARG(net && layer >= 0 && layer < static_cast<int>(net->layers.size()) && net->layers[layer].spec.kind == TDH_L_DROPOUT,
+                "tdh_net_set_dropout_generator: bad argument");
+  tdh_net::Layer &L = net->layers[layer];
+  if (!L.generates) ++net->mask_sources;
+  L.generates            = true;
+  const uint64_t state[2] = {seed, offset};
+  return tdh_memcpy_h2d(L.generator, state, sizeof(state));
+}
+// behind a pass of the train phase that drew masks: the next one draws others
+static int advance_generators(tdh_net *net) {
+  if (net->test_phase) return TDH_OK;
+  for (const tdh_net::Layer &L : net->layers)
+    if (L.generates) return seeded_dropout_advance(net->generators, net->n_generators);
+  return TDH_OK;
 }
 int tdh_net_clear_grads(tdh_net *net) {
   TDH_REQUIRE_INIT();
@@ -1099,7 +1141,8 @@ int tdh_net_forward(tdh_net *net, int batch, const float *x) {
   TDH_CHECK_ARG(net && x && batch > 0 && batch <= net->max_batch, "tdh_net_forward: bad argument");
   distrust_copies(net);
   TDH_TRY(pack_copies(net, batch, x, /*training=*/false, /*leave=*/true));
-  return forward(net, batch, x);
+  TDH_TRY(forward(net, batch, x));
+  return advance_generators(net);
 }
 
 // Queues one whole train step on the library stream. forked (only while the stream is being
@@ -1447,6 +1490,11 @@ static int enqueue_step(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, co
         break;
       case TDH_L_DROPOUT:    // dropout_layer.h:62-82
         if (fold.kind != TDH_ACT_NONE) return set_error(TDH_ERR_INVALID, "dropout behind a folded activation");
+        if (L.generates && !net->test_phase) {
+          TDH_TRY(seeded_dropout(TDH_F32, L.out_size * static_cast<size_t>(batch), s.dropout_rate, 0, 0, L.generator, L.dout, nullptr, dx,
+                                 "dropout_seeded_bwd"));
+          break;
+        }
         if (const tdh_net::Layer &A = net->layers[i - 1]; A.spec.kind == TDH_L_ACT && is_pointwise_act(A.spec.act) && !A.grad_folded) {
           // the activation in front leaves the same kernel
           const DxTarget through = dx_target(net, i - 1);
@@ -1512,7 +1560,7 @@ static bool same_key(const tdh_net::GraphKey &a, const tdh_net::GraphKey &b) {
   const tdh_opt &p = a.hyper, &q = b.hyper;
   return a.batch == b.batch && a.loss == b.loss && a.do_update == b.do_update && a.test_phase == b.test_phase &&
          a.powers_at == b.powers_at && a.n_steps == b.n_steps && a.packs == b.packs &&
-         std::equal(a.x, a.x + a.n_steps, b.x) && std::equal(a.t, a.t + a.n_steps, b.t) && a.scratch == b.scratch && p.kind == q.kind && p.alpha == q.alpha &&
+         std::equal(a.x, a.x + a.n_steps, b.x) && std::equal(a.t, a.t + a.n_steps, b.t) && a.scratch == b.scratch && a.mask_sources == b.mask_sources && p.kind == q.kind && p.alpha == q.alpha &&
          p.lambda == q.lambda && p.mu == q.mu && p.b1 == q.b1 && p.b2 == q.b2 && p.eps == q.eps;
 }
 
@@ -1534,6 +1582,7 @@ static int train_steps(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, int
     for (int s = 0; s < n_steps; ++s) {
       if (net->flags & TDH_NET_GRAPH) TDH_TRY(ws_begin(net->scratch));
       TDH_TRY(enqueue_step(net, opt, loss_kind, batch, xs[s], ts[s], do_update, nullptr, nullptr, keeps(s)));
+      TDH_TRY(advance_generators(net));
     }
     return TDH_OK;
   }
@@ -1555,6 +1604,7 @@ static int train_steps(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, int
   }
   TDH_TRY(ws_begin(net->scratch));  // may move the scratch buffer if another op outgrew it
   key.scratch = ctx().workspace;
+  key.mask_sources = net->mask_sources;
   tdh_net::GraphSlot *slot = nullptr;
   for (auto &g : net->graphs)
     if (g.exec && same_key(key, g.key)) slot = &g;
@@ -1587,6 +1637,7 @@ static int train_steps(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, int
         rc = enqueue_step(net, opt ? &capture_opt : nullptr, loss_kind, batch, xs[s], ts[s], do_update,
                           net->dev_powers + 4 * at, net->dev_powers + 4 * (1 - at), keeps(s),
                           /*forked=*/net_forks(net, batch));
+        if (rc == TDH_OK) rc = advance_generators(net);
       }
       e = hipStreamEndCapture(c.stream, &graph);
     }
@@ -1656,9 +1707,9 @@ int tdh_net_train_steps(tdh_net *net, tdh_opt *opt, int loss_kind, int batch, in
                 n_steps <= tdh_net::kMaxSteps, "tdh_net_train_steps: bad argument (1 to %d steps a call)",
                 tdh_net::kMaxSteps);
   for (int s = 0; s < n_steps; ++s) TDH_CHECK_ARG(x[s] && t[s], "tdh_net_train_steps: null batch %d", s);
-  // a dropout layer's masks are handed over once per step, between the steps
+  // a dropout layer's masks are handed over once per step, between the steps, unless it draws them itself
   for (const tdh_net::Layer &L : net->layers)
-    TDH_CHECK_ARG(L.spec.kind != TDH_L_DROPOUT || net->test_phase,
+    TDH_CHECK_ARG(L.spec.kind != TDH_L_DROPOUT || L.generates || net->test_phase,
                   "tdh_net_train_steps: a net with a dropout layer trains one step a call");
   return train_steps(net, opt, loss_kind, batch, n_steps, x, t, 1);
 }

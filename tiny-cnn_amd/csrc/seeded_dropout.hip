@@ -41,9 +41,9 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], const uint64_t block, c
 template <class T, bool VEC, bool RES>
 __global__ void __launch_bounds__(SD_NT)
 seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const uint32_t threshold, const float scale,
-                      const uint64_t seed, const uint64_t offset0, const uint64_t *__restrict__ step) {
+                      const uint64_t seed_arg, const uint64_t offset_arg, const uint64_t *__restrict__ state) {
   constexpr int E = VEC ? Word<T>::N : 4;   // elements a thread takes at a time
-  const uint64_t offset = offset0 + (step ? *step : 0);
+  const uint64_t seed = state ? state[0] : seed_arg, offset = state ? state[1] : offset_arg;
   const size_t items = (n + E - 1) / E, stride = static_cast<size_t>(gridDim.x) * SD_NT;
   for (size_t i = static_cast<size_t>(blockIdx.x) * SD_NT + threadIdx.x; i < items; i += stride) {
     const size_t at = i * E;
@@ -72,9 +72,13 @@ seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const
   }
 }
 
+__global__ void advance_kernel(uint64_t *state, const int n) {
+  for (int i = threadIdx.x; i < n; i += 64) ++state[2 * i + 1];
+}
+
 }  // namespace
 
-int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offset, const uint64_t *step, const void *x,
+int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offset, const uint64_t *state, const void *x,
                    const void *residual, void *y, const char *tag) {
   const size_t size = dtype_size(dtype);
   ProfScope prof(tag, static_cast<double>(size) * n * (residual ? 3 : 2), WORK_BYTE);
@@ -87,13 +91,20 @@ int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offs
     const dim3 grid(static_cast<unsigned>(std::min<size_t>(ceil_div_sz(items, SD_NT), GRID_X_MAX)));
     auto go = [&](auto kernel) {
       TDH_LAUNCH(kernel, grid, dim3(SD_NT), 0, ctx().stream, static_cast<const T *>(x), static_cast<const T *>(residual),
-                 static_cast<T *>(y), n, threshold, scale, seed, offset, step);
+                 static_cast<T *>(y), n, threshold, scale, seed, offset, state);
       TDH_LAUNCH_CHECK();
       return static_cast<int>(TDH_OK);
     };
     if (vec) return residual ? go(seeded_dropout_kernel<T, true, true>) : go(seeded_dropout_kernel<T, true, false>);
     return residual ? go(seeded_dropout_kernel<T, false, true>) : go(seeded_dropout_kernel<T, false, false>);
   });
+}
+
+int seeded_dropout_advance(uint64_t *state, int n) {
+  ProfScope prof("dropout_advance", 16.0 * n, WORK_BYTE);
+  TDH_LAUNCH(advance_kernel, dim3(1), dim3(64), 0, ctx().stream, state, n);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
 }
 
 }  // namespace tdh
