@@ -111,7 +111,6 @@ struct EpiGate {
   const T *bias;       // or null
   float *partial;      // slices of z, [split][rows][2 half], that a sum of them reads
   int rows, hidden, half, act;
-  bool wide;           // h's rows lie on 16-byte boundaries
   // g and u at (m, n) to h; writes z
   template <int KIND>
   __device__ __forceinline__ float one(const size_t m, const int n, const float g, const float u) const {
@@ -155,13 +154,10 @@ struct EpiGate {
         turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
           if (m0 + 32 * i + row >= rows) return;
           T *p = h + static_cast<size_t>(m0 + 32 * i + row) * hidden + n0 + col;
-          if (wide) {
-            if (n0 + col < hidden) store8(p, v);
-          } else {
+          if (n0 + col + 8 <= hidden) return store8(p, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n0 + col + e < hidden) p[e] = from_f32<T>(v[e]);
-          }
+          for (int e = 0; e < 8; ++e)
+            if (n0 + col + e < hidden) p[e] = from_f32<T>(v[e]);
         });
       }
     });
@@ -176,13 +172,13 @@ struct EpiGrad {
   int rows, cols;      // of C
   int hidden, half;    // two halves of columns, as above (one: both are cols)
   int accumulate;
-  bool wide;           // out's rows lie on 16-byte boundaries, and its columns are C's
-  __device__ __forceinline__ void one(const size_t m, int n, float v) const {
-    if (n >= hidden) {
-      if (n < half || n - half >= hidden) return;
-      n += hidden - half;
-    }
-    T *p = out + m * (cols > half ? 2 * hidden : hidden) + n;
+  // where column n of C's row m goes (n is in use)
+  __device__ __forceinline__ T *at(const size_t m, const int n) const {
+    return out + m * (cols > half ? 2 * hidden : hidden) + (n < half ? n : n - half + hidden);
+  }
+  __device__ __forceinline__ void one(const size_t m, const int n, float v) const {
+    if ((n < half ? n : n - half) >= hidden) return;
+    T *p = at(m, n);
     if (accumulate) v += to_f32(*p);
     *p = from_f32<T>(v);
   }
@@ -211,9 +207,8 @@ struct EpiGrad {
       turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
         const int m = m0 + 32 * i + row, n = n0 + col;
         if (m >= rows) return;
-        if (wide) {
-          if (n >= cols) return;
-          T *p = out + static_cast<size_t>(m) * cols + n;
+        if (n < cols && (n < half ? n : n - half) + 8 <= hidden) {   // (half is a multiple of eight, or all there is)
+          T *p = at(m, n);
           if (!accumulate) return store8(p, v);
           float o[8];
           load8(p, o);
@@ -301,21 +296,28 @@ pack_kernel(const PackJobs<T> jobs) {
   int c = static_cast<int>(i - row * (per * j.halves)), h = c >= per ? 1 : 0;
   c = (c - h * per) * 8;
   const T *p = j.src + (row * j.halves + h) * j.used + c;
-  T v[8];
+  uint4 v;
+  if (c + 8 <= j.used) {
+    v = load_word(p).raw;
+  } else {
+    float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = c + e < j.used ? p[e] : T{};
-  *reinterpret_cast<uint4 *>(j.dst + i * 8) = *reinterpret_cast<const uint4 *>(v);
+    for (int e = 0; e < 8; ++e) f[e] = c + e < j.used ? to_f32(p[e]) : 0.0f;
+    v = Word<T>::from(f).raw;
+  }
+  *reinterpret_cast<uint4 *>(j.dst + i * 8) = v;
 }
 
 // dz as the products read it (type Z), [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
-// workgroup's band (in fp32, before the rounding). A thread takes E columns: a 16-byte word where every row lies on a 16-byte
-// boundary, else one.
-template <class T, class Z, int E>
+// workgroup's band (in fp32, before the rounding). A thread takes a word of T's columns.
+template <class T, class Z>
 __global__ void __launch_bounds__(GF_NT)
 gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restrict__ dz, float *__restrict__ bias_part,
                const int rows, const int hidden, const int half, const int act, const int blocks_n, const int band_rows) {
+  constexpr int E = Word<T>::N;
   const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
   if (n >= half) return;
+  const bool whole = n + E <= hidden;
   float sg[E] = {}, su[E] = {};
   const int end = min(rows, (band + 1) * band_rows);
   with_gate(act, [&](auto kind) {
@@ -324,24 +326,27 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restr
       float g[E], u[E], d[E], dg[E], du[E];
       const float *zr = z + static_cast<size_t>(m) * 2 * hidden + n;
       const T *dr     = dh + static_cast<size_t>(m) * hidden + n;
-      if constexpr (E > 1) {
+      if (whole) {
 #pragma unroll
         for (int q = 0; q < E / 4; ++q) {
-          const float4 gq = reinterpret_cast<const float4 *>(zr)[q], uq = reinterpret_cast<const float4 *>(zr + hidden)[q];
+          const Word<float> gq = load_word(zr + 4 * q), uq = load_word(zr + hidden + 4 * q);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            g[4 * q + e] = (&gq.x)[e];
-            u[4 * q + e] = (&uq.x)[e];
+            g[4 * q + e] = gq[e];
+            u[4 * q + e] = uq[e];
           }
         }
-        const Word<T> w{*reinterpret_cast<const uint4 *>(dr)};
+        const Word<T> w = load_word(dr);
 #pragma unroll
         for (int e = 0; e < E; ++e) d[e] = w[e];
       } else {
-        const bool in = n < hidden;
-        g[0] = in ? zr[0] : 0.0f;
-        u[0] = in ? zr[hidden] : 0.0f;
-        d[0] = in ? to_f32(dr[0]) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool in = n + e < hidden;
+          g[e] = in ? zr[e] : 0.0f;
+          u[e] = in ? zr[hidden + e] : 0.0f;
+          d[e] = in ? to_f32(dr[e]) : 0.0f;
+        }
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -349,47 +354,53 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restr
         const float a = gate_act<decltype(kind)::value>(g[e], &slope);
         dg[e] = d[e] * u[e] * slope;
         du[e] = d[e] * a;
+        if (!whole && n + e >= hidden) dg[e] = du[e] = 0.0f;
         sg[e] += dg[e];
         su[e] += du[e];
       }
       if (dz) {
         Z *o = dz + static_cast<size_t>(m) * 2 * half + n;
-        if constexpr (E > 1 && sizeof(Z) == 2) {
-          *reinterpret_cast<uint4 *>(o)        = Word<Z>::from(dg).raw;
-          *reinterpret_cast<uint4 *>(o + half) = Word<Z>::from(du).raw;
-        } else if constexpr (E > 1) {
+        if (n + E <= half) {
 #pragma unroll
-          for (int q = 0; q < E / 4; ++q) {
-            reinterpret_cast<float4 *>(o)[q]        = make_float4(dg[4 * q], dg[4 * q + 1], dg[4 * q + 2], dg[4 * q + 3]);
-            reinterpret_cast<float4 *>(o + half)[q] = make_float4(du[4 * q], du[4 * q + 1], du[4 * q + 2], du[4 * q + 3]);
+          for (int s = 0; s < 2; ++s) {
+            const float(&v)[E] = s ? du : dg;
+#pragma unroll
+            for (int q = 0; q < E / Word<Z>::N; ++q) {
+              float w[Word<Z>::N];
+#pragma unroll
+              for (int e = 0; e < Word<Z>::N; ++e) w[e] = v[q * Word<Z>::N + e];
+              store_word(o + s * half + q * Word<Z>::N, Word<Z>::from(w).raw);
+            }
           }
         } else {
-          o[0]    = from_f32<Z>(dg[0]);
-          o[half] = from_f32<Z>(du[0]);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (n + e < half) {
+              o[e]        = from_f32<Z>(dg[e]);
+              o[half + e] = from_f32<Z>(du[e]);
+            }
         }
       }
     }
   });
-  if (bias_part && n < hidden) {
+  if (bias_part) {
     float *p = bias_part + static_cast<size_t>(band) * 2 * hidden + n;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      p[e]          = sg[e];
-      p[hidden + e] = su[e];
-    }
+    for (int e = 0; e < E; ++e)
+      if (n + e < hidden) {
+        p[e]          = sg[e];
+        p[hidden + e] = su[e];
+      }
   }
 }
 // rows of a band: 32, or as few as it takes for four workgroups a compute unit (bias sums: no more than 128 bands up to 4096 samples)
 struct DzPlan {
-  bool wide;
   int blocks_n, band_rows, bands;
 };
 template <class T>
-DzPlan dz_plan(int hidden, int half, int batch, const float *z, const T *dh, bool sums) {
-  constexpr int E = Word<T>::N;
+DzPlan dz_plan(int half, int batch, bool sums) {
   DzPlan p;
-  p.wide      = hidden % E == 0 && ((reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dh)) & 15) == 0;
-  p.blocks_n  = ceil_div(half, p.wide ? E * GF_NT : GF_NT);
+  p.blocks_n  = ceil_div(half, Word<T>::N * GF_NT);
   p.band_rows = std::max(1, std::min<int>(32, static_cast<long>(batch) * p.blocks_n / 1024));
   if (sums) p.band_rows = std::max(p.band_rows, std::min(32, ceil_div(batch, 128)));
   p.bands = ceil_div(batch, p.band_rows);
@@ -398,13 +409,10 @@ DzPlan dz_plan(int hidden, int half, int batch, const float *z, const T *dh, boo
 template <class T, class Z>
 int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, Z *dz, float *bias_part) {
   ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
-  auto go = [&](auto kernel) {
-    TDH_LAUNCH(kernel, dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half, act,
-               p.blocks_n, p.band_rows);
-    TDH_LAUNCH_CHECK();
-    return static_cast<int>(TDH_OK);
-  };
-  return p.wide ? go(gate_dz_kernel<T, Z, Word<T>::N>) : go(gate_dz_kernel<T, Z, 1>);
+  TDH_LAUNCH((gate_dz_kernel<T, Z>), dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
+             act, p.blocks_n, p.band_rows);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
 }
 // db (+)= the bands' sums: 32 columns a workgroup, eight groups of bands, their sums in order
 template <class T>
@@ -443,13 +451,13 @@ constexpr int FEW_ROWS = 4, FEW_NT = 512;
 // rows matter more than anything: 1 KB of a row at a time reaches 6.4 TB/s, 128 bytes of many rows 4.1 to 4.4. So
 // large matrices are split along k, gate and up columns apart, and their slices added up by a launch of its own (BOTH =
 // false); where a strip is small a workgroup takes the gate's columns and the up columns that belong to them, and
-// finishes (BOTH = true). E = 1: columns one by one, for rows that do not lie on 16-byte boundaries. 4096 -> 2 x 12288
-// in bf16, one row: 31.5 us and 2.5 for the sum of 16 slices; through the caches 35.6.
+// finishes (BOTH = true). 4096 -> 2 x 12288 in bf16, one row: 31.5 us and 2.5 for the sum of 16 slices; through the caches
+// 35.6.
 constexpr int FEW_X = 8192;   // values of x in LDS
-template <class T, int E, int M, int LANES, bool BOTH, bool ONCE>
+template <class T, int M, int LANES, bool BOTH, bool ONCE>
 __global__ void __launch_bounds__(FEW_NT)
 few_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const EpiGate<T> epi, const int in, const int strips, const int split_rows) {
-  constexpr int COLS = LANES * E, KG = FEW_NT / LANES, H = BOTH ? 2 : 1;
+  constexpr int E = Word<T>::N, COLS = LANES * E, KG = FEW_NT / LANES, H = BOTH ? 2 : 1;
   constexpr int SLICE = FEW_X / M, SUMS = FEW_NT / 64 * H * COLS;
   __shared__ float lds[FEW_X > SUMS ? FEW_X : SUMS];
   const int tid = threadIdx.x, lc = tid % LANES, kg = tid / LANES, hidden = epi.hidden;
@@ -466,29 +474,37 @@ few_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const EpiGate<T
     for (int m = 0; m < M; ++m)
       for (int k = tid; k < len; k += FEW_NT) lds[m * SLICE + k] = m < epi.rows ? to_f32(x[static_cast<size_t>(m) * in + k0 + k]) : 0.0f;
     __syncthreads();
-    if (n < hidden) {
-      const T *wp = w + static_cast<size_t>(k0 + kg) * ld + half * hidden + n;
+    const T *wp = w + static_cast<size_t>(k0 + kg) * ld + half * hidden + n;
+    auto add = [&](int k, const float (&v)[H][E]) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const float xv = lds[m * SLICE + k];
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[m][s][e] = __builtin_fmaf(xv, v[s][e], acc[m][s][e]);
+      }
+    };
+    if (n + E <= hidden) {
 #pragma unroll 8
       for (int k = kg; k < len; k += KG, wp += KG * ld) {
         float v[H][E];
 #pragma unroll
         for (int s = 0; s < H; ++s) {
-          if constexpr (E > 1) {
-            const Word<T> word = load_word<T, ONCE>(wp + s * hidden);
+          const Word<T> word = load_word<T, ONCE>(wp + s * hidden);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[s][e] = word[e];
-          } else {
-            v[s][0] = to_f32(wp[s * hidden]);
-          }
+          for (int e = 0; e < E; ++e) v[s][e] = word[e];
         }
+        add(k, v);
+      }
+    } else if (n < hidden) {   // (the lane that has the last columns)
+      for (int k = kg; k < len; k += KG, wp += KG * ld) {
+        float v[H][E];
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          const float xv = lds[m * SLICE + k];
+        for (int s = 0; s < H; ++s)
 #pragma unroll
-          for (int s = 0; s < H; ++s)
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[m][s][e] = __builtin_fmaf(xv, v[s][e], acc[m][s][e]);
-        }
+          for (int e = 0; e < E; ++e) v[s][e] = n + e < hidden ? to_f32(wp[s * hidden + e]) : 0.0f;
+        add(k, v);
       }
     }
   }
@@ -530,10 +546,11 @@ few_fwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const EpiGate<T
 // Backward: dx[m][i] = sum_c dz[m][c] w[i][c] and dw[i][c] (+)= sum_m x[m][i] dz[m][c] in one pass over c: a workgroup has
 // FEW_I rows of w and dw, its four waves take turns along c. dz is in fp32 (there is little of it). dx null: only dw, and w is not read; dw null: only dx.
 constexpr int FEW_I = 4;
-template <class T, int E, int M, bool ONCE>
+template <class T, int M, bool ONCE>
 __global__ void __launch_bounds__(256)
 few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const float *__restrict__ dz, T *__restrict__ dx, T *__restrict__ dw,
                const int in, const int cols, const int batch, const int accumulate) {
+  constexpr int E = Word<T>::N;
   __shared__ float sums[4][M * FEW_I];
   const int tid = threadIdx.x, lane = tid & 63, i0 = blockIdx.x * FEW_I;
   float xv[M][FEW_I], acc[M][FEW_I] = {};
@@ -544,31 +561,36 @@ few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const float *__
 #pragma unroll
     for (int m = 0; m < M; ++m) xv[m][i] = dw && m < batch ? to_f32(x[m * static_cast<size_t>(in) + row[i]]) : 0.0f;
   }
-#pragma unroll 2
-  for (int c = tid * E; c < cols; c += 256 * E) {
-    float d[M][E];
-    Word<T> wv[FEW_I];
-    T w1[FEW_I];
+  // the columns c .. c + E - 1, of which `n` are in use (WHOLE: all)
+  auto chunk = [&](const int c, auto all, const int n) {
+    constexpr bool WHOLE = decltype(all)::value;
+    float d[M][E], wv[FEW_I][E];
 #pragma unroll
     for (int i = 0; i < FEW_I; ++i) {
       if (!dx) break;
-      if constexpr (E > 1)
-        wv[i] = load_word<T, ONCE>(w + row[i] * cols + c);
-      else
-        w1[i] = w[row[i] * cols + c];
+      const T *p = w + row[i] * cols + c;
+      if constexpr (WHOLE) {
+        const Word<T> v = load_word<T, ONCE>(p);
+#pragma unroll
+        for (int e = 0; e < E; ++e) wv[i][e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) wv[i][e] = e < n ? to_f32(p[e]) : 0.0f;
+      }
     }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const float *p = dz + static_cast<size_t>(m < batch ? m : 0) * cols + c;
-      if constexpr (E > 1) {
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q) {
-          const float4 v = reinterpret_cast<const float4 *>(p)[q];
+      for (int q = 0; q < E / 4; ++q) {
+        if constexpr (WHOLE) {
+          const Word<float> v = load_word(p + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[m][4 * q + e] = m < batch ? (&v.x)[e] : 0.0f;
+          for (int e = 0; e < 4; ++e) d[m][4 * q + e] = m < batch ? v[e] : 0.0f;
+        } else {
+#pragma unroll
+          for (int e = 4 * q; e < 4 * q + 4; ++e) d[m][e] = m < batch && e < n ? p[e] : 0.0f;
         }
-      } else {
-        d[m][0] = m < batch ? p[0] : 0.0f;
       }
     }
     if (dx) {
@@ -577,35 +599,36 @@ few_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const float *__
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            float v;
-            if constexpr (E > 1) v = wv[i][e]; else v = to_f32(w1[i]);
-            acc[m][i] = __builtin_fmaf(d[m][e], v, acc[m][i]);
-          }
+          for (int e = 0; e < E; ++e) acc[m][i] = __builtin_fmaf(d[m][e], wv[i][e], acc[m][i]);
     }
-    if (dw) {
+    if (!dw) return;
 #pragma unroll
-      for (int i = 0; i < FEW_I; ++i) {
-        if (i0 + i >= in) break;
-        T *p = dw + row[i] * cols + c;
-        float o[E] = {};
+    for (int i = 0; i < FEW_I; ++i) {
+      if (i0 + i >= in) break;
+      T *p = dw + row[i] * cols + c;
+      float o[E] = {};
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = m < batch ? __builtin_fmaf(xv[m][i], d[m][e], o[e]) : o[e];
-        if constexpr (E > 1) {
-          if (accumulate) {
-            const Word<T> was = load_word<T, ONCE>(p);
+        for (int e = 0; e < E; ++e) o[e] = m < batch ? __builtin_fmaf(xv[m][i], d[m][e], o[e]) : o[e];
+      if constexpr (WHOLE) {
+        if (accumulate) {
+          const Word<T> was = load_word<T, ONCE>(p);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += was[e];
-          }
-          store_word16<ONCE>(p, Word<T>::from(o).raw);
-        } else {
-          *p = from_f32<T>(accumulate ? o[0] + to_f32(*p) : o[0]);
+          for (int e = 0; e < E; ++e) o[e] += was[e];
         }
+        store_word<ONCE>(p, Word<T>::from(o).raw);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (e < n) p[e] = from_f32<T>(accumulate ? o[e] + to_f32(p[e]) : o[e]);
       }
     }
-  }
+  };
+  int c = tid * E;
+#pragma unroll 2
+  for (; c + E <= cols; c += 256 * E) chunk(c, std::true_type(), E);
+  if (c < cols) chunk(c, std::false_type(), cols - c);
   if (!dx) return;
 #pragma unroll
   for (int m = 0; m < M; ++m)
@@ -631,47 +654,37 @@ int with_rows(int batch, const F &f) {
   if (batch <= 2) return f(std::integral_constant<int, 2>());
   return f(std::integral_constant<int, 4>());
 }
-template <class T>
-bool in_words(std::initializer_list<const void *> tensors, int cols) {
-  uintptr_t all = 0;
-  for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
-  return (all & 15) == 0 && cols % Word<T>::N == 0;
-}
-
 // matrices that the L2 caches (8 x 4 MB) do not hold are read past them
 constexpr size_t FEW_ONCE_BYTES = 32u << 20;
 
 template <class T>
 int few_fwd(int act, int in, int hidden, int batch, const T *x, const T *w, const T *b, T *h, float *z) {
-  const bool words = in_words<T>({w}, hidden), wide = hidden >= 256;
+  const bool wide = hidden >= 256;
   const size_t bytes = sizeof(T) * static_cast<size_t>(in) * 2 * hidden;
-  const int cols = (wide ? 64 : 16) * (words ? Word<T>::N : 1), strips = ceil_div(hidden, cols);
+  const int cols = (wide ? 64 : 16) * Word<T>::N, strips = ceil_div(hidden, cols);
   // a workgroup reads 256 KB at most, or an equal part of one of 768
   const long want  = std::min<long>(768, static_cast<long>(bytes >> 17));
   const bool both  = bytes / strips <= (256u << 10);
   const int most   = std::max(1, in / 32), splits = both ? 1 : static_cast<int>(std::min<long>(most, std::max(1L, (want + 2 * strips - 1) / (2 * strips))));
   const int rows_s = ceil_div(in, splits), used = ceil_div(in, rows_s);
   const size_t part = static_cast<size_t>(batch) * 2 * hidden;
-  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, hidden, act, false};
+  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, hidden, act};
   if (!both) {
     TDH_TRY(ws_begin(ws_align(4 * part * used)));
     TDH_TRY(take(part * used, &epi.partial));
   }
   const bool once = bytes > FEW_ONCE_BYTES;
   TDH_TRY(with_rows(batch, [&](auto rows) {
-    constexpr int M = decltype(rows)::value, E = Word<T>::N;
+    constexpr int M = decltype(rows)::value;
     ProfScope prof("gated_ff_few_fwd", static_cast<double>(bytes), WORK_BYTE);
     auto go = [&](auto kernel) {
       TDH_LAUNCH(kernel, dim3(both ? strips : 2 * strips * used), dim3(FEW_NT), 0, ctx().stream, x, w, epi, in, strips, rows_s);
       TDH_LAUNCH_CHECK();
       return static_cast<int>(TDH_OK);
     };
-    if (words && wide)
-      return both ? go(few_fwd_kernel<T, E, M, 64, true, false>)
-             : once ? go(few_fwd_kernel<T, E, M, 64, false, true>) : go(few_fwd_kernel<T, E, M, 64, false, false>);
-    if (words) return both ? go(few_fwd_kernel<T, E, M, 16, true, false>) : go(few_fwd_kernel<T, E, M, 16, false, false>);
-    if (wide) return both ? go(few_fwd_kernel<T, 1, M, 64, true, false>) : go(few_fwd_kernel<T, 1, M, 64, false, false>);
-    return both ? go(few_fwd_kernel<T, 1, M, 16, true, false>) : go(few_fwd_kernel<T, 1, M, 16, false, false>);
+    if (both) return wide ? go(few_fwd_kernel<T, M, 64, true, false>) : go(few_fwd_kernel<T, M, 16, true, false>);
+    if (!wide) return go(few_fwd_kernel<T, M, 16, false, false>);
+    return once ? go(few_fwd_kernel<T, M, 64, false, true>) : go(few_fwd_kernel<T, M, 64, false, false>);
   }));
   return both ? static_cast<int>(TDH_OK) : launch_gate_reduce(epi, used);
 }
@@ -680,7 +693,7 @@ template <class T>
 int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
             int accumulate) {
   const int cols = 2 * hidden;
-  const DzPlan pz = dz_plan(hidden, hidden, batch, z, dh, db != nullptr);
+  const DzPlan pz = dz_plan<T>(hidden, batch, db != nullptr);
   TDH_TRY(ws_begin(ws_align(sizeof(float) * batch * cols) + ws_align(4 * static_cast<size_t>(pz.bands) * cols)));
   float *dz = nullptr, *bias_part = nullptr;
   if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * cols, &dz));
@@ -696,9 +709,7 @@ int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, cons
       TDH_LAUNCH_CHECK();
       return static_cast<int>(TDH_OK);
     };
-    if (!in_words<T>({w, dw}, cols)) return go(few_bwd_kernel<T, 1, M, false>);
-    return sizeof(T) * static_cast<size_t>(in) * cols > FEW_ONCE_BYTES ? go(few_bwd_kernel<T, Word<T>::N, M, true>)
-                                                                       : go(few_bwd_kernel<T, Word<T>::N, M, false>);
+    return sizeof(T) * static_cast<size_t>(in) * cols > FEW_ONCE_BYTES ? go(few_bwd_kernel<T, M, true>) : go(few_bwd_kernel<T, M, false>);
   });
 }
 
@@ -826,10 +837,10 @@ int ff_fwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   TDH_TRY(packer.add(x, batch, in, 1, &A));
   TDH_TRY(packer.add(w, in, hidden, 2, &B));
   TDH_TRY(packer.run());
-  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act, fits(h, hidden)};
+  EpiGate<T> epi{h, z, b, nullptr, batch, hidden, half, act};
   if (plan.splits == 1) return ff_gemm<T, true, false, true>(plan, A, B, epi, batch, 2 * half, in, "gated_ff_fwd");
   TDH_TRY(take(plan.splits * part, &epi.partial));
-  const EpiGrad<T> slices{nullptr, epi.partial, batch, 2 * half, hidden, half, 0, false};
+  const EpiGrad<T> slices{nullptr, epi.partial, batch, 2 * half, hidden, half, 0};
   TDH_TRY((ff_gemm<T, true, false, false>(plan, A, B, slices, batch, 2 * half, in, "gated_ff_fwd")));
   return launch_gate_reduce(epi, plan.splits);
 }
@@ -845,7 +856,7 @@ template <class T>
 int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, const float *z, const T *dh, T *dx, T *dw, T *db,
               int accumulate) {
   const int half = padded(hidden);
-  const DzPlan pz = dz_plan(hidden, half, batch, z, dh, db != nullptr);
+  const DzPlan pz = dz_plan<T>(half, batch, db != nullptr);
   const int bands = pz.bands;
   const FfPlan px = ff_plan(batch, in, 2 * half), pw = ff_plan(in, 2 * half, batch);
   const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
@@ -865,10 +876,10 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   if (dw) TDH_TRY(packer.add(x, batch, in, 1, &X));
   TDH_TRY(packer.run());
   if (dx) {
-    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0, fits(dx, in)}, 2 * half, "gated_ff_dx")));
+    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx")));
   }
   if (dw) {
-    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate, fits(dw, hidden)}, batch, "gated_ff_dw")));
+    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw")));
   }
   return TDH_OK;
 }
@@ -898,12 +909,7 @@ split_kernel(const SplitJobs jobs) {
   const bool turn  = j.sign == 1 ? (row / X3P_BK) & 1 : j.sign == 2 ? (col / X3P_BK) & 1 : false;
   const float scale = turn ? -X3_SCALE : X3_SCALE;
   float v[8];
-  if ((reinterpret_cast<uintptr_t>(j.src) & 15) == 0) {
-    load8(j.src + i * 8, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = j.src[i * 8 + e];
-  }
+  load8(j.src + i * 8, v);
   uint4 out[X3_PARTS];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -999,10 +1005,10 @@ int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
     TDH_TRY(split.add(w, in, 2 * hidden, 0, &W));
     TDH_TRY(split.run());
     const X3Source src{x, w, in, 1, 2L * hidden, 1, batch, 2 * hidden};
-    EpiGate<float> epi{h, z, b, nullptr, batch, hidden, hidden, act, fits(h, hidden)};
+    EpiGate<float> epi{h, z, b, nullptr, batch, hidden, hidden, act};
     if (plan.splits == 1) return x3_gemm<true, false, true>(plan, X, W, src, epi, in, "gated_ff_fwd_x3");
     TDH_TRY(take(plan.splits * nz, &epi.partial));
-    const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * hidden, hidden, hidden, 0, false};
+    const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * hidden, hidden, hidden, 0};
     TDH_TRY((x3_gemm<true, false, false>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
     return launch_gate_reduce(epi, plan.splits);
   }
@@ -1020,7 +1026,7 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   const int cols = 2 * hidden;
   const bool planes_x = dx && x3_weights(in, hidden, batch), planes_w = dw && x3_dw(in, hidden, batch);
   const bool own_db   = db && planes_w;   // (else the sums ride along with dw's launch)
-  const DzPlan pz     = dz_plan(hidden, hidden, batch, z, dh, own_db);
+  const DzPlan pz     = dz_plan<float>(hidden, batch, own_db);
   const size_t nz = static_cast<size_t>(batch) * cols, nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * cols;
   TDH_TRY(ws_begin(ws_align(4 * nz) + (own_db ? ws_align(4 * static_cast<size_t>(pz.bands) * cols) : 0) +
                    (planes_x || planes_w ? Splitter::bytes(batch, cols) : 0) +
@@ -1041,12 +1047,12 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   TDH_TRY(split.run());
   if (planes_w)
     TDH_TRY((x3_grad<false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, cols},
-                                   EpiGrad<float>{dw, nullptr, in, cols, hidden, hidden, accumulate, fits(dw, hidden)}, batch, "gated_ff_dw_x3")));
+                                   EpiGrad<float>{dw, nullptr, in, cols, hidden, hidden, accumulate}, batch, "gated_ff_dw_x3")));
   if (planes_x) {
     TDH_TRY(weights.add(w, in, cols, 2, &W));
     TDH_TRY(weights.run());
     TDH_TRY((x3_grad<true, true>(Z, W, X3Source{dz, w, cols, 1, 1, cols, batch, in},
-                                 EpiGrad<float>{dx, nullptr, batch, in, in, in, 0, fits(dx, in)}, cols, "gated_ff_dx_x3")));
+                                 EpiGrad<float>{dx, nullptr, batch, in, in, in, 0}, cols, "gated_ff_dx_x3")));
   }
   if ((dx && !planes_x) || (dw && !planes_w) || (db && !own_db))
     return fc_bwd(in, cols, db && !own_db, batch, x, w, dz, planes_x ? nullptr : dx, planes_w ? nullptr : dw, own_db ? nullptr : db,
@@ -1057,7 +1063,7 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
 // the gradients of no samples
 template <class T>
 int no_rows(int in, int hidden, T *dw, T *db) {
-  if (dw) TDH_TRY(launch_grad_reduce(EpiGrad<T>{dw, nullptr, in, 2 * hidden, hidden, hidden, 0, false}, 0));
+  if (dw) TDH_TRY(launch_grad_reduce(EpiGrad<T>{dw, nullptr, in, 2 * hidden, hidden, hidden, 0}, 0));
   return db ? launch_db<T>(nullptr, db, 0, hidden, 0) : static_cast<int>(TDH_OK);
 }
 

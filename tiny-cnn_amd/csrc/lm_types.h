@@ -53,31 +53,29 @@ struct Word {
   }
 };
 
-// A word from memory; ONCE: past the caches (data larger than they are, read once).
-template <class T, bool ONCE>
+// Sixteen bytes of memory on any element's boundary (the memory instructions take them there; where rows have an odd length every
+// other one starts off a 16-byte boundary). ONCE: past the caches (data larger than they are, read or written once).
+typedef uint32_t any_word __attribute__((ext_vector_type(4), aligned(2)));
+template <class T, bool ONCE = false>
 __device__ __forceinline__ Word<T> load_word(const T *p) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const any_word *q = reinterpret_cast<const any_word *>(p);
+  return Word<T>{__builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(q) : *q)};
+}
+template <bool ONCE = false>
+__device__ __forceinline__ void store_word(void *p, const uint4 v) {
+  any_word *q = static_cast<any_word *>(p);
   if constexpr (ONCE)
-    return Word<T>{__builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)))};
+    __builtin_nontemporal_store(__builtin_bit_cast(any_word, v), q);
   else
-    return Word<T>{*reinterpret_cast<const uint4 *>(p)};
+    *q = __builtin_bit_cast(any_word, v);
 }
 
-template <bool ONCE>
-__device__ __forceinline__ void store_word16(void *p, const uint4 v) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  if constexpr (ONCE)
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4 *>(p));
-  else
-    *static_cast<uint4 *>(p) = v;
-}
-
-// Eight neighbours on a 16-byte boundary.
+// Eight neighbours.
 template <class T>
 __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
 #pragma unroll
   for (int q = 0; q < 8 / Word<T>::N; ++q) {
-    const Word<T> w{reinterpret_cast<const uint4 *>(p)[q]};
+    const Word<T> w = load_word(p + q * Word<T>::N);
 #pragma unroll
     for (int e = 0; e < Word<T>::N; ++e) v[q * Word<T>::N + e] = w[e];
   }
@@ -89,7 +87,7 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
     float w[Word<T>::N];
 #pragma unroll
     for (int e = 0; e < Word<T>::N; ++e) w[e] = v[q * Word<T>::N + e];
-    reinterpret_cast<uint4 *>(p)[q] = Word<T>::from(w).raw;
+    store_word(p + q * Word<T>::N, Word<T>::from(w).raw);
   }
 }
 

@@ -36,13 +36,12 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], const uint64_t block, c
   }
 }
 
-// y = [residual +] keep * scale * x. VEC: all tensors lie on 16-byte boundaries, so that a thread takes
-// whole words; the elements behind the last whole one are taken one by one.
-template <class T, bool VEC, bool RES>
+// y = [residual +] keep * scale * x, a 16-byte word a thread at a time.
+template <class T, bool RES>
 __global__ void __launch_bounds__(SD_NT)
 seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const uint32_t threshold, const float scale,
                       const uint64_t seed_arg, const uint64_t offset_arg, const uint64_t *__restrict__ state) {
-  constexpr int E = VEC ? Word<T>::N : 4;   // elements a thread takes at a time
+  constexpr int E = Word<T>::N;
   const uint64_t seed = state ? state[0] : seed_arg, offset = state ? state[1] : offset_arg;
   const size_t items = (n + E - 1) / E, stride = static_cast<size_t>(gridDim.x) * SD_NT;
   for (size_t i = static_cast<size_t>(blockIdx.x) * SD_NT + threadIdx.x; i < items; i += stride) {
@@ -50,17 +49,15 @@ seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const
     uint32_t c[E / 4][4];
 #pragma unroll
     for (int q = 0; q < E / 4; ++q) philox(c[q], i * (E / 4) + q, offset, seed);
-    if (VEC && at + E <= n) {
-      const Word<T> v{*reinterpret_cast<const uint4 *>(x + at)};
-      Word<T> r{};
-      if (RES) r.raw = *reinterpret_cast<const uint4 *>(residual + at);
-      float o[Word<T>::N];
+    if (at + E <= n) {
+      const Word<T> v = load_word(x + at), r = RES ? load_word(residual + at) : Word<T>{};
+      float o[E];
 #pragma unroll
-      for (int e = 0; e < Word<T>::N; ++e) {
+      for (int e = 0; e < E; ++e) {
         const float d = c[e / 4][e % 4] >= threshold ? v[e] * scale : 0.0f;
         o[e] = RES ? r[e] + d : d;
       }
-      *reinterpret_cast<uint4 *>(y + at) = Word<T>::from(o).raw;
+      store_word(y + at, Word<T>::from(o).raw);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -84,10 +81,9 @@ int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offs
   ProfScope prof(tag, static_cast<double>(size) * n * (residual ? 3 : 2), WORK_BYTE);
   const uint32_t threshold = static_cast<uint32_t>(static_cast<double>(rate) * 4294967296.0);
   const float scale        = static_cast<float>(1.0 / (1.0 - static_cast<double>(rate)));
-  const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const size_t items = ceil_div_sz(n, vec ? Word<T>::N : 4);
+    const size_t items = ceil_div_sz(n, Word<T>::N);
     const dim3 grid(static_cast<unsigned>(std::min<size_t>(ceil_div_sz(items, SD_NT), GRID_X_MAX)));
     auto go = [&](auto kernel) {
       TDH_LAUNCH(kernel, grid, dim3(SD_NT), 0, ctx().stream, static_cast<const T *>(x), static_cast<const T *>(residual),
@@ -95,8 +91,7 @@ int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offs
       TDH_LAUNCH_CHECK();
       return static_cast<int>(TDH_OK);
     };
-    if (vec) return residual ? go(seeded_dropout_kernel<T, true, true>) : go(seeded_dropout_kernel<T, true, false>);
-    return residual ? go(seeded_dropout_kernel<T, false, true>) : go(seeded_dropout_kernel<T, false, false>);
+    return residual ? go(seeded_dropout_kernel<T, true>) : go(seeded_dropout_kernel<T, false>);
   });
 }
 

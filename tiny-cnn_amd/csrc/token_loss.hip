@@ -50,10 +50,10 @@ struct Row {
 
 // Writes word k (in the numbering of the row of logits) of the gradient's row.
 template <class T>
-__device__ __forceinline__ void store_word(const Row<T> &r, T *out, const int k, const float (&v)[Word<T>::N]) {
+__device__ __forceinline__ void store_row_word(const Row<T> &r, T *out, const int k, const float (&v)[Word<T>::N]) {
   T *at = out + (static_cast<long>(k) * Word<T>::N - r.shift);
   if (r.whole(k) && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-    store_word16<true>(at, Word<T>::from(v).raw);
+    store_word<true>(at, Word<T>::from(v).raw);
     return;
   }
 #pragma unroll
@@ -186,7 +186,7 @@ row_kernel(const RowArgs a) {
     if (tid == 0) skip_row<MODE>(a, row);
     if (dx) {
       const float zero[N] = {};
-      for (int k = tid; k < r.words; k += NT) store_word(r, dx, k, zero);
+      for (int k = tid; k < r.words; k += NT) store_row_word(r, dx, k, zero);
     }
     return;
   }
@@ -258,7 +258,7 @@ row_kernel(const RowArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) g[e] = e == at ? g[e] + d : g[e];
       }
-      store_word(r, dx, k, g);
+      store_row_word(r, dx, k, g);
     };
     if constexpr (W > 0) {
 #pragma unroll
@@ -374,7 +374,7 @@ dlogits_kernel(const GradArgs a) {
     const float zero[N] = {};
 #pragma unroll
     for (int i = 0; i < GRAD_WORDS; ++i)
-      if (k0 + i * GRAD_NT < r.words) store_word(r, dx, k0 + i * GRAD_NT, zero);
+      if (k0 + i * GRAD_NT < r.words) store_row_word(r, dx, k0 + i * GRAD_NT, zero);
     return;
   }
   if (t >= a.vocab) d = __builtin_nanf("");
@@ -395,7 +395,7 @@ dlogits_kernel(const GradArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e) g[e] = e == at ? g[e] + d : g[e];
     }
-    store_word(r, dx, k, g);
+    store_row_word(r, dx, k, g);
   }
 }
 
