@@ -39,6 +39,15 @@ struct Word {
     else
       return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(e & 1 ? w >> 16 : w)));
   }
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  __device__ __forceinline__ static uint32_t pair(bf16, const float a, const float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+  }
+  __device__ __forceinline__ static uint32_t pair(f16, const float a, const float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+  }
   __device__ __forceinline__ static Word from(const float (&v)[N]) {
     Word o;
 #pragma unroll
@@ -46,8 +55,7 @@ struct Word {
       if constexpr (sizeof(T) == 4)
         (&o.raw.x)[i] = __float_as_uint(v[i]);
       else
-        (&o.raw.x)[i] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * i]))) |
-                        static_cast<uint32_t>(__builtin_bit_cast(uint16_t, from_f32<T>(v[2 * i + 1]))) << 16;
+        (&o.raw.x)[i] = pair(T(), v[2 * i], v[2 * i + 1]);   // (one instruction for the two)
     }
     return o;
   }

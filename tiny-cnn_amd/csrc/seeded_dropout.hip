@@ -14,7 +14,9 @@ constexpr int SD_NT = 256;
 
 __device__ __forceinline__ void philox_round(uint32_t (&c)[4], const uint32_t k0, const uint32_t k1) {
   const uint64_t a = static_cast<uint64_t>(0xD2511F53u) * c[0], b = static_cast<uint64_t>(0xCD9E8D57u) * c[2];
-  const uint32_t c0 = static_cast<uint32_t>(b >> 32) ^ c[1] ^ k0, c2 = static_cast<uint32_t>(a >> 32) ^ c[3] ^ k1;
+  // (a ^ b ^ c in one instruction)
+  const uint32_t c0 = __builtin_amdgcn_bitop3_b32(static_cast<uint32_t>(b >> 32), c[1], k0, 0x96);
+  const uint32_t c2 = __builtin_amdgcn_bitop3_b32(static_cast<uint32_t>(a >> 32), c[3], k1, 0x96);
   c[1] = static_cast<uint32_t>(b);
   c[3] = static_cast<uint32_t>(a);
   c[0] = c0;
@@ -36,8 +38,11 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], const uint64_t block, c
   }
 }
 
-// y = [residual +] keep * scale * x, a 16-byte word a thread at a time.
-template <class T, bool RES>
+// y = [residual +] keep * scale * x, a 16-byte word a thread at a time. Tensors that the L2 caches do not hold go past them. Bound by
+// memory with a residual (33.5 M bf16 values: 32.7 us, 6.2 TB/s; through the caches 36.8), without one by the generator's
+// 64-bit products, two a round.
+constexpr size_t SD_ONCE_BYTES = 32u << 20;
+template <class T, bool RES, bool ONCE>
 __global__ void __launch_bounds__(SD_NT)
 seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const uint32_t threshold, const float scale,
                       const uint64_t seed_arg, const uint64_t offset_arg, const uint64_t *__restrict__ state) {
@@ -50,14 +55,14 @@ seeded_dropout_kernel(const T *x, const T *residual, T *y, const size_t n, const
 #pragma unroll
     for (int q = 0; q < E / 4; ++q) philox(c[q], i * (E / 4) + q, offset, seed);
     if (at + E <= n) {
-      const Word<T> v = load_word(x + at), r = RES ? load_word(residual + at) : Word<T>{};
+      const Word<T> v = load_word<T, ONCE>(x + at), r = RES ? load_word<T, ONCE>(residual + at) : Word<T>{};
       float o[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float d = c[e / 4][e % 4] >= threshold ? v[e] * scale : 0.0f;
         o[e] = RES ? r[e] + d : d;
       }
-      store_word(y + at, Word<T>::from(o).raw);
+      store_word<ONCE>(y + at, Word<T>::from(o).raw);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -91,7 +96,8 @@ int seeded_dropout(int dtype, size_t n, float rate, uint64_t seed, uint64_t offs
       TDH_LAUNCH_CHECK();
       return static_cast<int>(TDH_OK);
     };
-    return residual ? go(seeded_dropout_kernel<T, true>) : go(seeded_dropout_kernel<T, false>);
+    if (size * n > SD_ONCE_BYTES) return residual ? go(seeded_dropout_kernel<T, true, true>) : go(seeded_dropout_kernel<T, false, true>);
+    return residual ? go(seeded_dropout_kernel<T, true, false>) : go(seeded_dropout_kernel<T, false, false>);
   });
 }
 
