@@ -267,13 +267,12 @@ int tdh_softmax_xent_grad(int batch, int len, const float *y, const float *t, fl
 /* -------------------------------------------- operators of language models
  * They have no counterpart in the reference. `dtype` (TDH_F32, TDH_BF16, TDH_F16) is the element type of the
  * tensors declared void *; those declared float * are fp32 in every type. Sums are held in 32 bits or more, and
- * results are rounded once, to nearest. Tensors are aligned to their elements; where they lie on 16-byte
- * boundaries and rows are multiples of 16 bytes apart, they move in words of that size. The same inputs give
- * the same bits. */
+ * results are rounded once, to nearest. Tensors are aligned to their elements. The same inputs give the same bits. */
 
 /* Gated feed-forward block: z = x W + b, h = act(z_gate) * z_up. x [batch][in], w [in][2*hidden] with the gate's
  * columns first, b [2*hidden] (has_bias), h [batch][hidden]. z [batch][2*hidden], fp32, is what the backward pass
- * reads; NULL where there is none (inference). */
+ * reads; NULL where there is none (inference). No output may overlap another tensor of the call. in up to 2^21,
+ * hidden up to 2^20, batch up to 2^24, and no tensor of 2^31 elements. */
 int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
                      const void *b, void *h, float *z);
 /* dz = (dh * z_up * act'(z_gate), dh * act(z_gate)), dx = dz W^T, dw = x^T dz, db = the sum of dz over the batch. dx is overwritten;
@@ -309,7 +308,8 @@ int tdh_token_logprob_bwd(int dtype, int rows, int vocab, const void *logits, si
  *   ratio = exp(logp - old_logp), gap = ref_logp - logp,
  *   row_loss = weight * (-min(ratio * advantage, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantage)
  *                        + kl_coef * (exp(gap) - gap - 1)),
- * loss[0] = the sum of row_loss, and dlogits its gradient. weight NULL: 1 for every row (1 / rows makes a mean);
+ * loss[0] = the sum of row_loss, and dlogits its gradient. weight NULL: 1 for every row (1 / rows makes a mean). It is a
+ * factor and no mask: 0 times an infinite loss is NaN, and rows whose values mean nothing have a negative target.
  * ref_logp NULL: no KL term. Any of logp, row_loss, loss and dlogits may be NULL; dlogits as in
  * tdh_token_logprob_bwd. Where the two sides of the minimum are equal the gradient is the first one's. */
 typedef struct tdh_policy_desc {

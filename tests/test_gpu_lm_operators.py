@@ -193,6 +193,27 @@ def test_gated_ff_activations(T, dtype, act):
 
 
 @pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_gated_ff_activations_far_from_zero(T, dtype, act, n):
+    """Beyond 2^10 every activation is 0, 1 or the gate itself, and its derivative 0 or 1, without a rounding: squares and
+    cubes that overflow on the way there must not show."""
+    top = 15 if dtype == "f16" else 126
+    g = np.array([s * 2.0 ** e for e in (10, 15, 30, 42, 63, 66, 90, 126) if e <= top for s in (1, -1)])
+    f = len(g)
+    want_h = {"sigmoid": (g > 0) * 1.0, "none": g}.get(act, np.maximum(g, 0))
+    slope = {"sigmoid": 0 * g, "none": 0 * g + 1}.get(act, (g > 0) * 1.0)
+    z = np.tile(np.concatenate([g, np.ones(f)]), (n, 1))
+    x, w = Buf(T, np.ones((n, 1)), dtype), Buf(T, z[:1], dtype)
+    h, bz = out(T, (n, f), dtype), out(T, (n, 2 * f))
+    T.gated_ff_fwd(1, f, False, n, x, w, None, h, bz, act=act, dtype=dtype)
+    assert np.array_equal(bz.read(), z) and np.array_equal(h.read(), np.tile(want_h, (n, 1)))
+    db, dh = out(T, 2 * f, dtype), Buf(T, np.eye(n)[:, :1] * np.ones((n, f)), dtype)   # (one sample has a gradient)
+    T.gated_ff_bwd(1, f, True, n, x, w, bz, dh, None, None, db, act=act, dtype=dtype)
+    assert np.array_equal(db.read(), np.concatenate([slope, want_h]))
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
 @pytest.mark.parametrize("shape", [(1, 64, 32), (6, 40, 48), (70, 64, 128)], ids=lambda s: "x".join(map(str, s)))
 def test_gated_ff_unaligned_and_accumulating(T, dtype, shape):
     ff_case(T, shape, "gelu_tanh", dtype, bias=True, skew=1)

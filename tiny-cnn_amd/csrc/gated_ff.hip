@@ -32,9 +32,11 @@ __device__ __forceinline__ float gate_act(const float g, float *slope) {
     *slope = cdf + g * (0.39894228040143268f * e);
     return g * cdf;
   } else if constexpr (KIND == TDH_GATE_GELU_TANH) {
-    // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3)
-    const float s = logistic(1.5957691216057308f * (g + 0.044715f * g * g * g));
-    *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * g * g));
+    // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3); beyond 16 it is 0 or 1, and the
+    // square in the derivative would overflow where its factor is 0
+    const float c = __builtin_amdgcn_fmed3f(g, -16.0f, 16.0f);
+    const float s = logistic(1.5957691216057308f * (c + 0.044715f * c * c * c));
+    *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * c * c));
     return g * s;
   } else if constexpr (KIND == TDH_GATE_SIGMOID) {
     const float s = logistic(g);
@@ -1073,8 +1075,9 @@ int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch)
   TDH_CHECK_ARG(in > 0 && hidden > 0 && batch >= 0, "%s: bad shape %d->2*%d batch %d", who, in, hidden, batch);
   TDH_CHECK_ARG(2L * in * hidden < (1L << 31) && static_cast<long>(batch) * in < (1L << 31) && 2L * batch * hidden < (1L << 31),
                 "%s: tensor exceeds 2^31 elements", who);
-  // (offsets within a tile of 256 rows are 32 bits)
-  TDH_CHECK_ARG(dtype == TDH_F32 || (in <= (1 << 21) && hidden <= (1 << 20)), "%s: %d->2*%d is too wide for 16-bit types", who, in, hidden);
+  // (offsets within a tile of 256 rows are 32 bits, and a launch has fewer than 2^24 workgroups)
+  TDH_CHECK_ARG(in <= (1 << 21) && hidden <= (1 << 20) && batch <= (1 << 24), "%s: %d->2*%d batch %d is beyond 2^21->2*2^20 batch 2^24", who,
+                in, hidden, batch);
   return TDH_OK;
 }
 int check_aligned(const char *who, int dtype, std::initializer_list<const void *> tensors) {
