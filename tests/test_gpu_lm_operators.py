@@ -164,6 +164,14 @@ def test_gated_ff_of_many_samples_unaligned_and_accumulating(T, dtype):
     ff_case(T, (1001, 1024, 1000), "gelu", dtype, bias=True, skew=1, accumulate=True)
 
 
+@pytest.mark.parametrize("skew", [0, 1])
+@pytest.mark.parametrize("shape", [(1001, 1027, 1001), (402, 1401, 1803), (130, 2811, 2797), (1500, 1340, 501), (20001, 65, 801)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ff_of_many_samples_with_rows_of_any_length(T, shape, skew):
+    """(fp32 products in three parts, whose copies are padded to whole words)"""
+    ff_case(T, shape, "silu", "f32", bias=True, skew=skew, accumulate=skew == 1)
+
+
 @pytest.mark.parametrize("dtype", L.DTYPES)
 def test_gated_ff_of_many_samples_with_infinities(T, dtype):
     """An infinite or NaN value reaches the sums that it is part of, which are what fp32 arithmetic gives, and no others."""
@@ -219,6 +227,13 @@ def test_gated_ff_unaligned_and_accumulating(T, dtype, shape):
     ff_case(T, shape, "gelu_tanh", dtype, bias=True, skew=1)
     ff_case(T, shape, "gelu_tanh", dtype, bias=True, accumulate=True)
     ff_case(T, shape, "gelu_tanh", dtype, bias=True, skew=3, accumulate=True)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("shape", [(513, 40, 48), (900, 41, 33), (5000, 24, 40), (9001, 9, 5), (4000, 1, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_ff_of_many_samples_and_narrow_matrices(T, dtype, shape, accumulate):
+    ff_case(T, shape, "silu", dtype, bias=True, accumulate=accumulate)
 
 
 @pytest.mark.parametrize("dtype", L.DTYPES)

@@ -5,8 +5,8 @@
 //   up to FEW_ROWS samples   the weights are read once, as they lie, by vector kernels (few_fwd_kernel, few_bwd_kernel)
 //   16-bit types             three products on the matrix cores (gemm16.h); the forward one takes gate and up columns in
 //                            pairs and leaves h, and z for the way back
-//   fp32                     products of many samples on operands in three bf16 parts (gemm_x3.h), the others the
-//                            fully-connected layer's
+//   fp32                     products of many samples on operands in three bf16 parts (gemm_x3.h), at any row length, the
+//                            others the fully-connected layer's
 //
 // z is kept in fp32 in every type, so that the derivative sees what the activation saw. dz is rounded to the 16-bit type once,
 // as the products' operand: in two parts each, dx and dW would cost twice the matrix work for one rounding among as
@@ -431,30 +431,32 @@ int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const f
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
-// db (+)= the bands' sums: 32 columns a workgroup, eight groups of bands, their sums in order (128 bands of 8192 columns 4.1 us, a launch;
+// db (+)= the bands' sums: 32 columns a workgroup, 32 groups of bands, their sums in order (128 bands of 8192 columns 4.1 us, a launch;
 // a thread a column, all bands in turn: 45)
+constexpr int BS_GROUPS = 32;
 template <class T>
-__global__ void __launch_bounds__(GF_NT)
+__global__ void __launch_bounds__(32 * BS_GROUPS)
 bias_sum_kernel(const float *__restrict__ part, T *__restrict__ db, const int bands, const int cols, const int accumulate) {
-  __shared__ float lds[8][32];
+  __shared__ float lds[BS_GROUPS][32];
   const int c = threadIdx.x & 31, group = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
   float s = 0.0f;
   if (n < cols) {
 #pragma unroll 4
-    for (int b = group; b < bands; b += 8) s += part[static_cast<size_t>(b) * cols + n];
+    for (int b = group; b < bands; b += BS_GROUPS) s += part[static_cast<size_t>(b) * cols + n];
   }
   lds[group][c] = s;
   __syncthreads();
   if (group || n >= cols) return;
 #pragma unroll
-  for (int g = 1; g < 8; ++g) s += lds[g][c];
+  for (int g = 1; g < BS_GROUPS; ++g) s += lds[g][c];
   if (accumulate) s += to_f32(db[n]);
   db[n] = from_f32<T>(s);
 }
 template <class T>
 int launch_db(const float *part, T *db, int bands, int hidden, int accumulate) {
   ProfScope prof("gated_ff_db", 8.0 * bands * hidden, WORK_BYTE);
-  TDH_LAUNCH((bias_sum_kernel<T>), dim3(ceil_div(2 * hidden, 32)), dim3(GF_NT), 0, ctx().stream, part, db, bands, 2 * hidden, accumulate);
+  TDH_LAUNCH((bias_sum_kernel<T>), dim3(ceil_div(2 * hidden, 32)), dim3(32 * BS_GROUPS), 0, ctx().stream, part, db, bands, 2 * hidden,
+             accumulate);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
@@ -910,11 +912,12 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
 // fp32 matrices to their three planes, a thread eight neighbours. sign: 1 turns every other group of 32 rows, 2 of columns.
 // Bound by memory, 4 bytes in and 6 out (1344 -> 2 x 2640 and 2000 samples, three launches of a step: 54 us, 5.6 TB/s). A pass of its own:
 // within a product the split would be made again by every tile that reads the element, on the vector units beside its products.
+// Columns come in one or two halves of `used` values, `half` (a multiple of 8) apart in the planes, zero behind a half.
 struct SplitJobs {
   struct Job {
     const float *src;
-    uint16_t *dst;   // planes, rows * cols elements each
-    int cols, sign;
+    uint16_t *dst;   // planes, 8 * words elements each
+    int used, half, halves, sign;
     unsigned blocks;
     size_t words;    // of eight elements
   } job[2];
@@ -925,33 +928,41 @@ split_kernel(const SplitJobs jobs) {
   const SplitJobs::Job &j = jobs.job[second];
   const size_t i = static_cast<size_t>(blockIdx.x - (second ? jobs.job[0].blocks : 0)) * GF_NT + threadIdx.x;
   if (i >= j.words) return;
-  const size_t row = i / (j.cols / 8);
-  const int col    = static_cast<int>(i - row * (j.cols / 8)) * 8;
+  const int per = j.half / 8;   // words of a half
+  const size_t row = i / (per * j.halves);
+  const int col = static_cast<int>(i - row * (per * j.halves)) * 8, h = col >= j.half ? 1 : 0, c0 = col - h * j.half;
   const bool turn  = j.sign == 1 ? (row / X3P_BK) & 1 : j.sign == 2 ? (col / X3P_BK) & 1 : false;
   const float scale = turn ? -X3_SCALE : X3_SCALE;
+  const float *p = j.src + (row * j.halves + h) * j.used + c0;
   float v[8];
-  load8(j.src + i * 8, v);
+  if (c0 + 8 <= j.used) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c0 + e < j.used ? p[e] : 0.0f;
+  }
   uint4 out[X3_PARTS];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     uint32_t part[X3_PARTS];
     split_pair(scale * v[2 * c], scale * v[2 * c + 1], part);
 #pragma unroll
-    for (int p = 0; p < X3_PARTS; ++p) (&out[p].x)[c] = part[p];
+    for (int q = 0; q < X3_PARTS; ++q) (&out[q].x)[c] = part[q];
   }
 #pragma unroll
-  for (int p = 0; p < X3_PARTS; ++p) reinterpret_cast<uint4 *>(j.dst)[p * j.words + i] = out[p];
+  for (int q = 0; q < X3_PARTS; ++q) reinterpret_cast<uint4 *>(j.dst)[q * j.words + i] = out[q];
 }
 struct Splitter {
   SplitJobs jobs{};
   int n = 0;
-  static size_t bytes(size_t rows, int cols) { return ws_align(6 * rows * cols); }
-  int add(const float *src, int rows, int cols, int sign, G16Matrix *out) {
+  static size_t bytes(size_t rows, int used, int halves) { return ws_align(6 * rows * halves * padded(used)); }
+  int add(const float *src, int rows, int used, int halves, int sign, G16Matrix *out) {
+    const int half = padded(used);
     SplitJobs::Job &j = jobs.job[n++];
-    j = {src, nullptr, cols, sign, 0, static_cast<size_t>(rows) * cols / 8};
+    j = {src, nullptr, used, half, halves, sign, 0, static_cast<size_t>(rows) * halves * half / 8};
     j.blocks = static_cast<unsigned>(ceil_div_sz(j.words, GF_NT));
     TDH_TRY(take(j.words * 24, &j.dst));
-    *out = G16Matrix{j.dst, cols, rows, cols};
+    *out = G16Matrix{j.dst, static_cast<long>(halves) * half, rows, halves * half};
     return TDH_OK;
   }
   int run() {
@@ -1004,32 +1015,40 @@ int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad
 }
 
 // Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do. us of a
-// training step on them and on the fully-connected layer's products: 1024 -> 2 x 2048, 1200 samples 271 / 272, 2400 463 / 473; 1344
-// -> 2 x 2640, 800 samples 307 / 305, 2000 633 / 681; numbers of samples that are no multiple of four, for which that
-// layer's three-part products do not apply: 801 208 / 255, 1601 330 / 447.
-bool x3_fits(int in, int hidden) { return in % 8 == 0 && hidden % 8 == 0; }
-constexpr int X3P_BATCH = 1000, X3P_BATCH_ODD = 320, X3P_DW_BATCH = 128;
-constexpr double X3P_FLOP = 4e9;   // below that the products are short
-bool x3_weights(int in, int hidden, int batch) {
-  return x3_fits(in, hidden) && batch >= (batch % 4 ? X3P_BATCH_ODD : X3P_BATCH) && 4.0 * batch * in * hidden >= X3P_FLOP;
+// training step on planes and on the fully-connected layer's products: 1024 -> 2 x 2048, 1200 samples 271 / 272, 2400 463 / 473; 1344
+// -> 2 x 2640, 800 samples 307 / 305, 2000 633 / 681; 2000 -> 2 x 64, 20000 samples 483 / 407; 12 -> 2 x 2000, 20000 samples 689 / 782. Sizes that are no multiple of four, which
+// that layer's own three-part products do not take and its others read element by element: 1023 -> 2 x 2047, 128 samples 91 / 79, 200 105 /
+// 122, 801 202 / 377; 4097 -> 2 x 4099, 100 samples 378 / 332, 257 598 / 1039; 2002 -> 2 x 301, 200 samples 75 / 66, 1000
+// 120 / 166; 1999 -> 2 x 25, 20001 samples 454 / 426, 2 x 37 481 / 550.
+constexpr int X3P_BATCH = 1000, X3P_BATCH_ODD = 160, X3P_DW_BATCH = 128;
+constexpr double X3P_FLOP = 4e9, X3P_FLOP_ODD = 1e9;   // below that the products are short
+constexpr int X3P_IN = 12, X3P_HIDDEN = 128, X3P_HIDDEN_ODD = 32;   // narrower ones leave most of a tile empty
+bool x3_pays(int in, int hidden, int batch, int from) {
+  const bool odd = batch % 4 || in % 4 || hidden % 2;
+  return in >= X3P_IN && hidden >= (odd ? X3P_HIDDEN_ODD : X3P_HIDDEN) && batch >= (odd ? X3P_BATCH_ODD : from) &&
+         4.0 * batch * in * hidden >= (odd ? X3P_FLOP_ODD : X3P_FLOP);
 }
-bool x3_dw(int in, int hidden, int batch) { return x3_fits(in, hidden) && batch >= X3P_DW_BATCH && 4.0 * batch * in * hidden >= X3P_FLOP; }
+bool x3_weights(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_BATCH); }
+bool x3_dw(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_DW_BATCH); }
 
+constexpr int FF_OWN_DB = 512;
 int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *b, float *h, float *z) {
   const size_t nz = static_cast<size_t>(batch) * 2 * hidden;
   if (x3_weights(in, hidden, batch)) {
-    const FfPlan plan = x3_plan(batch, 2 * hidden, in);
-    TDH_TRY(ws_begin(Splitter::bytes(batch, in) + Splitter::bytes(in, 2 * hidden) + ff_partial_bytes(plan, nz)));
+    const int half    = padded(hidden);
+    const size_t part = static_cast<size_t>(batch) * 2 * half;
+    const FfPlan plan = x3_plan(batch, 2 * half, in);
+    TDH_TRY(ws_begin(Splitter::bytes(batch, in, 1) + Splitter::bytes(in, hidden, 2) + ff_partial_bytes(plan, part)));
     Splitter split;
     G16Matrix X, W;
-    TDH_TRY(split.add(x, batch, in, 2, &X));
-    TDH_TRY(split.add(w, in, 2 * hidden, 0, &W));
+    TDH_TRY(split.add(x, batch, in, 1, 2, &X));
+    TDH_TRY(split.add(w, in, hidden, 2, 0, &W));
     TDH_TRY(split.run());
-    const X3Source src{x, w, in, 1, 2L * hidden, 1, batch, 2 * hidden};
-    EpiGate<float> epi{h, z, b, nullptr, batch, hidden, hidden, act};
+    const X3Source src{x, w, in, 1, 2L * hidden, 1, batch, 2 * half, {in, in}, {hidden, half}};
+    EpiGate<float> epi{h, z, b, nullptr, batch, hidden, half, act};
     if (plan.splits == 1) return x3_gemm<true, false, true>(plan, X, W, src, epi, in, "gated_ff_fwd_x3");
-    TDH_TRY(take(plan.splits * nz, &epi.partial));
-    const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * hidden, hidden, hidden, 0};
+    TDH_TRY(take(plan.splits * part, &epi.partial));
+    const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * half, hidden, half, 0};
     TDH_TRY((x3_gemm<true, false, false>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
     return launch_gate_reduce(epi, plan.splits);
   }
@@ -1044,36 +1063,38 @@ int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
 }
 int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *z, const float *dh, float *dx,
                float *dw, float *db, int accumulate) {
-  const int cols = 2 * hidden;
+  const int cols = 2 * hidden, half = padded(hidden);
   const bool planes_x = dx && x3_weights(in, hidden, batch), planes_w = dw && x3_dw(in, hidden, batch);
-  const bool own_db   = db && planes_w;   // (else the sums ride along with dw's launch)
+  // db by the bands of the dz pass, 4 us; without planes the layer's column sums, which ride along with dw's launch or take 5 us at
+  // 500 samples, 24 at 4000, 540 at 100000
+  const bool own_db   = db && (planes_w || batch > FF_OWN_DB);
   const DzPlan pz     = dz_plan<float>(hidden, batch, own_db);
-  const size_t nz = static_cast<size_t>(batch) * cols, nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * cols;
+  const size_t nz = static_cast<size_t>(batch) * cols, nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
   TDH_TRY(ws_begin(ws_align(4 * nz) + (own_db ? ws_align(4 * static_cast<size_t>(pz.bands) * cols) : 0) +
-                   (planes_x || planes_w ? Splitter::bytes(batch, cols) : 0) +
-                   (planes_x ? Splitter::bytes(in, cols) + ff_partial_bytes(x3_plan(batch, in, cols), nx) : 0) +
-                   (planes_w ? Splitter::bytes(batch, in) + ff_partial_bytes(x3_plan(in, cols, batch), nw) : 0) +
+                   (planes_x || planes_w ? Splitter::bytes(batch, hidden, 2) : 0) +
+                   (planes_x ? Splitter::bytes(in, hidden, 2) + ff_partial_bytes(x3_plan(batch, in, 2 * half), nx) : 0) +
+                   (planes_w ? Splitter::bytes(batch, in, 1) + ff_partial_bytes(x3_plan(in, 2 * half, batch), nw) : 0) +
                    (planes_x && planes_w ? 0 : fc_workspace_bytes(in, cols, batch))));
   float *dz = nullptr, *bias_part = nullptr;
   TDH_TRY(take(nz, &dz));
   if (own_db) TDH_TRY(take(static_cast<size_t>(pz.bands) * cols, &bias_part));
   TDH_TRY(launch_dz(pz, act, hidden, hidden, batch, z, dh, dz, bias_part));
   if (own_db) TDH_TRY(launch_db(bias_part, db, pz.bands, hidden, accumulate));
-  if (!planes_x && !planes_w)
-    return fc_bwd(in, cols, db != nullptr, batch, x, w, dz, dx, dw, db, accumulate, ActGrad());
-  G16Matrix Z, X, W;
-  Splitter split, weights;
-  TDH_TRY(split.add(dz, batch, cols, 0, &Z));
-  if (planes_w) TDH_TRY(split.add(x, batch, in, 1, &X));
-  TDH_TRY(split.run());
-  if (planes_w)
-    TDH_TRY((x3_grad<false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, cols},
-                                   EpiGrad<float>{dw, nullptr, in, cols, hidden, hidden, accumulate}, batch, "gated_ff_dw_x3")));
-  if (planes_x) {
-    TDH_TRY(weights.add(w, in, cols, 2, &W));
-    TDH_TRY(weights.run());
-    TDH_TRY((x3_grad<true, true>(Z, W, X3Source{dz, w, cols, 1, 1, cols, batch, in},
-                                 EpiGrad<float>{dx, nullptr, batch, in, in, in, 0}, cols, "gated_ff_dx_x3")));
+  if (planes_x || planes_w) {
+    G16Matrix Z, X, W;
+    Splitter split, weights;
+    TDH_TRY(split.add(dz, batch, hidden, 2, 0, &Z));
+    if (planes_w) TDH_TRY(split.add(x, batch, in, 1, 1, &X));
+    TDH_TRY(split.run());
+    if (planes_w)
+      TDH_TRY((x3_grad<false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, 2 * half, {batch, batch}, {hidden, half}},
+                                     EpiGrad<float>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw_x3")));
+    if (planes_x) {
+      TDH_TRY(weights.add(w, in, hidden, 2, 2, &W));
+      TDH_TRY(weights.run());
+      TDH_TRY((x3_grad<true, true>(Z, W, X3Source{dz, w, cols, 1, 1, cols, batch, in, {hidden, half}, {in, in}},
+                                   EpiGrad<float>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx_x3")));
+    }
   }
   if ((dx && !planes_x) || (dw && !planes_w) || (db && !own_db))
     return fc_bwd(in, cols, db && !own_db, batch, x, w, dz, planes_x ? nullptr : dx, planes_w ? nullptr : dw, own_db ? nullptr : db,

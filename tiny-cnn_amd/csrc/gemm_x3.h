@@ -2,7 +2,7 @@
 //
 // fc_x3.hip splits its operands on the way into LDS, once for every tile that reads them, which costs more vector
 // instructions than there are matrix instructions to hide them behind. Here every element is split once, by a pass of
-// its own that writes three planes (10 bytes moved an element), and tiles of 32 reduction indices of all three planes
+// its own that writes three planes (10 bytes moved an element; rows of any length, padded to whole words), and tiles of 32 reduction indices of all three planes
 // go straight into LDS. Worth its pass where an operand is read by many tiles. One operand's planes carry the sign
 // of their step (split_bf16.h: steps take turns between the product and its negative).
 //
@@ -20,12 +20,19 @@ namespace {
 
 constexpr int X3P_BK = 32;
 
+// The planes' columns come in one or two halves, `half` apart, of which `used` are in use and have neighbours in the fp32 matrix.
+struct X3Span {
+  int used, half;
+  // where column i of the planes lies in the matrix, or -1
+  __device__ __forceinline__ int at(const int i) const { return i < used ? i : i >= half && i - half < used ? i - half + used : -1; }
+};
 // The fp32 matrices themselves, for sums that come out infinite or NaN: element (m, k) at a[m am + k ak], (k, n) at
-// b[k bk + n bn]; rows and cols of C.
+// b[k bk + n bn] with k and n in the matrices' own columns; rows and cols of C, in the planes'.
 struct X3Source {
   const float *a, *b;
   long am, ak, bk, bn;
   int rows, cols;
+  X3Span k, n;
 };
 
 template <bool A_KC, bool B_KC, bool PAIR, class Epi>
@@ -99,8 +106,8 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
     int col[TN];   // (PAIR: of either half)
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int hidden = src.cols >> 1, n = PAIR ? nw + 32 * (j >> 1) + l32 : nw + 32 * j + l32;
-      col[j] = n < (PAIR ? hidden : src.cols) ? n + (PAIR ? (j & 1) * hidden : 0) : -1;
+      const int n = PAIR ? nw + 32 * (j >> 1) + l32 : nw + 32 * j + l32;
+      col[j]      = n >= (PAIR ? src.n.half : src.cols) ? -1 : src.n.at(PAIR ? n + (j & 1) * src.n.half : n);
     }
     x3_redo(reinterpret_cast<floatx16_x3(&)[TM * TN]>(acc), [&](int b, int r) {
       return mw + 32 * (b / TN) + 8 * (r >> 2) + 4 * half + (r & 3) < src.rows && col[b % TN] >= 0;
@@ -110,14 +117,14 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
         float av[4][TM], bv[4][TN];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const int k = k0 + 2 * s + half;
+          const int kp = k0 + 2 * s + half, k = kp < kend ? src.k.at(kp) : -1;
 #pragma unroll
           for (int i = 0; i < TM; ++i) {
             const int m = mw + 32 * i + l32;
-            av[s][i] = k < kend && m < src.rows ? src.a[m * src.am + k * src.ak] : 0.0f;
+            av[s][i] = k >= 0 && m < src.rows ? src.a[m * src.am + k * src.ak] : 0.0f;
           }
 #pragma unroll
-          for (int j = 0; j < TN; ++j) bv[s][j] = k < kend && col[j] >= 0 ? src.b[k * src.bk + col[j] * src.bn] : 0.0f;
+          for (int j = 0; j < TN; ++j) bv[s][j] = k >= 0 && col[j] >= 0 ? src.b[k * src.bk + col[j] * src.bn] : 0.0f;
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s)
