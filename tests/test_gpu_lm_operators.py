@@ -164,6 +164,12 @@ def test_gated_ff_of_many_samples_unaligned_and_accumulating(T, dtype):
     ff_case(T, (1001, 1024, 1000), "gelu", dtype, bias=True, skew=1, accumulate=True)
 
 
+@pytest.mark.parametrize("shape", [(2000, 1208, 1224), (256, 1344, 1400), (2004, 1300, 1202)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_ff_of_many_samples_in_fours(T, shape):
+    """(fp32: the weight gradient alone on planes, and all three products)"""
+    ff_case(T, shape, "silu", "f32", bias=True)
+
+
 @pytest.mark.parametrize("skew", [0, 1])
 @pytest.mark.parametrize("shape", [(1001, 1027, 1001), (402, 1401, 1803), (130, 2811, 2797), (1500, 1340, 501), (20001, 65, 801)],
                          ids=lambda s: "x".join(map(str, s)))
@@ -175,7 +181,15 @@ def test_gated_ff_of_many_samples_with_rows_of_any_length(T, shape, skew):
 @pytest.mark.parametrize("dtype", L.DTYPES)
 def test_gated_ff_of_many_samples_with_infinities(T, dtype):
     """An infinite or NaN value reaches the sums that it is part of, which are what fp32 arithmetic gives, and no others."""
-    n, d, f = 1001, 1024, 1000
+    many_samples_with_infinities(T, dtype, 1001, 1024, 1000)
+
+
+@pytest.mark.parametrize("shape", [(1002, 1027, 1001), (1001, 1025, 505)])
+def test_gated_ff_of_many_samples_with_infinities_at_any_length(T, shape):
+    many_samples_with_infinities(T, "f32", *shape)
+
+
+def many_samples_with_infinities(T, dtype, n, d, f):
     rng = np.random.RandomState(12)
     x, w, dh = rng.randn(n, d), rng.randn(d, 2 * f) / 32, rng.randn(n, f)
     x[3, 17], x[900, 5], x[1000, 1023] = np.inf, np.nan, -np.inf

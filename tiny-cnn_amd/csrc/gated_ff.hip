@@ -1014,19 +1014,20 @@ int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad
   return plan.splits > 1 ? launch_grad_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
 }
 
-// Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do. us of a
-// training step on planes and on the fully-connected layer's products: 1024 -> 2 x 2048, 1200 samples 271 / 272, 2400 463 / 473; 1344
-// -> 2 x 2640, 800 samples 307 / 305, 2000 633 / 681; 2000 -> 2 x 64, 20000 samples 483 / 407; 12 -> 2 x 2000, 20000 samples 689 / 782. Sizes that are no multiple of four, which
-// that layer's own three-part products do not take and its others read element by element: 1023 -> 2 x 2047, 128 samples 91 / 79, 200 105 /
-// 122, 801 202 / 377; 4097 -> 2 x 4099, 100 samples 378 / 332, 257 598 / 1039; 2002 -> 2 x 301, 200 samples 75 / 66, 1000
-// 120 / 166; 1999 -> 2 x 25, 20001 samples 454 / 426, 2 x 37 481 / 550.
-constexpr int X3P_BATCH = 1000, X3P_BATCH_ODD = 160, X3P_DW_BATCH = 128;
-constexpr double X3P_FLOP = 4e9, X3P_FLOP_ODD = 1e9;   // below that the products are short
-constexpr int X3P_IN = 12, X3P_HIDDEN = 128, X3P_HIDDEN_ODD = 32;   // narrower ones leave most of a tile empty
+// Whether the weights' planes pay for themselves (they are made anew in every call), and whether those of x and dz do: the pass that
+// writes planes grows with in + 2 hidden, what the product gains by them with in * hidden. us of a training step with all three products
+// on planes, dW alone, and none (the fully-connected layer's products): 1024 -> 2 x 2048, 256 samples 105 / 95 / 104, 1200 266 / 266 /
+// 262, 4000 658 / 695 / 686; 1344 -> 2 x 2640, 200 samples 135 / 110 / 129, 2000 632 / 652 / 654; 4096 -> 2 x 4096, 256 samples 472 / 358 /
+// 396; 2000 -> 2 x 200, 8000 samples 378 / 363 / 344; 128 -> 2 x 2000, 20000 samples 818 / 945 / 798.
+// Sizes that are no multiple of four the layer's own three-part products do not take, and its others read element by element: 1023 ->
+// 2 x 2047, 128 samples 91 / - / 79, 200 105 / - / 122, 801 202 / - / 377; 4097 -> 2 x 4099, 100 samples 378 / - / 332, 257 598 / - / 1039;
+// 331 -> 2 x 333, 1501 samples 85 / 96 / 98; 61 -> 2 x 1999, 20001 samples 838 / 962 / 895; 1999 -> 2 x 50 505 / 520 / 493, 2 x 61 496 / 563 / 550.
+constexpr int X3P_BATCH = 2000, X3P_DW_BATCH = 128, X3P_BATCH_ODD = 160, X3P_SIZE = 400, X3P_SIZE_ODD = 40;
+constexpr double X3P_FLOP = 6e8;   // below that the products are short
 bool x3_pays(int in, int hidden, int batch, int from) {
   const bool odd = batch % 4 || in % 4 || hidden % 2;
-  return in >= X3P_IN && hidden >= (odd ? X3P_HIDDEN_ODD : X3P_HIDDEN) && batch >= (odd ? X3P_BATCH_ODD : from) &&
-         4.0 * batch * in * hidden >= (odd ? X3P_FLOP_ODD : X3P_FLOP);
+  return batch >= (odd ? X3P_BATCH_ODD : from) && 4.0 * batch * in * hidden >= X3P_FLOP &&
+         static_cast<double>(in) * hidden >= (odd ? X3P_SIZE_ODD : X3P_SIZE) * (in + 2.0 * hidden);
 }
 bool x3_weights(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_BATCH); }
 bool x3_dw(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_DW_BATCH); }
