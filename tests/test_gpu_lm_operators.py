@@ -171,7 +171,7 @@ def test_gated_ff_of_many_samples_in_fours(T, shape):
 
 
 @pytest.mark.parametrize("skew", [0, 1])
-@pytest.mark.parametrize("shape", [(1001, 1027, 1001), (402, 1401, 1803), (130, 2811, 2797), (1500, 1340, 501), (20001, 65, 801)],
+@pytest.mark.parametrize("shape", [(1001, 1027, 1001), (402, 1401, 1803), (130, 2811, 2797), (1500, 1340, 501), (20001, 65, 801), (161, 1027, 2049), (67, 4097, 4099)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_gated_ff_of_many_samples_with_rows_of_any_length(T, shape, skew):
     """(fp32 products in three parts, whose copies are padded to whole words)"""
@@ -184,7 +184,7 @@ def test_gated_ff_of_many_samples_with_infinities(T, dtype):
     many_samples_with_infinities(T, dtype, 1001, 1024, 1000)
 
 
-@pytest.mark.parametrize("shape", [(1002, 1027, 1001), (1001, 1025, 505)])
+@pytest.mark.parametrize("shape", [(1002, 1027, 1001), (1001, 1025, 505), (501, 1031, 1003)])
 def test_gated_ff_of_many_samples_with_infinities_at_any_length(T, shape):
     many_samples_with_infinities(T, "f32", *shape)
 
@@ -192,7 +192,7 @@ def test_gated_ff_of_many_samples_with_infinities_at_any_length(T, shape):
 def many_samples_with_infinities(T, dtype, n, d, f):
     rng = np.random.RandomState(12)
     x, w, dh = rng.randn(n, d), rng.randn(d, 2 * f) / 32, rng.randn(n, f)
-    x[3, 17], x[900, 5], x[1000, 1023] = np.inf, np.nan, -np.inf
+    x[3, 17], x[n - 101, 5], x[n - 1, 1023] = np.inf, np.nan, -np.inf
     w[40, 7] = np.inf
     x, w, dh = (L.rounded(v, dtype) for v in (x, w, dh))
     bx, bw, bdh = (Buf(T, v, dtype) for v in (x, w, dh))

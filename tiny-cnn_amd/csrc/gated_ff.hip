@@ -995,22 +995,22 @@ FfPlan x3_plan(int M, int N, int K) {
   }
   return best;
 }
-template <bool A_KC, bool B_KC, bool PAIR, class Epi>
+template <bool A_KC, bool B_KC, bool PAIR, bool ON_THE_WAY, class Epi>
 int x3_gemm(const FfPlan &p, const G16Matrix &A, const G16Matrix &B, const X3Source &src, const Epi &epi, int K, const char *tag) {
   ProfScope prof(tag, src.rows, src.cols, K);
   const int tiles_m = ceil_div(src.rows, X3P_TILE), tiles_n = PAIR ? ceil_div(src.cols / 2, X3P_TILE / 2) : ceil_div(src.cols, X3P_TILE);
-  TDH_LAUNCH((gemm_x3_kernel<A_KC, B_KC, PAIR, Epi>), dim3(static_cast<unsigned>(tiles_m) * tiles_n * p.splits), dim3(256), 0,
+  TDH_LAUNCH((gemm_x3_kernel<A_KC, B_KC, PAIR, ON_THE_WAY, Epi>), dim3(static_cast<unsigned>(tiles_m) * tiles_n * p.splits), dim3(256), 0,
              ctx().stream, A, B, static_cast<long>(A.rows) * A.cols, static_cast<long>(B.rows) * B.cols, src, epi, tiles_m, tiles_n, K,
              p.k_per_split);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
-template <bool A_KC, bool B_KC>
+template <bool A_KC, bool B_KC, bool ON_THE_WAY>
 int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad<float> epi, int K, const char *tag) {
   const FfPlan plan  = x3_plan(src.rows, src.cols, K);
   const size_t total = static_cast<size_t>(src.rows) * src.cols;
   if (plan.splits > 1) TDH_TRY(take(plan.splits * total, &epi.partial));
-  TDH_TRY((x3_gemm<A_KC, B_KC, false>(plan, A, B, src, epi, K, tag)));
+  TDH_TRY((x3_gemm<A_KC, B_KC, false, ON_THE_WAY>(plan, A, B, src, epi, K, tag)));
   return plan.splits > 1 ? launch_grad_reduce(epi, plan.splits) : static_cast<int>(TDH_OK);
 }
 
@@ -1020,15 +1020,20 @@ int x3_grad(const G16Matrix &A, const G16Matrix &B, const X3Source &src, EpiGrad
 // 262, 4000 658 / 695 / 686; 1344 -> 2 x 2640, 200 samples 135 / 110 / 129, 2000 632 / 652 / 654; 4096 -> 2 x 4096, 256 samples 472 / 358 /
 // 396; 2000 -> 2 x 200, 8000 samples 378 / 363 / 344; 128 -> 2 x 2000, 20000 samples 818 / 945 / 798.
 // Sizes that are no multiple of four the layer's own three-part products do not take, and its others read element by element: 1023 ->
-// 2 x 2047, 128 samples 91 / - / 79, 200 105 / - / 122, 801 202 / - / 377; 4097 -> 2 x 4099, 100 samples 378 / - / 332, 257 598 / - / 1039;
-// 331 -> 2 x 333, 1501 samples 85 / 96 / 98; 61 -> 2 x 1999, 20001 samples 838 / 962 / 895; 1999 -> 2 x 50 505 / 520 / 493, 2 x 61 496 / 563 / 550.
-constexpr int X3P_BATCH = 2000, X3P_DW_BATCH = 128, X3P_BATCH_ODD = 160, X3P_SIZE = 400, X3P_SIZE_ODD = 40;
-constexpr double X3P_FLOP = 6e8;   // below that the products are short
+// 2 x 2047, 128 samples 85 / - / 79, 200 105 / - / 122, 801 202 / - / 377; 4097 -> 2 x 4099, 33 samples 227 / - / 198, 65 244 / - / 330, 257 543 / -
+// / 1034; 331 -> 2 x 333, 1501 samples 85 / 96 / 98; 61 -> 2 x 1999, 20001 samples 838 / 962 / 895; 1999 -> 2 x 50 505 / 520 / 493, 2 x 61 496 /
+// 563 / 550.
+constexpr int X3P_BATCH = 2000, X3P_DW_BATCH = 128, X3P_BATCH_ODD = 160, X3P_BATCH_ODD_LARGE = 65, X3P_SIZE = 400, X3P_SIZE_ODD = 40;
+constexpr double X3P_FLOP = 6e8, X3P_FLOP_LARGE = 4e9;   // below the first the products are short
 bool x3_pays(int in, int hidden, int batch, int from) {
-  const bool odd = batch % 4 || in % 4 || hidden % 2;
-  return batch >= (odd ? X3P_BATCH_ODD : from) && 4.0 * batch * in * hidden >= X3P_FLOP &&
+  const bool odd    = batch % 4 || in % 4 || hidden % 2;
+  const double flop = 4.0 * batch * in * hidden;
+  return batch >= (!odd ? from : flop >= X3P_FLOP_LARGE ? X3P_BATCH_ODD_LARGE : X3P_BATCH_ODD) && flop >= X3P_FLOP &&
          static_cast<double>(in) * hidden >= (odd ? X3P_SIZE_ODD : X3P_SIZE) * (in + 2.0 * hidden);
 }
+// Up to so many samples few tiles read a weight, and the forward product and dX split it on the way into LDS: 4097 -> 2 x 4099, 257
+// samples 543, with planes 598; 701 -> 2 x 703, 501 samples 87 / 91; 1023 -> 2 x 2047, 801 samples 215 / 202.
+constexpr int X3P_ON_THE_WAY = 512;
 bool x3_weights(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_BATCH); }
 bool x3_dw(int in, int hidden, int batch) { return x3_pays(in, hidden, batch, X3P_DW_BATCH); }
 
@@ -1039,18 +1044,24 @@ int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
     const int half    = padded(hidden);
     const size_t part = static_cast<size_t>(batch) * 2 * half;
     const FfPlan plan = x3_plan(batch, 2 * half, in);
-    TDH_TRY(ws_begin(Splitter::bytes(batch, in, 1) + Splitter::bytes(in, hidden, 2) + ff_partial_bytes(plan, part)));
+    const bool way    = batch <= X3P_ON_THE_WAY;
+    TDH_TRY(ws_begin(Splitter::bytes(batch, in, 1) + (way ? 0 : Splitter::bytes(in, hidden, 2)) + ff_partial_bytes(plan, part)));
     Splitter split;
-    G16Matrix X, W;
-    TDH_TRY(split.add(x, batch, in, 1, 2, &X));
-    TDH_TRY(split.add(w, in, hidden, 2, 0, &W));
+    G16Matrix X, W{};
+    TDH_TRY(split.add(x, batch, in, 1, way ? 0 : 2, &X));
+    if (!way) TDH_TRY(split.add(w, in, hidden, 2, 0, &W));
     TDH_TRY(split.run());
     const X3Source src{x, w, in, 1, 2L * hidden, 1, batch, 2 * half, {in, in}, {hidden, half}};
     EpiGate<float> epi{h, z, b, nullptr, batch, hidden, half, act};
-    if (plan.splits == 1) return x3_gemm<true, false, true>(plan, X, W, src, epi, in, "gated_ff_fwd_x3");
+    if (plan.splits == 1)
+      return way ? x3_gemm<true, false, true, true>(plan, X, W, src, epi, in, "gated_ff_fwd_x3")
+                 : x3_gemm<true, false, true, false>(plan, X, W, src, epi, in, "gated_ff_fwd_x3");
     TDH_TRY(take(plan.splits * part, &epi.partial));
     const EpiGrad<float> slices{nullptr, epi.partial, batch, 2 * half, hidden, half, 0};
-    TDH_TRY((x3_gemm<true, false, false>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
+    if (way)
+      TDH_TRY((x3_gemm<true, false, false, true>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
+    else
+      TDH_TRY((x3_gemm<true, false, false, false>(plan, X, W, src, slices, in, "gated_ff_fwd_x3")));
     return launch_gate_reduce(epi, plan.splits);
   }
   TDH_TRY(ws_begin(fc_workspace_bytes(in, 2 * hidden, batch) + (z ? 0 : ws_align(4 * nz))));
@@ -1065,7 +1076,7 @@ int ff_fwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
 int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const float *w, const float *z, const float *dh, float *dx,
                float *dw, float *db, int accumulate) {
   const int cols = 2 * hidden, half = padded(hidden);
-  const bool planes_x = dx && x3_weights(in, hidden, batch), planes_w = dw && x3_dw(in, hidden, batch);
+  const bool planes_x = dx && x3_weights(in, hidden, batch), planes_w = dw && x3_dw(in, hidden, batch), way = batch <= X3P_ON_THE_WAY;
   // db by the bands of the dz pass, 4 us; without planes the layer's column sums, which ride along with dw's launch or take 5 us at
   // 500 samples, 24 at 4000, 540 at 100000
   const bool own_db   = db && (planes_w || batch > FF_OWN_DB);
@@ -1073,7 +1084,7 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   const size_t nz = static_cast<size_t>(batch) * cols, nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
   TDH_TRY(ws_begin(ws_align(4 * nz) + (own_db ? ws_align(4 * static_cast<size_t>(pz.bands) * cols) : 0) +
                    (planes_x || planes_w ? Splitter::bytes(batch, hidden, 2) : 0) +
-                   (planes_x ? Splitter::bytes(in, hidden, 2) + ff_partial_bytes(x3_plan(batch, in, 2 * half), nx) : 0) +
+                   (planes_x ? (way ? 0 : Splitter::bytes(in, hidden, 2)) + ff_partial_bytes(x3_plan(batch, in, 2 * half), nx) : 0) +
                    (planes_w ? Splitter::bytes(batch, in, 1) + ff_partial_bytes(x3_plan(in, 2 * half, batch), nw) : 0) +
                    (planes_x && planes_w ? 0 : fc_workspace_bytes(in, cols, batch))));
   float *dz = nullptr, *bias_part = nullptr;
@@ -1082,19 +1093,24 @@ int ff_bwd_f32(int act, int in, int hidden, int batch, const float *x, const flo
   TDH_TRY(launch_dz(pz, act, hidden, hidden, batch, z, dh, dz, bias_part));
   if (own_db) TDH_TRY(launch_db(bias_part, db, pz.bands, hidden, accumulate));
   if (planes_x || planes_w) {
-    G16Matrix Z, X, W;
+    G16Matrix Z, X, W{};
     Splitter split, weights;
     TDH_TRY(split.add(dz, batch, hidden, 2, 0, &Z));
     if (planes_w) TDH_TRY(split.add(x, batch, in, 1, 1, &X));
     TDH_TRY(split.run());
     if (planes_w)
-      TDH_TRY((x3_grad<false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, 2 * half, {batch, batch}, {hidden, half}},
+      TDH_TRY((x3_grad<false, false, false>(X, Z, X3Source{x, dz, 1, in, cols, 1, in, 2 * half, {batch, batch}, {hidden, half}},
                                      EpiGrad<float>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw_x3")));
     if (planes_x) {
-      TDH_TRY(weights.add(w, in, hidden, 2, 2, &W));
-      TDH_TRY(weights.run());
-      TDH_TRY((x3_grad<true, true>(Z, W, X3Source{dz, w, cols, 1, 1, cols, batch, in, {hidden, half}, {in, in}},
-                                   EpiGrad<float>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx_x3")));
+      const X3Source src{dz, w, cols, 1, 1, cols, batch, in, {hidden, half}, {in, in}};
+      const EpiGrad<float> epi{dx, nullptr, batch, in, in, in, 0};
+      if (way) {
+        TDH_TRY((x3_grad<true, true, true>(Z, W, src, epi, 2 * half, "gated_ff_dx_x3")));
+      } else {
+        TDH_TRY(weights.add(w, in, hidden, 2, 2, &W));
+        TDH_TRY(weights.run());
+        TDH_TRY((x3_grad<true, true, false>(Z, W, src, epi, 2 * half, "gated_ff_dx_x3")));
+      }
     }
   }
   if ((dx && !planes_x) || (dw && !planes_w) || (db && !own_db))

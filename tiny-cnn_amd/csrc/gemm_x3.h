@@ -2,9 +2,10 @@
 //
 // fc_x3.hip splits its operands on the way into LDS, once for every tile that reads them, which costs more vector
 // instructions than there are matrix instructions to hide them behind. Here every element is split once, by a pass of
-// its own that writes three planes (10 bytes moved an element; rows of any length, padded to whole words), and tiles of 32 reduction indices of all three planes
-// go straight into LDS. Worth its pass where an operand is read by many tiles. One operand's planes carry the sign
-// of their step (split_bf16.h: steps take turns between the product and its negative).
+// its own that writes three planes (10 bytes moved an element, rows padded to whole words), and tiles of 32 reduction indices
+// of all three planes go straight into LDS. Worth its pass where an operand is read by many tiles; where few read B, it is split on
+// its way into LDS after all (ON_THE_WAY). One operand carries the sign of its step (split_bf16.h: steps take turns between the
+// product and its negative).
 //
 // Tiles of 128 x 128 on four waves, one of them in LDS at a time (48 KB), two workgroups a compute unit that cover each
 // other's loads and epilogues: 4096 x 8192 with k of 256 in 102 us, 4096 x 4096 with k of 2048 in 314 (m, n), 351 (k, k)
@@ -35,7 +36,62 @@ struct X3Source {
   X3Span k, n;
 };
 
-template <bool A_KC, bool B_KC, bool PAIR, class Epi>
+// B's tile of Side from the fp32 matrix, split on the way into LDS: what a thread has of it, eight neighbours a chunk.
+template <class Side, bool KC, bool PAIR, int NT>
+struct X3OnTheWay {
+  float v[Side::PER][8];
+  uint4 part[Side::PER][X3_PARTS];
+  // asks for the tile at k0 (`left`: reduction indices from there), whose first column is `first`
+  __device__ __forceinline__ void load(const X3Source &src, const int first, const int k0, const int left, const int tid) {
+#pragma unroll
+    for (int i = 0; i < Side::PER; ++i) {
+      int row, chunk;
+      Side::place(tid, i, row, chunk);
+      const X3Span &span = KC ? src.k : src.n;   // of the fast index, eight of which lie in one half
+      int h, c, slow;
+      bool in;
+      if (KC) {
+        h    = k0 + 8 * chunk >= span.half ? 1 : 0;
+        c    = k0 + 8 * chunk - h * span.half;
+        slow = first + row;
+        in   = slow < src.cols && 8 * chunk < left;
+      } else {
+        const int col = 8 * chunk;
+        h    = PAIR ? (col >> 5) & 1 : first + col >= span.half ? 1 : 0;
+        c    = PAIR ? first + (col >> 6) * 32 + (col & 31) : first + col - h * span.half;
+        slow = k0 + row;
+        in   = row < left;
+      }
+      const float *p = src.b + slow * (KC ? src.bn : src.bk) + static_cast<long>(h) * span.used + c;
+      if (in && c + 8 <= span.used) {
+        load8(p, v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = in && c + e < span.used ? p[e] : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ void split(const float scale) {
+#pragma unroll
+    for (int i = 0; i < Side::PER; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t q[X3_PARTS];
+        split_pair(scale * v[i][2 * c], scale * v[i][2 * c + 1], q);
+#pragma unroll
+        for (int x = 0; x < X3_PARTS; ++x) (&part[i][x].x)[c] = q[x];
+      }
+  }
+  __device__ __forceinline__ void put(char *lds, const int tid) const {
+#pragma unroll
+    for (int x = 0; x < X3_PARTS; ++x)
+#pragma unroll
+      for (int i = 0; i < Side::PER; ++i) *reinterpret_cast<uint4 *>(lds + x * Side::BYTES + (i * NT + tid) * 16) = part[i][x];
+  }
+};
+
+// ON_THE_WAY: B is src.b itself, asked for in front of the products of the tile before.
+template <bool A_KC, bool B_KC, bool PAIR, bool ON_THE_WAY, class Epi>
 __global__ void __launch_bounds__(256, 2)
 gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const X3Source src, const Epi epi,
                const int tiles_m, const int tiles_n, const int K, const int k_per_split) {
@@ -57,7 +113,7 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
   SideA sa;
   SideB sb;
   sa.plan(A, m0, tid);
-  sb.plan(B, n0, tid);
+  if constexpr (!ON_THE_WAY) sb.plan(B, n0, tid);
   floatx16_x3 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -74,17 +130,25 @@ gemm_x3_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const l
       SideA a = sa;
       SideB b = sb;
       a.base += 2 * p * a_plane;
-      b.base += 2 * p * b_plane;
       a.fetch(A, lds + p * SideA::BYTES, k0, kend - k0, tid);
-      b.fetch(B, lds + X3_PARTS * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
+      if constexpr (!ON_THE_WAY) {
+        b.base += 2 * p * b_plane;
+        b.fetch(B, lds + X3_PARTS * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
+      }
     }
   };
+  X3OnTheWay<SideB, B_KC, PAIR, NT> own;
+  if constexpr (ON_THE_WAY) own.load(src, n0, kbeg, kend - kbeg, tid);
 #pragma unroll 1
   for (int k0 = kbeg; k0 < kend; k0 += X3P_BK) {
+    if constexpr (ON_THE_WAY) own.split(k0 / X3P_BK & 1 ? -X3_SCALE : X3_SCALE);
     __syncthreads();   // everyone has read the tile before
     fetch(k0);
+    if constexpr (ON_THE_WAY) own.put(lds + X3_PARTS * SideA::BYTES, tid);
     g16_arrived<0>();
     __syncthreads();
+    if constexpr (ON_THE_WAY)
+      if (k0 + X3P_BK < kend) own.load(src, n0, k0 + X3P_BK, kend - k0 - X3P_BK, tid);
     bf16x8 a[2][TM][X3_PARTS], b[2][TN][X3_PARTS];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
