@@ -559,6 +559,13 @@ def test_preference_loss_long_and_many(T):
     preference_case(T, "bf16", list(np.random.RandomState(8).randint(0, 9, 300)), 17, "sigmoid", 0.0, 17, 0, True)
 
 
+@pytest.mark.parametrize("kind", ["sigmoid", "squared", "hinge"])
+def test_preference_loss_with_and_without_a_launch_for_the_pairs(T, kind):
+    preference_case(T, "f32", [600, 400], 50, kind, 0.0, 50, 0, True)
+    preference_case(T, "bf16", [3, 4, 0, 65, 2, 1, 9, 9, 1, 0, 5, 6, 7, 8, 64, 63], 1200, kind, 0.0, 1201, 0, False, lead=1, trail=2)
+    preference_case(T, "bf16", [3, 4, 0, 65, 2, 1, 9, 9, 1, 0, 5, 6, 7, 8, 64, 63, 2, 2], 1200, kind, 0.0, 1201, 0, False, lead=1, trail=2)
+
+
 def test_preference_loss_without_pairs_rows_or_outputs(T):
     loss = out(T, 1)
     i32 = Buf(T, np.zeros(5, np.int32), "i32")

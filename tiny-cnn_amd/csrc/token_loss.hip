@@ -313,6 +313,60 @@ short_row_kernel(const RowArgs a, float *__restrict__ loss) {
   }
 }
 
+// What the sequences of a pair come to.
+struct PairArgs {
+  const double *logp64;
+  const int32_t *seq_start;
+  const float *ref_logp;
+  int pairs, rows, kind;
+  double beta, smoothing;
+  float *seq_logp, *margin, *pair_loss, *d;
+};
+struct PairValue {
+  double margin, loss, d;   // d: of the chosen sequence's gradient, -d of the rejected one's
+};
+// ... of the sums c and r over the two sequences
+__device__ __forceinline__ PairValue pair_value(const PairArgs &a, const int pair, const double c, const double r) {
+  const double rc = a.ref_logp ? a.ref_logp[2 * pair] : 0.0, rr = a.ref_logp ? a.ref_logp[2 * pair + 1] : 0.0;
+  const double m = a.beta * ((c - rc) - (r - rr));
+  double loss, dm;
+  switch (a.kind) {
+    case TDH_PREF_SIGMOID: {
+      // log(1 + exp(-|m|)) on the side where it cannot overflow, and the linear part of the other
+      const double e = exp(-fabs(m)), l = log1p(e);
+      const double neg = m > 0 ? l : l - m, pos = m > 0 ? l + m : l;   // softplus(-m), softplus(m)
+      const double up = (m > 0 ? e : 1.0) / (1.0 + e);                 // sigmoid(-m)
+      loss = (1.0 - a.smoothing) * neg + a.smoothing * pos;
+      dm   = a.smoothing * ((m > 0 ? 1.0 : e) / (1.0 + e)) - (1.0 - a.smoothing) * up;
+    } break;
+    case TDH_PREF_SQUARED: {
+      const double v = (m - 0.5) / a.beta;
+      loss = v * v;
+      dm   = 2.0 * v / a.beta;
+    } break;
+    default:
+      loss = m < 1.0 ? 1.0 - m : m >= 1.0 ? 0.0 : m;   // (NaN stays)
+      dm   = m < 1.0 ? -1.0 : m >= 1.0 ? 0.0 : m;
+      break;
+  }
+  return PairValue{m, loss, a.beta * dm / a.pairs};
+}
+// a lane's share of the sum over sequence s, `lanes` of them
+__device__ __forceinline__ double sequence_share(const PairArgs &a, const int s, const int t, const int lanes) {
+  const int beg = max(0, min(a.rows, a.seq_start[s])), end = max(beg, min(a.rows, a.seq_start[s + 1]));
+  double sum = 0.0;
+#pragma unroll 4
+  for (int i = beg + t; i < end; i += lanes) sum += a.logp64[i];
+  return sum;
+}
+__device__ __forceinline__ void keep_pair(const PairArgs &a, const int pair, const double c, const double r, const PairValue &v) {
+  if (a.seq_logp) {
+    a.seq_logp[2 * pair]     = static_cast<float>(c);
+    a.seq_logp[2 * pair + 1] = static_cast<float>(r);
+  }
+  if (a.margin) a.margin[pair] = static_cast<float>(v.margin);
+}
+
 // dlogits = d ([j = t] - exp(x - m) / s), row by row; workgroups of 256 threads take SPAN words of a row, each of its threads
 // GRAD_WORDS that are on their way together. Bound by memory: 4096 x 131072 in bf16 308 us, 7.0 TB/s (the last rows of the pass
 // before are still in the memory-side cache).
@@ -331,6 +385,7 @@ struct GradArgs {
   // the mean of these, which a workgroup behind the others computes (null: none)
   const float *pair_loss;
   float *loss;
+  PairArgs pair;   // WITH_PAIRS: what d comes from
 };
 // out[0] = scale * (v[0] + ... + v[n-1]), by one workgroup, in an order that n and its size set
 template <int NT>
@@ -347,11 +402,32 @@ __device__ __forceinline__ void sum_of(const float *v, const int n, const double
     out[0] = static_cast<float>(scale * sum);
   }
 }
-template <class T>
+// WITH_PAIRS: few short sequences, every workgroup adds up those of its row's pair itself, and one behind the others leaves what
+// belongs to the pairs: a launch less. us of a loss with a launch for the pairs / so: 3 pairs of up to 41 rows of 1003 logits 12.0 / 9.0; 8 of
+// 20 rows of 30000 17.2 / 14.9; 16 of 60 rows of 1000 14.1 / 14.2; one of 1000 rows 13.4 / 15.0; 60 of 10 rows 13.4 / 27.2.
+template <class T, bool WITH_PAIRS>
 __global__ void __launch_bounds__(GRAD_NT)
 dlogits_kernel(const GradArgs a) {
   constexpr int N = Word<T>::N;
-  if (a.loss && blockIdx.x == gridDim.x - 1) {
+  __shared__ double sums[GRAD_NT / 64];
+  if (WITH_PAIRS && blockIdx.x == gridDim.x - 1) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double loss = 0.0;
+    for (int p = wave; p < a.pair.pairs; p += GRAD_NT / 64) {
+      const double c = wave_sum(sequence_share(a.pair, 2 * p, lane, 64)), r = wave_sum(sequence_share(a.pair, 2 * p + 1, lane, 64));
+      const PairValue v = pair_value(a.pair, p, c, r);
+      loss += v.loss;
+      if (lane == 0) keep_pair(a.pair, p, c, r, v);
+    }
+    if (lane == 0) sums[wave] = loss;
+    __syncthreads();
+    if (threadIdx.x == 0 && a.loss) {
+      for (int w = 1; w < GRAD_NT / 64; ++w) loss += sums[w];
+      a.loss[0] = static_cast<float>(loss / a.pair.pairs);
+    }
+    return;
+  }
+  if (!WITH_PAIRS && a.loss && blockIdx.x == gridDim.x - 1) {
     sum_of<GRAD_NT>(a.pair_loss, a.sequences / 2, 2.0 / a.sequences, a.loss);
     return;
   }
@@ -365,7 +441,17 @@ dlogits_kernel(const GradArgs a) {
       if (a.seq_start[mid] <= row) lo = mid; else hi = mid;
     }
     if (row < a.seq_start[0] || row >= a.seq_start[a.sequences]) return;   // in no sequence: left as it is
-    d = a.d[lo];
+    if constexpr (WITH_PAIRS) {
+      if (tid < 128) {
+        const double sum = wave_sum(sequence_share(a.pair, (lo & ~1) + (tid >> 6), tid & 63, 64));
+        if ((tid & 63) == 0) sums[tid >> 6] = sum;
+      }
+      __syncthreads();
+      d = static_cast<float>(pair_value(a.pair, lo >> 1, sums[0], sums[1]).d);
+      if (lo & 1) d = -d;
+    } else {
+      d = a.d[lo];
+    }
   } else {
     d = a.d[row];
   }
@@ -408,58 +494,21 @@ sum_kernel(const float *__restrict__ v, const int n, const double scale, float *
   sum_of<SUM_NT>(v, n, scale, out);
 }
 
-// One workgroup a pair: the sums over its two sequences, its margin, its loss and the factors of its gradient. 4 us, a launch.
-struct PairArgs {
-  const double *logp64;
-  const int32_t *seq_start;
-  const float *ref_logp;
-  int pairs, rows, kind;
-  double beta, smoothing;
-  float *seq_logp, *margin, *pair_loss, *d;
-};
 constexpr int PAIR_NT = 256;
+// One workgroup a pair: the sums over its two sequences, its margin, its loss and the factors of its gradient. 4 us, a launch.
 __global__ void __launch_bounds__(PAIR_NT)
 pair_kernel(const PairArgs a) {
   __shared__ double part[PAIR_NT / 64];
-  const int pair = blockIdx.x, tid = threadIdx.x, half = tid >> 7, t = tid & 127;
-  const int s = 2 * pair + half;
-  const int beg = max(0, min(a.rows, a.seq_start[s])), end = max(beg, min(a.rows, a.seq_start[s + 1]));
-  double sum = 0.0;
-  for (int i = beg + t; i < end; i += 128) sum += a.logp64[i];
-  sum = wave_sum(sum);
+  const int pair = blockIdx.x, tid = threadIdx.x;
+  const double sum = wave_sum(sequence_share(a, 2 * pair + (tid >> 7), tid & 127, 128));
   if ((tid & 63) == 0) part[tid >> 6] = sum;
   __syncthreads();
   if (tid) return;
   const double c = part[0] + part[1], r = part[2] + part[3];
-  if (a.seq_logp) {
-    a.seq_logp[2 * pair]     = static_cast<float>(c);
-    a.seq_logp[2 * pair + 1] = static_cast<float>(r);
-  }
-  const double rc = a.ref_logp ? a.ref_logp[2 * pair] : 0.0, rr = a.ref_logp ? a.ref_logp[2 * pair + 1] : 0.0;
-  const double m = a.beta * ((c - rc) - (r - rr));
-  double loss, dm;
-  switch (a.kind) {
-    case TDH_PREF_SIGMOID: {
-      // log(1 + exp(-|m|)) on the side where it cannot overflow, and the linear part of the other
-      const double e = exp(-fabs(m)), l = log1p(e);
-      const double neg = m > 0 ? l : l - m, pos = m > 0 ? l + m : l;   // softplus(-m), softplus(m)
-      const double up = (m > 0 ? e : 1.0) / (1.0 + e);                 // sigmoid(-m)
-      loss = (1.0 - a.smoothing) * neg + a.smoothing * pos;
-      dm   = a.smoothing * ((m > 0 ? 1.0 : e) / (1.0 + e)) - (1.0 - a.smoothing) * up;
-    } break;
-    case TDH_PREF_SQUARED: {
-      const double v = (m - 0.5) / a.beta;
-      loss = v * v;
-      dm   = 2.0 * v / a.beta;
-    } break;
-    default:
-      loss = m < 1.0 ? 1.0 - m : m >= 1.0 ? 0.0 : m;   // (NaN stays)
-      dm   = m < 1.0 ? -1.0 : m >= 1.0 ? 0.0 : m;
-      break;
-  }
-  if (a.margin) a.margin[pair] = static_cast<float>(m);
-  a.pair_loss[pair]   = static_cast<float>(loss);
-  const float d       = static_cast<float>(a.beta * dm / a.pairs);
+  const PairValue v = pair_value(a, pair, c, r);
+  keep_pair(a, pair, c, r, v);
+  a.pair_loss[pair]   = static_cast<float>(v.loss);
+  const float d       = static_cast<float>(v.d);
   a.d[2 * pair]       = d;
   a.d[2 * pair + 1]   = -d;
 }
@@ -503,7 +552,11 @@ int grad_blocks(int vocab, size_t size) { return ceil_div(static_cast<int>((voca
 template <class T>
 int launch_dlogits(GradArgs a) {
   a.blocks_per_row = grad_blocks(a.vocab, sizeof(T));
-  TDH_LAUNCH((dlogits_kernel<T>), dim3(a.rows * a.blocks_per_row + (a.loss ? 1 : 0)), dim3(GRAD_NT), 0, ctx().stream, a);
+  const dim3 grid(a.rows * a.blocks_per_row + (a.loss || a.pair.pairs ? 1 : 0));
+  if (a.pair.pairs)
+    TDH_LAUNCH((dlogits_kernel<T, true>), grid, dim3(GRAD_NT), 0, ctx().stream, a);
+  else
+    TDH_LAUNCH((dlogits_kernel<T, false>), grid, dim3(GRAD_NT), 0, ctx().stream, a);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
@@ -514,6 +567,8 @@ int launch_sum(const float *v, int n, double scale, float *out) {
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
+
+constexpr int WITH_PAIRS_PAIRS = 8, WITH_PAIRS_ROWS = 1024, WITH_PAIRS_BLOCKS = 2048;
 
 double logits_bytes(int dtype, int rows, int vocab, int passes) {
   return static_cast<double>(dtype_size(dtype)) * rows * vocab * passes;
@@ -642,13 +697,16 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
     ProfScope prof("preference_logprob", logits_bytes(dtype, rows, vocab, 1), WORK_BYTE);
     TDH_TRY(with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t), ROW_LOGP>(a, dlogits != nullptr); }));
   }
-  {
-    PairArgs a{};
-    a.logp64 = static_cast<const double *>(logp64); a.seq_start = seq_start; a.ref_logp = ref_logp;
-    a.pairs = pairs; a.rows = rows; a.kind = p->kind; a.beta = p->beta; a.smoothing = p->smoothing;
-    a.seq_logp = seq_logp; a.margin = margin; a.pair_loss = static_cast<float *>(pair_loss); a.d = static_cast<float *>(d);
+  PairArgs pa{};
+  pa.logp64 = static_cast<const double *>(logp64); pa.seq_start = seq_start; pa.ref_logp = ref_logp;
+  pa.pairs = pairs; pa.rows = rows; pa.kind = p->kind; pa.beta = p->beta; pa.smoothing = p->smoothing;
+  pa.seq_logp = seq_logp; pa.margin = margin; pa.pair_loss = static_cast<float *>(pair_loss); pa.d = static_cast<float *>(d);
+  // few pairs, short sequences, and a gradient whose workgroups are all on the chip at once
+  const bool with_pairs = dlogits && rows && pairs <= WITH_PAIRS_PAIRS && rows <= WITH_PAIRS_ROWS &&
+                          static_cast<long>(rows) * grad_blocks(vocab, dtype_size(dtype)) <= WITH_PAIRS_BLOCKS;
+  if (!with_pairs) {
     ProfScope prof("preference_pairs", 8.0 * rows, WORK_BYTE);
-    TDH_LAUNCH(pair_kernel, dim3(pairs), dim3(PAIR_NT), 0, ctx().stream, a);
+    TDH_LAUNCH(pair_kernel, dim3(pairs), dim3(PAIR_NT), 0, ctx().stream, pa);
     TDH_LAUNCH_CHECK();
   }
   if (dlogits && rows) {
@@ -657,6 +715,7 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
     g.stats = static_cast<const float *>(stats); g.d = static_cast<const float *>(d);
     g.seq_start = seq_start; g.sequences = 2 * pairs; g.dlogits = dlogits; g.ld_d = ld_d;
     g.pair_loss = static_cast<const float *>(pair_loss); g.loss = loss;
+    if (with_pairs) g.pair = pa;
     ProfScope prof("preference_grad", logits_bytes(dtype, rows, vocab, 2), WORK_BYTE);
     return with_dtype(dtype, [&](auto t) { return launch_dlogits<decltype(t)>(g); });
   }
