@@ -10,8 +10,10 @@
 // them in turns: the next ones are on their way while this one is multiplied, one barrier a tile. LDS holds a tile as it
 // lies in memory, its 16-byte chunks permuted within each row so that the reads hit different banks (the lanes fetch
 // permuted chunks: the way into LDS is linear in the lane):
-//   along k      rows of 64 k (128 bytes), chunk c of row r at c ^ (r mod 8) (rows of 32 k: at c ^ (r/2 mod 4)); a lane's
-//                operand, 8 k of its row, is one 16-byte read;
+//   along k      rows of 64 k (128 bytes), chunk c of row r at c ^ (r/2 mod 8) (rows of 32 k: at c ^ (r/4 mod 4)), so that 16 rows in
+//                a row fill the 256 bytes that LDS reads at a time (at c ^ (r mod 8) rows r and r + 8 meet: 4 cycles a read, and
+//                the product with both operands along k in 662-708 us for 650); a lane's operand, 8 k of its row, is one
+//                16-byte read;
 //   along m, n   rows of one k each, 64-byte segments permuted by k mod 4; ds_read_b64_tr_b16 hands every lane 4 k of
 //                its column out of 4 rows.
 //
@@ -63,8 +65,8 @@ struct G16Side {
   static_assert(BYTES % (NT * 16) == 0, "");
   const char *base;   // of the tile's k = 0
   unsigned off[PER];  // bytes from there, by load
-  // chunk c of row r lies at c ^ turn(r) (KC): the eight lanes that read at a time hit different banks
-  __device__ __forceinline__ static int turn(const int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
+  // chunk c of row r lies at c ^ turn(r) (KC): the sixteen lanes that read at a time hit different banks
+  __device__ __forceinline__ static int turn(const int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
   __device__ __forceinline__ static int swizzle(const int k) { return ROWS >= 128 ? (k & 3) * 4 : ROWS == 64 ? ((k >> 1) & 1) * 4 : 0; }
   // where thread tid's load i lies: row of the tile and 16-byte chunk (of memory) in it
   __device__ __forceinline__ static void place(const int tid, const int i, int &row, int &chunk) {
