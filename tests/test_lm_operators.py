@@ -43,6 +43,11 @@ def test_gated_ff_refusals(T):
     for shape in ((1 << 22, 1, 1), (1, 1 << 21, 1), (1, 1, 1 << 25)):
         refuses(T, "beyond", T.gated_ff_fwd, shape[0], shape[1], False, shape[2], A, B, None, D, **ok)
         refuses(T, "beyond", T.gated_ff_bwd, shape[0], shape[1], False, shape[2], A, B, D, D, None, D, None, **ok)
+    far, near = At(0x500000000), At(0x500000000 + 4 * 64)
+    refuses(T, "overlaps an input", T.gated_ff_fwd, 8, 16, False, 8, A, far, None, near, **ok)
+    refuses(T, "two outputs overlap", T.gated_ff_fwd, 8, 16, False, 8, A, B, None, far, z=near, **ok)
+    refuses(T, "overlaps an input", T.gated_ff_bwd, 8, 16, False, 8, A, B, D, far, near, None, None, **ok)
+    refuses(T, "two outputs overlap", T.gated_ff_bwd, 8, 16, False, 8, A, B, D, At(0x700000000), near, far, None, **ok)
     refuses(T, "aligned", T.gated_ff_fwd, 8, 8, False, 1, At(0x100000001), B, None, D, act="silu", dtype="bf16")
     refuses(T, "aligned", T.gated_ff_fwd, 8, 8, False, 1, A, B, None, D, z=At(0x300000002), act="silu", dtype="bf16")
     refuses(T, "null tensor", T.gated_ff_bwd, 8, 8, False, 1, A, B, None, D, None, None, None, **ok)

@@ -1137,6 +1137,22 @@ int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch)
                 in, hidden, batch);
   return TDH_OK;
 }
+// no output overlaps another tensor of the call
+struct Span {
+  const void *p;
+  size_t bytes;
+};
+int check_apart(const char *who, std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  auto meet = [](const Span &a, const Span &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x && y && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+  };
+  for (const Span &o : outputs) {
+    for (const Span &i : inputs) TDH_CHECK_ARG(!meet(o, i), "%s: an output overlaps an input", who);
+    for (const Span *q = &o + 1; q != outputs.end(); ++q) TDH_CHECK_ARG(!meet(o, *q), "%s: two outputs overlap", who);
+  }
+  return TDH_OK;
+}
 int check_aligned(const char *who, int dtype, std::initializer_list<const void *> tensors) {
   for (const void *p : tensors)
     TDH_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0, "%s: a tensor that is not aligned to its elements", who);
@@ -1157,6 +1173,8 @@ int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int b
   TDH_CHECK_ARG(batch == 0 || !has_bias || b, "tdh_gated_ff_fwd: has_bias set but b is null");
   TDH_TRY(check_aligned("tdh_gated_ff_fwd", dtype, {x, w, b, h}));
   TDH_TRY(check_aligned("tdh_gated_ff_fwd", TDH_F32, {z}));
+  const size_t e = dtype_size(dtype), nx = static_cast<size_t>(batch) * in, nh = static_cast<size_t>(batch) * hidden, nw = 2 * static_cast<size_t>(in) * hidden;
+  TDH_TRY(check_apart("tdh_gated_ff_fwd", {{h, e * nh}, {z, 8 * nh}}, {{x, e * nx}, {w, e * nw}, {has_bias ? b : nullptr, 2 * e * hidden}}));
   TDH_REQUIRE_INIT();
   if (batch == 0) return TDH_OK;
   return with_dtype(dtype, [&](auto t) {
@@ -1176,6 +1194,9 @@ int tdh_gated_ff_bwd(int dtype, int act, int in, int hidden, int has_bias, int b
   TDH_CHECK_ARG(batch == 0 || (x && w && z && dh), "tdh_gated_ff_bwd: null tensor");
   TDH_TRY(check_aligned("tdh_gated_ff_bwd", dtype, {x, w, dh, dx, dw, db}));
   TDH_TRY(check_aligned("tdh_gated_ff_bwd", TDH_F32, {z}));
+  const size_t e = dtype_size(dtype), nx = static_cast<size_t>(batch) * in, nh = static_cast<size_t>(batch) * hidden, nw = 2 * static_cast<size_t>(in) * hidden;
+  TDH_TRY(check_apart("tdh_gated_ff_bwd", {{dx, e * nx}, {dw, e * nw}, {has_bias ? db : nullptr, 2 * e * hidden}},
+                      {{x, e * nx}, {batch ? w : nullptr, e * nw}, {z, 8 * nh}, {dh, e * nh}}));
   TDH_REQUIRE_INIT();
   if (batch == 0 && accumulate) return TDH_OK;
   return with_dtype(dtype, [&](auto t) {
