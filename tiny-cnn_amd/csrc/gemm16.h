@@ -18,7 +18,7 @@
 //                its column out of 4 rows.
 //
 // Bound by the card's power on large products: 4096 x 24576 x 4096 in bf16, tiles of 256 x 256 by eight waves, random operands
-// 1170-1215 TFLOP/s, all zero 1440-1490 (whose sums no bits toggle). Slower: tiles of 32 indices, four of them in turns 1100-1113; four
+// 1150-1270 TFLOP/s without the gate, all zero 1440-1490 (whose sums no bits toggle). Slower: tiles of 32 indices, four of them in turns 1100-1113; four
 // waves of 128 x 128 each 1074-1111.
 #pragma once
 #include "lm_types.h"
