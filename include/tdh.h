@@ -272,7 +272,7 @@ int tdh_softmax_xent_grad(int batch, int len, const float *y, const float *t, fl
 /* Gated feed-forward block: z = x W + b, h = act(z_gate) * z_up. x [batch][in], w [in][2*hidden] with the gate's
  * columns first, b [2*hidden] (has_bias), h [batch][hidden]. z [batch][2*hidden], fp32, is what the backward pass
  * reads; NULL where there is none (inference). No output may overlap another tensor of the call. in up to 2^21,
- * hidden up to 2^20, batch up to 2^24, and no tensor of 2^31 elements. */
+ * hidden up to 2^20, batch up to 2^24 (TDH_F32: 2^20), and no tensor of 2^31 elements. */
 int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
                      const void *b, void *h, float *z);
 /* dz = (dh * z_up * act'(z_gate), dh * act(z_gate)), dx = dz W^T, dw = x^T dz, db = the sum of dz over the batch. dx is overwritten;

@@ -250,6 +250,12 @@ def test_gated_ff_of_many_samples_and_narrow_matrices(T, dtype, shape, accumulat
     ff_case(T, shape, "silu", dtype, bias=True, accumulate=accumulate)
 
 
+@pytest.mark.parametrize("dtype,n", [("f32", 1 << 20), ("bf16", (1 << 21) + 3)])
+def test_gated_ff_of_the_most_samples(T, dtype, n):
+    ff_case(T, (n, 1, 1), "sigmoid", dtype, bias=True)
+    ff_case(T, (n, 3, 2), "sigmoid", dtype, bias=False)
+
+
 @pytest.mark.parametrize("dtype", L.DTYPES)
 def test_gated_ff_gradients_left_out(T, dtype):
     """Each of dx, dw and db asked for alone. Another kernel may compute it then, in another order of its sums: two

@@ -40,7 +40,7 @@ def test_gated_ff_refusals(T):
     refuses(T, "null tensor", T.gated_ff_fwd, 8, 8, False, 1, None, B, None, D, **ok)
     refuses(T, "has_bias", T.gated_ff_fwd, 8, 8, True, 1, A, B, None, D, **ok)
     refuses(T, "2\\^31", T.gated_ff_fwd, 1 << 16, 1 << 15, False, 1, A, B, None, D, **ok)
-    for shape in ((1 << 22, 1, 1), (1, 1 << 21, 1), (1, 1, 1 << 25)):
+    for shape in ((1 << 22, 1, 1), (1, 1 << 21, 1), (1, 1, 1 << 25), (1, 1, (1 << 20) + 1)):
         refuses(T, "beyond", T.gated_ff_fwd, shape[0], shape[1], False, shape[2], A, B, None, D, **ok)
         refuses(T, "beyond", T.gated_ff_bwd, shape[0], shape[1], False, shape[2], A, B, D, D, None, D, None, **ok)
     far, near = At(0x500000000), At(0x500000000 + 4 * 64)

@@ -1132,9 +1132,11 @@ int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch)
   TDH_CHECK_ARG(in > 0 && hidden > 0 && batch >= 0, "%s: bad shape %d->2*%d batch %d", who, in, hidden, batch);
   TDH_CHECK_ARG(2L * in * hidden < (1L << 31) && static_cast<long>(batch) * in < (1L << 31) && 2L * batch * hidden < (1L << 31),
                 "%s: tensor exceeds 2^31 elements", who);
-  // (offsets within a tile of 256 rows are 32 bits, and a launch has fewer than 2^24 workgroups)
-  TDH_CHECK_ARG(in <= (1 << 21) && hidden <= (1 << 20) && batch <= (1 << 24), "%s: %d->2*%d batch %d is beyond 2^21->2*2^20 batch 2^24", who,
-                in, hidden, batch);
+  // (offsets within a tile of 256 rows are 32 bits, a launch has fewer than 2^24 workgroups, and the fully-connected layer's products,
+  // in fp32, fewer than 2^16 tiles of rows)
+  const int most = dtype == TDH_F32 ? 1 << 20 : 1 << 24;
+  TDH_CHECK_ARG(in <= (1 << 21) && hidden <= (1 << 20) && batch <= most, "%s: %d->2*%d batch %d is beyond 2^21->2*2^20 batch %d", who,
+                in, hidden, batch, most);
   return TDH_OK;
 }
 // no output overlaps another tensor of the call
