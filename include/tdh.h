@@ -267,12 +267,13 @@ int tdh_softmax_xent_grad(int batch, int len, const float *y, const float *t, fl
 /* -------------------------------------------- operators of language models
  * They have no counterpart in the reference. `dtype` (TDH_F32, TDH_BF16, TDH_F16) is the element type of the
  * tensors declared void *; those declared float * are fp32 in every type. Sums are held in 32 bits or more, and
- * results are rounded once, to nearest. Tensors are aligned to their elements. The same inputs give the same bits. */
+ * results are rounded once, to nearest. Tensors are aligned to their elements. No output may overlap
+ * an input or another output, except where it is said that it may be an input. The same inputs give the same bits. */
 
 /* Gated feed-forward block: z = x W + b, h = act(z_gate) * z_up. x [batch][in], w [in][2*hidden] with the gate's
  * columns first, b [2*hidden] (has_bias), h [batch][hidden]. z [batch][2*hidden], fp32, is what the backward pass
- * reads; NULL where there is none (inference). No output may overlap another tensor of the call. in up to 2^21,
- * hidden up to 2^20, batch up to 2^24 (TDH_F32: 2^20), and no tensor of 2^31 elements. */
+ * reads; NULL where there is none (inference). in up to 2^21, hidden up to 2^20, batch up to 2^24 (TDH_F32: 2^20), and
+ * no tensor of 2^31 elements. */
 int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
                      const void *b, void *h, float *z);
 /* dz = (dh * z_up * act'(z_gate), dh * act(z_gate)), dx = dz W^T, dw = x^T dz, db = the sum of dz over the batch. dx is overwritten;

@@ -100,6 +100,17 @@ def test_loss_refusals(T):
                                    C.c_size_t(8)) == -1
 
 
+def test_loss_refusals_of_overlapping_tensors(T):
+    one = dict(rows=4, vocab=8, logits=A, target=B)
+    refuses(T, "overlaps an input", T.token_logprob_fwd, 4, 8, A, B, At(B.ptr.value + 12))
+    refuses(T, "two outputs overlap", T.token_logprob_fwd, 4, 8, A, B, D, stats=At(D.ptr.value + 12))
+    refuses(T, "overlaps an input", T.token_logprob_bwd, 4, 8, A, B, D, At(0x400000000), At(D.ptr.value + 28))
+    refuses(T, "overlaps an input", T.policy_loss, old_logp=D, ref_logp=None, advantage=At(0x400000000), logp=D, **one)
+    refuses(T, "overlaps an input", T.policy_loss, old_logp=D, ref_logp=None, advantage=D, loss=At(A.ptr.value + 124), **one)
+    refuses(T, "overlaps an input", T.preference_loss, 1, seq_start=D, ref_logp=At(0x400000000), seq_logp=At(0x400000004), **one)
+    refuses(T, "two outputs overlap", T.preference_loss, 1, seq_start=D, margin=At(0x400000000), loss=At(0x400000000), **one)
+
+
 def test_cast_refusals(T):
     refuses(T, "null tensor", T.cast, 4, None, B, "f32", "bf16")
     refuses(T, "overlap", T.cast, 4, A, At(0x100000008), "f32", "bf16")

@@ -1139,22 +1139,6 @@ int check_ff(const char *who, int dtype, int act, int in, int hidden, int batch)
                 in, hidden, batch, most);
   return TDH_OK;
 }
-// no output overlaps another tensor of the call
-struct Span {
-  const void *p;
-  size_t bytes;
-};
-int check_apart(const char *who, std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
-  auto meet = [](const Span &a, const Span &b) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    return x && y && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
-  };
-  for (const Span &o : outputs) {
-    for (const Span &i : inputs) TDH_CHECK_ARG(!meet(o, i), "%s: an output overlaps an input", who);
-    for (const Span *q = &o + 1; q != outputs.end(); ++q) TDH_CHECK_ARG(!meet(o, *q), "%s: two outputs overlap", who);
-  }
-  return TDH_OK;
-}
 int check_aligned(const char *who, int dtype, std::initializer_list<const void *> tensors) {
   for (const void *p : tensors)
     TDH_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0, "%s: a tensor that is not aligned to its elements", who);

@@ -3,6 +3,8 @@
 #pragma once
 #include "common.h"
 
+#include <initializer_list>
+
 namespace tdh {
 
 struct bf16 {
@@ -101,6 +103,23 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
 
 inline bool dtype_known(int dtype) { return dtype == TDH_F32 || dtype == TDH_BF16 || dtype == TDH_F16; }
 inline size_t dtype_size(int dtype) { return dtype == TDH_F32 ? 4 : 2; }
+
+// No output of a call may overlap an input or another output of it.
+struct Span {
+  const void *p;
+  size_t bytes;
+};
+inline int check_apart(const char *who, std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  auto meet = [](const Span &a, const Span &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x && y && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+  };
+  for (const Span &o : outputs) {
+    for (const Span &i : inputs) TDH_CHECK_ARG(!meet(o, i), "%s: an output overlaps an input", who);
+    for (const Span *q = &o + 1; q != outputs.end(); ++q) TDH_CHECK_ARG(!meet(o, *q), "%s: two outputs overlap", who);
+  }
+  return TDH_OK;
+}
 
 // Calls f with a value of the device type that `dtype` names.
 template <class F>

@@ -596,6 +596,11 @@ int check_dlogits(const char *who, int dtype, int rows, int vocab, const void *l
   return TDH_OK;
 }
 
+// the memory that `rows` rows of logits or gradients take
+Span span_of(int dtype, int rows, int vocab, const void *p, size_t ld) {
+  return Span{p, rows > 0 ? dtype_size(dtype) * ((rows - 1) * ld + vocab) : 0};
+}
+
 }  // namespace
 }  // namespace tdh
 
@@ -607,6 +612,8 @@ int tdh_token_logprob_fwd(int dtype, int rows, int vocab, const void *logits, si
                           float *stats) {
   TDH_TRY(check_logits("tdh_token_logprob_fwd", dtype, rows, vocab, logits, ld, target));
   TDH_CHECK_ARG(rows == 0 || logp, "tdh_token_logprob_fwd: null tensor");
+  const size_t r4 = 4 * static_cast<size_t>(rows);
+  TDH_TRY(check_apart("tdh_token_logprob_fwd", {{logp, r4}, {stats, 2 * r4}}, {span_of(dtype, rows, vocab, logits, ld), {target, r4}}));
   TDH_REQUIRE_INIT();
   if (rows == 0) return TDH_OK;
   RowArgs a{};
@@ -621,6 +628,8 @@ int tdh_token_logprob_bwd(int dtype, int rows, int vocab, const void *logits, si
   TDH_TRY(check_logits("tdh_token_logprob_bwd", dtype, rows, vocab, logits, ld, target));
   TDH_TRY(check_dlogits("tdh_token_logprob_bwd", dtype, rows, vocab, logits, ld, dlogits, ld_d));
   TDH_CHECK_ARG(rows == 0 || (stats && dlogp && dlogits), "tdh_token_logprob_bwd: null tensor");
+  const size_t r4 = 4 * static_cast<size_t>(rows);
+  TDH_TRY(check_apart("tdh_token_logprob_bwd", {span_of(dtype, rows, vocab, dlogits, ld_d)}, {{target, r4}, {stats, 2 * r4}, {dlogp, r4}}));
   TDH_REQUIRE_INIT();
   if (rows == 0) return TDH_OK;
   GradArgs g{};
@@ -640,6 +649,10 @@ int tdh_policy_loss(const tdh_policy_desc *p, int dtype, int rows, int vocab, co
   TDH_CHECK_ARG(p->kl_coef >= 0.0f && p->kl_coef <= FLT_MAX, "tdh_policy_loss: KL coefficient %g", p->kl_coef);
   TDH_CHECK_ARG(rows == 0 || (old_logp && advantage), "tdh_policy_loss: null tensor");
   if (dlogits) TDH_TRY(check_dlogits("tdh_policy_loss", dtype, rows, vocab, logits, ld, dlogits, ld_d));
+  const size_t r4 = 4 * static_cast<size_t>(rows);
+  TDH_TRY(check_apart("tdh_policy_loss", {{logp, r4}, {row_loss, r4}, {loss, 4}, span_of(dtype, rows, vocab, dlogits, ld_d)},
+                      {{target, r4}, {old_logp, r4}, {ref_logp, r4}, {advantage, r4}, {weight, r4}}));
+  TDH_TRY(check_apart("tdh_policy_loss", {{logp, r4}, {row_loss, r4}, {loss, 4}}, {span_of(dtype, rows, vocab, logits, ld)}));
   TDH_REQUIRE_INIT();
   if (rows == 0) return loss ? launch_sum(nullptr, 0, 1.0, loss) : static_cast<int>(TDH_OK);
   if (loss && !row_loss) {
@@ -679,6 +692,10 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
   TDH_CHECK_ARG(pairs >= 0 && pairs <= (1 << 23), "tdh_preference_loss: %d pairs", pairs);
   TDH_CHECK_ARG(pairs == 0 || seq_start, "tdh_preference_loss: null tensor");
   if (dlogits) TDH_TRY(check_dlogits("tdh_preference_loss", dtype, rows, vocab, logits, ld, dlogits, ld_d));
+  const size_t r4 = 4 * static_cast<size_t>(rows), p4 = 4 * static_cast<size_t>(pairs);
+  TDH_TRY(check_apart("tdh_preference_loss", {{logp, r4}, {seq_logp, 2 * p4}, {margin, p4}, {loss, 4}, span_of(dtype, rows, vocab, dlogits, ld_d)},
+                      {{target, r4}, {seq_start, 2 * p4 + 4}, {ref_logp, 2 * p4}}));
+  TDH_TRY(check_apart("tdh_preference_loss", {{logp, r4}, {seq_logp, 2 * p4}, {margin, p4}, {loss, 4}}, {span_of(dtype, rows, vocab, logits, ld)}));
   TDH_REQUIRE_INIT();
   if (pairs == 0) return loss ? launch_sum(nullptr, 0, 1.0, loss) : static_cast<int>(TDH_OK);
   const size_t nr = static_cast<size_t>(rows), np = static_cast<size_t>(pairs);
