@@ -278,7 +278,8 @@ int tdh_gated_ff_fwd(int dtype, int act, int in, int hidden, int has_bias, int b
                      const void *b, void *h, float *z);
 /* dz = (dh * z_up * act'(z_gate), dh * act(z_gate)), dx = dz W^T, dw = x^T dz, db = the sum of dz over the batch. dx is overwritten;
  * dw and db (as in tdh_fc_bwd) overwritten, or added to with accumulate != 0. Any of dx, dw, db may be NULL.
- * In the 16-bit types dz is rounded to that type once, as the operand of the two products (not for up to four samples).
+ * In the 16-bit types dz is rounded to that type once, as the operand of the two products (not for up to four samples); in
+ * TDH_F16 times a power of two that brings its largest finite value into [2^14, 2^15), so dz need not be in the type's range.
  * The derivative of relu at zero is 0. */
 int tdh_gated_ff_bwd(int dtype, int act, int in, int hidden, int has_bias, int batch, const void *x, const void *w,
                      const float *z, const void *dh, void *dx, void *dw, void *db, int accumulate);

@@ -1,0 +1,86 @@
+"""The language-model operators at values far from one, each result held to its own size: gradients in fp16 whose dz fp16 does not
+hold, and activations and their derivatives in the tails. Bounds come from the number of roundings."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import lm_common as L  # noqa: E402
+from test_gpu_lm_operators import Buf, out  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------ dz in fp16
+
+def f16_bounds(x, w, z, dh):
+    """(want, bound) of dx and dw under the identity as gate. dz is rounded to fp16 times a power of two that brings the
+    largest into [2^14, 2^15): half a step of 2^-24 there is 2^-39 of the largest."""
+    dz, dx, dw, _ = L.ff_backward(x, w, z, dh, "none")
+    half = (2.0 ** -11 + 2.0 ** -22) * np.abs(dz) + 2.0 ** -39 * np.abs(dz).max()
+    n, m = dz.shape
+
+    def final(v, e):
+        return e + 2.0 ** -11 * (np.abs(v) + e) + 2.0 ** -25
+
+    size = np.abs(dz) + half
+    return ((dx, final(dx, half @ np.abs(w).T + L.sum_bound(m, size @ np.abs(w).T))),
+            (dw, final(dw, np.abs(x).T @ half + L.sum_bound(n, np.abs(x).T @ size))))
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("size", ["large", "small", "mixed"])
+@pytest.mark.parametrize("shape", [(5, 40, 24), (6, 65, 521), (40, 72, 88), (300, 333, 129), (1001, 1024, 1000), (5000, 24, 41)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ff_gradients_whose_dz_fp16_does_not_hold(T, shape, size, accumulate):
+    """dz of 10^6 beside weights of 10^-5, dz of 2^-28 beside weights of 2^13, and one sample of 10^6 among ordinary ones: dx and dw
+    are well within fp16, which without a scale would have them infinite, or zero."""
+    n, d, f = shape
+    rng = np.random.RandomState(n + d)
+    x, w, dh, z = rng.randn(n, d), rng.randn(d, 2 * f), rng.randn(n, f), rng.randn(n, 2 * f)
+    if size == "large":
+        x, w, dh, z = 6e-5 * x, 6e-5 * w, 1e4 * np.clip(dh, -6, 6), 100 * z
+    elif size == "small":
+        x, w, dh, z = 2.0 ** 13 * np.clip(x, -7, 7), 2.0 ** 13 * np.clip(w, -7, 7), 2.0 ** -8 * dh, 2.0 ** -20 * z
+    else:
+        x[n // 2], dh[n // 2], z[n // 2], w = 1e-4 * x[n // 2], 1e4 * np.clip(dh[n // 2], -6, 6), 100 * z[n // 2], w / 2.0 ** 14
+    x, w, dh, z = (L.rounded(v, t) for v, t in ((x, "f16"), (w, "f16"), (dh, "f16"), (z, "f32")))
+    bx, bw, bdh, bz = Buf(T, x, "f16"), Buf(T, w, "f16"), Buf(T, dh, "f16"), Buf(T, z)
+    want = f16_bounds(x, w, z, dh)
+    assert all(np.abs(v).max() < 3e4 for v, _ in want)
+    before = L.rounded(rng.randn(d, 2 * f) * np.median(np.abs(want[1][0])), "f16")
+    for alone in (False, True):
+        dx, dw = out(T, (n, d), "f16"), Buf(T, before, "f16")
+        if alone:
+            T.gated_ff_bwd(d, f, False, n, bx, bw, bz, bdh, dx, None, None, act="none", dtype="f16")
+            T.gated_ff_bwd(d, f, False, n, bx, bw, bz, bdh, None, dw, None, act="none", dtype="f16", accumulate=accumulate)
+        else:
+            T.gated_ff_bwd(d, f, False, n, bx, bw, bz, bdh, dx, dw, None, act="none", dtype="f16", accumulate=accumulate)
+        L.within(dx.read(), *want[0], f"{size} dx")
+        v, e = want[1]
+        if accumulate:
+            v, e = v + before, e + 2.0 ** -10 * (np.abs(v) + np.abs(before)) + 2.0 ** -25
+        L.within(dw.read(), v, e, f"{size} dw")
+
+
+def test_gated_ff_gradients_of_no_size_in_fp16(T):
+    """dz of zero throughout, and infinities beside ordinary values: those stay what they are."""
+    n, d, f = 9, 40, 24
+    rng = np.random.RandomState(1)
+    x, w, dh, z = (L.rounded(rng.randn(*s), "f16") for s in ((n, d), (d, 2 * f), (n, f), (n, 2 * f)))
+    bx, bw, bz = Buf(T, x, "f16"), Buf(T, w, "f16"), Buf(T, z)
+    dx, dw = out(T, (n, d), "f16"), out(T, (d, 2 * f), "f16")
+    T.gated_ff_bwd(d, f, False, n, bx, bw, bz, Buf(T, 0 * dh, "f16"), dx, dw, None, act="none", dtype="f16")
+    assert (dx.read() == 0).all() and (dw.read() == 0).all()
+    dh[3, 5] = np.inf
+    T.gated_ff_bwd(d, f, False, n, bx, bw, bz, Buf(T, dh, "f16"), dx, dw, None, act="none", dtype="f16")
+    got = dx.read()
+    rest = [r for r in range(n) if r != 3]
+    assert not np.isfinite(got[3]).any()
+    want = f16_bounds(x[rest], w, z[rest], dh[rest])[0]
+    L.within(got[rest], *want, "rows beside an infinite one")
+    hit = np.zeros(2 * f, bool)
+    hit[[5, f + 5]] = True
+    assert np.isfinite(dw.read()[:, ~hit]).all() and not np.isfinite(dw.read()[:, hit]).any()

@@ -10,7 +10,9 @@
 //
 // z is kept in fp32 in every type, so that the derivative sees what the activation saw. dz is rounded to the 16-bit type once,
 // as the products' operand: in two parts each, dx and dW would cost twice the matrix work for one rounding among as
-// many as there are products' operands. db is summed before that rounding.
+// many as there are products' operands. db is summed before that rounding. fp16 has not the range of dz, which is a product of three
+// numbers: there dz is held times a power of two that brings its largest finite value into [2^14, 2^15), so what vanishes is 2^-39 of that
+// at most, and the products' sums are taken back by the same power (gate_dz_peak_kernel).
 #include "gemm16.h"
 #include "gemm_x3.h"
 
@@ -185,6 +187,11 @@ struct EpiGrad {
   int rows, cols;      // of C
   int hidden, half;    // two halves of columns, as above (one: both are cols)
   int accumulate;
+  const float *unscale = nullptr;   // fp16: what C has to be multiplied with (device memory; null: nothing)
+  __device__ __forceinline__ float factor() const {
+    if constexpr (std::is_same<T, f16>::value) return unscale ? *unscale : 1.0f;
+    return 1.0f;
+  }
   // where column n of C's row m goes (n is in use)
   __device__ __forceinline__ T *at(const size_t m, const int n) const {
     return out + m * (cols > half ? 2 * hidden : hidden) + (n < half ? n : n - half + hidden);
@@ -213,10 +220,11 @@ struct EpiGrad {
       return;
     }
     const G16Turn<32 * TN> turn{lds};
+    const float f = factor();
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) turn.put(lane, j, [&](int r) { return acc[i][j][r]; });
+      for (int j = 0; j < TN; ++j) turn.put(lane, j, [&](int r) { return f * acc[i][j][r]; });
       turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
         const int m = m0 + 32 * i + row, n = n0 + col;
         if (m >= rows) return;
@@ -274,7 +282,7 @@ grad_reduce_kernel(const EpiGrad<T> epi, const int splits) {
   float v = 0.0f;
 #pragma unroll 8
   for (int s = 0; s < splits; ++s) v += epi.partial[s * total + i];
-  epi.one(m, static_cast<int>(i - m * epi.cols), v);
+  epi.one(m, static_cast<int>(i - m * epi.cols), epi.factor() * v);
 }
 
 template <class T>
@@ -323,23 +331,15 @@ pack_kernel(const PackJobs<T> jobs) {
   *reinterpret_cast<uint4 *>(j.dst + i * 8) = v;
 }
 
-// dz as the products read it (type Z), [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
-// workgroup's band (in fp32, before the rounding). A thread takes a word of T's columns. Bound by memory: 4096 x 12288 in bf16 136-142 us,
-// 5.0 TB/s (z is 8 of its 14 bytes an element; read past the caches 142). A pass of its own: as a part of the products it would read
-// z and dh once a tile of columns, and dW reads dz with the other fast index.
-template <class T, class Z>
-__global__ void __launch_bounds__(GF_NT)
-gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restrict__ dz, float *__restrict__ bias_part,
-               const int rows, const int hidden, const int half, const int act, const int blocks_n, const int band_rows) {
-  constexpr int E = Word<T>::N;
-  const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
-  if (n >= half) return;
+// dz of the columns n .. of a word of T, row by row: take(m, dg, du), zero behind `hidden`
+template <class T, class F>
+__device__ __forceinline__ void gate_dz_rows(const float *__restrict__ z, const T *__restrict__ dh, const int n, const int hidden, const int act,
+                                             const int first, const int end, const F &take) {
+  constexpr int E  = Word<T>::N;
   const bool whole = n + E <= hidden;
-  float sg[E] = {}, su[E] = {};
-  const int end = min(rows, (band + 1) * band_rows);
   with_gate(act, [&](auto kind) {
 #pragma unroll 2
-    for (int m = band * band_rows; m < end; ++m) {
+    for (int m = first; m < end; ++m) {
       float g[E], u[E], d[E], dg[E], du[E];
       const float *zr = z + static_cast<size_t>(m) * 2 * hidden + n;
       const T *dr     = dh + static_cast<size_t>(m) * hidden + n;
@@ -372,32 +372,107 @@ gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restr
         dg[e] = d[e] * u[e] * slope;
         du[e] = d[e] * a;
         if (!whole && n + e >= hidden) dg[e] = du[e] = 0.0f;
-        sg[e] += dg[e];
-        su[e] += du[e];
       }
-      if (dz) {
-        Z *o = dz + static_cast<size_t>(m) * 2 * half + n;
-        if (n + E <= half) {
+      take(m, dg, du);
+    }
+  });
+}
+
+// The largest finite |dz| of a workgroup's part, in front of gate_dz_kernel: which power of two fp16 holds dz times. It reads what that pass
+// reads, as dz is known only then: 4096 x 12288 114 us (4.4 TB/s) of a step of 2480, 300 x 1000 4, a launch. A workgroup has no more than 1024 others beside it (or a row of them), as
+// every workgroup of the next pass reads all their peaks.
+template <class T>
+__global__ void __launch_bounds__(GF_NT)
+gate_dz_peak_kernel(const float *__restrict__ z, const T *__restrict__ dh, float *__restrict__ peaks, const int rows, const int hidden,
+                    const int act, const int blocks_n, const int band_rows) {
+  constexpr int E = Word<T>::N;
+  __shared__ float part[GF_NT / 64];
+  const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, first = blockIdx.x / blocks_n * band_rows;
+  float peak = 0.0f;
+  if (n < hidden)
+    gate_dz_rows(z, dh, n, hidden, act, first, min(rows, first + band_rows), [&](int, const float (&dg)[E], const float (&du)[E]) {
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const float(&v)[E] = s ? du : dg;
+      for (int e = 0; e < E; ++e) {
+        const float a = __builtin_fabsf(dg[e]), b = __builtin_fabsf(du[e]);
+        if (a < INFINITY) peak = fmaxf(peak, a);
+        if (b < INFINITY) peak = fmaxf(peak, b);
+      }
+    });
 #pragma unroll
-            for (int q = 0; q < E / Word<Z>::N; ++q) {
-              float w[Word<Z>::N];
+  for (int o = 32; o; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = peak;
+  __syncthreads();
+  if (threadIdx.x) return;
 #pragma unroll
-              for (int e = 0; e < Word<Z>::N; ++e) w[e] = v[q * Word<Z>::N + e];
-              store_word(o + s * half + q * Word<Z>::N, Word<Z>::from(w).raw);
-            }
-          }
-        } else {
+  for (int w = 1; w < GF_NT / 64; ++w) peak = fmaxf(peak, part[w]);
+  peaks[blockIdx.x] = peak;
+}
+// 2^k that brings the largest of n peaks into [2^14, 2^15) (as far as 2^126 does), the same in every thread of the workgroup
+__device__ __forceinline__ float gate_dz_scale(const float *__restrict__ peaks, const int n) {
+  __shared__ float part[GF_NT / 64];
+  float peak = 0.0f;
+  for (int i = threadIdx.x; i < n; i += GF_NT) peak = fmaxf(peak, peaks[i]);
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (n + e < half) {
-              o[e]        = from_f32<Z>(dg[e]);
-              o[half + e] = from_f32<Z>(du[e]);
-            }
+  for (int o = 32; o; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = peak;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < GF_NT / 64; ++w) peak = fmaxf(peak, part[w]);
+  // (exponents as they are held: the scale's is 127 + 14 - (peak's - 127))
+  return __uint_as_float(min(268u - (__float_as_uint(peak) >> 23), 253u) << 23);
+}
+// the peaks of a call, and where the inverse of the scale is left for the products (null: dz is not scaled)
+struct DzPeaks {
+  const float *peaks;
+  int n;
+  float *unscale;
+};
+
+// dz as the products read it (type Z), [rows][2 half], zero behind each half; and with `bias_part` the sums of dz over the rows of this
+// workgroup's band (in fp32, before the rounding). A thread takes a word of T's columns. Bound by memory: 4096 x 12288 in bf16 136-142 us,
+// 5.0 TB/s (z is 8 of its 14 bytes an element; read past the caches 142). A pass of its own: as a part of the products it would read
+// z and dh once a tile of columns, and dW reads dz with the other fast index.
+template <class T, class Z>
+__global__ void __launch_bounds__(GF_NT)
+gate_dz_kernel(const float *__restrict__ z, const T *__restrict__ dh, Z *__restrict__ dz, float *__restrict__ bias_part,
+               const int rows, const int hidden, const int half, const int act, const int blocks_n, const int band_rows, const DzPeaks peaks) {
+  constexpr int E = Word<T>::N;
+  float scale     = 1.0f;
+  if constexpr (std::is_same<Z, f16>::value)
+    if (peaks.unscale) {
+      scale = gate_dz_scale(peaks.peaks, peaks.n);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *peaks.unscale = __uint_as_float((254u << 23) - __float_as_uint(scale));
+    }
+  const int n = (blockIdx.x % blocks_n * GF_NT + threadIdx.x) * E, band = blockIdx.x / blocks_n;
+  if (n >= half) return;
+  float sg[E] = {}, su[E] = {};
+  gate_dz_rows(z, dh, n, hidden, act, band * band_rows, min(rows, (band + 1) * band_rows), [&](int m, const float (&dg)[E], const float (&du)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      sg[e] += dg[e];
+      su[e] += du[e];
+    }
+    if (!dz) return;
+    Z *o = dz + static_cast<size_t>(m) * 2 * half + n;
+    if (n + E <= half) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float(&v)[E] = s ? du : dg;
+#pragma unroll
+        for (int q = 0; q < E / Word<Z>::N; ++q) {
+          float w[Word<Z>::N];
+#pragma unroll
+          for (int e = 0; e < Word<Z>::N; ++e) w[e] = scale * v[q * Word<Z>::N + e];
+          store_word(o + s * half + q * Word<Z>::N, Word<Z>::from(w).raw);
         }
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (n + e < half) {
+          o[e]        = from_f32<Z>(scale * dg[e]);
+          o[half + e] = from_f32<Z>(scale * du[e]);
+        }
     }
   });
   if (bias_part) {
@@ -423,11 +498,29 @@ DzPlan dz_plan(int half, int batch, bool sums) {
   p.bands = ceil_div(batch, p.band_rows);
   return p;
 }
+// ... of the pass for the largest dz: four workgroups a compute unit at most, where a row of columns has no more
+template <class T>
+DzPlan dz_peak_plan(int hidden, int batch) {
+  DzPlan p;
+  p.blocks_n  = ceil_div(hidden, Word<T>::N * GF_NT);
+  p.band_rows = std::max(1, static_cast<int>((static_cast<long>(batch) * p.blocks_n + 1023) / 1024));
+  p.bands     = ceil_div(batch, p.band_rows);
+  return p;
+}
 template <class T, class Z>
-int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, Z *dz, float *bias_part) {
+int launch_dz(const DzPlan &p, int act, int hidden, int half, int batch, const float *z, const T *dh, Z *dz, float *bias_part,
+              const DzPeaks &peaks = DzPeaks{}) {
   ProfScope prof("gated_ff_dz", (8.0 + 3 * sizeof(T)) * batch * hidden, WORK_BYTE);
   TDH_LAUNCH((gate_dz_kernel<T, Z>), dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, dz, bias_part, batch, hidden, half,
-             act, p.blocks_n, p.band_rows);
+             act, p.blocks_n, p.band_rows, peaks);
+  TDH_LAUNCH_CHECK();
+  return TDH_OK;
+}
+template <class T>
+int launch_dz_peak(const DzPlan &p, int act, int hidden, int batch, const float *z, const T *dh, float *peaks) {
+  ProfScope prof("gated_ff_dz_peak", (8.0 + sizeof(T)) * batch * hidden, WORK_BYTE);
+  TDH_LAUNCH((gate_dz_peak_kernel<T>), dim3(p.blocks_n * p.bands), dim3(GF_NT), 0, ctx().stream, z, dh, peaks, batch, hidden, act, p.blocks_n,
+             p.band_rows);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
@@ -881,14 +974,25 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   const int bands = pz.bands;
   const FfPlan px = ff_plan(batch, in, 2 * half), pw = ff_plan(in, 2 * half, batch);
   const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
-  TDH_TRY(ws_begin(ws_align(sizeof(T) * batch * 2 * half) + ws_align(4 * static_cast<size_t>(bands) * 2 * hidden) +
+  const bool scaled = std::is_same<T, f16>::value && (dx || dw);
+  const DzPlan pp   = dz_peak_plan<T>(hidden, batch);
+  DzPeaks peaks{nullptr, pp.blocks_n * pp.bands, nullptr};
+  TDH_TRY(ws_begin((scaled ? ws_align(4 * (static_cast<size_t>(peaks.n) + 1)) : 0) +
+                   ws_align(sizeof(T) * batch * 2 * half) + ws_align(4 * static_cast<size_t>(bands) * 2 * hidden) +
                    (dx ? pack_bytes(w, in, hidden, 2) + ff_partial_bytes(px, nx) : 0) +
                    (dw ? pack_bytes(x, batch, in, 1) + ff_partial_bytes(pw, nw) : 0)));
   T *dz = nullptr;
   float *bias_part = nullptr;
   if (dx || dw) TDH_TRY(take(static_cast<size_t>(batch) * 2 * half, &dz));
   if (db) TDH_TRY(take(static_cast<size_t>(bands) * 2 * hidden, &bias_part));
-  TDH_TRY(launch_dz(pz, act, hidden, half, batch, z, dh, dz, bias_part));
+  if (scaled) {
+    float *p = nullptr;
+    TDH_TRY(take(static_cast<size_t>(peaks.n) + 1, &p));
+    peaks.peaks   = p;
+    peaks.unscale = p + peaks.n;
+    TDH_TRY(launch_dz_peak(pp, act, hidden, batch, z, dh, p));
+  }
+  TDH_TRY(launch_dz(pz, act, hidden, half, batch, z, dh, dz, bias_part, peaks));
   if (db) TDH_TRY(launch_db(bias_part, db, bands, hidden, accumulate));
   const G16Matrix Z{dz, 2L * half, batch, 2 * half};
   G16Matrix W, X;   // w: [in][2 half], of which the rows are the product's columns
@@ -897,10 +1001,10 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   if (dw) TDH_TRY(packer.add(x, batch, in, 1, &X));
   TDH_TRY(packer.run());
   if (dx) {
-    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0}, 2 * half, "gated_ff_dx")));
+    TDH_TRY((ff_grad<T, true, true>(px, Z, W, EpiGrad<T>{dx, nullptr, batch, in, in, in, 0, peaks.unscale}, 2 * half, "gated_ff_dx")));
   }
   if (dw) {
-    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate}, batch, "gated_ff_dw")));
+    TDH_TRY((ff_grad<T, false, false>(pw, X, Z, EpiGrad<T>{dw, nullptr, in, 2 * half, hidden, half, accumulate, peaks.unscale}, batch, "gated_ff_dw")));
   }
   return TDH_OK;
 }
