@@ -84,3 +84,47 @@ def test_gated_ff_gradients_of_no_size_in_fp16(T):
     hit = np.zeros(2 * f, bool)
     hit[[5, f + 5]] = True
     assert np.isfinite(dw.read()[:, ~hit]).all() and not np.isfinite(dw.read()[:, hit]).any()
+
+
+# ------------------------------------------- activations by their own size
+
+EPS = 2.0 ** -24   # of a rounding in fp32
+
+
+def gelu_off(g):
+    """What fp32 may be off: seven half-steps of each result with a reciprocal and an exponential rounded to nearest, and one
+    ulp (two half-steps) more for each of the two where they are the machine's; a few for the last products."""
+    from scipy.special import erfc
+    cdf, pdf = 0.5 * erfc(-g / np.sqrt(2)), np.exp(-g * g / 2) / np.sqrt(2 * np.pi)
+    return 16 * EPS * np.abs(g) * cdf, 16 * EPS * (cdf + np.abs(g) * pdf)
+
+
+ACT_OFF = {"gelu": (gelu_off, np.linspace(-12.5, 8, 1641))}   # (below, results of less than 2^-126)
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("n", [1, 9, 40])
+@pytest.mark.parametrize("act", ACT_OFF)
+def test_gated_ff_activations_by_their_own_size(T, act, n, dtype):
+    """One input of 1, up columns of 1 and a gate of whatever the weight is: h is the activation itself and db, of one sample with a
+    gradient, its derivative, both to be as near as their own size asks, in the tails too."""
+    off, g = ACT_OFF[act]
+    g = np.unique(L.rounded(g, dtype))
+    f = len(g)
+    z = np.tile(np.concatenate([g, np.ones(f)]), (n, 1))
+    x, w = Buf(T, np.ones((n, 1)), dtype), Buf(T, z[:1], dtype)
+    h, bz, db = out(T, (n, f), dtype), out(T, (n, 2 * f)), out(T, 2 * f, dtype)
+    T.gated_ff_fwd(1, f, False, n, x, w, None, h, bz, act=act, dtype=dtype)
+    assert np.array_equal(bz.read(), z)
+    dh = Buf(T, np.eye(n)[:, :1] * np.ones((n, f)), dtype)
+    T.gated_ff_bwd(1, f, True, n, x, w, bz, dh, None, None, db, act=act, dtype=dtype)
+    a, slope = L.gate(act, g)
+    a_off, slope_off = off(g)
+
+    def final(v, e):
+        return e + (0 if dtype == "f32" else L.HALF_ULP[dtype] * (np.abs(v) + e) + L.TINY[dtype])
+
+    L.within(h.read(), np.tile(a, (n, 1)), final(a, a_off), "h")
+    got = db.read()
+    L.within(got[f:], a, final(a, a_off), "the up half of db")
+    L.within(got[:f], slope, final(slope, slope_off), "the derivative")

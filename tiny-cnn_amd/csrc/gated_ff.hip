@@ -35,12 +35,21 @@ __device__ __forceinline__ float gate_act(const float g, float *slope) {
     *slope = s * (1.0f + g * (1.0f - s));
     return g * s;
   } else if constexpr (KIND == TDH_GATE_GELU) {
-    // erfc(x) for x >= 0 as a polynomial in 1 / (1 + p x) times exp(-x^2), off by 1.5e-7 at most (Abramowitz and
-    // Stegun, Handbook of Mathematical Functions, 7.1.26)
-    const float x = 0.70710678118654752f * __builtin_fabsf(g), e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
-    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
-    const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float cdf  = g < 0.0f ? tail : 1.0f - tail;   // (NaN stays)
+    // Beside zero cdf(-|g|) = erfc(x) / 2, x = |g| / sqrt(2), falls like exp(-x^2), and so that h keeps its figures there, the fit is one of
+    // erfc(x) exp(x^2) / 2, a polynomial in t = 1 / (1 + 0.38 x) without a constant term, off by 2.7e-8 of the value at most for 0 <= x <= 14.2
+    // (fitted for the least relative error), and g^2 brings its rounding along. In fp32 h is off by 7 half-ulps at most for
+    // -13 <= g <= 8, the derivative by 7 of cdf + |g| pdf.
+    const float c = __builtin_amdgcn_fmed3f(g, -20.0f, 20.0f);   // (exp(-200) is 0, and the square stays finite)
+    const float q = c * c, a = -0.72134752044448170f * q;
+    const float lo = __builtin_fmaf(q, -0.72134752044448170f, -a) - 0.72134752044448170f * __builtin_fmaf(c, c, -q) - 9.6298e-9f * q;
+    const float e0 = __builtin_amdgcn_exp2f(a), e = __builtin_fmaf(e0, 0.69314718055994531f * lo, e0);
+    const float t  = __builtin_amdgcn_rcpf(__builtin_fmaf(0.26870057f, __builtin_fabsf(c), 1.0f));
+    constexpr float fit[9] = {0.10720470547676086f, 0.10697626322507858f, 0.10180984437465668f, 0.06998414546251297f, 0.1132340133190155f,
+                              -0.07782156765460968f, 0.1790992021560669f, -0.12963144481182098f, 0.029144831001758575f};
+    float r = fit[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) r = __builtin_fmaf(r, t, fit[i]);
+    const float tail = e * (t * r), cdf = g < 0.0f ? tail : 1.0f - tail;   // (NaN stays)
     *slope = cdf + g * (0.39894228040143268f * e);
     return g * cdf;
   } else if constexpr (KIND == TDH_GATE_GELU_TANH) {
