@@ -99,7 +99,46 @@ def gelu_off(g):
     return 16 * EPS * np.abs(g) * cdf, 16 * EPS * (cdf + np.abs(g) * pdf)
 
 
-ACT_OFF = {"gelu": (gelu_off, np.linspace(-12.5, 8, 1641))}   # (below, results of less than 2^-126)
+def gate(kind, g):
+    """The activation and its derivative with 1 - s from an exponential, which keeps its figures in 64 bits too."""
+    from scipy.special import expit
+    if kind == "gelu":
+        return L.gate(kind, g)
+    k = 2 * np.sqrt(2 / np.pi)
+    y, dy = (k * (g + 0.044715 * g ** 3), k * (1 + 3 * 0.044715 * g * g)) if kind == "gelu_tanh" else (g, 1)
+    s, rest = expit(y), expit(-y)
+    return (s, s * rest) if kind == "sigmoid" else (g * s, s + g * s * rest * dy)
+
+
+def logistic_off(y):
+    """Of 1 / (1 + exp(-y)) and of 1 minus it, relative: y's rounding and its factor's, an ulp of the exponential and the reciprocal each,
+    a sum and a product."""
+    return EPS * (3 * np.abs(y) + 8)
+
+
+def sigmoid_off(g):
+    a, slope = gate("sigmoid", g)
+    return logistic_off(g) * a, 2 * (logistic_off(g) + EPS) * slope
+
+
+def silu_off(g):
+    s, ds = gate("sigmoid", g)
+    terms = s + np.abs(g) * ds     # of s (1 + g (1 - s))
+    return (logistic_off(g) + EPS) * np.abs(g) * s, (2 * logistic_off(g) + 4 * EPS) * terms
+
+
+def gelu_tanh_off(g):
+    from scipy.special import expit
+    k = 2 * np.sqrt(2 / np.pi)
+    y, dy = k * (g + 0.044715 * g ** 3), k * (1 + 3 * 0.044715 * g * g)
+    s, rest = expit(y), expit(-y)
+    off = EPS * (6 * np.abs(y) + 8)   # (a cube's two products and their sum more in y)
+    return (off + EPS) * np.abs(g) * s, (2 * off + 8 * EPS) * (s + np.abs(g) * s * rest * dy)
+
+
+# (where a result is less than 2^-126 it may be flushed)
+ACT_OFF = {"gelu": (gelu_off, np.linspace(-12.5, 8, 1641)), "sigmoid": (sigmoid_off, np.linspace(-80, 80, 1601)),
+           "silu": (silu_off, np.linspace(-80, 80, 1601)), "gelu_tanh": (gelu_tanh_off, np.linspace(-9.5, 9.5, 1521))}
 
 
 @pytest.mark.parametrize("dtype", L.DTYPES)
@@ -118,7 +157,7 @@ def test_gated_ff_activations_by_their_own_size(T, act, n, dtype):
     assert np.array_equal(bz.read(), z)
     dh = Buf(T, np.eye(n)[:, :1] * np.ones((n, f)), dtype)
     T.gated_ff_bwd(1, f, True, n, x, w, bz, dh, None, None, db, act=act, dtype=dtype)
-    a, slope = L.gate(act, g)
+    a, slope = gate(act, g)
     a_off, slope_off = off(g)
 
     def final(v, e):

@@ -22,17 +22,21 @@ namespace {
 
 constexpr int GF_NT = 256;
 
-// 1 / (1 + exp(-x)); the two instructions are off by an ulp each
-__device__ __forceinline__ float logistic(const float x) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+// s = 1 / (1 + exp(-x)); the two instructions are off by an ulp each. rest: 1 - s, from the exponential, as a difference it has nothing
+// left where s is next to 1 (the derivative of a sigmoid gate at 17 and more would be 0).
+__device__ __forceinline__ float logistic(const float x, float *rest) {
+  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * __builtin_fabsf(x)), big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+  *rest = x < 0.0f ? big : small;
+  return x < 0.0f ? small : big;
 }
 
 // the gate's activation, and its derivative
 template <int KIND>
 __device__ __forceinline__ float gate_act(const float g, float *slope) {
   if constexpr (KIND == TDH_GATE_SILU) {
-    const float s = logistic(g);
-    *slope = s * (1.0f + g * (1.0f - s));
+    float rest;
+    const float s = logistic(g, &rest);
+    *slope = s * (1.0f + g * rest);
     return g * s;
   } else if constexpr (KIND == TDH_GATE_GELU) {
     // Beside zero cdf(-|g|) = erfc(x) / 2, x = |g| / sqrt(2), falls like exp(-x^2), and so that h keeps its figures there, the fit is one of
@@ -56,12 +60,14 @@ __device__ __forceinline__ float gate_act(const float g, float *slope) {
     // 0.5 (1 + tanh(y)) = 1 / (1 + exp(-2 y)), y = sqrt(2/pi) (g + 0.044715 g^3); beyond 16 it is 0 or 1, and the
     // square in the derivative would overflow where its factor is 0
     const float c = __builtin_amdgcn_fmed3f(g, -16.0f, 16.0f);
-    const float s = logistic(1.5957691216057308f * (c + 0.044715f * c * c * c));
-    *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * c * c));
+    float rest;
+    const float s = logistic(1.5957691216057308f * (c + 0.044715f * c * c * c), &rest);
+    *slope = s + g * s * rest * (1.5957691216057308f * (1.0f + 0.134145f * c * c));
     return g * s;
   } else if constexpr (KIND == TDH_GATE_SIGMOID) {
-    const float s = logistic(g);
-    *slope = s * (1.0f - s);
+    float rest;
+    const float s = logistic(g, &rest);
+    *slope = s * rest;
     return s;
   } else if constexpr (KIND == TDH_GATE_RELU) {
     *slope = g > 0.0f ? 1.0f : 0.0f;
