@@ -725,6 +725,7 @@ inline GemmPlan plan_gemm(int M, int N, int K, bool allow_split) {
     const TileCfg &t = kTiles[c];
     if (t.bm > 32 && t.bm >= 2 * M && M > 0 && t.bm / 2 >= 32) continue;  // half the rows empty
     if (t.bn > 32 && t.bn >= 2 * N && t.bn / 2 >= 32) continue;
+    if (ceil_div(M, t.bm) > GRID_Y_MAX) continue;
     const double tiles = static_cast<double>(ceil_div(M, t.bm)) * ceil_div(N, t.bn);
     const double slots = kSlots * 256.0 / (64.0 * t.wm * t.wn);
     int splits = 1;
