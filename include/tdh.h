@@ -298,7 +298,8 @@ int tdh_dropout_seeded_bwd(int dtype, size_t n, float rate, uint64_t seed, uint6
 /* Log-probabilities of given tokens: logp[r] = logits[r][target[r]] - m - log(s), m the row's maximum and
  * s = sum_j exp(logits[r][j] - m). Row r starts ld elements behind row r-1 (ld >= vocab). A row with a negative
  * target does not count (prompt, padding): its logits are not read, logp and stats are 0. A target of vocab or more
- * gives NaN. stats [rows][2] receives (m, s), from which the gradient is computed; NULL where there is none. */
+ * gives NaN. stats [rows][2] receives (m, s), from which the gradient is computed; NULL where there is none. vocab up to
+ * 2^30, and fewer than 2^24 rows, of more than 65504 bytes fewer than 2^22; the same of the losses below. */
 int tdh_token_logprob_fwd(int dtype, int rows, int vocab, const void *logits, size_t ld, const int32_t *target,
                           float *logp, float *stats);
 /* dlogits[r][j] = dlogp[r] * ((j == target[r]) - exp(logits[r][j] - m) / s), zero in rows that do not count.

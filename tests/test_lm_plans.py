@@ -29,3 +29,28 @@ def test_fully_connected_products_have_no_more_tiles_of_rows_than_a_launch_takes
             for k in range(1, 40):
                 p = plan_gemm(m, n, k, split)
                 assert -(-m // p.bm) <= 65535, (m, n, k, p.cfg)
+
+
+class At:
+    """An address that no call may follow."""
+
+    def __init__(self, address):
+        self.ptr = C.c_void_p(address)
+
+
+@pytest.mark.parametrize("dtype,longest", [("f32", 16376), ("bf16", 32752), ("f16", 32752)])
+def test_long_rows_are_as_many_as_a_launch_has_threads_for(dtype, longest):
+    """A row of more than 4096 words gets up to 1024 threads, and 2^22 such rows are 2^32 threads, where a launch's number wraps and
+    it does nothing of the work without an error. (Calls that are not refused for that end where the library is not initialised, or at
+    a null tensor.)"""
+    a, b, d = At(1 << 44), At(1 << 45), At(1 << 46)
+    calls = {"logprob": lambda rows, v, t: T.token_logprob_fwd(rows, v, a, b, t, dtype=dtype),
+             "logprob_bwd": lambda rows, v, t: T.token_logprob_bwd(rows, v, a, b, d, d, t, dtype=dtype),
+             "policy": lambda rows, v, t: T.policy_loss(rows, v, a, b, t, None, d, dtype=dtype),
+             "preference": lambda rows, v, t: T.preference_loss(1, rows, v, a, b, t, dtype=dtype)}
+    for call in calls.values():
+        with pytest.raises(T.TdhError, match="64 KB"):
+            call(1 << 22, longest + 1, None)
+        for rows, v in (((1 << 22) - 1, longest + 1), (1 << 22, longest)):
+            with pytest.raises(T.TdhError, match="null tensor|too many"):
+                call(rows, v, None)

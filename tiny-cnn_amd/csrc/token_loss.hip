@@ -574,9 +574,12 @@ double logits_bytes(int dtype, int rows, int vocab, int passes) {
   return static_cast<double>(dtype_size(dtype)) * rows * vocab * passes;
 }
 
+constexpr size_t LONG_ROW = 65536 - 32;   // bytes of a row that is 4096 words at any alignment
 int check_logits(const char *who, int dtype, int rows, int vocab, const void *logits, size_t ld, const int32_t *target) {
   TDH_CHECK_ARG(dtype_known(dtype), "%s: element type %d", who, dtype);
   TDH_CHECK_ARG(rows >= 0 && rows <= GRID_X_MAX && vocab > 0 && vocab <= (1 << 30), "%s: %d rows of %d logits", who, rows, vocab);
+  // (a long row has up to 1024 threads, and a launch fewer than 2^32)
+  TDH_CHECK_ARG(rows < (1 << 22) || vocab * dtype_size(dtype) <= LONG_ROW, "%s: %d rows of %d logits, more than 64 KB each", who, rows, vocab);
   TDH_CHECK_ARG(ld >= static_cast<size_t>(vocab) && ld <= (static_cast<size_t>(1) << 40), "%s: rows of %d logits %zu elements apart", who, vocab, ld);
   TDH_CHECK_ARG(rows == 0 || (logits && target), "%s: null tensor", who);
   TDH_CHECK_ARG((reinterpret_cast<uintptr_t>(logits) & (dtype_size(dtype) - 1)) == 0, "%s: logits not aligned to their elements", who);
