@@ -54,3 +54,14 @@ def test_long_rows_are_as_many_as_a_launch_has_threads_for(dtype, longest):
         for rows, v in (((1 << 22) - 1, longest + 1), (1 << 22, longest)):
             with pytest.raises(T.TdhError, match="null tensor|too many"):
                 call(rows, v, None)
+
+
+def test_no_kernel_of_the_losses_that_nothing_launches():
+    """The row kernels that the library holds, by how many waves and words they have: log-probabilities of rows past 4096 words
+    are read as they come, and the policy loss never reads past the caches."""
+    import re
+    with open(os.path.join(os.path.dirname(T.__file__), "lib", "libtdh.so"), "rb") as f:
+        names = set(re.findall(rb"row_kernelI[A-Za-z0-9_]+?Li(\d)ELi(\d+)ELi(\d+)ELb([01])EEEvNS", f.read()))
+    got = {tuple(int(v) for v in n) for n in names}
+    both = {(1, 1), (1, 2), (1, 4), (1, 8), (4, 4), (4, 8), (4, 16), (16, 0), (16, 1), (16, 4)}
+    assert got == {(m, w, k, 0) for m in (0, 1) for w, k in both} | {(0, 8, 0, 0), (0, 8, 0, 1), (1, 16, 8, 0), (1, 16, 16, 0)}

@@ -537,13 +537,14 @@ int launch_rows(const RowArgs &a, bool again) {
     if (words <= 1024) return go(row_kernel<T, MODE, 4, 4, false>, 4);
     if (words <= 2048) return go(row_kernel<T, MODE, 4, 8, false>, 4);
     if (words <= 4096) return go(row_kernel<T, MODE, 4, 16, false>, 4);
-    if (MODE == ROW_LOGP) return again ? go(row_kernel<T, MODE, 8, 0, false>, 8) : go(row_kernel<T, MODE, 8, 0, true>, 8);
+    if constexpr (MODE == ROW_LOGP) return again ? go(row_kernel<T, MODE, 8, 0, false>, 8) : go(row_kernel<T, MODE, 8, 0, true>, 8);
   }
   if (words <= 1024) return go(row_kernel<T, MODE, 16, 1, false>, 16);
   if (words <= 4096) return go(row_kernel<T, MODE, 16, 4, false>, 16);
-  if (MODE == ROW_LOGP) return go(row_kernel<T, MODE, 16, 0, false>, 16);
-  if (words <= 8192) return go(row_kernel<T, MODE, 16, 8, false>, 16);
-  if (words <= 16384) return go(row_kernel<T, MODE, 16, 16, false>, 16);
+  if constexpr (MODE == ROW_POLICY) {
+    if (words <= 8192) return go(row_kernel<T, MODE, 16, 8, false>, 16);
+    if (words <= 16384) return go(row_kernel<T, MODE, 16, 16, false>, 16);
+  }
   return go(row_kernel<T, MODE, 16, 0, false>, 16);
 }
 
