@@ -65,3 +65,18 @@ def test_no_kernel_of_the_losses_that_nothing_launches():
     got = {tuple(int(v) for v in n) for n in names}
     both = {(1, 1), (1, 2), (1, 4), (1, 8), (4, 4), (4, 8), (4, 16), (16, 0), (16, 1), (16, 4)}
     assert got == {(m, w, k, 0) for m in (0, 1) for w, k in both} | {(0, 8, 0, 0), (0, 8, 0, 1), (1, 16, 8, 0), (1, 16, 16, 0)}
+
+
+def test_assembly_that_writes_m0_leaves_it_as_it_was():
+    """The compiler keeps m0 for itself (named as clobbered it is warned about and no more)."""
+    import glob
+    import re
+    found = 0
+    for path in glob.glob(os.path.join(os.path.dirname(T.__file__), "csrc", "*.h*")):
+        with open(path) as f:
+            for asm in re.findall(r"asm\s+volatile\s*\((.*?)\);", f.read(), re.S):
+                if "s_mov_b32 m0" in asm:
+                    found += 1
+                    text = "".join(re.findall(r'"([^"]*)"', asm.split("\n")[0])).replace("\\n\\t", "\n").split("\n")
+                    assert text[0] == "s_mov_b32 %0, m0" and text[-1] == "s_mov_b32 m0, %0" and '"=&s"' in asm, (path, asm)
+    assert found

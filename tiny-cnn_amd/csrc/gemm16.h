@@ -110,10 +110,15 @@ struct G16Side {
       // (a wave's 64 lanes fill 1024 bytes of LDS from an address that is the same for all of them)
       const unsigned to = __builtin_amdgcn_readfirstlane(
           static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds)) + (tid & ~63) * 16);
+      // (m0 holds where the load writes; the compiler keeps that register for itself, and finds it as it was)
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * NT * 16), "v"(off[i]), "s"(desc)
+      for (int i = 0; i < PER; ++i) {
+        unsigned was;
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                     : "=&s"(was)
+                     : "s"(to + i * NT * 16), "v"(off[i]), "s"(desc)
                      : "memory");
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
