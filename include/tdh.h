@@ -313,7 +313,7 @@ int tdh_token_logprob_bwd(int dtype, int rows, int vocab, const void *logits, si
  *                        + kl_coef * (exp(gap) - gap - 1)),
  * loss[0] = the sum of row_loss, and dlogits its gradient. weight NULL: 1 for every row (1 / rows makes a mean). It is a
  * factor and no mask: 0 times an infinite loss is NaN, and rows whose values mean nothing have a negative target.
- * ref_logp NULL: no KL term. Any of logp, row_loss, loss and dlogits may be NULL; dlogits as in
+ * ref_logp NULL or kl_coef 0: no KL term. Any of logp, row_loss, loss and dlogits may be NULL; dlogits as in
  * tdh_token_logprob_bwd. Where the two sides of the minimum are equal the gradient is the first one's. */
 typedef struct tdh_policy_desc {
   float clip_low, clip_high, kl_coef;
@@ -327,7 +327,8 @@ int tdh_policy_loss(const tdh_policy_desc *p, int dtype, int rows, int vocab, co
  * seq_logp[s] the sum of logp over the sequence's rows that count and ref_logp[s] the same of the reference
  * model (NULL: 0),
  *   margin = beta * ((seq_logp - ref_logp)[2p] - (seq_logp - ref_logp)[2p+1]), and its loss
- *   TDH_PREF_SIGMOID  (1 - smoothing) * log(1 + exp(-margin)) + smoothing * log(1 + exp(margin))
+ *   TDH_PREF_SIGMOID  (1 - smoothing) * log(1 + exp(-margin)) + smoothing * log(1 + exp(margin)), without the side whose
+ *                     factor is 0
  *   TDH_PREF_SQUARED  ((margin - 1/2) / beta)^2
  *   TDH_PREF_HINGE    max(0, 1 - margin)   (derivative 0 at 1)
  * loss[0] = the mean over the pairs, dlogits its gradient. Any of logp [rows], seq_logp [2*pairs], margin [pairs],

@@ -167,3 +167,46 @@ def test_gated_ff_activations_by_their_own_size(T, act, n, dtype):
     got = db.read()
     L.within(got[f:], a, final(a, a_off), "the up half of db")
     L.within(got[:f], slope, final(slope, slope_off), "the derivative")
+
+
+# ------------------------------------------------- losses of impossible tokens
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("vocab", [9, 40, 5000])
+def test_policy_loss_whose_kl_coefficient_is_zero(T, dtype, vocab):
+    """A token that the model has at -inf, or 1500 below the others, beside a reference that has it: a KL term of infinity, of which a
+    coefficient of 0 takes nothing. The call is the one without a reference, bit for bit."""
+    rng = np.random.RandomState(vocab)
+    x = L.rounded(rng.randn(5, vocab), dtype)
+    x[1, 3], x[2, 3] = -np.inf, L.rounded(np.array([-1500.0]), dtype)[0]
+    target, adv = np.full(5, 3, np.int32), np.ones(5)
+    now = np.full(5, -2.0)
+    got = []
+    for ref in (None, Buf(T, now)):
+        row, loss, g = out(T, 5), out(T, 1), out(T, (5, vocab), dtype)
+        T.policy_loss(5, vocab, Buf(T, x, dtype), Buf(T, target, "i32"), Buf(T, now), ref, Buf(T, adv), None, None, row, loss, g, kl_coef=0.0,
+                      dtype=dtype)
+        got.append((row.bits(), loss.bits(), g.bits()))
+        assert np.isfinite(row.read()).all() and np.isfinite(loss.read()).all() and np.isfinite(g.read()).all()
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("pairs", [1, 12])
+@pytest.mark.parametrize("smoothing", [0.0, 1.0, 0.25])
+@pytest.mark.parametrize("impossible", ["rejected", "chosen"])
+def test_preference_loss_of_an_infinite_margin(T, impossible, smoothing, pairs):
+    """An answer that the model cannot give makes its pair's margin infinite. The side that has no share in the loss adds nothing:
+    without smoothing an impossible rejected answer costs nothing, and an impossible chosen one everything."""
+    rows, vocab = 2 * pairs, 7
+    x = np.zeros((rows, vocab))
+    x[0 if impossible == "chosen" else 1, 2] = -np.inf
+    start, target = np.arange(rows + 1).astype(np.int32), np.full(rows, 2, np.int32)
+    margin, loss, g = out(T, pairs), out(T, 1), out(T, (rows, vocab))
+    T.preference_loss(pairs, rows, vocab, Buf(T, x), Buf(T, target, "i32"), Buf(T, start, "i32"), margin=margin, loss=loss, dlogits=g,
+                      beta=0.5, smoothing=smoothing)
+    assert margin.read()[0] == (np.inf if impossible == "rejected" else -np.inf) and (margin.read()[1:] == 0).all()
+    share = {"rejected": smoothing, "chosen": 1 - smoothing}[impossible]
+    want = np.inf if share else (pairs - 1) * np.log(2.0) / pairs
+    L.within(loss.read(), [want], 0 if share else 2.0 ** -23 * want)
+    assert np.isfinite(g.read()).all()

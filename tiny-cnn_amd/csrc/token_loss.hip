@@ -126,7 +126,7 @@ __device__ __forceinline__ double policy_row(const RowArgs &a, const int row, co
   const double low = 1.0 - static_cast<double>(a.clip_low), high = 1.0 + static_cast<double>(a.clip_high);
   const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
   double l = -(free <= held || free != free ? free : held), d = free <= held ? -free : free > held ? 0.0 : free;
-  if (a.ref_logp) {
+  if (a.ref_logp && a.kl_coef != 0.0f) {   // (a coefficient of 0 leaves the term out, which may be infinite)
     const double gap = static_cast<double>(a.ref_logp[row]) - logp, e = expm1(gap), k = a.kl_coef;
     l += k * (e - gap);
     d -= k * e;
@@ -336,7 +336,8 @@ __device__ __forceinline__ PairValue pair_value(const PairArgs &a, const int pai
       const double e = exp(-fabs(m)), l = log1p(e);
       const double neg = m > 0 ? l : l - m, pos = m > 0 ? l + m : l;   // softplus(-m), softplus(m)
       const double up = (m > 0 ? e : 1.0) / (1.0 + e);                 // sigmoid(-m)
-      loss = (1.0 - a.smoothing) * neg + a.smoothing * pos;
+      // (a share of 0 leaves its side out: at an infinite margin the other one is infinite)
+      loss = (a.smoothing == 1.0 ? 0.0 : (1.0 - a.smoothing) * neg) + (a.smoothing == 0.0 ? 0.0 : a.smoothing * pos);
       dm   = a.smoothing * ((m > 0 ? 1.0 : e) / (1.0 + e)) - (1.0 - a.smoothing) * up;
     } break;
     case TDH_PREF_SQUARED: {
