@@ -80,3 +80,23 @@ def test_assembly_that_writes_m0_leaves_it_as_it_was():
                     text = "".join(re.findall(r'"([^"]*)"', asm.split("\n")[0])).replace("\\n\\t", "\n").split("\n")
                     assert text[0] == "s_mov_b32 %0, m0" and text[-1] == "s_mov_b32 m0, %0" and '"=&s"' in asm, (path, asm)
     assert found
+
+
+class FfPlan(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("cfg", "splits", "k_per_split")]
+
+
+def test_the_gpu_tests_reach_every_tile_of_the_16_bit_products():
+    """Forward, input and weight gradient, each on all five tiles, split along the reduction and whole."""
+    import test_gpu_lm_sizes as sizes
+    f = T.lib()._ZN3tdh7ff_planEiiib   # tdh::ff_plan
+    f.restype, f.argtypes = FfPlan, [C.c_int] * 3 + [C.c_bool]
+    for aligned in (False, True):
+        reached = set()
+        for n, d, h in sizes.TILE_SHAPES:
+            half = (h + 7) & ~7
+            d = (d + 7) & ~7 if aligned else d
+            for product, plan in (("forward", f(n, 2 * half, d, True)), ("dx", f(n, d, 2 * half, False)), ("dw", f(d, 2 * half, n, False))):
+                reached.add((product, plan.cfg, plan.splits > 1))
+        missing = {(p, c, s) for p in ("forward", "dx", "dw") for c in range(5) for s in (False, True)} - reached
+        assert not missing, (aligned, missing)

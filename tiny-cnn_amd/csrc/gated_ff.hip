@@ -843,10 +843,12 @@ int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, cons
 }
 
 // ---- plans
+}  // namespace
 struct FfPlan {
   int cfg;       // index into FF_TILES
   int splits, k_per_split;
 };
+namespace {
 // A tile shape: the workgroups that a compute unit holds, us of a tile of 64 reduction indices with one, two, ... of them on a
 // compute unit (all of them take that long), us of a round of workgroups beside that, and of the launch. Measured on
 // products of 256 to 1024 tiles with k of 64 to 2048; 256 x 256 reaches 1100 TFLOP/s there, 128 x 128 990, 64 x 128 760,
@@ -867,7 +869,8 @@ constexpr FfTile FF_TILES[] = {{256, 256, 2, 1, {1.65}, 5.0, 5.0},
 // 11), and of rows of 64 or 128 bytes 0.4 or 0.6 of that (pair: an unsplit tile takes half of its columns from either half of
 // the matrix; the product above, 64 x 128: 64 us, 39 if its columns lie together). A split's slices are written and
 // read once and its sum is another launch.
-FfPlan ff_plan(int M, int N, int K, bool pair = false) {
+}  // namespace
+FfPlan ff_plan(int M, int N, int K, bool pair) {
   const long cus    = ctx().compute_units > 0 ? ctx().compute_units : 256;
   const int ktiles  = std::max(1, ceil_div(K, G16_BK));
   const double read = 2.0 * (static_cast<double>(M) + N) * K;
@@ -898,6 +901,7 @@ FfPlan ff_plan(int M, int N, int K, bool pair = false) {
   }
   return best;
 }
+namespace {
 size_t ff_partial_bytes(const FfPlan &p, size_t elements) { return p.splits > 1 ? ws_align(4 * p.splits * elements) : 0; }
 
 // N: the columns of B in use (PAIR: both halves)
@@ -987,7 +991,7 @@ int ff_bwd_16(int act, int in, int hidden, int batch, const T *x, const T *w, co
   const int half = padded(hidden);
   const DzPlan pz = dz_plan<T>(half, batch, db != nullptr);
   const int bands = pz.bands;
-  const FfPlan px = ff_plan(batch, in, 2 * half), pw = ff_plan(in, 2 * half, batch);
+  const FfPlan px = ff_plan(batch, in, 2 * half, false), pw = ff_plan(in, 2 * half, batch, false);
   const size_t nx = static_cast<size_t>(batch) * in, nw = static_cast<size_t>(in) * 2 * half;
   const bool scaled = std::is_same<T, f16>::value && (dx || dw);
   const DzPlan pp   = dz_peak_plan<T>(hidden, batch);
