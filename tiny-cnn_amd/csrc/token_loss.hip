@@ -166,7 +166,9 @@ __device__ __forceinline__ void skip_row(const RowArgs &a, const int row) {
 
 // WAVES waves a row; W 16-byte words a thread in registers, or W = 0: any number, read once more for the gradient. Rows in
 // registers of few waves are fastest as long as several workgroups fit a compute unit (policy loss of 8192 x 32000 in
-// bf16: 4 waves 198 us, 8 waves 208, 16 waves 258, read twice 214).
+// bf16, 4000 words: 4 waves 198 us, 8 waves 208, 16 waves 258, read twice 214). Longer rows do not fit 4 waves; 16 of them hold
+// up to 16384 words, beyond which the 16 read twice. us so / with 8 waves that read twice: 4096 x 50001 in bf16 197 / 190, 4096 x 32001 in
+// fp32 202 / 230, 1024 x 100000 in bf16 88 / 107, 4096 x 131072 in bf16 424 / 452, 2048 x 131075 in fp32 478 / 554.
 template <class T, int MODE, int WAVES, int W, bool ONCE>
 __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256)
 row_kernel(const RowArgs a) {
