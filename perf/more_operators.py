@@ -244,13 +244,14 @@ def _plain_sample(c, t):
     keep &= (mass - w < top_p.double() * mass[:, -1:]) | (top_p >= 1)
     keep &= w >= min_p.double()
     kept = torch.zeros_like(keep).scatter_(1, order, keep)
+    # (what the others add to the likeliest token's 1, whose logarithm is that small where one token has it all)
+    rest = (w * keep)[:, 1:].sum(1, keepdim=True)
     w = torch.where(kept, torch.exp((x - top) / temperature.double()), torch.zeros((), device=x.device, dtype=torch.float64))
     mass = torch.cumsum(w, 1)
-    total = mass[:, -1:]
-    token = torch.searchsorted(mass, t["u"].double()[:, None] * total, right=True).clamp(max=v - 1)
+    token = torch.searchsorted(mass, t["u"].double()[:, None] * mass[:, -1:], right=True).clamp(max=v - 1)
     chosen = x.gather(1, token) - top
-    logp = chosen - torch.log(torch.exp(x - top).sum(1, keepdim=True))
-    logq = chosen / temperature.double() - torch.log(total)
+    logp = chosen - torch.log1p(torch.exp(sorted_x[:, 1:] - top).sum(1, keepdim=True))
+    logq = chosen / temperature.double() - torch.log1p(rest)
     return {"token": token[:, 0].to(torch.int32), "kept": kept.sum(1).to(torch.int32), "logp": logp[:, 0].float(), "logq": logq[:, 0].float()}
 
 
@@ -332,13 +333,14 @@ def _exact_sample(c, t):
             order, prob = order[:n], prob[:n]
         n = int((prob >= q * prob[0]).sum())
         ids, _ = torch.sort(order[:n])
-        logq = torch.log_softmax(x[ids] / temp, 0)
-        edge = torch.cumsum(torch.exp(logq), 0)
+        edge = torch.cumsum(torch.softmax(x[ids] / temp, 0), 0)
         at = min(int((edge <= t["u"][r].double() * edge[-1]).sum()), n - 1)
         out["token"].append(ids[at])
         out["kept"].append(torch.tensor(n))
-        out["logq"].append(logq[at])
-        out["logp"].append(x[ids[at]] - torch.logsumexp(x, 0))
+        first = x[order[0]]
+        for name, others, scale in (("logq", order[1:n], temp), ("logp", fine[fine != order[0]], 1.0)):
+            log_sum = torch.logaddexp(torch.zeros_like(first), torch.logsumexp((x[others] - first) / scale, 0))
+            out[name].append((x[ids[at]] - first) / scale - log_sum)
     return {k: torch.stack([v.to("cuda") for v in vs]).to(torch.int32 if k in ("token", "kept") else torch.float64) for k, vs in out.items()}
 
 
