@@ -341,6 +341,18 @@ int tdh_preference_loss(const tdh_preference_desc *p, int dtype, int pairs, int 
                         const int32_t *target, const int32_t *seq_start, const float *ref_logp, float *logp,
                         float *seq_logp, float *margin, float *loss, void *dlogits, size_t ld_d);
 
+/* Layer normalisation of rows: y = (x - mean) * rstd * gamma + beta with the row's mean and rstd = 1 / sqrt(variance + eps), the variance
+ * over len. Rows of x are ld elements apart, of y ld_y (both >= len). gamma [len] and beta [len], or NULL for 1 and 0. stats [rows][2]
+ * receives (mean, rstd), which the backward pass reads; NULL where there is none. y may be x (with ld_y == ld). eps is positive and
+ * normal, len up to 2^24, fewer than 2^24 rows; sums are fp32, so the squares of a row's deviations have to add up to less than 2^127. */
+int tdh_layernorm_fwd(int dtype, int rows, int len, float eps, const void *x, size_t ld, const void *gamma, const void *beta,
+                      void *y, size_t ld_y, float *stats);
+/* With xhat = (x - mean) * rstd and g = dy * gamma: dx = rstd * (g - mean(g) - xhat * mean(g * xhat)), means over the row; dgamma = the sum
+ * over the rows of dy * xhat, dbeta = that of dy. dx is overwritten, and may be dy (with ld_dx == ld_dy); dgamma and dbeta are
+ * overwritten, or added to with accumulate != 0. Any of dx, dgamma and dbeta may be NULL. */
+int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, const void *gamma, const float *stats,
+                      const void *dy, size_t ld_dy, void *dx, size_t ld_dx, void *dgamma, void *dbeta, int accumulate);
+
 /* n elements from one element type to another, rounded to nearest: fp32 weights to the 16-bit ones that a block
  * computes with, and its 16-bit gradients to the fp32 ones that tdh_opt_update takes */
 int tdh_cast(int dst_dtype, int src_dtype, size_t n, const void *src, void *dst);

@@ -1,0 +1,52 @@
+"""What layer normalisation, the orthogonalised update, token sampling and products in 8-bit integers refuse, before anything reaches a
+device."""
+import ctypes as C
+import importlib
+import os
+import sys
+
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_lm_operators import A, B, D, At, refuses  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def T():
+    return importlib.import_module("tiny-cnn_amd")
+
+
+F, G = At(0x400000000), At(0x500000000)
+
+
+def test_layernorm_refusals(T):
+    fwd, bwd = T.layernorm_fwd, T.layernorm_bwd
+    refuses(T, "rows of", fwd, -1, 8, A, B, B, D)
+    refuses(T, "rows of", fwd, 4, 0, A, B, B, D)
+    refuses(T, "rows of", fwd, 1 << 24, 8, A, B, B, D)
+    refuses(T, "rows of", bwd, 4, (1 << 24) + 1, A, None, F, D, G, None, None)
+    for eps in (0.0, -1e-5, 1e-42, float("inf"), float("nan")):
+        refuses(T, "eps", fwd, 4, 8, A, B, B, D, eps=eps)
+    refuses(T, "null tensor", fwd, 4, 8, None, B, B, D)
+    refuses(T, "null tensor", fwd, 4, 8, A, B, B, None)
+    refuses(T, "null tensor", bwd, 4, 8, A, None, None, D, G, None, None)
+    refuses(T, "null tensor", bwd, 4, 8, A, None, F, None, G, None, None)
+    refuses(T, "of x 7 apart", fwd, 4, 8, A, B, B, D, ld=7)
+    refuses(T, "of y 7 apart", fwd, 4, 8, A, B, B, D, ld_y=7)
+    refuses(T, "of dy 7 apart", bwd, 4, 8, A, None, F, D, G, None, None, ld_dy=7)
+    refuses(T, "of dx 7 apart", bwd, 4, 8, A, None, F, D, G, None, None, ld_dx=7)
+    refuses(T, "aligned", fwd, 4, 8, At(A.ptr.value + 1), B, B, D, dtype="f16")
+    refuses(T, "aligned", fwd, 4, 8, A, At(B.ptr.value + 1), B, D, dtype="f16")
+    refuses(T, "aligned", fwd, 4, 8, A, B, B, D, At(F.ptr.value + 2), dtype="f16")
+    refuses(T, "aligned", bwd, 4, 8, A, None, F, D, G, At(B.ptr.value + 2), None)
+    refuses(T, "overlaps an input", fwd, 4, 8, A, B, B, At(A.ptr.value + 4))
+    refuses(T, "overlaps an input", fwd, 4, 8, A, B, B, A, ld=16)
+    refuses(T, "overlaps an input", fwd, 4, 8, A, B, B, B)
+    refuses(T, "overlaps an input", fwd, 4, 8, A, B, B, D, At(A.ptr.value + 120))
+    refuses(T, "two outputs overlap", fwd, 4, 8, A, B, B, D, At(D.ptr.value + 120))
+    refuses(T, "overlaps an input", bwd, 4, 8, A, None, F, D, A, None, None)
+    refuses(T, "overlaps an input", bwd, 4, 8, A, None, F, D, At(D.ptr.value + 4), None, None)
+    refuses(T, "overlaps an input", bwd, 4, 8, A, None, F, D, G, At(D.ptr.value + 8), None)
+    refuses(T, "two outputs overlap", bwd, 4, 8, A, None, F, D, None, G, At(G.ptr.value + 28))
+    assert T.lib().tdh_layernorm_fwd(3, 4, 8, C.c_float(1e-5), A.ptr, C.c_size_t(8), None, None, D.ptr, C.c_size_t(8), None) == -1
+    assert b"element type" in T.lib().tdh_last_error()

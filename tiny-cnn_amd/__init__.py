@@ -524,6 +524,19 @@ def preference_loss(pairs, rows, vocab, logits, target, seq_start, ref_logp=None
                                     _p(dlogits), C.c_size_t(ld_d or vocab)), "tdh_preference_loss")
 
 
+def layernorm_fwd(rows, length, x, gamma, beta, y, stats=None, eps=1e-5, dtype="f32", ld=None, ld_y=None):
+    """y = (x - mean) * rstd * gamma + beta row by row; stats [rows][2], (mean, rstd) in fp32, is what layernorm_bwd reads"""
+    check(lib().tdh_layernorm_fwd(DTYPE[dtype], rows, length, C.c_float(eps), _p(x), C.c_size_t(ld or length), _p(gamma), _p(beta),
+                                  _p(y), C.c_size_t(ld_y or length), _p(stats)), "tdh_layernorm_fwd")
+
+
+def layernorm_bwd(rows, length, x, gamma, stats, dy, dx, dgamma, dbeta, dtype="f32", accumulate=False, ld=None, ld_dy=None,
+                  ld_dx=None):
+    check(lib().tdh_layernorm_bwd(DTYPE[dtype], rows, length, _p(x), C.c_size_t(ld or length), _p(gamma), _p(stats), _p(dy),
+                                  C.c_size_t(ld_dy or length), _p(dx), C.c_size_t(ld_dx or length), _p(dgamma), _p(dbeta),
+                                  int(accumulate)), "tdh_layernorm_bwd")
+
+
 def cast(n, src, dst, src_dtype, dst_dtype):
     check(lib().tdh_cast(DTYPE[dst_dtype], DTYPE[src_dtype], C.c_size_t(n), _p(src), _p(dst)), "tdh_cast")
 
