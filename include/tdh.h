@@ -353,6 +353,39 @@ int tdh_layernorm_fwd(int dtype, int rows, int len, float eps, const void *x, si
 int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, const void *gamma, const float *stats,
                       const void *dy, size_t ld_dy, void *dx, size_t ld_dx, void *dgamma, void *dbeta, int accumulate);
 
+/* A token of every row of logits, drawn with the row's number u in [0, 1). Of the tokens whose logit is not -inf, likeliest first and equal ones
+ * by their index, these are left:
+ *   the first top_k (0: all), of those
+ *   the shortest beginning whose share of their probability softmax(logits / temperature) is top_p or more (1: all), of those
+ *   the ones with at least min_p times the probability of the likeliest (0: all),
+ * always the first one. token[r] is the first one left, by index, at which the sum of the probabilities of those left exceeds u times the sum
+ * over all of them. temperature 0 takes the likeliest. logp[r] is the token's log-probability under softmax(logits), which
+ * tdh_policy_loss takes as old_logp; logq[r] the one that it was drawn with; kept[r] how many were left; any of the three may be NULL. A u below 0
+ * or NaN counts as 0, of 1 or more as the last number below 1. A row with NaN or +inf, or nothing but -inf, gives token -1, kept 0 and NaN.
+ * Probabilities are summed as whole multiples of 2^-45 of the likeliest's (vocab up to 2^17; 2^-50 up to 2^12, 2^(b - 62) from vocab 2^b on), so the
+ * same inputs give the same token.
+ * settings (device, [rows]): each row's own descriptor in the place of p, or NULL. Values out of range there: top_k below 1
+ * and top_p of 1 or more, and NaN, leave all; top_p of 0 or less the likeliest; min_p of 0 or less, and NaN, all, above 1 what has the likeliest's
+ * logit; a temperature that is 0 or less or NaN takes the likeliest, an infinite one leaves all equal. vocab up to 2^30, fewer than 2^22 rows,
+ * ld elements apart. */
+typedef struct tdh_sample_desc {
+  float temperature;
+  int32_t top_k;
+  float top_p, min_p;
+} tdh_sample_desc;
+int tdh_sample_tokens(const tdh_sample_desc *p, const tdh_sample_desc *settings, int dtype, int rows, int vocab, const void *logits, size_t ld,
+                      const float *u, int32_t *token, float *logp, float *logq, int32_t *kept);
+
+/* Products with weights in 8 bits. A row of weights holds one output's, wq [out][tdh_q8_row(in)], where bytes behind `in` are 0; output n stands for
+ * wq[n] * wscale[n]. tdh_fc_q8_pack makes them of w [in][out]: wscale[n] = max |w[.][n]| / 127, wq = w / wscale rounded to nearest. */
+size_t tdh_q8_row(int in); /* `in` rounded up to 16 */
+int tdh_fc_q8_pack(int dtype, int in, int out, const void *w, int8_t *wq, float *wscale);
+/* y = x W + b with every sample of x in 8 bits too: scale = max |x| / 127 of the sample (fp32), q = x / scale (fp32) rounded to nearest, ties to
+ * even; y[m][n] = (sum_k q[m][k] wq[n][k]) * scale[m] * wscale[n] + b[n], the sum in 32-bit integers, which is exact. A sample with NaN or an
+ * infinity gives NaN. in up to 2^17, out up to 2^20, batch up to 2^24, no tensor of 2^31 elements. wq lies on a 16-byte boundary. */
+int tdh_fc_q8_fwd(int dtype, int in, int out, int has_bias, int batch, const void *x, const int8_t *wq, const float *wscale,
+                  const void *b, void *y);
+
 /* n elements from one element type to another, rounded to nearest: fp32 weights to the 16-bit ones that a block
  * computes with, and its 16-bit gradients to the fp32 ones that tdh_opt_update takes */
 int tdh_cast(int dst_dtype, int src_dtype, size_t n, const void *src, void *dst);
@@ -367,6 +400,29 @@ int tdh_cast(int dst_dtype, int src_dtype, size_t n, const void *src, void *dst)
 int tdh_opt_update(tdh_opt *o, size_t n, const float *merged_grad, float grad_scale, float *w,
                    float *s0, float *s1);
 void tdh_opt_default(tdh_opt *o, int kind);
+
+/* The update of a matrix by its orthogonalised momentum (K. Jordan et al., "Muon: an optimizer for hidden layers in neural networks", 2024). It has no
+ * counterpart in the reference. Of a matrix U, steps times from X = U / (|U| + eps), |U| the root of the sum of squares:
+ *   A = X X^T, X <- a X + (b A + c A A) X       (A = X^T X on the right-hand side where there are more rows than columns)
+ * which takes every singular value s to s (a + b s^2 + c s^4) and leaves the singular vectors: the result O is near the orthogonal factor of U.
+ * products: TDH_F32 or TDH_F16, what the products' operands are held in. TDH_F32: in three bf16 parts, as precise as fp32. TDH_F16:
+ * rounded to fp16 around known magnitudes; X itself and all sums stay in fp32, and O is off by 1e-3 of its size for a, b, c as they are by default.
+ * Coefficients that take a singular value of at most 1 beyond 4 in any step are refused. Up to 16384 on the shorter side, 2^20 on the longer and
+ * 2^30 elements in all. */
+typedef struct tdh_muon {
+  float alpha, mu, lambda; /* learning rate, momentum, decay */
+  float scale;             /* of the update, beside alpha: sqrt(max(1, out / in)) and the like */
+  int32_t nesterov;
+  int32_t steps;           /* 0 to 32 */
+  float a, b, c, eps;
+  int32_t products;
+} tdh_muon;
+void tdh_muon_default(tdh_muon *o);
+/* y = O of x [rows][cols]; may be x. alpha, mu, lambda, scale and nesterov are not read. */
+int tdh_orthogonalize(const tdh_muon *o, int dtype, int rows, int cols, const void *x, void *y);
+/* With g = merged_grad * grad_scale (merged_grad in dtype, weights and momentum in fp32, all [rows][cols]):
+ *   momentum = mu * momentum + g, U = nesterov ? g + mu * momentum : momentum, w = w - alpha * (scale * O + lambda * w) */
+int tdh_muon_update(const tdh_muon *o, int dtype, int rows, int cols, const void *merged_grad, float grad_scale, float *w, float *momentum);
 
 /* ------------------------------------------------------ sequential network */
 /* network<sequential>::fit / train_onebatch (tiny_dnn/network.h:840-926) with

@@ -50,3 +50,29 @@ def test_layernorm_refusals(T):
     refuses(T, "two outputs overlap", bwd, 4, 8, A, None, F, D, None, G, At(G.ptr.value + 28))
     assert T.lib().tdh_layernorm_fwd(3, 4, 8, C.c_float(1e-5), A.ptr, C.c_size_t(8), None, None, D.ptr, C.c_size_t(8), None) == -1
     assert b"element type" in T.lib().tdh_last_error()
+
+
+def test_sample_refusals(T):
+    f, one = T.sample_tokens, (4, 8, A, B, D)
+    refuses(T, "rows of", f, -1, 8, A, B, D)
+    refuses(T, "rows of", f, 1 << 22, 8, A, B, D)
+    refuses(T, "rows of", f, 4, 0, A, B, D)
+    refuses(T, "rows of", f, 4, (1 << 30) + 1, A, B, D)
+    refuses(T, "elements apart", f, *one, ld=7)
+    for i in (2, 3, 4):
+        refuses(T, "null tensor", f, *[None if i == k else v for k, v in enumerate(one)])
+    for t in (-0.5, float("inf"), float("nan")):
+        refuses(T, "temperature", f, *one, temperature=t)
+    refuses(T, "top_k", f, *one, top_k=-1)
+    for p in (0.0, 1.5, float("nan")):
+        refuses(T, "top_p", f, *one, top_p=p)
+    for q in (-0.1, 1.5, float("nan")):
+        refuses(T, "min_p", f, *one, min_p=q)
+    refuses(T, "aligned", f, 4, 8, At(A.ptr.value + 1), B, D, dtype="bf16")
+    refuses(T, "aligned", f, 4, 8, A, B, D, logp=At(F.ptr.value + 2), dtype="bf16")
+    refuses(T, "overlaps an input", f, 4, 8, A, B, At(A.ptr.value + 124))
+    refuses(T, "overlaps an input", f, 4, 8, A, B, D, logq=B)
+    refuses(T, "overlaps an input", f, 4, 8, A, B, D, settings=F, kept=At(F.ptr.value + 60))
+    refuses(T, "two outputs overlap", f, 4, 8, A, B, D, logp=At(D.ptr.value + 12))
+    assert T.lib().tdh_sample_tokens(None, None, 0, 4, 8, A.ptr, C.c_size_t(8), B.ptr, D.ptr, None, None, None) == -1
+    assert b"descriptor" in T.lib().tdh_last_error()

@@ -62,6 +62,15 @@ class PreferenceDesc(C.Structure):
     _fields_ = [("kind", C.c_int32), ("beta", C.c_float), ("smoothing", C.c_float)]
 
 
+class SampleDesc(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
+class MuonDesc(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("alpha", "mu", "lam", "scale")] + [("nesterov", C.c_int32), ("steps", C.c_int32)] + [
+        (n, C.c_float) for n in ("a", "b", "c", "eps")] + [("products", C.c_int32)]
+
+
 class LayerDesc(C.Structure):
     _fields_ = [("kind", C.c_int32), ("act", C.c_int32), ("conv", ConvDesc), ("pool", PoolDesc),
                 ("fc_in", C.c_int32), ("fc_out", C.c_int32), ("fc_bias", C.c_int32),
@@ -93,13 +102,14 @@ def lib():
         l.tdh_last_error.restype = C.c_char_p
         l.tdh_version.restype = C.c_char_p
         for n in ("tdh_net_in_size", "tdh_net_out_size", "tdh_net_layer_out_size",
-                  "tdh_net_param_size"):
+                  "tdh_net_param_size", "tdh_q8_row"):
             getattr(l, n).restype = C.c_size_t
         for n in ("tdh_net_param", "tdh_net_layer_out", "tdh_net_layer_dx", "tdh_net_layer_grad",
                   "tdh_net_layer_argmax"):
             getattr(l, n).restype = C.c_void_p
         l.tdh_opt_default.restype = None
         l.tdh_act_default_params.restype = None
+        l.tdh_muon_default.restype = None
         _lib = l
     return _lib
 
@@ -537,6 +547,32 @@ def layernorm_bwd(rows, length, x, gamma, stats, dy, dx, dgamma, dbeta, dtype="f
                                   int(accumulate)), "tdh_layernorm_bwd")
 
 
+def sample_tokens(rows, vocab, logits, u, token, logp=None, logq=None, kept=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  settings=None, dtype="f32", ld=None):
+    """token[r] drawn from logits[r] with u[r] in [0, 1); settings: a device buffer of SampleDesc, one a row, in the place of the
+    four numbers. logp is the token's log-probability under the logits as they are (policy_loss's old_logp), logq the one that it was
+    drawn with, kept how many tokens were left to draw from."""
+    p = SampleDesc(temperature, top_k, top_p, min_p)
+    check(lib().tdh_sample_tokens(C.byref(p), _p(settings), DTYPE[dtype], rows, vocab, _p(logits), C.c_size_t(ld or vocab), _p(u),
+                                  _p(token), _p(logp), _p(logq), _p(kept)), "tdh_sample_tokens")
+
+
+def q8_row(n_in):
+    """Bytes of an output's row of 8-bit weights"""
+    return lib().tdh_q8_row(n_in)
+
+
+def fc_q8_pack(n_in, n_out, w, wq, wscale, dtype="f32"):
+    """w [n_in][n_out] to 8-bit weights wq [n_out][q8_row(n_in)] (int8) and their scales (fp32)"""
+    check(lib().tdh_fc_q8_pack(DTYPE[dtype], n_in, n_out, _p(w), _p(wq), _p(wscale)), "tdh_fc_q8_pack")
+
+
+def fc_q8_fwd(n_in, n_out, has_bias, batch, x, wq, wscale, b, y, dtype="f32"):
+    """y = x w + b with x in 8 bits sample by sample and w in 8 bits output by output, sums in integers"""
+    check(lib().tdh_fc_q8_fwd(DTYPE[dtype], n_in, n_out, int(has_bias), batch, _p(x), _p(wq), _p(wscale), _p(b), _p(y)),
+          "tdh_fc_q8_fwd")
+
+
 def cast(n, src, dst, src_dtype, dst_dtype):
     check(lib().tdh_cast(DTYPE[dst_dtype], DTYPE[src_dtype], C.c_size_t(n), _p(src), _p(dst)), "tdh_cast")
 
@@ -544,6 +580,27 @@ def cast(n, src, dst, src_dtype, dst_dtype):
 def opt_update(o, n, merged_grad, w, s0=None, s1=None, grad_scale=1.0):
     check(lib().tdh_opt_update(C.byref(o), C.c_size_t(n), _p(merged_grad), C.c_float(grad_scale),
                                _p(w), _p(s0), _p(s1)), "tdh_opt_update")
+
+
+def muon_desc(products="f32", **kw):
+    """The update by the orthogonalised momentum: alpha, mu, lambda_, scale, nesterov, steps, a, b, c and eps; products f32 or f16."""
+    o = MuonDesc()
+    lib().tdh_muon_default(C.byref(o))
+    o.products = DTYPE[products]
+    for k, v in kw.items():
+        setattr(o, "lam" if k == "lambda_" else k, v)
+    return o
+
+
+def orthogonalize(o, rows, cols, x, y, dtype="f32"):
+    """y [rows][cols]: x with its singular values brought near one"""
+    check(lib().tdh_orthogonalize(C.byref(o), DTYPE[dtype], rows, cols, _p(x), _p(y)), "tdh_orthogonalize")
+
+
+def muon_update(o, rows, cols, merged_grad, w, momentum, grad_scale=1.0, dtype="f32"):
+    """w -= alpha * (scale * O + lambda * w), O the orthogonalised momentum; dtype: the gradient's (weights and momentum are fp32)"""
+    check(lib().tdh_muon_update(C.byref(o), DTYPE[dtype], rows, cols, _p(merged_grad), C.c_float(grad_scale), _p(w), _p(momentum)),
+          "tdh_muon_update")
 
 
 # ------------------------------------------------------------ sequential net

@@ -35,25 +35,6 @@ struct NormBwdArgs {
   int accumulate;
 };
 
-// The N elements of word k of a row of `len`: those behind its end read as `rest`.
-template <class T>
-__device__ __forceinline__ Word<T> row_word(const T *p, const int k, const int len, const float rest) {
-  constexpr int N = Word<T>::N;
-  if (k * N + N <= len) return load_word(p + k * N);
-  float v[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = k * N + e < len ? to_f32(p[k * N + e]) : rest;
-  return Word<T>::from(v);
-}
-template <class T>
-__device__ __forceinline__ void put_row_word(T *p, const int k, const int len, const float (&v)[Word<T>::N]) {
-  constexpr int N = Word<T>::N;
-  if (k * N + N <= len) return store_word(p + k * N, Word<T>::from(v).raw);
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (k * N + e < len) p[k * N + e] = from_f32<T>(v[e]);
-}
-
 // Sums over the LANES lanes that have a row (a power of two; more than a wave: LANES / 64 whole waves, through LDS). `turn` tells two
 // calls behind each other apart, which need no barrier between them then; every thread of the workgroup calls.
 template <int LANES, int K, int NT>
