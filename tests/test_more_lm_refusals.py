@@ -76,3 +76,30 @@ def test_sample_refusals(T):
     refuses(T, "two outputs overlap", f, 4, 8, A, B, D, logp=At(D.ptr.value + 12))
     assert T.lib().tdh_sample_tokens(None, None, 0, 4, 8, A.ptr, C.c_size_t(8), B.ptr, D.ptr, None, None, None) == -1
     assert b"descriptor" in T.lib().tdh_last_error()
+
+
+def test_muon_refusals(T):
+    d = T.muon_desc
+    refuses(T, "bad shape", T.orthogonalize, d(), -1, 8, A, B)
+    refuses(T, "beyond", T.orthogonalize, d(), 16385, 16385, A, B)
+    refuses(T, "beyond", T.orthogonalize, d(), 1, (1 << 20) + 1, A, B)
+    refuses(T, "beyond", T.orthogonalize, d(), 1 << 20, 1025, A, B)
+    refuses(T, "null tensor", T.orthogonalize, d(), 8, 8, None, B)
+    refuses(T, "null tensor", T.orthogonalize, d(), 8, 8, A, None)
+    refuses(T, "null tensor", T.muon_update, d(), 8, 8, A, B, None)
+    refuses(T, "aligned", T.orthogonalize, d(), 8, 8, At(A.ptr.value + 1), B, dtype="f16")
+    refuses(T, "aligned", T.muon_update, d(), 8, 8, A, At(B.ptr.value + 2), D, dtype="f16")
+    refuses(T, "overlaps an input", T.orthogonalize, d(), 8, 8, A, At(A.ptr.value + 4))
+    refuses(T, "overlaps an input", T.muon_update, d(), 8, 8, A, B, At(A.ptr.value + 252))
+    refuses(T, "two outputs overlap", T.muon_update, d(), 8, 8, A, B, At(B.ptr.value + 252))
+    refuses(T, "steps", T.orthogonalize, d(steps=33), 8, 8, A, B)
+    refuses(T, "steps", T.orthogonalize, d(steps=-1), 8, 8, A, B)
+    for eps in (0.0, float("nan"), float("inf"), 1e-42):
+        refuses(T, "eps", T.orthogonalize, d(eps=eps), 8, 8, A, B)
+    for k in (dict(a=5.0), dict(b=1.0), dict(c=float("nan")), dict(a=float("inf")), dict(a=3.0, b=0.5, c=0.0)):
+        refuses(T, "coefficients", T.orthogonalize, d(**k), 8, 8, A, B)
+    refuses(T, "products", T.orthogonalize, d(products="bf16"), 8, 8, A, B)
+    assert T.lib().tdh_orthogonalize(None, 0, 8, 8, A.ptr, B.ptr) == -1
+    o = d()
+    assert T.lib().tdh_muon_update(C.byref(o), 3, 8, 8, A.ptr, C.c_float(1.0), B.ptr, D.ptr) == -1
+    assert b"element type" in T.lib().tdh_last_error()

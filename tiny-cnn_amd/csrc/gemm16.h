@@ -163,6 +163,21 @@ __device__ __forceinline__ void g16_tile(int id, const int tiles_m, const int ti
   tn = id / rows;
 }
 
+// All tiles, or those on and below the diagonal of a symmetric product.
+struct G16AllTiles {
+  __host__ __device__ static int count(const int tiles_m, const int tiles_n) { return tiles_m * tiles_n; }
+  __device__ __forceinline__ static void place(const int id, const int tiles_m, const int tiles_n, int &tm, int &tn) { g16_tile(id, tiles_m, tiles_n, tm, tn); }
+};
+struct G16LowerTiles {
+  __host__ __device__ static int count(const int tiles_m, const int) { return tiles_m * (tiles_m + 1) / 2; }
+  __device__ __forceinline__ static void place(const int id, const int, const int, int &tm, int &tn) {
+    tm = static_cast<int>((sqrtf(8.0f * id + 1.0f) - 1.0f) * 0.5f);   // (up to rounding)
+    while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
+    while (tm * (tm + 1) / 2 > id) --tm;
+    tn = id - tm * (tm + 1) / 2;
+  }
+};
+
 // 32 rows of COLS fp32 values that a wave turns in LDS, so that a lane has eight neighbours of one row: put() takes
 // block j in the matrix cores' layout, rows() hands out (row, column of the first, values).
 template <int COLS>
@@ -197,7 +212,7 @@ struct G16Turn {
 // Epi: done(acc, m0, n0, lane, split, lds) with the wave's blocks: register r of lane l of block (i, j) is row
 // m0 + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 and column n0 + 32 j + l % 32 (PAIR: of the tile's column order); lds:
 // G16Turn<32 TN>::BYTES of the wave's own.
-template <class T, int WM, int WN, int TM, int TN, int BUFS, bool A_KC, bool B_KC, bool PAIR, class Epi>
+template <class T, int WM, int WN, int TM, int TN, int BUFS, bool A_KC, bool B_KC, bool PAIR, class Epi, class Tiles = G16AllTiles>
 __global__ void __launch_bounds__(64 * WM * WN)
 gemm16_kernel(const G16Matrix A, const G16Matrix B, const Epi epi, const int tiles_m, const int tiles_n, const int K,
               const int k_per_split) {
@@ -206,12 +221,12 @@ gemm16_kernel(const G16Matrix A, const G16Matrix B, const Epi epi, const int til
   using SideB = G16Side<BN, B_KC, PAIR, NT>;
   __shared__ __align__(1024) char lds[BUFS][SideA::BYTES + SideB::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-  const int tiles = tiles_m * tiles_n;
+  const int tiles = Tiles::count(tiles_m, tiles_n);
   int id = xcd_compact_id(blockIdx.x, gridDim.x);
   const int split = id / tiles;
   id -= split * tiles;
   int tm, tn;
-  g16_tile(id, tiles_m, tiles_n, tm, tn);
+  Tiles::place(id, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * (PAIR ? BN / 2 : BN);
   const int kbeg = split * k_per_split, kend = min(K, kbeg + k_per_split);
 
