@@ -103,3 +103,32 @@ def test_muon_refusals(T):
     o = d()
     assert T.lib().tdh_muon_update(C.byref(o), 3, 8, 8, A.ptr, C.c_float(1.0), B.ptr, D.ptr) == -1
     assert b"element type" in T.lib().tdh_last_error()
+
+
+def test_q8_refusals(T):
+    f, one = T.fc_q8_fwd, (64, 8, False, 4, A, B, F, None, D)
+    refuses(T, "bad shape", f, 0, *one[1:])
+    refuses(T, "bad shape", f, 64, 0, *one[2:])
+    refuses(T, "beyond", f, (1 << 17) + 1, *one[1:])
+    refuses(T, "beyond", f, 64, (1 << 20) + 1, *one[2:])
+    refuses(T, "samples", f, 64, 8, False, -1, *one[4:])
+    refuses(T, "samples", f, 64, 8, False, (1 << 24) + 1, *one[4:])
+    refuses(T, "2\\^31", f, 1 << 17, 1 << 14, *one[2:])
+    refuses(T, "2\\^31", f, 64, 1 << 10, False, 1 << 21, *one[4:])
+    for i in (4, 5, 6, 8):
+        refuses(T, "null tensor", f, *[None if i == k else v for k, v in enumerate(one)])
+    refuses(T, "has_bias", f, 64, 8, True, *one[3:])
+    refuses(T, "16-byte", f, 64, 8, False, 4, A, At(B.ptr.value + 8), F, None, D)
+    refuses(T, "aligned", f, 64, 8, False, 4, At(A.ptr.value + 1), B, F, None, D, dtype="bf16")
+    refuses(T, "aligned", f, 64, 8, False, 4, A, B, At(F.ptr.value + 2), None, D, dtype="bf16")
+    refuses(T, "overlaps an input", f, 64, 8, False, 4, A, B, F, None, At(A.ptr.value + 1020))
+    refuses(T, "overlaps an input", f, 64, 8, False, 4, A, B, F, None, At(B.ptr.value + 508))
+    p = T.fc_q8_pack
+    refuses(T, "bad shape", p, -3, 8, A, B, D)
+    refuses(T, "null tensor", p, 64, 8, A, None, D)
+    refuses(T, "16-byte", p, 64, 8, A, At(B.ptr.value + 4), D)
+    refuses(T, "overlaps an input", p, 64, 8, A, At(A.ptr.value + 64), D)
+    refuses(T, "two outputs overlap", p, 64, 8, A, B, At(B.ptr.value + 500))
+    assert T.q8_row(0) == 0 and T.q8_row(1) == 16 and T.q8_row(16) == 16 and T.q8_row(17) == 32
+    assert T.lib().tdh_fc_q8_fwd(7, 64, 8, 0, 4, A.ptr, B.ptr, F.ptr, None, D.ptr) == -1
+    assert b"element type" in T.lib().tdh_last_error()

@@ -844,12 +844,6 @@ int few_bwd(int act, int in, int hidden, int batch, const T *x, const T *w, cons
 }
 
 // ---- plans
-}  // namespace
-struct FfPlan {
-  int cfg;       // index into FF_TILES
-  int splits, k_per_split;
-};
-namespace {
 // A tile shape: the workgroups that a compute unit holds, us of a tile of 64 reduction indices with one, two, ... of them on a
 // compute unit (all of them take that long), us of a round of workgroups beside that, and of the launch. Measured on
 // products of 256 to 1024 tiles with k of 64 to 2048; 256 x 256 reaches 1100 TFLOP/s there, 128 x 128 990, 64 x 128 760,

@@ -24,6 +24,14 @@
 #include "lm_types.h"
 
 namespace tdh {
+
+// A product's tile shape, and its split along k
+struct FfPlan {
+  int cfg;       // 0 to 4: 256 x 256 by eight waves, 128 x 128, 64 x 128, 64 x 64 by two waves, 32 x 256; four waves where none are named
+  int splits, k_per_split;
+};
+FfPlan ff_plan(int M, int N, int K, bool pair);   // (gated_ff.hip)
+
 namespace {
 
 typedef __bf16 g16_bf16x8 __attribute__((ext_vector_type(8)));
@@ -40,6 +48,18 @@ __device__ __forceinline__ g16_f32x16 mfma16(bf16, const g16_s16x8 a, const g16_
 }
 __device__ __forceinline__ g16_f32x16 mfma16(f16, const g16_s16x8 a, const g16_s16x8 b, const g16_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(g16_f16x8, a), __builtin_bit_cast(g16_f16x8, b), c, 0, 0, 0);
+}
+
+// Eight-bit integers in pairs, which take the place of 16-bit elements everywhere but in the products; their sums are whole numbers, held in the
+// bits of the accumulators.
+struct i8x2 {
+  int8_t v[2];
+};
+typedef int g16_i32x4 __attribute__((ext_vector_type(4)));
+typedef int g16_i32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ g16_f32x16 mfma16(i8x2, const g16_s16x8 a, const g16_s16x8 b, const g16_f32x16 c) {
+  return __builtin_bit_cast(g16_f32x16, __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(g16_i32x4, a), __builtin_bit_cast(g16_i32x4, b),
+                                                                             __builtin_bit_cast(g16_i32x16, c), 0, 0, 0));
 }
 
 // waits until all but the last LEFT of the wave's loads into LDS have arrived
