@@ -31,23 +31,32 @@ struct SampleArgs {
   float *logp, *logq;
 };
 
-// 2^t for t <= 0, to 4e-14 of the value: the fit is of (2^f - 1) / f for |f| <= 1/2 (Chebyshev nodes), so that 2^0 is 1
-__device__ __forceinline__ double exp2_64(double t) {
-  t = __builtin_fmax(t, -1000.0);   // (and where t is 0 times an infinity: nothing)
-  const double n = __builtin_rint(t), f = t - n;
-  double p = 1.0203121063391729e-07;
-  p = __builtin_fma(p, f, 1.3255224878668817e-06);
-  p = __builtin_fma(p, f, 1.525268684626772e-05);
-  p = __builtin_fma(p, f, 0.00015403455852453838);
-  p = __builtin_fma(p, f, 0.0013333558179043112);
-  p = __builtin_fma(p, f, 0.009618129159402558);
-  p = __builtin_fma(p, f, 0.055504108664760424);
-  p = __builtin_fma(p, f, 0.2402265069581299);
-  p = __builtin_fma(p, f, 0.6931471805599453);
+// 2^t for -1000 <= t < 1000, to 2e-12 of the value: the fit is of (2^f - 1) / f for |f| <= 1/2 (Chebyshev nodes), so that 2^0 is 1. Adding 1.5 * 2^52 leaves
+// t to the nearest whole number in the low bits, which go to the exponent as they are.
+__device__ __forceinline__ double exp2_64(const double t) {
+  constexpr double MAGIC = 6755399441055744.0;
+  const double big = t + MAGIC, f = t - (big - MAGIC);
+  double p = 1.325080551750225e-06;
+  p = __builtin_fma(p, f, 1.5303700711365693e-05);
+  p = __builtin_fma(p, f, 0.00015403475186530786);
+  p = __builtin_fma(p, f, 0.0013333478473685416);
+  p = __builtin_fma(p, f, 0.00961812913523614);
+  p = __builtin_fma(p, f, 0.055504109063258665);
+  p = __builtin_fma(p, f, 0.24022650695888503);
+  p = __builtin_fma(p, f, 0.6931471805568324);
   p = __builtin_fma(p, f, 1.0);
-  return __builtin_ldexp(p, static_cast<int>(n));
+  const u64 b = __builtin_bit_cast(u64, p);
+  const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(u64, big));
+  return __builtin_bit_cast(double, (b & 0xffffffffu) | static_cast<u64>(static_cast<uint32_t>(b >> 32) + (n << 20)) << 32);
 }
 constexpr double LOG2E_64 = 1.4426950408889634;
+
+// exp(d) in fp32, d <= 0: the product with log2(e) with its rounding
+__device__ __forceinline__ float exp_32(float d) {
+  d = fmaxf(d, -200.0f);
+  const float t = d * 1.44269504f, r = __builtin_fmaf(d, 1.44269504f, -t) + d * 1.925963033e-8f, e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, 0.69314718f * r, e);
+}
 
 // logits in an order of whole numbers, -0 as 0
 __device__ __forceinline__ uint32_t key_of(const float v) {
@@ -71,15 +80,243 @@ __device__ __forceinline__ V wave_scan(V v) {   // with this lane's own
   }
   return v;
 }
+__device__ __forceinline__ float wave_top(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ void no_token(const SampleArgs &a, const int row) {
+  a.token[row] = -1;
+  if (a.kept) a.kept[row] = 0;
+  if (a.logp) a.logp[row] = __builtin_nanf("");
+  if (a.logq) a.logq[row] = __builtin_nanf("");
+}
 
+// The words of a row, each wave's behind each other: word(i) of this thread, i < per, and a wave's share of the row's words.
+template <class T, int NT, bool HELD>
+struct RowWords {
+  static constexpr int N = Word<T>::N;
+  const T *x;
+  uint4 *held;   // (HELD) in LDS, where load() put them
+  int vocab, words, per, first;
+  __device__ __forceinline__ RowWords(const SampleArgs &a, uint4 *lds) : held(lds) {
+    x     = static_cast<const T *>(a.logits) + static_cast<size_t>(blockIdx.x) * a.ld;
+    vocab = a.vocab;
+    words = (vocab + N - 1) / N;
+    per   = (words + NT - 1) / NT;
+    first = (static_cast<int>(threadIdx.x) >> 6) * per * 64 + (threadIdx.x & 63);
+  }
+  __device__ __forceinline__ Word<T> load(const int k) const { return row_word(x, k, vocab, -INFINITY); }
+  __device__ __forceinline__ Word<T> at(const int k) const { return HELD ? Word<T>{held[k]} : load(k); }
+  // f(word) of every word that this thread has, the next two on their way meanwhile
+  template <class F>
+  __device__ __forceinline__ void each_word(const F &f) const {
+    const int mine = min(per, (words - first + 63) >> 6);
+    if (mine <= 0) return;
+    const int last = first + 64 * (mine - 1);
+    Word<T> now = at(first), next = at(min(first + 64, last));
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const Word<T> then = at(min(first + 64 * (i + 2), last));
+      f(now, i);
+      now  = next;
+      next = then;
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(const F &f) const {
+    each_word([&](const Word<T> &w, int) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(w[e]);
+    });
+  }
+};
+
+// (a single maximum: the logarithm of 1 + rest has rest's precision)
+__device__ __forceinline__ double log_of_sum(const double tops, const double rest) { return tops == 1.0 ? log1p(rest) : log(tops + rest); }
+
+// --------------------------------------------------------------- without filters
+// Long rows without top-k, top-p and min-p. The weights are taken by a reference near the maximum, the largest logit among every thread's first
+// words, so that one pass over the row gives the sums of its waves. A second pass has the maximum itself for its reference: where the first one was
+// too far below it for whole numbers of 62 bits, or where what is left beside the likeliest token has lost its figures beside that one's weight.
+// That wave's words, read once more, give the token.
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, 2)
+sample_all_kernel(const SampleArgs a) {
+  constexpr int WAVES = NT / 64, N = Word<T>::N;
+  __shared__ float tops[WAVES];
+  __shared__ int bads[WAVES], counts[WAVES], top_counts[WAVES];
+  __shared__ double sums[WAVES], raws[WAVES];
+  __shared__ u64 wholes[WAVES], wholes2[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, vocab = a.vocab;
+  const RowWords<T, NT, false> words(a, nullptr);
+  const double temperature = a.p.temperature, rate = LOG2E_64 / temperature, unit = __builtin_ldexp(1.0, min(a.fix, 45));
+  const bool with_raw = a.logp && temperature != 1.0;
+
+  float ref = -INFINITY;
+  if (words.first < words.words) {
+    const Word<T> w = words.load(words.first);
+#pragma unroll
+    for (int e = 0; e < N; ++e) ref = fmaxf(ref, w[e]);
+  }
+  ref = wave_top(ref);
+  if (lane == 0) tops[wave] = ref;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) ref = fmaxf(ref, tops[w]);
+  ref = fabsf(ref) <= FLT_MAX ? ref : 0.0f;
+
+  auto weight = [&](float v) { return exp2_64(__builtin_fmax((static_cast<double>(v) - static_cast<double>(ref)) * rate, -1000.0)); };
+  constexpr double SHIFT = 4503599627370496.0;   // 2^52: the sum's low bits are the rounded product
+  constexpr u64 SHIFT_BITS = 0x4330000000000000ull;
+  // (weights of 2^6 and more of the reference's: to 2^6 of the unit)
+  auto whole = [&](double w) {
+    return w < 64.0 ? __builtin_bit_cast(u64, __builtin_fma(w, unit, SHIFT)) - SHIFT_BITS
+                    : (__builtin_bit_cast(u64, __builtin_fma(w, unit * 0x1p-10, SHIFT)) - SHIFT_BITS) << 10;
+  };
+  float top = -INFINITY;
+  double sum = 0.0, raw = 0.0;   // (second pass: of what is below the maximum)
+  int kept = 0, top_n = 0;
+  bool second = false;
+#pragma unroll 1
+  for (;;) {
+    u64 s = 0;
+    double f = 0.0, q = 0.0;
+    int n = 0, tn = 0;
+    bool bad = false;
+    float t = -INFINITY;
+    const float large = ref + static_cast<float>(4.0 * temperature);   // (e^4 of the reference's weight)
+    words.each_word([&](const Word<T> &w, int) {
+      float m = w[0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) m = fmaxf(m, w[e]);
+      t = fmaxf(t, m);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        bad = bad || !(w[e] < INFINITY);
+        n += __builtin_popcountll(__ballot(w[e] > -INFINITY));
+      }
+      if (__builtin_expect(second || m > large, 0)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v  = w[e];
+          const double x = weight(v);
+          s += whole(x);
+          f += second && v == ref ? 0.0 : x;
+          tn += v == ref;
+          if (with_raw) q += second && v == ref ? 0.0 : static_cast<double>(exp_32(v - ref));
+        }
+      } else {
+        u64 c = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const double x = weight(w[e]);
+          c += __builtin_bit_cast(u64, __builtin_fma(x, unit, SHIFT));
+          f += x;
+        }
+        s += c - N * SHIFT_BITS;
+        if (with_raw)
+#pragma unroll
+          for (int e = 0; e < N; ++e) q += static_cast<double>(exp_32(w[e] - ref));
+      }
+    });
+    t  = wave_top(t);
+    s  = wave_total(s);
+    f  = wave_total(f);
+    tn = wave_total(tn);
+    n  = __shfl(n, 0);   // (the first lane has a word wherever another one has)
+    if (with_raw) q = wave_total(q);
+    const int any_bad = __any(bad);
+    __syncthreads();   // (what was there before has been read)
+    if (lane == 0) {
+      tops[wave] = t;
+      bads[wave] = any_bad;
+      counts[wave] = n;
+      top_counts[wave] = tn;
+      wholes[wave] = s;
+      sums[wave] = f;
+      raws[wave] = q;
+    }
+    __syncthreads();
+    sum = raw = 0.0;
+    kept = top_n = 0;
+    int all_bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      top = fmaxf(top, tops[w]);
+      all_bad |= bads[w];
+      kept += counts[w];
+      top_n += top_counts[w];
+      sum += sums[w];
+      raw += raws[w];
+    }
+    if (all_bad || top == -INFINITY) {   // (the whole workgroup)
+      if (tid == 0) no_token(a, row);
+      return;
+    }
+    if (second) break;
+    // whole numbers that add up to less than 2^62; the likeliest's share below 1 - 10^-4, of fp32's exponentials 0.9
+    const double beyond = (static_cast<double>(top) - static_cast<double>(ref)) * rate;
+    if (beyond < 60.0 && sum * unit < 0x1p61 && sum > 1.0001 * weight(top) &&
+        (!with_raw || (top - ref < 80.0f && raw > 1.1 * static_cast<double>(exp_32(top - ref)))))
+      break;
+    ref    = top;
+    second = true;
+  }
+  u64 all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) all += wholes[w];
+  const double u = a.u[row];
+  u64 r = static_cast<u64>((u > 0.0 ? fmin(u, 1.0) : 0.0) * static_cast<double>(all));
+  r = min(r, all - 1);
+  u64 before = 0;
+  int where = 0;
+#pragma unroll 1
+  for (; where < WAVES - 1 && before + wholes[where] <= r; ++where) before += wholes[where];
+  const int span = words.per * 64, share = (span + NT - 1) / NT, beg = where * span + tid * share;
+  const int end = min(min(beg + share, (where + 1) * span), words.words);
+  u64 mine = 0;
+  for (int k = beg; k < end; ++k) {
+    const Word<T> w = words.load(k);
+#pragma unroll
+    for (int e = 0; e < N; ++e) mine += whole(weight(w[e]));
+  }
+  const u64 scan = wave_scan(mine);
+  if (lane == 63) wholes2[wave] = scan;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+    if (w < wave) before += wholes2[w];
+  before += scan - mine;
+  if (before > r || before + mine <= r) return;
+  // one thread is left
+  int token = -1;
+  float chosen = 0.0f;
+  for (int i = beg * N; i < min(end * N, vocab) && token < 0; ++i) {
+    chosen = to_f32(words.x[i]);
+    before += whole(weight(chosen));
+    if (before > r) token = i;
+  }
+  a.token[row] = token;
+  if (a.kept) a.kept[row] = kept;
+  const double d = static_cast<double>(chosen) - static_cast<double>(ref);
+  const double lq = d / temperature - (second ? log_of_sum(top_n, sum) : log(sum));
+  if (a.logq) a.logq[row] = static_cast<float>(lq);
+  if (a.logp) a.logp[row] = static_cast<float>(!with_raw ? lq : d - (second ? log_of_sum(top_n, raw) : log(raw)));
+}
+
+// ------------------------------------------------------------------ with filters
+constexpr int SAMPLE_LIST = 2048, SAMPLE_SHORT = 128;   // logits that a list takes, and that one wave goes through by itself
 // LDS of a row's workgroup
 template <int NT>
 struct SampleShared {
   static constexpr int WAVES = NT / 64, BINS = 2 * NT;
   u64 hist[BINS];   // (counts: the first half of it)
+  float list[SAMPLE_LIST];
   u64 sum[WAVES];
-  u64 found_above;
-  int found_bin;
+  u64 found_above, found_upto, found_ties;
+  float found_v;
+  int found_bin, listed;
   float top[WAVES], far[WAVES];
   int bad[WAVES], n[WAVES];
   // what is left, wave by wave: weight and number above V, number with V; weights below the maximum in floating point, number of maxima
@@ -88,44 +325,15 @@ struct SampleShared {
   double rest[WAVES], raw[WAVES];
 };
 
-// W words a thread, each wave's behind each other (W = 0: any number, read in every pass)
-template <class T, int NT, int W>
+template <class T, int NT, bool HELD>
 __global__ void __launch_bounds__(NT)
 sample_kernel(const SampleArgs a) {
   using Shared = SampleShared<NT>;
   constexpr int WAVES = Shared::WAVES, BINS = Shared::BINS, N = Word<T>::N;
+  extern __shared__ uint4 row_lds[];
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, vocab = a.vocab;
-  const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
-  const int words = (vocab + N - 1) / N, per = (words + NT - 1) / NT;   // words a thread
-  const int first_word = wave * per * 64 + lane;
-  auto load = [&](int k) { return row_word(x, k, vocab, -INFINITY); };
-  Word<T> held[W ? W : 1];
-  if constexpr (W > 0) {
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      if (i < per && first_word + 64 * i < words) held[i] = load(first_word + 64 * i);
-  }
-  // f(logit) of every logit that this thread has
-  auto each = [&](auto f) {
-    if constexpr (W > 0) {
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        // (a word at a time: left alone the compiler keeps what it unpacks from one pass to the next, and spills)
-        asm volatile("" : "+v"(held[i].raw.x), "+v"(held[i].raw.y), "+v"(held[i].raw.z), "+v"(held[i].raw.w));
-        if (i < per && first_word + 64 * i < words)
-#pragma unroll
-          for (int e = 0; e < N; ++e) f(held[i][e]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-      for (int i = 0; i < per && first_word + 64 * i < words; ++i) {
-        const Word<T> w = load(first_word + 64 * i);
-#pragma unroll
-        for (int e = 0; e < N; ++e) f(w[e]);
-      }
-    }
-  };
+  const RowWords<T, NT, HELD> words(a, row_lds);
 
   // the row's settings
   const tdh_sample_desc p = a.settings ? a.settings[row] : a.p;
@@ -134,29 +342,35 @@ sample_kernel(const SampleArgs a) {
   const int top_k = greedy ? 1 : p.top_k;
   const bool with_k = top_k > 0 && top_k < vocab, with_p = !greedy && p.top_p < 1.0f, with_q = !greedy && p.min_p > 0.0f;
 
-  // maximum, and how far the others lie from it on average
+  // maximum, and how far others lie from it on average: those of every thread's first word will do
   float top = -INFINITY, far = 0.0f;
-  int bad = 0, n = 0;
-  each([&](float v) {
-    top = fmaxf(top, v);
-    bad |= !(v < INFINITY);
-  });
-  if (with_k || with_p)
-    each([&](float v) {
-      far += v > -INFINITY ? v : 0.0f;
-      n += v > -INFINITY;
-    });
+  int n = 0;
+  bool strange = false;
+  RowWords<T, NT, false>(a, nullptr).each_word([&](const Word<T> &w, int i) {
+    if (HELD) row_lds[words.first + 64 * i] = w.raw;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int e = 0; e < N; ++e) {
+      top     = fmaxf(top, w[e]);
+      strange = strange || !(w[e] < INFINITY);
+    }
+    if (i == 0)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        far += w[e] > -INFINITY ? w[e] : 0.0f;
+        n += w[e] > -INFINITY;
+      }
+  });
+  top = wave_top(top);
   far = wave_total(far);
   n   = wave_total(n);
-  bad = __any(bad);
+  int bad = __any(strange);
   if (lane == 0) {
     sh.top[wave] = top;
     sh.far[wave] = far;
     sh.bad[wave] = bad;
     sh.n[wave]   = n;
   }
+  if (tid == 0) sh.listed = 0;
   __syncthreads();
   far = 0.0f;
   n = bad = 0;
@@ -168,71 +382,131 @@ sample_kernel(const SampleArgs a) {
     bad |= sh.bad[w];
   }
   if (bad || top == -INFINITY) {   // (the whole workgroup)
-    if (tid == 0) {
-      a.token[row] = -1;
-      if (a.kept) a.kept[row] = 0;
-      if (a.logp) a.logp[row] = __builtin_nanf("");
-      if (a.logq) a.logq[row] = __builtin_nanf("");
-    }
+    if (tid == 0) no_token(a, row);
     return;
   }
   const double top64 = top, unit = __builtin_ldexp(1.0, a.fix);
-  auto weight = [&](float v) { return exp2_64((static_cast<double>(v) - top64) * rate); };
+  // (of 2^-1000 nothing is left, nor where t is 0 times an infinity)
+  auto weight = [&](float v) { return exp2_64(__builtin_fmax((static_cast<double>(v) - top64) * rate, -1000.0)); };
   constexpr double SHIFT = 4503599627370496.0;   // 2^52: the sum's low bits are the rounded product
   auto whole = [&](double w) { return __builtin_bit_cast(u64, __builtin_fma(w, unit, SHIFT)) - __builtin_bit_cast(u64, SHIFT); };
 
   // What is left: logits above V, and the first `ties` of those that are V
   float V  = -INFINITY;
   u64 ties = 0;
+  bool in_list = false;   // all that is left is in the list
+
+  const float mean = n ? top - far / static_cast<float>(n) : 16.0f, scale = mean > 0.0f ? BINS / (4.0f * mean) : 0.0f;
+  // the first round's ranges: equal ones of the distance from the maximum, the last for what is beyond four times the average
+  auto bin_of = [&](float v) { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); };
 
   // The logit at which the sum over what is left, from the largest logit on, reaches a target: top_k (counts) or the share top_p of
-  // all (weights). V becomes that logit and ties what is missing there.
+  // all (weights). V becomes that logit and ties what is missing there. The first round is over the row, those behind it over the logits that the first
+  // one leaves in question, in the list if they fit.
   auto select = [&](auto zero) {
     using M = decltype(zero);
     constexpr bool MASS = sizeof(M) == 8;
     M *hist = reinterpret_cast<M *>(sh.hist);
-    const float mean = top - far / static_cast<float>(n), scale = mean > 0.0f ? BINS / (4.0f * mean) : 0.0f;
-    // the first round's ranges: equal ones of the distance from the maximum, the last for what is beyond four times the average
-    auto bin_of = [&](float v) { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); };
     const u64 v_weight = MASS ? whole(weight(V)) : 0;
     u64 above = 0, target = MASS ? 0 : static_cast<u64>(top_k);
     int bin = 0, shift = 0;
     uint32_t lo = 0, hi = 0;
+    bool listed = in_list;
+    // A short list in one wave: each lane has a logit, and what the larger ones come to. `whole_sum`: the list has all that is left.
+    auto in_short_list = [&](const bool whole_sum) {
+      __syncthreads();
+      if (wave == 0) {
+        const int m = sh.listed;
+        float v_new = V;
+        u64 here = 0;
+        bool done = false;
+        for (int i0 = 0; !done && (i0 == 0 || i0 < m); i0 += 64) {
+          const bool in = i0 + lane < m && sh.list[i0 + lane] > V;
+          const float v = in ? sh.list[i0 + lane] : 0.0f;
+          u64 larger = above, equal = 0, total = above;
+          for (int j = 0; j < m; ++j) {
+            const float o = sh.list[j];
+            const u64 w = !(o > V) ? 0 : MASS ? sh.hist[j] : 1;
+            total += w;
+            larger += o > v ? w : 0;
+            equal += o == v ? w : 0;
+          }
+          if (MASS && whole_sum) {
+            const u64 all = total + ties * v_weight;
+            target = max(1ull, min(all, static_cast<u64>(__builtin_ceil(static_cast<double>(p.top_p) * static_cast<double>(all)))));
+          }
+          const u64 hit = __ballot(in && larger < target && larger + equal >= target);
+          if (hit) {
+            const int from = __builtin_ctzll(hit);
+            v_new = __shfl(v, from);
+            here  = target - __shfl(larger, from);
+            if (MASS) {
+              const u64 w = whole(weight(v_new));
+              here = (here + w - 1) / w;
+            }
+            done = true;
+          } else if (MASS && total < target && total + ties * v_weight >= target) {   // among those that are V already
+            here = min(ties, (target - total + v_weight - 1) / max(1ull, v_weight));
+            done = true;
+          }
+        }
+        if (lane == 0) {
+          sh.found_v    = v_new;
+          sh.found_ties = here;
+        }
+      }
+      __syncthreads();
+      V    = sh.found_v;
+      ties = sh.found_ties;
+    };
+    auto weigh_list = [&] {
+      if (MASS) {
+        __syncthreads();
+        for (int i = tid; i < sh.listed; i += NT) sh.hist[i] = whole(weight(sh.list[i]));
+      }
+    };
+    if (listed && sh.listed <= SAMPLE_SHORT) {   // (what top-k left; more than one of them)
+      weigh_list();
+      return in_short_list(true);
+    }
     for (int round = 0; round < 6; ++round) {   // (32 bits of logits, 7 or more a round behind the first)
       __syncthreads();   // (the histogram of before has been read)
       hist[tid] = hist[tid + NT] = 0;
       __syncthreads();
       M last = 0;   // (the first round's last range has the most, and one sum a lane)
-      auto add = [&](float v, M what) {
+      auto add = [&](float v, auto what) {
         if (round == 0) {
           const int b = bin_of(v);
           if (b == BINS - 1)
-            last += what;
+            last += what();
           else
-            atomicAdd(&hist[b], what);
+            atomicAdd(&hist[b], what());
         } else {
           const uint32_t k = key_of(v);
-          if (k >= lo && k <= hi && bin_of(v) == bin) atomicAdd(&hist[(hi - k) >> shift], what);
+          if (k >= lo && k <= hi && bin_of(v) == bin) atomicAdd(&hist[(hi - k) >> shift], what());
         }
       };
-      if constexpr (MASS) {
-        const float from = round ? of_key(lo) : V;
-        each([&](float v) {
-          if (v > V && v >= from) add(v, whole(weight(v)));
-        });
-        if (ties && tid == 0) add(V, ties * v_weight);
+      auto one = [&](float v) {
+        if constexpr (MASS) {
+          if (v > V) add(v, [&] { return whole(weight(v)); });
+        } else {
+          if (v > -INFINITY) add(v, [] { return 1u; });
+        }
+      };
+      if (listed) {
+        const int m = sh.listed;
+        for (int i = tid; i < m; i += NT) one(sh.list[i]);
       } else {
-        each([&](float v) {
-          if (v > -INFINITY) add(v, 1);
-        });
+        words.each(one);
       }
+      if (MASS && ties && tid == 0) add(V, [&] { return ties * v_weight; });
       if (round == 0) {
         last = wave_total(last);
         if (lane == 0 && last) atomicAdd(&hist[BINS - 1], last);
       }
       __syncthreads();
-      const u64 one = hist[2 * tid], two = hist[2 * tid + 1];
-      u64 upto = wave_scan(one + two);
+      const u64 first = hist[2 * tid], second = hist[2 * tid + 1];
+      u64 upto = wave_scan(first + second);
       if (lane == 63) sh.sum[wave] = upto;
       __syncthreads();
       u64 total = 0;
@@ -246,10 +520,11 @@ sample_kernel(const SampleArgs a) {
         if (total < target) return;   // fewer than top_k (the whole workgroup)
       }
       const u64 want = target - above;
-      if (upto >= want && upto - one - two < want) {
-        const bool second = upto - two < want;
-        sh.found_bin   = 2 * tid + second;
-        sh.found_above = above + upto - two - (second ? 0 : one);
+      if (upto >= want && upto - first - second < want) {
+        const bool later = upto - second < want;
+        sh.found_bin   = 2 * tid + later;
+        sh.found_above = above + upto - second - (later ? 0 : first);
+        sh.found_upto  = above + upto - (later ? 0 : second);
       }
       __syncthreads();
       above = sh.found_above;
@@ -261,6 +536,26 @@ sample_kernel(const SampleArgs a) {
         hi = scale > 0.0f ? key_of(static_cast<float>(x1 + 1e-6 * __builtin_fabs(x1) + 1e-37)) : key_of(top);
         lo = scale > 0.0f && b < BINS - 1 ? key_of(__builtin_fmaxf(static_cast<float>(x0 - 1e-6 * __builtin_fabs(x0) - 1e-37), -FLT_MAX)) : key_of(-FLT_MAX);
         hi = min(hi, key_of(top));
+        // Of top-k all from the maximum on, which is what top-p looks at next; of weights that range alone.
+        if (!listed && (MASS || sh.found_upto <= SAMPLE_LIST)) {
+          words.each([&](float v) {
+            const bool in = v > -INFINITY && (MASS ? v > V && bin_of(v) == bin : bin_of(v) <= bin);
+            const u64 lanes = __ballot(in);
+            if (!lanes) return;
+            int at = 0;
+            if (lane == __builtin_ctzll(lanes)) at = atomicAdd(&sh.listed, __builtin_popcountll(lanes));
+            at = __shfl(at, __builtin_ctzll(lanes)) + __builtin_popcountll(lanes & ((1ull << lane) - 1));
+            if (in && at < SAMPLE_LIST) sh.list[at] = v;
+          });
+          __syncthreads();
+          listed = sh.listed <= SAMPLE_LIST;
+          if (!MASS) in_list = true;
+          if (sh.listed <= SAMPLE_SHORT) {
+            if (!MASS) above = 0;
+            weigh_list();
+            return in_short_list(false);
+          }
+        }
       } else {
         hi -= static_cast<uint32_t>(b) << shift;
         if (shift == 0) break;
@@ -298,7 +593,8 @@ sample_kernel(const SampleArgs a) {
     u64 gt = 0;
     int gt_n = 0, at = 0, tops = 0;
     double rest = 0.0, raw = 0.0;
-    each([&](float v) {
+    const bool same = !(with_k || with_p || with_q) && temperature == 1.0, with_raw = a.logp && !same;
+    words.each([&](float v) {
       if (v > V) {
         const double w = weight(v);
         gt += whole(w);
@@ -307,29 +603,21 @@ sample_kernel(const SampleArgs a) {
       }
       at += v == V;
       tops += v == top;
+      if (with_raw) raw += v < top && v > -INFINITY ? static_cast<double>(exp_32(v - top)) : 0.0;
     });
-    const bool same = a.logp && !(with_k || with_p || with_q) && temperature == 1.0;
-    if (a.logp && !same) {
-      // exp(v - top) in fp32, the product with log2(e) with its rounding
-      each([&](float v) {
-        const float d = fmaxf(v - top, -200.0f), t = d * 1.44269504f, r = __builtin_fmaf(d, 1.44269504f, -t) + d * 1.925963033e-8f;
-        const float e = __builtin_amdgcn_exp2f(t);
-        raw += v < top && v > -INFINITY ? static_cast<double>(__builtin_fmaf(e, 0.69314718f * r, e)) : 0.0;
-      });
-    }
     gt   = wave_total(gt);
     gt_n = wave_total(gt_n);
     at   = wave_total(at);
     tops = wave_total(tops);
     rest = wave_total(rest);
-    raw  = wave_total(same ? rest : raw);
+    raw  = same ? rest : wave_total(raw);
     if (lane == 0) {
       sh.gt[wave]   = gt;
       sh.gt_n[wave] = gt_n;
       sh.ties[wave] = at;
       sh.tops[wave] = tops;
       sh.rest[wave] = rest;
-      sh.raw[wave]  = same ? rest : raw;
+      sh.raw[wave]  = raw;
     }
   }
   __syncthreads();
@@ -355,11 +643,12 @@ sample_kernel(const SampleArgs a) {
     t0 = t1;
   }
   // that wave's words, a share for every thread
-  const int share = (per * 64 + NT - 1) / NT, beg = where * per * 64 + tid * share, end = min(min(beg + share, (where + 1) * per * 64), words);
+  const int span = words.per * 64, share = (span + NT - 1) / NT, beg = where * span + tid * share;
+  const int end = min(min(beg + share, (where + 1) * span), words.words);
   u64 gt = 0;
   int at = 0;
   for (int k = beg; k < end; ++k) {
-    const Word<T> w = load(k);
+    const Word<T> w = words.at(k);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       if (w[e] > V) gt += whole(weight(w[e]));
@@ -385,16 +674,13 @@ sample_kernel(const SampleArgs a) {
   // one thread is left
   int token = -1;
   float chosen = V;
-  for (int k = beg; k < end && token < 0; ++k) {
-#pragma unroll 1
-    for (int e = 0; e < N && token < 0; ++e) {
-      const float v = to_f32(x[min(k * N + e, vocab - 1)]);
-      if (k * N + e >= vocab || v < V) continue;
-      if (v > V) g0 += whole(weight(v)); else ++t0;
-      if (upto(g0, t0) > r) {
-        token  = k * N + e;
-        chosen = v;
-      }
+  for (int i = beg * N; i < min(end * N, vocab) && token < 0; ++i) {
+    const float v = to_f32(words.x[i]);
+    if (v < V) continue;
+    if (v > V) g0 += whole(weight(v)); else ++t0;
+    if (upto(g0, t0) > r) {
+      token  = i;
+      chosen = v;
     }
   }
   a.token[row] = token;
@@ -410,28 +696,29 @@ sample_kernel(const SampleArgs a) {
   }
   if (a.kept) a.kept[row] = static_cast<int>(gt_count + ties_left);
   const double d = static_cast<double>(chosen) - top64;
-  // (a single maximum: the logarithm of 1 + rest has rest's precision)
-  auto log_of = [](double tops, double rest) { return tops == 1.0 ? log1p(rest) : log(tops + rest); };
   if (a.logq) a.logq[row] = static_cast<float>(V == top ? -log(static_cast<double>(ties_left))
-                                                        : d / temperature - log_of(tops, rest + v_weight64 * static_cast<double>(ties_left)));
-  if (a.logp) a.logp[row] = static_cast<float>(d - log_of(tops, raw));
+                                                        : d / temperature - log_of_sum(tops, rest + v_weight64 * static_cast<double>(ties_left)));
+  if (a.logp) a.logp[row] = static_cast<float>(d - log_of_sum(tops, raw));
 }
 
+constexpr size_t SAMPLE_HELD = 128 << 10;   // bytes of a row that stay in LDS
 template <class T>
 int launch_sample(const SampleArgs &a, int rows) {
   const int words = static_cast<int>((static_cast<long>(a.vocab) + Word<T>::N - 1) / Word<T>::N);
-  auto go = [&](auto kernel, int nt) {
-    TDH_LAUNCH(kernel, dim3(rows), dim3(nt), 0, ctx().stream, a);
+  const size_t bytes = 16 * static_cast<size_t>(words);
+  auto go = [&](auto kernel, int nt, size_t lds) {
+    if (lds > (32 << 10))
+      TDH_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SAMPLE_HELD)));
+    TDH_LAUNCH(kernel, dim3(rows), dim3(nt), lds, ctx().stream, a);
     TDH_LAUNCH_CHECK();
     return static_cast<int>(TDH_OK);
   };
-  if (words <= 64) return go(sample_kernel<T, 64, 1>, 64);
-  if (words <= 512) return go(sample_kernel<T, 256, 2>, 256);
-  if (words <= 1024) return go(sample_kernel<T, 1024, 1>, 1024);
-  if (words <= 4096) return go(sample_kernel<T, 1024, 4>, 1024);
-  if (words <= 8192) return go(sample_kernel<T, 1024, 8>, 1024);
-  if (words <= 16384) return go(sample_kernel<T, 1024, 16>, 1024);
-  return go(sample_kernel<T, 1024, 0>, 1024);
+  if (words <= 128) return go(sample_kernel<T, 64, true>, 64, bytes);
+  if (words <= 1024) return go(sample_kernel<T, 256, true>, 256, bytes);
+  const bool filters = a.settings || !(a.p.temperature > 0.0f) || (a.p.top_k > 0 && a.p.top_k < a.vocab) || a.p.top_p < 1.0f || a.p.min_p > 0.0f;
+  if (!filters) return rows > 2 * ctx().compute_units ? go(sample_all_kernel<T, 512>, 512, 0) : go(sample_all_kernel<T, 1024>, 1024, 0);
+  if (bytes <= SAMPLE_HELD) return go(sample_kernel<T, 1024, true>, 1024, bytes);
+  return go(sample_kernel<T, 1024, false>, 1024, 0);
 }
 
 }  // namespace
