@@ -45,9 +45,10 @@ __device__ __forceinline__ double exp2_64(const double t) {
   p = __builtin_fma(p, f, 0.24022650695888503);
   p = __builtin_fma(p, f, 0.6931471805568324);
   p = __builtin_fma(p, f, 1.0);
-  const u64 b = __builtin_bit_cast(u64, p);
-  const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(u64, big));
-  return __builtin_bit_cast(double, (b & 0xffffffffu) | static_cast<u64>(static_cast<uint32_t>(b >> 32) + (n << 20)) << 32);
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 b = __builtin_bit_cast(u32x2, p);
+  b.y += __builtin_bit_cast(u32x2, big).x << 20;
+  return __builtin_bit_cast(double, b);
 }
 constexpr double LOG2E_64 = 1.4426950408889634;
 
@@ -108,16 +109,21 @@ struct RowWords {
   }
   __device__ __forceinline__ Word<T> load(const int k) const { return row_word(x, k, vocab, -INFINITY); }
   __device__ __forceinline__ Word<T> at(const int k) const { return HELD ? Word<T>{held[k]} : load(k); }
-  // f(word) of every word that this thread has, the next two on their way meanwhile
+  // f(word, i) of every word that this wave has, the next two on their way meanwhile. All lanes take part in all of them; behind the
+  // row's end a word is nothing but -inf.
   template <class F>
   __device__ __forceinline__ void each_word(const F &f) const {
-    const int mine = min(per, (words - first + 63) >> 6);
+    const int begin = first - (threadIdx.x & 63), mine = min(per, (words - begin + 63) >> 6), last = words - 1;
     if (mine <= 0) return;
-    const int last = first + 64 * (mine - 1);
-    Word<T> now = at(first), next = at(min(first + 64, last));
+    auto get = [&](int i) { return at(min(first + 64 * i, last)); };
+    Word<T> now = get(0), next = get(min(1, mine - 1));
 #pragma unroll 1
     for (int i = 0; i < mine; ++i) {
-      const Word<T> then = at(min(first + 64 * (i + 2), last));
+      const Word<T> then = get(min(i + 2, mine - 1));
+      if (first + 64 * i > last) {
+        constexpr uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u;
+        now.raw = make_uint4(nothing, nothing, nothing, nothing);
+      }
       f(now, i);
       now  = next;
       next = then;
@@ -224,7 +230,6 @@ sample_all_kernel(const SampleArgs a) {
     s  = wave_total(s);
     f  = wave_total(f);
     tn = wave_total(tn);
-    n  = __shfl(n, 0);   // (the first lane has a word wherever another one has)
     if (with_raw) q = wave_total(q);
     const int any_bad = __any(bad);
     __syncthreads();   // (what was there before has been read)
@@ -347,7 +352,7 @@ sample_kernel(const SampleArgs a) {
   int n = 0;
   bool strange = false;
   RowWords<T, NT, false>(a, nullptr).each_word([&](const Word<T> &w, int i) {
-    if (HELD) row_lds[words.first + 64 * i] = w.raw;
+    if (HELD && words.first + 64 * i < words.words) row_lds[words.first + 64 * i] = w.raw;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       top     = fmaxf(top, w[e]);
@@ -396,9 +401,7 @@ sample_kernel(const SampleArgs a) {
   u64 ties = 0;
   bool in_list = false;   // all that is left is in the list
 
-  const float mean = n ? top - far / static_cast<float>(n) : 16.0f, scale = mean > 0.0f ? BINS / (4.0f * mean) : 0.0f;
-  // the first round's ranges: equal ones of the distance from the maximum, the last for what is beyond four times the average
-  auto bin_of = [&](float v) { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); };
+  const float mean = n ? top - far / static_cast<float>(n) : 16.0f;
 
   // The logit at which the sum over what is left, from the largest logit on, reaches a target: top_k (counts) or the share top_p of
   // all (weights). V becomes that logit and ties what is missing there. The first round is over the row, those behind it over the logits that the first
@@ -407,9 +410,26 @@ sample_kernel(const SampleArgs a) {
     using M = decltype(zero);
     constexpr bool MASS = sizeof(M) == 8;
     M *hist = reinterpret_cast<M *>(sh.hist);
+    // The first round's ranges: equal ones of the distance from the maximum, the last for what is beyond. That one's sum takes no atomics, so it
+    // begins behind the average where a target is likely to be nearer: 131072 logits, top_p 0.9 ... us, up to four times the average ... .
+    const bool near    = MASS ? p.top_p <= 0.95f : top_k <= vocab / 8;
+    const float reach  = (near ? 1.2f : 4.0f) * mean, scale = reach > 0.0f ? BINS / reach : 0.0f;
+    auto bin_of = [&](float v) { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); };
+    // the smallest logit, as a key, in range b or one before it; by all the lanes of every wave
+    auto first_in = [&](const int b) {
+      uint32_t from = key_of(-FLT_MAX), to = key_of(top);
+      while (from < to) {
+        const uint32_t at = from + static_cast<uint32_t>((static_cast<u64>(to - from) * lane) / 63);
+        const int hit = __builtin_ctzll(__ballot(bin_of(of_key(at)) <= b));   // (the last lane's is the maximum, or known to be)
+        to = __shfl(at, hit);
+        if (hit == 0) break;
+        from = __shfl(at, hit - 1) + 1;
+      }
+      return to;
+    };
     const u64 v_weight = MASS ? whole(weight(V)) : 0;
     u64 above = 0, target = MASS ? 0 : static_cast<u64>(top_k);
-    int bin = 0, shift = 0;
+    int shift = 0;
     uint32_t lo = 0, hi = 0;
     bool listed = in_list;
     // A short list in one wave: each lane has a logit, and what the larger ones come to. `whole_sum`: the list has all that is left.
@@ -469,41 +489,23 @@ sample_kernel(const SampleArgs a) {
       weigh_list();
       return in_short_list(true);
     }
-    for (int round = 0; round < 6; ++round) {   // (32 bits of logits, 7 or more a round behind the first)
+    auto clear = [&] {
       __syncthreads();   // (the histogram of before has been read)
       hist[tid] = hist[tid + NT] = 0;
       __syncthreads();
-      M last = 0;   // (the first round's last range has the most, and one sum a lane)
-      auto add = [&](float v, auto what) {
-        if (round == 0) {
-          const int b = bin_of(v);
-          if (b == BINS - 1)
-            last += what();
-          else
-            atomicAdd(&hist[b], what());
-        } else {
-          const uint32_t k = key_of(v);
-          if (k >= lo && k <= hi && bin_of(v) == bin) atomicAdd(&hist[(hi - k) >> shift], what());
-        }
-      };
-      auto one = [&](float v) {
-        if constexpr (MASS) {
-          if (v > V) add(v, [&] { return whole(weight(v)); });
-        } else {
-          if (v > -INFINITY) add(v, [] { return 1u; });
-        }
-      };
-      if (listed) {
-        const int m = sh.listed;
-        for (int i = tid; i < m; i += NT) one(sh.list[i]);
-      } else {
-        words.each(one);
-      }
-      if (MASS && ties && tid == 0) add(V, [&] { return ties * v_weight; });
-      if (round == 0) {
-        last = wave_total(last);
-        if (lane == 0 && last) atomicAdd(&hist[BINS - 1], last);
-      }
+    };
+    M last = 0;   // (the first round's last range has the most, and one sum a lane)
+    auto first_round = [&](float v, M what) {
+      const int b = bin_of(v);
+      last += b == BINS - 1 ? what : 0;
+      if (b < BINS - 1) atomicAdd(&hist[b], what);
+    };
+    auto add_last = [&] {
+      last = wave_total(last);
+      if (lane == 0 && last) atomicAdd(&hist[BINS - 1], last);
+    };
+    // where the sums over the ranges reach what `want(total)` says (or false: they do not)
+    auto find = [&](auto want_of) {
       __syncthreads();
       const u64 first = hist[2 * tid], second = hist[2 * tid + 1];
       u64 upto = wave_scan(first + second);
@@ -515,39 +517,109 @@ sample_kernel(const SampleArgs a) {
         if (w == wave) upto += total;
         total += sh.sum[w];
       }
-      if (round == 0) {
-        if (MASS) target = max(1ull, min(total, static_cast<u64>(__builtin_ceil(static_cast<double>(p.top_p) * static_cast<double>(total)))));
-        if (total < target) return;   // fewer than top_k (the whole workgroup)
-      }
-      const u64 want = target - above;
+      const u64 want = want_of(total);
+      if (total < want) return false;
       if (upto >= want && upto - first - second < want) {
         const bool later = upto - second < want;
         sh.found_bin   = 2 * tid + later;
-        sh.found_above = above + upto - second - (later ? 0 : first);
-        sh.found_upto  = above + upto - (later ? 0 : second);
+        sh.found_above = upto - second - (later ? 0 : first);
+        sh.found_upto  = upto - (later ? 0 : second);
       }
       __syncthreads();
-      above = sh.found_above;
+      return true;
+    };
+    // all from `least` to `most` (and above V) into the list
+    auto gather = [&](const float least, const float most) {
+      words.each_word([&](const Word<T> &w, int) {
+        float m = w[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) m = fmaxf(m, w[e]);
+        if (!__any(m >= least)) return;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (w[e] >= least && w[e] <= most && w[e] > V) {   // (few)
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < SAMPLE_LIST) sh.list[at] = w[e];
+          }
+      });
+      __syncthreads();
+    };
+    // (of GRAIN neighbouring keys one is a number of the logits' type)
+    constexpr int GRAIN = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 16 : 13;
+    auto finer = [&] { shift = max(GRAIN, (32 - __builtin_clz((hi - lo) | 1)) - (31 - __builtin_clz(BINS))); };
+
+    int round = 0;
+    if constexpr (!MASS) {
+      // A rough bound first, from every thread's first word: where as many of those lie as top_k takes of them, and then some. Between top_k
+      // and SAMPLE_LIST of all logits are above it nearly always, and nothing else has to be looked at.
+      const float share = static_cast<float>(top_k) / words.per;
+      const int rough = static_cast<int>(1.3f * share + 4.0f * sqrtf(share)) + 7;
+      if (words.per >= 4 && static_cast<long>(rough) * words.per <= SAMPLE_LIST * 3 / 4) {
+        clear();
+        const int k = words.first;
+        if (k < words.words) {
+          const Word<T> w = words.at(k);
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (w[e] > -INFINITY) first_round(w[e], 1u);
+        }
+        last = 0;   // (a bound there would be none)
+        if (find([&](u64) { return static_cast<u64>(rough); })) {
+          lo = first_in(sh.found_bin);
+          hi = key_of(top);
+          gather(of_key(lo), top);
+          const int m = sh.listed;
+          if (m >= top_k && m <= SAMPLE_LIST) {
+            in_list = listed = true;
+            if (m <= SAMPLE_SHORT) return in_short_list(false);
+            finer();
+            round = 1;
+          } else {
+            __syncthreads();
+            if (tid == 0) sh.listed = 0;
+          }
+        }
+      }
+    }
+    for (; round < 6; ++round) {   // (32 bits of logits, 7 or more a round behind the first)
+      clear();
+      auto later_round = [&](float v, auto what) {
+        const uint32_t k = key_of(v);
+        if (k >= lo && k <= hi) atomicAdd(&hist[(hi - k) >> shift], what());
+      };
+      auto one = [&](float v) {
+        if constexpr (MASS) {
+          if (v > V) {
+            if (round) later_round(v, [&] { return whole(weight(v)); }); else first_round(v, whole(weight(v)));
+          }
+        } else if (v > -INFINITY) {
+          if (round) later_round(v, [] { return 1u; }); else first_round(v, 1u);
+        }
+      };
+      if (listed) {
+        const int m = sh.listed;
+        for (int i = tid; i < m; i += NT) one(sh.list[i]);
+      } else {
+        words.each(one);
+      }
+      if (MASS && ties && tid == 0) {
+        if (round) later_round(V, [&] { return ties * v_weight; }); else first_round(V, ties * v_weight);
+      }
+      if (round == 0) add_last();
+      const bool there = find([&](u64 total) {
+        if (MASS && round == 0)
+          target = max(1ull, min(total, static_cast<u64>(__builtin_ceil(static_cast<double>(p.top_p) * static_cast<double>(total)))));
+        return target - above;
+      });
+      if (!there) return;   // fewer than top_k (the whole workgroup)
+      above += sh.found_above;
       const int b = sh.found_bin;
       if (round == 0) {
-        bin = b;
-        // the logits of that range lie between these (and other ranges' beside it)
-        const double s = scale, x1 = top64 - b * 0.999999 / s, x0 = top64 - (b + 1) * 1.000001 / s;
-        hi = scale > 0.0f ? key_of(static_cast<float>(x1 + 1e-6 * __builtin_fabs(x1) + 1e-37)) : key_of(top);
-        lo = scale > 0.0f && b < BINS - 1 ? key_of(__builtin_fmaxf(static_cast<float>(x0 - 1e-6 * __builtin_fabs(x0) - 1e-37), -FLT_MAX)) : key_of(-FLT_MAX);
-        hi = min(hi, key_of(top));
+        hi = bin_of(top) < b ? first_in(b - 1) - 1 : key_of(top);
+        lo = first_in(b);
         // Of top-k all from the maximum on, which is what top-p looks at next; of weights that range alone.
         if (!listed && (MASS || sh.found_upto <= SAMPLE_LIST)) {
-          words.each([&](float v) {
-            const bool in = v > -INFINITY && (MASS ? v > V && bin_of(v) == bin : bin_of(v) <= bin);
-            const u64 lanes = __ballot(in);
-            if (!lanes) return;
-            int at = 0;
-            if (lane == __builtin_ctzll(lanes)) at = atomicAdd(&sh.listed, __builtin_popcountll(lanes));
-            at = __shfl(at, __builtin_ctzll(lanes)) + __builtin_popcountll(lanes & ((1ull << lane) - 1));
-            if (in && at < SAMPLE_LIST) sh.list[at] = v;
-          });
-          __syncthreads();
+          gather(of_key(lo), MASS ? of_key(hi) : top);
           listed = sh.listed <= SAMPLE_LIST;
           if (!MASS) in_list = true;
           if (sh.listed <= SAMPLE_SHORT) {
@@ -558,10 +630,16 @@ sample_kernel(const SampleArgs a) {
         }
       } else {
         hi -= static_cast<uint32_t>(b) << shift;
-        if (shift == 0) break;
+        if (shift == GRAIN) {
+          if (GRAIN) {   // positive numbers' keys end in zeros, negative ones' in ones
+            const uint32_t down = hi >> GRAIN << GRAIN;
+            hi = down & 0x80000000u ? down : ((hi + 1) >> GRAIN << GRAIN) - 1;
+          }
+          break;
+        }
         lo = max(lo, hi - ((1u << shift) - 1));
       }
-      shift = max(0, (32 - __builtin_clz((hi - lo) | 1)) - (31 - __builtin_clz(BINS)));
+      finer();
     }
     const float before = V;
     V = of_key(hi);
@@ -574,6 +652,19 @@ sample_kernel(const SampleArgs a) {
     ties = here;
   };
   if (with_k) select(0u);
+  if (with_p && in_list && top_k <= SAMPLE_SHORT && sh.listed > SAMPLE_SHORT) {   // what is above V in a short list again
+    float mine[SAMPLE_LIST / NT];
+    const int m = sh.listed;
+#pragma unroll
+    for (int i = 0; i < SAMPLE_LIST / NT; ++i) mine[i] = tid + i * NT < m ? sh.list[tid + i * NT] : -INFINITY;
+    __syncthreads();
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SAMPLE_LIST / NT; ++i)
+      if (mine[i] > V) sh.list[atomicAdd(&sh.listed, 1)] = mine[i];
+    __syncthreads();
+  }
   if (with_p) select(0ull);
   if (with_q) {
     const double cut = top64 + temperature * log(static_cast<double>(fminf(p.min_p, 1.0f)));
@@ -594,21 +685,51 @@ sample_kernel(const SampleArgs a) {
     int gt_n = 0, at = 0, tops = 0;
     double rest = 0.0, raw = 0.0;
     const bool same = !(with_k || with_p || with_q) && temperature == 1.0, with_raw = a.logp && !same;
-    words.each([&](float v) {
-      if (v > V) {
-        const double w = weight(v);
-        gt += whole(w);
-        ++gt_n;
-        rest += v < top ? w : 0.0;
+    // What is left is put behind each other in a queue of the wave's own (where the histogram was), and weighed 64 at a time.
+    float *queue = reinterpret_cast<float *>(sh.hist) + wave * 256;
+    int queued = 0;
+    auto weigh = [&](const int m) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      queued -= m;
+      if (lane < m) {
+        const float v  = queue[queued + lane];
+        const double x = weight(v);
+        gt += whole(x);
+        rest += v < top ? x : 0.0;
+        tops += v == top;
       }
-      at += v == V;
-      tops += v == top;
-      if (with_raw) raw += v < top && v > -INFINITY ? static_cast<double>(exp_32(v - top)) : 0.0;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+    __syncthreads();   // (the histogram has been read)
+    words.each_word([&](const Word<T> &w, int) {
+      float m = w[0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) m = fmaxf(m, w[e]);
+      if (__any(m >= V))
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v  = w[e];
+          const u64 keep = __ballot(v > V);
+          at += __builtin_popcountll(__ballot(v == V));
+          if (v > V) queue[queued + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(keep >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(keep), 0))] = v;
+          queued += __builtin_popcountll(keep);
+          gt_n += __builtin_popcountll(keep);
+          if (e & 1)
+            while (queued >= 64) weigh(64);
+        }
+      if (with_raw) {
+        float r = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) r += w[e] < top ? exp_32(w[e] - top) : 0.0f;
+        raw += static_cast<double>(r);
+      }
     });
+    weigh(queued);
     gt   = wave_total(gt);
-    gt_n = wave_total(gt_n);
-    at   = wave_total(at);
-    tops = wave_total(tops);
+    tops = V == top ? at : wave_total(tops);
     rest = wave_total(rest);
     raw  = same ? rest : wave_total(raw);
     if (lane == 0) {
