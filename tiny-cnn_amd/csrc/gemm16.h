@@ -229,6 +229,16 @@ struct G16Turn {
   }
 };
 
+// A launch may have a part of a product's tiles: those from epi.first_tile on, epi.tiles_here of them (an Epi without these: all).
+template <class Epi>
+__device__ __forceinline__ auto g16_first_tile(const Epi &epi, int) -> decltype(epi.first_tile) { return epi.first_tile; }
+template <class Epi>
+__device__ __forceinline__ int g16_first_tile(const Epi &, long) { return 0; }
+template <class Epi>
+__device__ __forceinline__ auto g16_tiles_here(const Epi &epi, int, int) -> decltype(epi.tiles_here) { return epi.tiles_here; }
+template <class Epi>
+__device__ __forceinline__ int g16_tiles_here(const Epi &, const int all, long) { return all; }
+
 // Epi: done(acc, m0, n0, lane, split, lds) with the wave's blocks: register r of lane l of block (i, j) is row
 // m0 + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4 and column n0 + 32 j + l % 32 (PAIR: of the tile's column order); lds:
 // G16Turn<32 TN>::BYTES of the wave's own.
@@ -241,12 +251,12 @@ gemm16_kernel(const G16Matrix A, const G16Matrix B, const Epi epi, const int til
   using SideB = G16Side<BN, B_KC, PAIR, NT>;
   __shared__ __align__(1024) char lds[BUFS][SideA::BYTES + SideB::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-  const int tiles = Tiles::count(tiles_m, tiles_n);
+  const int tiles = g16_tiles_here(epi, Tiles::count(tiles_m, tiles_n), 0);
   int id = xcd_compact_id(blockIdx.x, gridDim.x);
   const int split = id / tiles;
   id -= split * tiles;
   int tm, tn;
-  Tiles::place(id, tiles_m, tiles_n, tm, tn);
+  Tiles::place(id + g16_first_tile(epi, 0), tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * (PAIR ? BN / 2 : BN);
   const int kbeg = split * k_per_split, kend = min(K, kbeg + k_per_split);
 

@@ -30,16 +30,18 @@ constexpr int MU_NT = 256;
 template <int WM, int WN, int TM, int TN, bool A_KC, bool B_KC, class Tiles, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const Epi epi, const int tiles_m, const int tiles_n,
-                const int K) {
+                const int K, const int k_per_split) {
   constexpr int NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 32;
   using SideA = G16Side<BM, A_KC, false, NT, BK>;
   using SideB = G16Side<BN, B_KC, false, NT, BK>;
   constexpr int STAGE = 2 * (SideA::BYTES + SideB::BYTES);
   __shared__ __align__(1024) char lds[2][STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-  int tm, tn;
-  Tiles::place(xcd_compact_id(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
+  int id = xcd_compact_id(blockIdx.x, gridDim.x), tm, tn;
+  const int split = id / epi.tiles_here;
+  id -= split * epi.tiles_here;
+  Tiles::place(id + epi.first_tile, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN, kbeg = split * k_per_split, kend = min(K, kbeg + k_per_split);
   SideA sa;
   SideB sb;
   sa.plan(A, m0, tid);
@@ -61,17 +63,17 @@ gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const 
       SideB b = sb;
       a.base += 2 * p * a_plane;
       b.base += 2 * p * b_plane;
-      a.fetch(A, lds[buf] + p * SideA::BYTES, k0, K - k0, tid);
-      b.fetch(B, lds[buf] + 2 * SideA::BYTES + p * SideB::BYTES, k0, K - k0, tid);
+      a.fetch(A, lds[buf] + p * SideA::BYTES, k0, kend - k0, tid);
+      b.fetch(B, lds[buf] + 2 * SideA::BYTES + p * SideB::BYTES, k0, kend - k0, tid);
     }
   };
-  fetch(0, 0);
+  fetch(kbeg, 0);
   int buf = 0;
 #pragma unroll 1
-  for (int k0 = 0; k0 < K; k0 += BK) {
+  for (int k0 = kbeg; k0 < kend; k0 += BK) {
     g16_arrived<0>();
     __syncthreads();   // this tile has arrived, and everyone has read the one before
-    if (k0 + BK < K) fetch(k0 + BK, buf ^ 1);
+    if (k0 + BK < kend) fetch(k0 + BK, buf ^ 1);
     const char *at = lds[buf];
     g16_s16x8 a[2][TM][2], b[2][TN][2];
 #pragma unroll
@@ -105,7 +107,7 @@ gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const 
   }
   static_assert(sizeof(lds) >= WM * WN * G16Turn<32 * TN>::BYTES, "");
   __syncthreads();
-  epi.template done<TM, TN>(acc, m0 + 32 * TM * wm, n0 + 32 * TN * wn, lane, 0, reinterpret_cast<float *>(lds[0] + wave * G16Turn<32 * TN>::BYTES));
+  epi.template done<TM, TN>(acc, m0 + 32 * TM * wm, n0 + 32 * TN * wn, lane, split, reinterpret_cast<float *>(lds[0] + wave * G16Turn<32 * TN>::BYTES));
 }
 
 // A matrix in two fp16 planes, rows of `ld` (a multiple of 8, zero behind `cols`).
@@ -139,9 +141,22 @@ __device__ __forceinline__ void join_halves(const uint4 hi, const uint4 lo, cons
 template <class F, bool SYM>
 struct EpiRows {
   F f;
-  int rows, cols, tile;   // of C; (SYM) of a side of the workgroup's tile
+  int rows, cols, tile;          // of C; of a side of the workgroup's tile
+  int first_tile, tiles_here;    // of the launch
+  float *partial;                // where the tiles are split along k: [split][tile of the launch][tile][tile], which rest_kernel() takes up
   template <int TM, int TN>
-  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int, float *lds) const {
+  __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split, float *lds) const {
+    if (partial) {
+      const int slot = xcd_compact_id(blockIdx.x, gridDim.x);   // split * tiles_here + the tile
+      float *p = partial + static_cast<size_t>(slot) * tile * tile + (m0 % tile + 4 * (lane >> 5)) * tile + n0 % tile + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) p[(32 * i + 8 * (r >> 2) + (r & 3)) * tile + 32 * j] = acc[i][j][r];
+      return;
+    }
     const G16Turn<32 * TN> turn{lds};
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -174,6 +189,39 @@ struct EpiRows {
     }
   }
 };
+
+// The tiles that were split along k: their parts added up, in order, and finished. Bound by reading them.
+template <class F, bool SYM, class Tiles>
+__global__ void __launch_bounds__(MU_NT)
+muon_rest_kernel(const EpiRows<F, SYM> epi, const int tiles_m, const int tiles_n, const int parts) {
+  const int side = epi.tile, at = blockIdx.y * MU_NT + threadIdx.x;   // of eight elements
+  int tm, tn;
+  Tiles::place(blockIdx.x + epi.first_tile, tiles_m, tiles_n, tm, tn);
+  const size_t slice = static_cast<size_t>(epi.tiles_here) * side * side;
+  const float *p = epi.partial + static_cast<size_t>(blockIdx.x) * side * side;
+  {
+    const int row = at / (side / 8), col = at % (side / 8) * 8;
+    if (tm * side + row < epi.rows && tn * side + col < epi.cols) {
+      float v[8] = {};
+      for (int s = 0; s < parts; ++s) {
+        float o[8];
+        load8(p + s * slice + row * side + col, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += o[e];
+      }
+      epi.f.finish(tm * side + row, tn * side + col, v);
+    }
+  }
+  if (!SYM || tm == tn) return;
+  const int row = at % side, col = at / side * 8;   // of the mirror image
+  if (tn * side + row < epi.rows && tm * side + col < epi.cols) {
+    float v[8] = {};
+    for (int s = 0; s < parts; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += p[s * slice + (col + e) * side + row];
+    epi.f.finish(tn * side + row, tm * side + col, v);
+  }
+}
 
 __device__ __forceinline__ void put_halves(const Planes &out, const int row, const int col, const Halves &h, const bool lo) {
   uint16_t *p = out.p + static_cast<long>(row) * out.ld + col;
@@ -267,56 +315,85 @@ struct LastFinish {
   }
 };
 
-// A tile's side, waves and blocks by the size of the product: us a round of workgroups, of 64 reduction indices and beside them
+// Tiles, by the size of the product: a side, the workgroups that a compute unit holds, us of 64 reduction indices and beside them. Whole rounds
+// of workgroups take whole tiles; the tiles of a last round that is not half full are split along k, which takes two more launches (4096 x 4096 of
+// two parts, symmetric: 528 tiles of 128 on 512 places ... us, unsplit ...).
 struct MuTile {
   int side, per_cu;
   double us, round_us;
 };
 constexpr MuTile MU_TILES[] = {{256, 1, 1.65, 8.0}, {128, 2, 0.92, 5.0}, {64, 4, 0.78, 3.0}};    // hi alone
 constexpr MuTile MU_TILES2[] = {{128, 2, 2.6, 6.0}, {64, 4, 2.2, 4.0}};                          // three products
+struct MuSplit {
+  int side, whole, parts, k_per_part;   // whole: tiles that are not split
+};
 template <int N>
-int mu_plan(const MuTile (&tiles)[N], int M, int Ncols, int K, bool sym) {
+MuSplit mu_plan(const MuTile (&tiles)[N], int M, int Ncols, int K, bool sym) {
   const long cus = std::max(1, ctx().compute_units);
-  int best = 0;
+  MuSplit best{};
   double best_us = 1e30;
-  for (int c = 0; c < N; ++c) {
-    const MuTile &t = tiles[c];
-    const long tm = ceil_div(M, t.side), tn = ceil_div(Ncols, t.side), groups = sym ? tm * (tm + 1) / 2 : tm * tn;
-    const long rounds = (groups + cus * t.per_cu - 1) / (cus * t.per_cu);
-    const double us = rounds * (ceil_div(K, 64) * t.us + t.round_us);
-    if (us < best_us) {
-      best_us = us;
-      best    = c;
-    }
+  const int ktiles = ceil_div(K, 64);
+  for (const MuTile &t : tiles) {
+    const long tm = ceil_div(M, t.side), tn = ceil_div(Ncols, t.side), all = sym ? tm * (tm + 1) / 2 : tm * tn, places = cus * t.per_cu;
+    const long rounds = all / places, rest = all % places;
+    const double round_us = ktiles * t.us + t.round_us;
+    auto take = [&](double us, const MuSplit &s) {
+      if (us < best_us) {
+        best_us = us;
+        best    = s;
+      }
+    };
+    take((rounds + (rest ? 1 : 0)) * round_us, MuSplit{t.side, static_cast<int>(all), 1, ktiles * 64});
+    if (!rest) continue;
+    const int per = ceil_div(ktiles, static_cast<int>(std::min<long>(std::max(1l, places / rest), std::min(16, std::max(1, ktiles / 2)))));
+    const int parts = ceil_div(ktiles, per);
+    if (parts < 2) continue;
+    const double bytes = 8.0 * rest * parts * t.side * t.side;
+    take(rounds * round_us + per * t.us + t.round_us + 8.0 + bytes / 4e6, MuSplit{t.side, static_cast<int>(all - rest), parts, per * 64});
   }
   return best;
 }
+MuSplit mu_plan(bool two, int M, int N, int K, bool sym) { return two ? mu_plan(MU_TILES2, M, N, K, sym) : mu_plan(MU_TILES, M, N, K, sym); }
+int mu_tiles(const MuSplit &s, int M, int N, bool sym) {
+  const int tm = ceil_div(M, s.side), tn = ceil_div(N, s.side);
+  return sym ? G16LowerTiles::count(tm, tn) : G16AllTiles::count(tm, tn);
+}
+size_t mu_partial_bytes(bool two, int M, int N, int K, bool sym) {
+  const MuSplit s = mu_plan(two, M, N, K, sym);
+  return s.parts > 1 ? ws_align(4 * static_cast<size_t>(mu_tiles(s, M, N, sym) - s.whole) * s.parts * s.side * s.side) : 0;
+}
 
 template <bool A_KC, bool B_KC, bool SYM, class F>
-int mu_gemm(bool two, const Planes &a, const Planes &b, const F &f, int M, int N, int K, const char *tag) {
+int mu_gemm(bool two, const Planes &a, const Planes &b, const F &f, int M, int N, int K, float *partial, const char *tag) {
   ProfScope prof(tag, M, N, K);
   using Tiles = typename std::conditional<SYM, G16LowerTiles, G16AllTiles>::type;
   using Epi   = EpiRows<F, SYM>;
-  const int c    = two ? mu_plan(MU_TILES2, M, N, K, SYM) : mu_plan(MU_TILES, M, N, K, SYM);
-  const int side = two ? MU_TILES2[c].side : MU_TILES[c].side;
-  const int tm = ceil_div(M, side), tn = ceil_div(N, side);
-  const Epi epi{f, M, N, side};
+  const MuSplit plan = mu_plan(two, M, N, K, SYM);
+  const int side = plan.side, tm = ceil_div(M, side), tn = ceil_div(N, side), rest = mu_tiles(plan, M, N, SYM) - plan.whole;
   const G16Matrix A = a.matrix(), B = b.matrix();
-  const dim3 grid(static_cast<unsigned>(Tiles::count(tm, tn)));
-  if (two) {
-    if (side == 128)
-      TDH_LAUNCH((gemm16x2_kernel<2, 2, 2, 2, A_KC, B_KC, Tiles, Epi>), grid, dim3(256), 0, ctx().stream, A, B, a.plane, b.plane, epi, tm, tn, K);
-    else
-      TDH_LAUNCH((gemm16x2_kernel<2, 1, 1, 2, A_KC, B_KC, Tiles, Epi>), grid, dim3(128), 0, ctx().stream, A, B, a.plane, b.plane, epi, tm, tn, K);
-  } else {
-    const int whole = ceil_div(K, G16_BK) * G16_BK;
-    if (side == 256)
-      TDH_LAUNCH((gemm16_kernel<f16, 2, 4, 4, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(512), 0, ctx().stream, A, B, epi, tm, tn, K, whole);
-    else if (side == 128)
-      TDH_LAUNCH((gemm16_kernel<f16, 2, 2, 2, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(256), 0, ctx().stream, A, B, epi, tm, tn, K, whole);
-    else
-      TDH_LAUNCH((gemm16_kernel<f16, 2, 1, 1, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(128), 0, ctx().stream, A, B, epi, tm, tn, K, whole);
-  }
+  auto launch = [&](const Epi &epi, int parts, int k_per_part) {
+    const dim3 grid(static_cast<unsigned>(epi.tiles_here * parts));
+    if (two) {
+      if (side == 128)
+        TDH_LAUNCH((gemm16x2_kernel<2, 2, 2, 2, A_KC, B_KC, Tiles, Epi>), grid, dim3(256), 0, ctx().stream, A, B, a.plane, b.plane, epi, tm, tn, K, k_per_part);
+      else
+        TDH_LAUNCH((gemm16x2_kernel<2, 1, 1, 2, A_KC, B_KC, Tiles, Epi>), grid, dim3(128), 0, ctx().stream, A, B, a.plane, b.plane, epi, tm, tn, K, k_per_part);
+    } else {
+      if (side == 256)
+        TDH_LAUNCH((gemm16_kernel<f16, 2, 4, 4, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(512), 0, ctx().stream, A, B, epi, tm, tn, K, k_per_part);
+      else if (side == 128)
+        TDH_LAUNCH((gemm16_kernel<f16, 2, 2, 2, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(256), 0, ctx().stream, A, B, epi, tm, tn, K, k_per_part);
+      else
+        TDH_LAUNCH((gemm16_kernel<f16, 2, 1, 1, 2, 2, A_KC, B_KC, false, Epi, Tiles>), grid, dim3(128), 0, ctx().stream, A, B, epi, tm, tn, K, k_per_part);
+    }
+    TDH_LAUNCH_CHECK();
+    return static_cast<int>(TDH_OK);
+  };
+  if (plan.whole) TDH_TRY(launch(Epi{f, M, N, side, 0, plan.whole, nullptr}, 1, ceil_div(K, 64) * 64));
+  if (!rest) return TDH_OK;
+  const Epi epi{f, M, N, side, plan.whole, rest, partial};
+  TDH_TRY(launch(epi, plan.parts, plan.k_per_part));
+  TDH_LAUNCH((muon_rest_kernel<F, SYM, Tiles>), dim3(rest, side * side / 8 / MU_NT), dim3(MU_NT), 0, ctx().stream, epi, tm, tn, plan.parts);
   TDH_LAUNCH_CHECK();
   return TDH_OK;
 }
@@ -468,9 +545,15 @@ struct MuBuffers {
 };
 size_t planes_bytes(int rows, int ld) { return ws_align(4 * static_cast<size_t>(rows) * ld); }
 int mu_ld(int cols) { return (cols + 7) & ~7; }
-size_t mu_bytes(int rows, int cols) {
+// the largest of what the three products of a step leave in parts
+size_t mu_partial_bytes(bool two, int rows, int cols) {
   const int m = std::min(rows, cols);
-  return ws_align(8 * MU_PARTS) + 2 * planes_bytes(rows, mu_ld(cols)) + 2 * planes_bytes(m, mu_ld(m));
+  return std::max({mu_partial_bytes(two, m, m, rows > cols ? rows : mu_ld(cols), true), mu_partial_bytes(two, m, m, mu_ld(m), true),
+                   rows > cols ? mu_partial_bytes(two, rows, m, mu_ld(m), false) : mu_partial_bytes(two, m, cols, m, false)});
+}
+size_t mu_bytes(bool two, int rows, int cols) {
+  const int m = std::min(rows, cols);
+  return ws_align(8 * MU_PARTS) + 2 * planes_bytes(rows, mu_ld(cols)) + 2 * planes_bytes(m, mu_ld(m)) + mu_partial_bytes(two, rows, cols);
 }
 int take_planes(int rows, int cols, Planes *out) {
   const int ld = mu_ld(cols);
@@ -488,13 +571,16 @@ int mu_run(const tdh_muon &o, int rows, int cols, const Momentum<T> &u, const Ap
   MuPlan plan;
   mu_scalars(o, m, &plan);
   MuBuffers w;
-  TDH_TRY(ws_begin(mu_bytes(rows, cols)));
+  TDH_TRY(ws_begin(mu_bytes(two, rows, cols)));
   void *partial = nullptr;
   TDH_TRY(ws_take(8 * MU_PARTS, &partial));
   w.partial = static_cast<double *>(partial);
   for (Planes &x : w.x) TDH_TRY(take_planes(rows, cols, &x));
   TDH_TRY(take_planes(m, m, &w.gram));
   TDH_TRY(take_planes(m, m, &w.poly));
+  void *parts_of_tiles = nullptr;
+  if (const size_t bytes = mu_partial_bytes(two, rows, cols)) TDH_TRY(ws_take(bytes, &parts_of_tiles));
+  float *tp = static_cast<float *>(parts_of_tiles);
 
   const size_t n  = static_cast<size_t>(rows) * cols;
   const int cus   = std::max(1, ctx().compute_units);
@@ -523,16 +609,16 @@ int mu_run(const tdh_muon &o, int rows, int cols, const Momentum<T> &u, const Ap
     const float alpha = plan.alpha[k];
     const GramFinish gram{w.gram, 1.0f / (xs * xs), alpha, as, two};
     if (tall)
-      TDH_TRY((mu_gemm<false, false, true>(two, x, x, gram, m, m, rows, "muon_gram")));
+      TDH_TRY((mu_gemm<false, false, true>(two, x, x, gram, m, m, rows, tp, "muon_gram")));
     else
-      TDH_TRY((mu_gemm<true, true, true>(two, x, x, gram, m, m, x.ld, "muon_gram")));
+      TDH_TRY((mu_gemm<true, true, true>(two, x, x, gram, m, m, x.ld, tp, "muon_gram")));
     const PolyFinish poly{w.poly, w.gram, (o.b + 2.0f * o.c * alpha) / as, o.c / (as * as), bs, two};
-    TDH_TRY((mu_gemm<true, true, true>(two, w.gram, w.gram, poly, m, m, w.gram.ld, "muon_poly")));
+    TDH_TRY((mu_gemm<true, true, true>(two, w.gram, w.gram, poly, m, m, w.gram.ld, tp, "muon_poly")));
     const double a64 = alpha;
     const float keep = static_cast<float>((o.a + o.b * a64 + o.c * a64 * a64) / xs), part = 1.0f / (bs * xs);
     auto step = [&](const auto &finish) {
-      return tall ? mu_gemm<true, true, false>(two, x, w.poly, finish, rows, m, w.poly.ld, "muon_step")
-                  : mu_gemm<true, false, false>(two, w.poly, x, finish, m, cols, m, "muon_step");
+      return tall ? mu_gemm<true, true, false>(two, x, w.poly, finish, rows, m, w.poly.ld, tp, "muon_step")
+                  : mu_gemm<true, false, false>(two, w.poly, x, finish, m, cols, m, tp, "muon_step");
     };
     if (k + 1 < o.steps)
       TDH_TRY(step(StepFinish{x, next, keep, part, xs}));
