@@ -31,7 +31,7 @@ template <int WM, int WN, int TM, int TN, bool A_KC, bool B_KC, class Tiles, cla
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const Epi epi, const int tiles_m, const int tiles_n,
                 const int K, const int k_per_split) {
-  constexpr int NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 32;
+  constexpr int NT = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, BK = 32, TOGETHER = 32;
   using SideA = G16Side<BM, A_KC, false, NT, BK>;
   using SideB = G16Side<BN, B_KC, false, NT, BK>;
   constexpr int STAGE = 2 * (SideA::BYTES + SideB::BYTES);
@@ -46,11 +46,11 @@ gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const 
   SideB sb;
   sa.plan(A, m0, tid);
   sb.plan(B, n0, tid);
-  g16_f32x16 acc[TM][TN];
+  g16_f32x16 acc[TM][TN], sum[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = g16_f32x16{};
+    for (int j = 0; j < TN; ++j) acc[i][j] = sum[i][j] = g16_f32x16{};
   int oa[TM], ob[TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i) oa[i] = SideA::lane_offset(lane, 32 * (wm * TM + i));
@@ -86,23 +86,23 @@ gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const 
         for (int j = 0; j < TN; ++j) b[s][j][p] = SideB::read(at + p * SideB::BYTES, ob[j], lane, s);
       }
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      g16_f32x16 sum[TN];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) sum[j] = g16_f32x16{};
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int q = 0; q < 3; ++q)   // the small ones first
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) sum[j] = mfma16(f16(), a[s][i][q == 0], b[s][j][q == 1], sum[j]);
+          for (int j = 0; j < TN; ++j) sum[i][j] = mfma16(f16(), a[s][i][q == 0], b[s][j][q == 1], sum[i][j]);
+    if ((k0 - kbeg) / BK % TOGETHER == TOGETHER - 1 || k0 + BK >= kend)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] += sum[j][r];
-        asm volatile("" : "+v"(acc[i][j]));   // (here and now)
-      }
-    }
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            acc[i][j][r] += sum[i][j][r];
+            sum[i][j][r] = 0.0f;
+          }
     buf ^= 1;
   }
   static_assert(sizeof(lds) >= WM * WN * G16Turn<32 * TN>::BYTES, "");
@@ -271,6 +271,10 @@ struct Apply {
   int cols;
   bool add;
   float keep, take;
+  __device__ __forceinline__ void one(const int row, const int col, const float v) const {
+    T *p = out + static_cast<long>(row) * cols + col;
+    *p = from_f32<T>(add ? keep * to_f32(*p) + take * v : v);
+  }
   __device__ __forceinline__ void operator()(const int row, const int col, const float (&v)[8]) const {
     T *p = out + static_cast<long>(row) * cols + col;
     float o[8];
@@ -407,6 +411,14 @@ struct Momentum {
   float *momentum;   // or null: U is g
   float grad_scale, mu;
   bool nesterov;
+  // one element, with the momentum's update
+  __device__ __forceinline__ float one(const size_t at) const {
+    const float v = to_f32(g[at]);
+    if (!momentum) return v;
+    const float s = v * grad_scale, m = mu * momentum[at] + s;
+    momentum[at] = m;
+    return nesterov ? s + mu * m : m;
+  }
   template <bool FIRST>
   __device__ __forceinline__ void get(const size_t at, const int n, float (&u)[8]) const {
     float m[8];
@@ -539,6 +551,191 @@ bool mu_scalars(const tdh_muon &o, int m, MuPlan *p) {
   return true;
 }
 
+// ------------------------------------------------------------- small matrices
+// All of it by one workgroup, in one launch: X in its two parts twice in LDS, along either index, and the Gram matrix, whose place the polynomial takes. A
+// wave has 32 x 32 of X, in fp32, from the first step to the last. Three products in either kind. 120 x 84: ... us, as launches of their own 117.
+constexpr int MS_NT = 1024, MS_PAD = 8;   // (rows of LDS of 16 bytes more: 32 of them are read at a time)
+struct MuSmall {
+  int m, n, mp, np, steps;   // mp, np: in whole blocks of 32
+  bool tall;                 // X is the matrix turned round
+  double a, b, c, eps;
+  MuPlan plan;
+};
+size_t mu_small_bytes(int mp, int np) {
+  return 2 * sizeof(uint16_t) * (static_cast<size_t>(mp) * (np + MS_PAD) + static_cast<size_t>(np) * (mp + MS_PAD) + static_cast<size_t>(mp) * (mp + MS_PAD));
+}
+constexpr size_t MS_LDS = 156 << 10;
+bool mu_small(int rows, int cols) {
+  const int mp = ceil_div(std::min(rows, cols), 32) * 32, np = ceil_div(std::max(rows, cols), 32) * 32;
+  return static_cast<long>(mp) * np <= 16 * 1024 && mu_small_bytes(mp, np) <= MS_LDS;
+}
+template <class T, class D>
+__global__ void __launch_bounds__(MS_NT)
+muon_small_kernel(const Momentum<T> u, const Apply<D> apply, const MuSmall s) {
+  extern __shared__ __align__(16) uint16_t small_lds[];
+  __shared__ double sums[MS_NT / 64];
+  struct Matrix {
+    uint16_t *hi, *lo;
+    int ld;
+    __device__ __forceinline__ void put(const int row, const int col, const float v) const {
+      const _Float16 h = static_cast<_Float16>(v), l = static_cast<_Float16>(v - static_cast<float>(h));
+      hi[row * ld + col] = __builtin_bit_cast(uint16_t, h);
+      lo[row * ld + col] = __builtin_bit_cast(uint16_t, l);
+    }
+    __device__ __forceinline__ float get(const int row, const int col) const {
+      return static_cast<float>(__builtin_bit_cast(_Float16, hi[row * ld + col])) + static_cast<float>(__builtin_bit_cast(_Float16, lo[row * ld + col]));
+    }
+    // four neighbours of a row, from a multiple of four on
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    __device__ __forceinline__ void put4(const int row, const int col, const float (&v)[4]) const {
+      f16x4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = static_cast<_Float16>(v[e]);
+        l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+      }
+      *reinterpret_cast<f16x4 *>(hi + row * ld + col) = h;
+      *reinterpret_cast<f16x4 *>(lo + row * ld + col) = l;
+    }
+    __device__ __forceinline__ void get4(const int row, const int col, float (&v)[4]) const {
+      const f16x4 h = *reinterpret_cast<const f16x4 *>(hi + row * ld + col), l = *reinterpret_cast<const f16x4 *>(lo + row * ld + col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(h[e]) + static_cast<float>(l[e]);
+    }
+  };
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, l32 = lane & 31;
+  Matrix X, Xt, G;
+  uint16_t *at = small_lds;
+  auto take = [&](Matrix &mat, int rows, int ld) {
+    mat = Matrix{at, at + rows * ld, ld};
+    at += 2 * rows * ld;
+  };
+  take(X, s.mp, s.np + MS_PAD);
+  take(Xt, s.np, s.mp + MS_PAD);
+  take(G, s.mp, s.mp + MS_PAD);
+  for (int i = tid; i < (at - small_lds) / 8; i += MS_NT) reinterpret_cast<uint4 *>(small_lds)[i] = make_uint4(0, 0, 0, 0);
+  const int total = s.m * s.n, cols = s.tall ? s.m : s.n;
+  float held[16];
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    held[i] = tid + i * MS_NT < total ? u.one(tid + i * MS_NT) : 0.0f;
+    sum = __builtin_fma(static_cast<double>(held[i]), static_cast<double>(held[i]), sum);
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < MS_NT / 64; ++w) sum += sums[w];
+  const double inverse = 1.0 / (sqrt(sum) + s.eps);
+  const float xs = s.plan.x_scale, as = s.plan.a_scale, bs = s.plan.b_scale;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int e = tid + i * MS_NT;
+    if (e >= total) break;
+    const int row = e / cols, col = e - row * cols, m = s.tall ? col : row, n = s.tall ? row : col;
+    const float v = static_cast<float>(static_cast<double>(held[i]) * inverse) * xs;
+    X.put(m, n, v);
+    Xt.put(n, m, v);
+  }
+  __syncthreads();
+  const int tn = s.np / 32, tg = s.mp / 32, x0 = wave / tn * 32, x1 = wave % tn * 32, g0 = wave / tg * 32, g1 = wave % tg * 32;
+  const bool has_x = wave < s.mp / 32 * tn, has_g = wave < tg * tg;
+  // the element of this lane's register r, of a block at (row0, col0): row0 + row_of(r), col0 + l32
+  auto row_of = [&](int r) { return 8 * (r >> 2) + 4 * half + (r & 3); };
+  float x[16];
+  if (has_x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = X.get(x0 + row_of(r), x1 + l32);
+  // a block of A B^T, both along their rows of `len` (a multiple of 32)
+  auto product = [&](const Matrix &A, const int a0, const Matrix &B, const int b0, const int len) {
+    g16_f32x16 acc{}, more{};
+    const int ao = (a0 + l32) * A.ld + 8 * half, bo = (b0 + l32) * B.ld + 8 * half;
+    auto part = [](const uint16_t *p) { return *reinterpret_cast<const g16_s16x8 *>(p); };
+#pragma unroll 1
+    for (int k = 0; k < len; k += 32) {   // (two sums, so that an instruction need not wait for the one before)
+      const g16_s16x8 ah = part(A.hi + ao + k), al = part(A.lo + ao + k), bh = part(B.hi + bo + k), bl = part(B.lo + bo + k);
+      const g16_s16x8 ch = part(A.hi + ao + k + 16), cl = part(A.lo + ao + k + 16), dh = part(B.hi + bo + k + 16), dl = part(B.lo + bo + k + 16);
+      acc  = mfma16(f16(), al, bh, acc);
+      more = mfma16(f16(), cl, dh, more);
+      acc  = mfma16(f16(), ah, bl, acc);
+      more = mfma16(f16(), ch, dl, more);
+      acc  = mfma16(f16(), ah, bh, acc);
+      more = mfma16(f16(), ch, dh, more);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] += more[r];
+    return acc;
+  };
+#pragma unroll 1
+  for (int k = 0; k < s.steps; ++k) {
+    // (addresses are made anew in every step: kept from one to the next they take more registers than there are)
+    asm volatile("" : "+s"(X.ld), "+s"(Xt.ld), "+s"(G.ld));
+    const double alpha = s.plan.alpha[k];
+    if (has_g) {
+      const g16_f32x16 acc = product(X, g0, X, g1, s.np);
+      const float from = 1.0f / (xs * xs), al = static_cast<float>(alpha);
+      // (a lane has four neighbours of a column, which are as well four of a row)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int row = g0 + row_of(r), col = g1 + l32;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = row + e < s.m && col < s.m ? (acc[r + e] * from - (row + e == col ? al : 0.0f)) * as : 0.0f;
+        G.put4(col, row, v);
+      }
+    }
+    __syncthreads();
+    float p[16];
+    if (has_g) {
+      const g16_f32x16 acc = product(G, g0, G, g1, s.mp);
+      const float one = static_cast<float>(s.b + 2.0 * s.c * alpha) / as, square = static_cast<float>(s.c) / (as * as);
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        float v[4];
+        G.get4(g1 + l32, g0 + row_of(r), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[r + e] = __builtin_fmaf(acc[r + e], square, one * v[e]) * bs;
+      }
+    }
+    __syncthreads();
+    asm volatile("" : "+s"(G.ld));
+    if (has_g)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float v[4] = {p[r], p[r + 1], p[r + 2], p[r + 3]};
+        G.put4(g1 + l32, g0 + row_of(r), v);
+      }
+    __syncthreads();
+    if (has_x) {
+      const g16_f32x16 acc = product(G, x0, Xt, x1, s.mp);
+      const float keep = static_cast<float>(s.a + s.b * alpha + s.c * alpha * alpha), part = 1.0f / bs;   // (x is xs times X)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(acc[r], part, keep * x[r]);
+    }
+    __syncthreads();
+    if (k + 1 == s.steps) break;
+    asm volatile("" : "+s"(X.ld), "+s"(Xt.ld));
+    if (has_x)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float v[4] = {x[r], x[r + 1], x[r + 2], x[r + 3]};
+        Xt.put4(x1 + l32, x0 + row_of(r), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) X.put(x0 + row_of(r + e), x1 + l32, v[e]);
+      }
+    __syncthreads();
+  }
+  if (!has_x) return;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int m = x0 + row_of(r), n = x1 + l32;
+    if (m < s.m && n < s.n) apply.one(s.tall ? n : m, s.tall ? m : n, x[r] / xs);
+  }
+}
+
 struct MuBuffers {
   Planes x[2], gram, poly;
   double *partial;
@@ -570,6 +767,16 @@ int mu_run(const tdh_muon &o, int rows, int cols, const Momentum<T> &u, const Ap
   const bool tall = rows > cols, two = o.products == TDH_F32;
   MuPlan plan;
   mu_scalars(o, m, &plan);
+  if (mu_small(rows, cols)) {
+    const int n = std::max(rows, cols), mp = ceil_div(m, 32) * 32, np = ceil_div(n, 32) * 32;
+    const MuSmall small{m, n, mp, np, o.steps, tall, o.a, o.b, o.c, o.eps, plan};
+    const size_t lds = mu_small_bytes(mp, np);
+    ProfScope prof("muon_small", static_cast<double>(o.steps) * (3.0 * m * m * n + 1.0 * m * m * m), WORK_FLOP);
+    TDH_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(muon_small_kernel<T, D>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MS_LDS)));
+    TDH_LAUNCH((muon_small_kernel<T, D>), dim3(1), dim3(MS_NT), lds, ctx().stream, u, apply, small);
+    TDH_LAUNCH_CHECK();
+    return TDH_OK;
+  }
   MuBuffers w;
   TDH_TRY(ws_begin(mu_bytes(two, rows, cols)));
   void *partial = nullptr;
