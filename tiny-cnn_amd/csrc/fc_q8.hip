@@ -16,13 +16,25 @@ namespace tdh {
 
 namespace {
 
-// q of eight values and a scale, as packed bytes. The quotient is fp32's, rounded to nearest, ties to even, as the product's definition has it.
-__device__ __forceinline__ uint2 quantized(const float (&v)[8], const float scale) {
+// q of eight values and a scale, as packed bytes. The quotient is fp32's, rounded to nearest, ties to even, as the product's definition has it; a product with
+// the reciprocal is within 2^-15 of it and rounds to the same number, unless it lies beside a half (one in some thousands), where it is
+// divided. 4096 x 4096 in bf16: ... us, all of them divided 15.
+__device__ __forceinline__ uint2 quantized(const float (&v)[8], const float scale, const float inverse) {
   uint2 o = make_uint2(0, 0);
   if (!(scale > 0.0f)) return o;   // (all zero, or NaN)
+  float r[8], near = scale < 0x1p-100f ? 1.0f : 0.0f;   // (whose reciprocal is no number, or has few figures)
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int q = static_cast<int>(__builtin_amdgcn_fmed3f(__builtin_rintf(v[e] / scale), -127.0f, 127.0f));
+    const float t = v[e] * inverse;
+    r[e] = __builtin_rintf(t);
+    near = fmaxf(near, __builtin_fabsf(t - r[e]));
+  }
+  if (near > 0.4999f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = __builtin_rintf(v[e] / scale);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int q = static_cast<int>(__builtin_amdgcn_fmed3f(r[e], -127.0f, 127.0f));
     (&o.x)[e / 4] |= static_cast<uint32_t>(q & 255) << (8 * (e & 3));
   }
   return o;
@@ -43,9 +55,15 @@ __device__ __forceinline__ float most_of(const float (&v)[8], float most) {
 }
 __device__ __forceinline__ float scale_of(const float most) { return most <= FLT_MAX ? most / 127.0f : __builtin_nanf(""); }
 
-// A result. In 64 bits: a product of the two scales alone, or of one and the sum, may leave fp32's range where the result does not.
-__device__ __forceinline__ float scaled(const int sum, const float s, const float w, const float b) {
-  return static_cast<float>(__builtin_fma(static_cast<double>(sum), static_cast<double>(s) * static_cast<double>(w), static_cast<double>(b)));
+// A scale as f 2^e, f in [1/2, 1): a product of the two scales alone, or of one and the sum, may leave fp32's range where the result does not. NaN stays
+// in f.
+struct Scale {
+  float f;
+  int e;
+};
+__device__ __forceinline__ Scale scale_parts(const float s) { return Scale{__builtin_amdgcn_frexp_mantf(s), __builtin_amdgcn_frexp_expf(s)}; }
+__device__ __forceinline__ float scaled(const int sum, const Scale s, const Scale w, const float b) {
+  return __builtin_ldexpf(static_cast<float>(sum) * (s.f * w.f), s.e + w.e) + b;
 }
 
 // LANES lanes a row, W eights a lane in registers (W = 0: any number, the row is read twice)
@@ -80,18 +98,18 @@ quantize_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restri
     most = most_of(most_of(part[0], part[1]), most_of(part[2], part[3]));
   }
   if (!live) return;
-  const float s = scale_of(most);
+  const float s = scale_of(most), inverse = 1.0f / s;
   if (lane == 0) scale[row] = s;
   uint2 *out = reinterpret_cast<uint2 *>(q + row * ld);
   if constexpr (W > 0) {
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      if (lane + i * LANES < eights) out[lane + i * LANES] = quantized(held[i], s);
+      if (lane + i * LANES < eights) out[lane + i * LANES] = quantized(held[i], s, inverse);
   } else {
     for (int k = lane; k < eights; k += LANES) {
       float v[8];
       row8(p, 8 * k, len, v);
-      out[k] = quantized(v, s);
+      out[k] = quantized(v, s, inverse);
     }
   }
 }
@@ -106,6 +124,7 @@ int launch_quantize(const T *x, int8_t *q, float *scale, int rows, int len, int 
   const int eights = ld / 8;
   if (eights <= 64) return go(quantize_kernel<T, 64, 1>, 64);
   if (eights <= 256) return go(quantize_kernel<T, 64, 4>, 64);
+  if (eights <= 512 && rows > 1024) return go(quantize_kernel<T, 64, 8>, 64);
   if (eights <= 1024) return go(quantize_kernel<T, 256, 4>, 256);
   return go(quantize_kernel<T, 256, 0>, 256);
 }
@@ -119,7 +138,7 @@ struct EpiQ8 {
   int *partial;       // slices instead, [split][rows][cols]
   int rows, cols;
   __device__ __forceinline__ float one(const int sum, const float s, const int n) const {
-    return scaled(sum, s, wscale[n], bias ? to_f32(bias[n]) : 0.0f);
+    return scaled(sum, scale_parts(s), scale_parts(wscale[n]), bias ? to_f32(bias[n]) : 0.0f);
   }
   template <int TM, int TN>
   __device__ __forceinline__ void done(const g16_f32x16 (&acc)[TM][TN], const int m0, const int n0, const int lane, const int split, float *lds) const {
@@ -138,25 +157,32 @@ struct EpiQ8 {
       return;
     }
     const G16Turn<32 * TN> turn{lds};
+    // a lane has the same eight columns in all of its rows
+    const int n = n0 + lane % (4 * TN) * 8;
+    Scale w[8];
+    float b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = min(n + e, cols - 1);
+      w[e] = scale_parts(wscale[c]);
+      b[e] = bias ? to_f32(bias[c]) : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
       for (int j = 0; j < TN; ++j) turn.put(lane, j, [&](int r) { return acc[i][j][r]; });
-      turn.rows(lane, [&](int row, int col, const float (&v)[8]) {
-        const int m = m0 + 32 * i + row, n = n0 + col;
+      turn.rows(lane, [&](int row, int, const float (&v)[8]) {
+        const int m = m0 + 32 * i + row;
         if (m >= rows || n >= cols) return;
-        const float s = scale[m];
+        const Scale s = scale_parts(scale[m]);
         T *p = y + static_cast<size_t>(m) * cols + n;
-        if (n + 8 <= cols) {
-          float o[8];
+        float o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = one(__float_as_int(v[e]), s, n + e);
-          store8(p, o);
-        } else {
+        for (int e = 0; e < 8; ++e) o[e] = scaled(__float_as_int(v[e]), s, w[e], b[e]);
+        if (n + 8 <= cols) return store8(p, o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < cols) p[e] = from_f32<T>(one(__float_as_int(v[e]), s, n + e));
-        }
+        for (int e = 0; e < 8; ++e)
+          if (n + e < cols) p[e] = from_f32<T>(o[e]);
       });
     }
   }
@@ -211,16 +237,48 @@ int q8_many(int in, int out, int batch, const T *x, const int8_t *wq, const floa
 }
 
 // ------------------------------------------------------------------ a few samples
-constexpr int Q8_FEW = 8, Q8_FEW_BYTES = 64 << 10, Q8_NT = 512, Q8_ROWS = 4;   // Q8_ROWS: outputs of a wave at a time
-// M samples in LDS (q, in rows of `ld`), a wave Q8_ROWS outputs at a time, 16 bytes of every row a lane at a time. The first words of weights are asked
-// for before the samples are looked at.
+constexpr int Q8_FEW = 8, Q8_FEW_BYTES = 48 << 10, Q8_NT = 512;
+// the sum over a wave, in its last lane
+__device__ __forceinline__ int last_lane_sum(int v) {
+  auto add = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+  using I = std::integral_constant<int, 0xf>;
+  add(std::integral_constant<int, 0x111>(), I());   // from 1, 2, 4 and 8 lanes before, within rows of 16
+  add(std::integral_constant<int, 0x112>(), I());
+  add(std::integral_constant<int, 0x114>(), I());
+  add(std::integral_constant<int, 0x118>(), I());
+  add(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());   // the last lane of a row to the next one
+  add(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());   // ... of the second row to the two behind it
+  return v;
+}
+// M samples in LDS (q, in rows of `ld`). A wave goes through its outputs' rows of weights two at a time, 4 KB of either, with the next two such pieces on
+// their way; the first three are asked for before the samples are looked at, and arrive while those are brought to 8 bits.
 template <class T, int M>
 __global__ void __launch_bounds__(Q8_NT)
 q8_few_kernel(const T *__restrict__ x, const int8_t *__restrict__ wq, const float *__restrict__ wscale, const T *__restrict__ bias, T *__restrict__ y,
               const int in, const int ld, const int out, const int batch, const int per_wave) {
+  constexpr int R = 2, K = 4, AHEAD = M <= 4 ? 3 : 2;
   extern __shared__ uint4 lds[];
   __shared__ float part[M][Q8_NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, eights = ld / 8, words = ld / 16;
+  const int first = (blockIdx.x * (Q8_NT / 64) + wave) * per_wave, last = min(out, first + per_wave);
+  const int blocks = (words + 64 * K - 1) / (64 * K), pieces = first < last ? (last - first + R - 1) / R * blocks : 0;
+  uint4 w[AHEAD][R][K];
+  auto fetch = [&](uint4 (&to)[R][K], const int piece) {
+    const int n = first + piece / blocks * R, k0 = piece % blocks * 64 * K + lane;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int at = min(k0 + 64 * k, words - 1);   // (behind the row: nothing is made of it)
+        const any_word t = __builtin_nontemporal_load(reinterpret_cast<const any_word *>(wq + static_cast<size_t>(min(n + i, out - 1)) * ld) + at);
+        to[i][k] = __builtin_bit_cast(uint4, t);
+      }
+  };
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a)
+    if (a < pieces) fetch(w[a], a);
+  __builtin_amdgcn_sched_barrier(0);
+
   float most[M] = {};
 #pragma unroll
   for (int m = 0; m < M; ++m) {
@@ -243,58 +301,61 @@ q8_few_kernel(const T *__restrict__ x, const int8_t *__restrict__ wq, const floa
   for (int m = 0; m < M; ++m) {
     float v = part[m][0];
 #pragma unroll
-    for (int w = 1; w < Q8_NT / 64; ++w) v = most_of(v, part[m][w]);
+    for (int i = 1; i < Q8_NT / 64; ++i) v = most_of(v, part[m][i]);
     scale[m] = scale_of(v);
     if (m >= batch) continue;
     uint2 *q = reinterpret_cast<uint2 *>(lds) + static_cast<size_t>(m) * eights;
+    const float inverse = 1.0f / scale[m];
     for (int k = tid; k < eights; k += Q8_NT) {
       float e[8];
       row8(x + static_cast<size_t>(m) * in, 8 * k, in, e);
-      q[k] = quantized(e, scale[m]);
+      q[k] = quantized(e, scale[m], inverse);
     }
   }
   __syncthreads();
-  const int first = (blockIdx.x * (Q8_NT / 64) + wave) * per_wave, last = min(out, first + per_wave);
-  for (int n = first; n < last; n += Q8_ROWS) {
-    int sum[M][Q8_ROWS] = {};
-    const uint4 *w[Q8_ROWS];
+  int sum[M][R] = {};
+  auto use = [&](const uint4 (&v)[R][K], const int piece) {
+    const int block = piece % blocks, n = first + piece / blocks * R;
 #pragma unroll
-    for (int i = 0; i < Q8_ROWS; ++i) w[i] = reinterpret_cast<const uint4 *>(wq + static_cast<size_t>(min(n + i, out - 1)) * ld);
-#pragma unroll 2
-    for (int k = lane; k < words; k += 64) {
-      uint4 v[Q8_ROWS];
-#pragma unroll
-      for (int i = 0; i < Q8_ROWS; ++i) {
-        const any_word t = __builtin_nontemporal_load(reinterpret_cast<const any_word *>(w[i] + k));
-        v[i] = __builtin_bit_cast(uint4, t);
-      }
+    for (int k = 0; k < K; ++k) {
+      const int at = block * 64 * K + lane + 64 * k;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const uint4 q = lds[(m < batch ? m : 0) * words + k];
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (at < words && m < batch) q = lds[m * words + at];
 #pragma unroll
-        for (int i = 0; i < Q8_ROWS; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum[m][i] = __builtin_amdgcn_sdot4(static_cast<int>((&q.x)[e]), static_cast<int>((&v[i].x)[e]), sum[m][i], false);
+          for (int e = 0; e < 4; ++e) sum[m][i] = __builtin_amdgcn_sdot4(static_cast<int>((&q.x)[e]), static_cast<int>((&v[i][k].x)[e]), sum[m][i], false);
       }
     }
+    if (block + 1 < blocks) return;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      if (m >= batch) break;
+    for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int i = 0; i < Q8_ROWS; ++i) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum[m][i] += __shfl_xor(sum[m][i], o);
-        if (lane == i && n + i < last)
-          y[static_cast<size_t>(m) * out + n + i] = from_f32<T>(scaled(sum[m][i], scale[m], wscale[n + i], bias ? to_f32(bias[n + i]) : 0.0f));
+      for (int i = 0; i < R; ++i) {
+        const int total = last_lane_sum(sum[m][i]);
+        sum[m][i] = 0;
+        if (lane == 63 && n + i < last && m < batch)
+          y[static_cast<size_t>(m) * out + n + i] =
+              from_f32<T>(scaled(total, scale_parts(scale[m]), scale_parts(wscale[n + i]), bias ? to_f32(bias[n + i]) : 0.0f));
       }
+  };
+#pragma unroll 1
+  for (int p = 0; p < pieces; p += AHEAD) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (p + a >= pieces) break;
+      use(w[a], p + a);
+      if (p + a + AHEAD < pieces) fetch(w[a], p + a + AHEAD);
     }
   }
 }
 template <class T>
 int q8_few(int in, int out, int batch, const T *x, const int8_t *wq, const float *wscale, const T *b, T *y) {
   const int ld = static_cast<int>(tdh_q8_row(in)), cus = std::max(1, ctx().compute_units), waves = Q8_NT / 64;
-  // as many workgroups as compute units, each wave whole groups of outputs
-  const int per_wave = std::max(Q8_ROWS, ceil_div(ceil_div(out, cus * waves), Q8_ROWS) * Q8_ROWS), grid = ceil_div(out, per_wave * waves);
+  // as many workgroups as compute units, each wave pairs of outputs
+  const int per_wave = ceil_div(ceil_div(out, cus * waves), 2) * 2, grid = ceil_div(out, per_wave * waves);
   ProfScope prof("q8_few", static_cast<double>(ld) * out, WORK_BYTE);
   auto go = [&](auto kernel) {
     TDH_LAUNCH(kernel, dim3(grid), dim3(Q8_NT), static_cast<size_t>(batch) * ld, ctx().stream, x, wq, wscale, b, y, in, ld, out, batch, per_wave);
@@ -343,7 +404,7 @@ q8_pack_kernel(const T *__restrict__ w, const float *__restrict__ wscale, int8_t
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[k + 8 * h + e][n];
-    o[h] = quantized(v, s);
+    o[h] = quantized(v, s, 1.0f / s);
   }
   *reinterpret_cast<uint4 *>(wq + static_cast<size_t>(n0 + n) * ld + k0 + k) = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
 }
