@@ -111,10 +111,10 @@ __device__ __forceinline__ Word<T> row_word(const T *p, const int k, const int l
   for (int e = 0; e < N; ++e) v[e] = k * N + e < len ? to_f32(p[k * N + e]) : rest;
   return Word<T>::from(v);
 }
-template <class T>
+template <class T, bool ONCE = false>
 __device__ __forceinline__ void put_row_word(T *p, const int k, const int len, const float (&v)[Word<T>::N]) {
   constexpr int N = Word<T>::N;
-  if (k * N + N <= len) return store_word(p + k * N, Word<T>::from(v).raw);
+  if (k * N + N <= len) return store_word<ONCE>(p + k * N, Word<T>::from(v).raw);
 #pragma unroll
   for (int e = 0; e < N; ++e)
     if (k * N + e < len) p[k * N + e] = from_f32<T>(v[e]);
