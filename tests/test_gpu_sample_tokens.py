@@ -80,8 +80,9 @@ def check(T, x, u, dtype, settings, got, what=""):
             if np.isnan(w):
                 assert np.isnan(g)
             else:
-                # one rounding of the result; the sum of exponentials is good to 2^-22 of itself
-                assert abs(g - w) <= 2.0 ** -24 * abs(w) + 2.0 ** -22 * min(1.0, -np.expm1(-abs(w))) + 2.0 ** -22 * abs(w), (what, i, g, w)
+                # one rounding of the result (below fp32's smallest number, 2^-149, to a multiple of that: half of it off at most, 2^-150);
+                # the sum of exponentials is good to 2^-22 of itself
+                assert abs(g - w) <= 2.0 ** -150 + 2.0 ** -24 * abs(w) + 2.0 ** -22 * min(1.0, -np.expm1(-abs(w))) + 2.0 ** -22 * abs(w), (what, i, g, w)
 
 
 def logits(rows, vocab, dtype, seed=0, spread=2.0):
@@ -202,3 +203,43 @@ def test_frequencies(T, kw):
     counts = np.bincount(got[0], minlength=vocab)
     assert (np.abs(counts - n * w / w.sum()) <= 1.001).all()
     assert (np.diff(got[0]) >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 1.9])
+@pytest.mark.parametrize("rows,vocab", [(5, 9001), (600, 8200), (9, 70001), (3, 200003)])
+def test_long_rows_without_filters(T, rows, vocab, temperature, dtype):
+    """One descriptor that leaves all, few rows and more than twice the compute units."""
+    x, u = logits(rows, vocab, dtype, 4)
+    got = run(T, x, u, dtype, temperature=temperature)
+    some = np.unique(np.concatenate([np.arange(min(rows, 12)), [rows - 1]]))
+    check(T, x[some], u[some], dtype, [(temperature, 0, 1.0, 0.0)] * len(some), [g[some] for g in got], f"{rows} x {vocab} {dtype}")
+
+
+@pytest.mark.parametrize("vocab", [9001, 70001])
+def test_masks_and_exceptional_long_rows_without_filters(T, vocab):
+    x, u = logits(22, vocab, "f32", 3)
+    x[0, 1:] = -np.inf                     # a single token, at the start, at the end and in between
+    x[1, :-1] = -np.inf
+    x[2] = -np.inf
+    x[2, vocab // 2 + 333] = -77.0
+    x[3] = -np.inf                         # none
+    x[4, vocab // 2], x[5, vocab - 1] = np.nan, np.inf
+    x[6, ::2] = -np.inf
+    x[7] = -3.0e38
+    x[8] = np.where(np.arange(vocab) % 3 == 0, 3.0e38, -3.0e38)
+    x[9], x[10] = 1e-3 * x[9], 1e4 * x[10]
+    x[11, 0] = -np.finfo(np.float32).max
+    for i, shift in ((12, -50.0), (13, -1e5), (14, 50.0), (15, 1e5)):   # little is left, far from zero
+        keep = np.arange(vocab) >= vocab - 5
+        x[i] = np.where(keep, x[i] + shift, -np.inf)
+    x[16, vocab // 3] += 70.0              # the maximum far above the others, all but certain, and the first
+    x[17, vocab - 2] += 9.0 + np.log(vocab)
+    x[18, 0] += 300.0
+    x[19] -= 1e5
+    x[20, :vocab - vocab // 50] = -np.inf
+    x[20] -= 60.0
+    x[21] = 0.0
+    x = L.rounded(x, "f32")
+    for t in (1.0, 0.9, 0.01, 30.0):
+        check(T, x, u, "f32", [(t, 0, 1.0, 0.0)] * len(u), run(T, x, u, "f32", temperature=t), f"{t}")

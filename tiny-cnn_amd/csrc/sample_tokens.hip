@@ -260,9 +260,10 @@ sample_all_kernel(const SampleArgs a) {
       return;
     }
     if (second) break;
-    // whole numbers that add up to less than 2^62; the likeliest's share below 1 - 10^-4, of fp32's exponentials 0.9
+    // whole numbers that add up to less than 2^62, and no reference above the maximum (0, where the first words hold nothing but -inf);
+    // the likeliest's share below 1 - 10^-4, of fp32's exponentials 0.9
     const double beyond = (static_cast<double>(top) - static_cast<double>(ref)) * rate;
-    if (beyond < 60.0 && sum * unit < 0x1p61 && sum > 1.0001 * weight(top) &&
+    if (beyond >= 0.0 && beyond < 60.0 && sum * unit < 0x1p61 && sum > 1.0001 * weight(top) &&
         (!with_raw || (top - ref < 80.0f && raw > 1.1 * static_cast<double>(exp_32(top - ref)))))
       break;
     ref    = top;
@@ -345,6 +346,7 @@ sample_kernel(const SampleArgs a) {
   const bool greedy = !(p.temperature > 0.0f);
   const double temperature = greedy ? 1.0 : static_cast<double>(p.temperature), rate = LOG2E_64 / temperature;
   const int top_k = greedy ? 1 : p.top_k;
+  const double share_p = fmaxf(p.top_p, 0.0f);
   const bool with_k = top_k > 0 && top_k < vocab, with_p = !greedy && p.top_p < 1.0f, with_q = !greedy && p.min_p > 0.0f;
 
   // maximum, and how far others lie from it on average: those of every thread's first word will do
@@ -453,7 +455,7 @@ sample_kernel(const SampleArgs a) {
           }
           if (MASS && whole_sum) {
             const u64 all = total + ties * v_weight;
-            target = max(1ull, min(all, static_cast<u64>(__builtin_ceil(static_cast<double>(p.top_p) * static_cast<double>(all)))));
+            target = max(1ull, min(all, static_cast<u64>(__builtin_ceil(share_p * static_cast<double>(all)))));
           }
           const u64 hit = __ballot(in && larger < target && larger + equal >= target);
           if (hit) {
@@ -608,7 +610,7 @@ sample_kernel(const SampleArgs a) {
       if (round == 0) add_last();
       const bool there = find([&](u64 total) {
         if (MASS && round == 0)
-          target = max(1ull, min(total, static_cast<u64>(__builtin_ceil(static_cast<double>(p.top_p) * static_cast<double>(total)))));
+          target = max(1ull, min(total, static_cast<u64>(__builtin_ceil(share_p * static_cast<double>(total)))));
         return target - above;
       });
       if (!there) return;   // fewer than top_k (the whole workgroup)
