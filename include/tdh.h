@@ -405,8 +405,9 @@ void tdh_opt_default(tdh_opt *o, int kind);
  * counterpart in the reference. Of a matrix U, steps times from X = U / (|U| + eps), |U| the root of the sum of squares:
  *   A = X X^T, X <- a X + (b A + c A A) X       (A = X^T X on the right-hand side where there are more rows than columns)
  * which takes every singular value s to s (a + b s^2 + c s^4) and leaves the singular vectors: the result O is near the orthogonal factor of U.
- * products: TDH_F32 or TDH_F16, what the products' operands are held in. TDH_F32: in three bf16 parts, as precise as fp32. TDH_F16:
- * rounded to fp16 around known magnitudes; X itself and all sums stay in fp32, and O is off by 1e-3 of its size for a, b, c as they are by default.
+ * products: TDH_F32 or TDH_F16, what the products' operands are held in. TDH_F32: in two fp16 parts, 22 bits, as precise as products in fp32. TDH_F16:
+ * rounded to fp16 around known magnitudes, and O is off by 1e-3 of its size for a, b, c as they are by default. X itself is held in 22 bits
+ * of either kind, and sums in fp32.
  * Coefficients that take a singular value of at most 1 beyond 4 in any step are refused. Up to 16384 on the shorter side, 2^20 on the longer and
  * 2^30 elements in all. */
 typedef struct tdh_muon {

@@ -210,3 +210,33 @@ def test_same_bits_again(T):
         T.orthogonalize(T.muon_desc(products=p), 300, 500, Buf(T, u, "bf16"), y, dtype="bf16")
         T.orthogonalize(T.muon_desc(products=p), 300, 500, Buf(T, u, "bf16"), z, dtype="bf16")
         assert np.array_equal(y.bits(), z.bits())
+
+
+@pytest.mark.parametrize("shape", [(1, 20000), (20001, 1), (2, 17001), (9003, 7), (31, 900), (1031, 33), (5, 70001)])
+@pytest.mark.parametrize("products", ["f32", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_step_of_long_thin_matrices(T, shape, products, dtype):
+    u = matrix(*shape, dtype)
+    bu, y = Buf(T, u, dtype, shape[1] % 2), out(T, shape, dtype, shape[1] % 2)
+    T.orthogonalize(T.muon_desc(steps=1, products=products), *shape, bu, y, dtype=dtype)
+    x = start(u)
+    want, e = step(x), step_bound(x, products, 1.0 / min(shape)) + 12 * U * np.abs(x)
+    e = e + 5 * U * np.abs(want)
+    L.within(y.read(), want, e + L.HALF_ULP[dtype] * (np.abs(want) + e) + L.TINY[dtype], f"{shape} {dtype} {products}")
+
+
+def test_many_steps_and_every_coefficient(T):
+    """32 steps, and coefficients whose largest polynomial or singular value lies inside the range rather than at its end."""
+    u = matrix(70, 300, "f32")
+    y = out(T, u.shape)
+    for co, steps in (((1.5, -0.5, 0.0), 32), ((1.875, -1.25, 0.375), 20), ((1.0, 0.0, 0.0), 7), ((2.0, -1.5, 0.5), 10), ((0.5, 0.25, 0.0), 9)):
+        T.orthogonalize(T.muon_desc(steps=steps, **dict(zip("abc", co))), 70, 300, Buf(T, u), y)
+        x, slope = start(u), 1.0
+        e = 12 * U * np.linalg.norm(x)
+        for _ in range(steps):
+            s = np.linspace(0, max(1.0, np.linalg.svd(x)[1][0]), 200)
+            slope = max(1.0, np.abs(co[0] + 3 * co[1] * s ** 2 + 5 * co[2] * s ** 4).max())
+            # a step's own: the operands' 2^-22, of X and of two Gram matrices, and the sums' of up to 300 products
+            e = slope * e + (8 * 2.0 ** -22 + 3 * sum_error(300)) * (abs(co[0]) + abs(co[1]) + abs(co[2])) * np.linalg.norm(x)
+            x = step(x, co)
+        assert np.linalg.norm(y.read() - x) <= e + U * np.linalg.norm(x), co

@@ -528,12 +528,26 @@ bool mu_scalars(const tdh_muon &o, int m, MuPlan *p) {
   if (!std::isfinite(a + b + c)) return false;
   double most = 1.0, worst = 1.0, poly = 0.0, gram = 0.0, flat = 1.0 / std::sqrt(static_cast<double>(m));
   for (int k = 0; k < o.steps; ++k) {
-    const double alpha = flat * flat, beta = b * alpha + c * alpha * alpha;
+    const double alpha = flat * flat, beta = b * alpha + c * alpha * alpha, top = most * most;
     double next = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double s = most * i / 4096, s2 = s * s, q = b * s2 + c * s2 * s2;
-      next = std::max(next, std::fabs(s * (a + q)));
+    auto at = [&](double t) {   // of a singular value whose square is t, up to `top`
+      if (!(t >= 0.0 && t <= top)) return;
+      const double q = b * t + c * t * t;
+      next = std::max(next, std::fabs(std::sqrt(t) * (a + q)));
       poly = std::max(poly, std::fabs(q - beta));
+    };
+    // the ends, and where a slope is none: a + 3 b t + 5 c t^2 = 0, or b + 2 c t = 0
+    const double root = 9.0 * b * b - 20.0 * a * c;
+    at(0.0);
+    at(top);
+    if (c != 0.0) {
+      at(-b / (2.0 * c));
+      if (root >= 0.0) {
+        at((-3.0 * b + std::sqrt(root)) / (10.0 * c));
+        at((-3.0 * b - std::sqrt(root)) / (10.0 * c));
+      }
+    } else if (b != 0.0) {
+      at(-a / (3.0 * b));
     }
     if (!(next <= 4.0)) return false;
     gram = std::max(gram, most * most + alpha);
