@@ -243,3 +243,39 @@ def test_masks_and_exceptional_long_rows_without_filters(T, vocab):
     x = L.rounded(x, "f32")
     for t in (1.0, 0.9, 0.01, 30.0):
         check(T, x, u, "f32", [(t, 0, 1.0, 0.0)] * len(u), run(T, x, u, "f32", temperature=t), f"{t}")
+
+
+@pytest.mark.parametrize("dtype", L.DTYPES)
+@pytest.mark.parametrize("rows", [1, 11, 64, 65])
+@pytest.mark.parametrize("s", [(1.0, 0, 0.9, 0.0), (0.8, 0, 0.99, 0.001), (1.5, 0, 0.3, 0.0)])
+def test_long_rows_with_top_p(T, rows, dtype, s):
+    """Rows that several workgroups look at, and one more of them than have that."""
+    vocab = 66001
+    x, u = logits(rows, vocab, dtype, 6)
+    x[0, : vocab // 2] = -np.inf
+    got = run(T, x, u, dtype, temperature=s[0], top_k=s[1], top_p=s[2], min_p=s[3])
+    some = np.unique(np.concatenate([np.arange(min(rows, 8)), [rows - 1]]))
+    check(T, x[some], u[some], dtype, [s] * len(some), [g[some] for g in got], f"{rows} {dtype}")
+    tok = Buf(T, np.zeros(rows, np.int32), "i32")
+    T.sample_tokens(rows, vocab, Buf(T, x, dtype), Buf(T, u), tok, temperature=s[0], top_k=s[1], top_p=s[2], min_p=s[3], dtype=dtype)
+    assert np.array_equal(tok.bits(), got[0])
+
+
+@pytest.mark.parametrize("vocab", [66001, 140001])
+@pytest.mark.parametrize("s", [(1.0, 0, 0.8, 0.0), (0.9, 0, 0.95, 1e-4), (30.0, 0, 0.5, 0.0), (0.01, 0, 0.999, 0.0)])
+def test_masks_and_exceptional_long_rows_with_top_p(T, vocab, s):
+    x, u = logits(16, vocab, "f32", 3)
+    x[0, 1:], x[1, :-1], x[2] = -np.inf, -np.inf, -np.inf
+    x[3, vocab // 2], x[4, vocab - 1], x[5, 0] = np.nan, np.inf, np.nan
+    x[6, ::2] = -np.inf
+    x[7] = -3.0e38
+    x[8] = np.where(np.arange(vocab) % 3 == 0, 3.0e38, -3.0e38)
+    x[9], x[10] = 1e-3 * x[9], 1e4 * x[10]
+    x[11] = np.round(x[11])
+    x[12] = np.where(np.arange(vocab) >= vocab - 5, x[12] - 50, -np.inf)
+    x[13, vocab // 3] += 70.0
+    x[14] = 0.0
+    x[15, : vocab // 2] = -np.finfo(np.float32).max
+    x = L.rounded(x, "f32")
+    check(T, x, u, "f32", [s] * 16, run(T, x, u, "f32", temperature=s[0], top_k=s[1], top_p=s[2], min_p=s[3]), f"{s}")
+    check(T, x, u, "f32", [s] * 16, run(T, x, u, "f32", [s] * 16), f"own {s}")

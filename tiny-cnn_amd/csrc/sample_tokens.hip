@@ -8,8 +8,10 @@
 // histograms over ever finer ranges of logits: of counts for top-k, of weights for top-p (select()). min-p is a bound on the logit itself. Nothing is
 // sorted.
 //
-// A workgroup has a row, whose words stay in its registers (of up to 16384 words, else they are read in every pass). Bound by the exponentials in
-// 64 bits, some 20 instructions a logit that counts, and by the latency of a chain of passes on one compute unit.
+// A workgroup has a row, whose words it keeps in LDS (up to 128 KB of them, else it reads them again in every pass). A few long rows have several
+// workgroups in the passes that look at all of a row. Bound by the exponentials in 64 bits, some 20 instructions a logit that counts, and by the
+// latency of a chain of passes on one compute unit. bf16, us: 64 rows of 131072 with top_p 0.9 73, with top_k 50 50; 2048 rows of 65536 as they are
+// 148, with top_k 50 268, with top_p 0.9 547.
 #include "lm_types.h"
 
 #include <cfloat>
@@ -154,7 +156,7 @@ sample_all_kernel(const SampleArgs a) {
   __shared__ int bads[WAVES], counts[WAVES], top_counts[WAVES];
   __shared__ double sums[WAVES], raws[WAVES];
   __shared__ u64 wholes[WAVES], wholes2[WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, vocab = a.vocab;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   const RowWords<T, NT, false> words(a, nullptr);
   const double temperature = a.p.temperature, rate = LOG2E_64 / temperature, unit = __builtin_ldexp(1.0, min(a.fix, 45));
   const bool with_raw = a.logp && temperature != 1.0;
@@ -298,10 +300,19 @@ sample_all_kernel(const SampleArgs a) {
   // one thread is left
   int token = -1;
   float chosen = 0.0f;
-  for (int i = beg * N; i < min(end * N, vocab) && token < 0; ++i) {
-    chosen = to_f32(words.x[i]);
-    before += whole(weight(chosen));
-    if (before > r) token = i;
+  for (int k = beg; k < end && token < 0; ++k) {
+    const Word<T> w = words.load(k);
+    u64 g[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = whole(weight(w[e]));
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      before += g[e];
+      if (token < 0 && before > r) {
+        token  = k * N + e;
+        chosen = w[e];
+      }
+    }
   }
   a.token[row] = token;
   if (a.kept) a.kept[row] = kept;
@@ -312,6 +323,191 @@ sample_all_kernel(const SampleArgs a) {
 }
 
 // ------------------------------------------------------------------ with filters
+struct RowSettings {
+  tdh_sample_desc p;
+  bool with_k, with_p, with_q, same;   // same: what is left is all, by its probability under the logits as they are
+  int top_k;
+  double temperature, rate, share_p;
+};
+__device__ __forceinline__ RowSettings row_settings(const SampleArgs &a, const int row) {
+  RowSettings s;
+  s.p = a.settings ? a.settings[row] : a.p;
+  const bool greedy = !(s.p.temperature > 0.0f);
+  s.temperature     = greedy ? 1.0 : static_cast<double>(s.p.temperature);
+  s.rate            = LOG2E_64 / s.temperature;
+  s.top_k           = greedy ? 1 : s.p.top_k;
+  s.with_k          = s.top_k > 0 && s.top_k < a.vocab;
+  s.with_p          = !greedy && s.p.top_p < 1.0f;
+  s.with_q          = !greedy && s.p.min_p > 0.0f;
+  s.same            = !(s.with_k || s.with_p || s.with_q) && s.temperature == 1.0;
+  s.share_p         = fmaxf(s.p.top_p, 0.0f);
+  return s;
+}
+// weights as whole numbers
+struct Weights {
+  double top, rate, unit;
+  // (of 2^-1000 nothing is left, nor where t is 0 times an infinity)
+  __device__ __forceinline__ double operator()(const float v) const { return exp2_64(__builtin_fmax((static_cast<double>(v) - top) * rate, -1000.0)); }
+  __device__ __forceinline__ u64 whole(const double w) const {
+    constexpr double SHIFT = 4503599627370496.0;   // 2^52: the sum's low bits are the rounded product
+    return __builtin_bit_cast(u64, __builtin_fma(w, unit, SHIFT)) - __builtin_bit_cast(u64, SHIFT);
+  }
+};
+// What is left of a wave's or a workgroup's words: weight and number above V, number with V; of the weights below the maximum, and of the exponentials of
+// all logits below it, the sums in floating point; number of maxima.
+struct Left {
+  u64 gt;
+  double rest, raw;
+  int gt_n, ties, tops;
+  __device__ __forceinline__ void add(const Left &o) {
+    gt += o.gt;
+    rest += o.rest;
+    raw += o.raw;
+    gt_n += o.gt_n;
+    ties += o.ties;
+    tops += o.tops;
+  }
+};
+// ... of a wave, whose words `each(f)` gives to f, by all of its lanes. Those above V are put behind each other in a queue of the wave's own, and weighed 64
+// at a time.
+constexpr int LEFT_QUEUE = 256;
+template <class Each>
+__device__ __forceinline__ Left weigh_left(const Each &each, const float V, const float top, const Weights &weight, const bool with_raw, float *queue) {
+  const int lane = threadIdx.x & 63;
+  Left l{};
+  int queued = 0;
+  auto weigh = [&](const int m) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    queued -= m;
+    if (lane < m) {
+      const float v  = queue[queued + lane];
+      const double x = weight(v);
+      l.gt += weight.whole(x);
+      l.rest += v < top ? x : 0.0;
+      l.tops += v == top;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  each([&](const auto &w) {
+    constexpr int N = std::remove_reference_t<decltype(w)>::N;
+    float m = w[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, w[e]);
+    if (__any(m >= V))
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v  = w[e];
+        const u64 keep = __ballot(v > V);
+        l.ties += __builtin_popcountll(__ballot(v == V));
+        if (v > V) queue[queued + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(keep >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(keep), 0))] = v;
+        queued += __builtin_popcountll(keep);
+        l.gt_n += __builtin_popcountll(keep);
+        if (e & 1)
+          while (queued >= 64) weigh(64);
+      }
+    if (with_raw) {
+      float r = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) r += w[e] < top ? exp_32(w[e] - top) : 0.0f;
+      l.raw += static_cast<double>(r);
+    }
+  });
+  weigh(queued);
+  l.gt   = wave_total(l.gt);
+  l.tops = V == top ? l.ties : wave_total(l.tops);
+  l.rest = wave_total(l.rest);
+  l.raw  = wave_total(l.raw);
+  return l;
+}
+// The token, of what is left in `count` pieces of `span` words each, and all results of the row. By the whole workgroup; get(k): word k.
+template <class T, int NT, class Get>
+__device__ __forceinline__ void draw_token(const SampleArgs &a, const RowSettings &set, const Weights &weight, const float top, const float V, const u64 ties,
+                                           const Left *left, const int count, const int span, const int words, const Get &get, u64 (&gt2)[NT / 64],
+                                           int (&ties2)[NT / 64]) {
+  constexpr int WAVES = NT / 64, N = Word<T>::N;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
+  const double v_weight64 = weight(V);
+  const u64 v_weight = weight.whole(v_weight64);
+  u64 gt_all = 0, ties_all = 0;
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    gt_all += left[i].gt;
+    ties_all += left[i].ties;
+  }
+  const u64 ties_left = min(ties, ties_all), all = gt_all + v_weight * ties_left;
+  const double u = a.u[row];
+  u64 r = static_cast<u64>((u > 0.0 ? fmin(u, 1.0) : 0.0) * static_cast<double>(all));
+  r = min(r, all - 1);
+  // the weights left up to a place with `g` above V and `t` with V in front of it
+  auto upto = [&](u64 g, u64 t) { return g + v_weight * min(t, ties_left); };
+  u64 g0 = 0, t0 = 0;
+  int where = 0;
+#pragma unroll 1
+  for (; where < count - 1; ++where) {
+    const u64 g1 = g0 + left[where].gt, t1 = t0 + left[where].ties;
+    if (upto(g1, t1) > r) break;
+    g0 = g1;
+    t0 = t1;
+  }
+  // that piece's words, a share for every thread
+  const int share = (span + NT - 1) / NT, beg = where * span + tid * share, end = min(min(beg + share, (where + 1) * span), words);
+  u64 gt = 0;
+  int at = 0;
+  for (int k = beg; k < end; ++k) {
+    const Word<T> w = get(k);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (w[e] > V) gt += weight.whole(weight(w[e]));
+      at += w[e] == V;
+    }
+  }
+  const u64 gt_scan = wave_scan(gt);
+  const int at_scan = wave_scan(at);
+  if (lane == 63) {
+    gt2[wave]   = gt_scan;
+    ties2[wave] = at_scan;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+    if (w < wave) {
+      g0 += gt2[w];
+      t0 += ties2[w];
+    }
+  g0 += gt_scan - gt;
+  t0 += at_scan - at;
+  if (upto(g0, t0) > r || upto(g0 + gt, t0 + at) <= r) return;
+  // one thread is left
+  int token = -1;
+  float chosen = V;
+  for (int k = beg; k < end && token < 0; ++k) {
+    const Word<T> w = get(k);
+    u64 g[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = w[e] > V ? weight.whole(weight(w[e])) : 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      g0 += g[e];
+      t0 += w[e] == V;
+      if (token < 0 && w[e] >= V && upto(g0, t0) > r) {
+        token  = k * N + e;
+        chosen = w[e];
+      }
+    }
+  }
+  a.token[row] = token;
+  Left sum{};
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) sum.add(left[i]);
+  if (a.kept) a.kept[row] = static_cast<int>(sum.gt_n + ties_left);
+  const double d = static_cast<double>(chosen) - weight.top;
+  if (a.logq) a.logq[row] = static_cast<float>(V == top ? -log(static_cast<double>(ties_left))
+                                                        : d / set.temperature - log_of_sum(sum.tops, sum.rest + v_weight64 * static_cast<double>(ties_left)));
+  if (a.logp) a.logp[row] = static_cast<float>(d - log_of_sum(sum.tops, set.same ? sum.rest : sum.raw));
+}
 constexpr int SAMPLE_LIST = 2048, SAMPLE_SHORT = 128;   // logits that a list takes, and that one wave goes through by itself
 // LDS of a row's workgroup
 template <int NT>
@@ -325,15 +521,215 @@ struct SampleShared {
   int found_bin, listed;
   float top[WAVES], far[WAVES];
   int bad[WAVES], n[WAVES];
-  // what is left, wave by wave: weight and number above V, number with V; weights below the maximum in floating point, number of maxima
-  u64 gt[WAVES], gt2[WAVES];
-  int gt_n[WAVES], ties[WAVES], ties2[WAVES], tops[WAVES];
-  double rest[WAVES], raw[WAVES];
+  Left left[WAVES];
+  u64 gt2[WAVES];
+  int ties2[WAVES];
 };
 
-template <class T, int NT, bool HELD>
+// The ranges of a first round: equal ones of the distance from the maximum, the last for what is beyond. That one's sum takes no atomics, so it
+// begins behind the average where a target is likely to be nearer: 131072 logits, top_p 0.9 PPP us, up to four times the average PPP.
+template <int BINS>
+struct FirstBins {
+  float top, scale;
+  __device__ __forceinline__ FirstBins(const float top, const float mean, const bool near) : top(top) {
+    const float reach = (near ? 1.2f : 4.0f) * mean;
+    scale             = reach > 0.0f ? BINS / reach : 0.0f;
+  }
+  __device__ __forceinline__ int operator()(const float v) const { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); }
+};
+__device__ __forceinline__ bool near_p(const RowSettings &s) { return s.p.top_p <= 0.95f; }
+
+// Few long rows: what needs all of a row's logits and is the same in any order comes from several workgroups a row, in two launches ahead of the row's
+// own: the maximum, and by it the sums of exponentials and the first histogram of top-p's.
+struct SamplePart {
+  float top, far;   // the largest logit, and the sum of `n` finite ones
+  int n, bad;
+};
+struct SampleBound {   // logits above v are left, and the first `ties` that are v
+  float v;
+  u64 ties;
+};
+struct SampleAhead {
+  SamplePart *parts;   // [rows][count]
+  double *raw;         // [rows][count]
+  u64 *hist;           // [rows][2048]
+  SampleBound *bounds; // [rows]
+  Left *left;          // [rows][count]
+  int count, chunk;    // workgroups of a row, words of each
+};
+constexpr int SAMPLE_BINS = 2048, AHEAD_NT = 512;
+struct RowTop {
+  float top, mean;
+  bool bad;
+};
+__device__ __forceinline__ RowTop row_top(const float top, const float far, const int n, const bool bad) {
+  return RowTop{top, n ? top - far / static_cast<float>(n) : 16.0f, bad || top == -INFINITY};
+}
+__device__ __forceinline__ RowTop row_top(const SampleAhead &ahead, const int row) {
+  float top = -INFINITY, far = 0.0f;
+  int n = 0, bad = 0;
+  for (int i = 0; i < ahead.count; ++i) {
+    const SamplePart p = ahead.parts[row * ahead.count + i];
+    top = fmaxf(top, p.top);
+    far += p.far;
+    n += p.n;
+    bad |= p.bad;
+  }
+  return row_top(top, far, n, bad);
+}
+template <class T>
+__global__ void __launch_bounds__(AHEAD_NT)
+sample_top_kernel(const SampleArgs a, const SampleAhead ahead) {
+  constexpr int WAVES = AHEAD_NT / 64, N = Word<T>::N;
+  __shared__ SamplePart waves[WAVES];
+  const int tid = threadIdx.x, row = blockIdx.y, part = blockIdx.x, words = (a.vocab + N - 1) / N;
+  const int beg = min(words, part * ahead.chunk), end = min(words, beg + ahead.chunk);
+  const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
+  for (int b = part * AHEAD_NT + tid; b < SAMPLE_BINS; b += ahead.count * AHEAD_NT) ahead.hist[static_cast<size_t>(row) * SAMPLE_BINS + b] = 0;
+  float top = -INFINITY, far = 0.0f;
+  int n = 0;
+  bool strange = false;
+#pragma unroll 4
+  for (int k = beg + tid; k < end; k += AHEAD_NT) {
+    const Word<T> w = row_word(x, k, a.vocab, -INFINITY);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      top     = fmaxf(top, w[e]);
+      strange = strange || !(w[e] < INFINITY);
+    }
+    if (k < beg + AHEAD_NT)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        far += w[e] > -INFINITY ? w[e] : 0.0f;
+        n += w[e] > -INFINITY;
+      }
+  }
+  top = wave_top(top);
+  far = wave_total(far);
+  n   = wave_total(n);
+  const int bad = __any(strange);
+  if ((tid & 63) == 0) waves[tid >> 6] = SamplePart{top, far, n, bad};
+  __syncthreads();
+  if (tid) return;
+  SamplePart all = waves[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    all.top = fmaxf(all.top, waves[w].top);
+    all.far += waves[w].far;
+    all.n += waves[w].n;
+    all.bad |= waves[w].bad;
+  }
+  ahead.parts[row * ahead.count + part] = all;
+}
+template <class T>
+__global__ void __launch_bounds__(AHEAD_NT)
+sample_sums_kernel(const SampleArgs a, const SampleAhead ahead) {
+  constexpr int WAVES = AHEAD_NT / 64, N = Word<T>::N;
+  __shared__ u64 hist[SAMPLE_BINS];
+  __shared__ double raws[WAVES];
+  const int tid = threadIdx.x, row = blockIdx.y, part = blockIdx.x, words = (a.vocab + N - 1) / N;
+  const int beg = min(words, part * ahead.chunk), end = min(words, beg + ahead.chunk);
+  const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
+  const RowSettings s = row_settings(a, row);
+  const RowTop r      = row_top(ahead, row);
+  const bool with_raw = a.logp && !s.same, with_hist = s.with_p && !s.with_k;
+  if (tid == 0) ahead.raw[row * ahead.count + part] = 0.0;
+  if (r.bad || !(with_raw || with_hist)) return;   // (the whole workgroup)
+  const Weights weight{r.top, s.rate, __builtin_ldexp(1.0, a.fix)};
+  const FirstBins<SAMPLE_BINS> bin_of(r.top, r.mean, near_p(s));
+  for (int b = tid; b < SAMPLE_BINS; b += AHEAD_NT) hist[b] = 0;
+  __syncthreads();
+  double raw = 0.0;
+  u64 last   = 0;
+#pragma unroll 1
+  for (int k = beg + tid; k < end; k += AHEAD_NT) {
+    const Word<T> w = row_word(x, k, a.vocab, -INFINITY);
+    if (with_hist)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const u64 v = weight.whole(weight(w[e]));
+        const int b = bin_of(w[e]);
+        last += b == SAMPLE_BINS - 1 ? v : 0;
+        if (b < SAMPLE_BINS - 1) atomicAdd(&hist[b], v);
+      }
+    if (with_raw) {
+      float f = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) f += w[e] < r.top ? exp_32(w[e] - r.top) : 0.0f;
+      raw += static_cast<double>(f);
+    }
+  }
+  last = wave_total(last);
+  raw  = wave_total(raw);
+  if ((tid & 63) == 0) {
+    if (last) atomicAdd(&hist[SAMPLE_BINS - 1], last);
+    raws[tid >> 6] = raw;
+  }
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) raw += raws[w];
+    ahead.raw[row * ahead.count + part] = raw;
+  }
+  if (with_hist)
+    for (int b = tid; b < SAMPLE_BINS; b += AHEAD_NT)
+      if (hist[b]) atomicAdd(&ahead.hist[static_cast<size_t>(row) * SAMPLE_BINS + b], hist[b]);
+}
+
+// the two of them for the rows of several workgroups
+template <class T>
+__global__ void __launch_bounds__(AHEAD_NT)
+sample_left_kernel(const SampleArgs a, const SampleAhead ahead) {
+  constexpr int WAVES = AHEAD_NT / 64, N = Word<T>::N;
+  __shared__ float queues[WAVES][LEFT_QUEUE];
+  __shared__ Left waves[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, part = blockIdx.x, words = (a.vocab + N - 1) / N;
+  const int beg = min(words, part * ahead.chunk), end = min(words, beg + ahead.chunk);
+  const RowSettings s = row_settings(a, row);
+  const RowTop r      = row_top(ahead, row);
+  if (r.bad) return;   // (the whole workgroup)
+  const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
+  const Weights weight{r.top, s.rate, __builtin_ldexp(1.0, a.fix)};
+  const Left mine = weigh_left(
+      [&](auto f) {
+#pragma unroll 1
+        for (int k0 = beg + 64 * wave; k0 < end; k0 += AHEAD_NT) {
+          float none[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) none[e] = -INFINITY;
+          f(k0 + lane < end ? row_word(x, k0 + lane, a.vocab, -INFINITY) : Word<T>::from(none));
+        }
+      },
+      ahead.bounds[row].v, r.top, weight, false, queues[wave]);
+  if (lane == 0) waves[wave] = mine;
+  __syncthreads();
+  if (tid) return;
+  Left all = waves[0];
+  for (int w = 1; w < WAVES; ++w) all.add(waves[w]);
+  all.raw = ahead.raw[row * ahead.count + part];
+  ahead.left[row * ahead.count + part] = all;
+}
+constexpr int DRAW_NT = 1024;
+template <class T>
+__global__ void __launch_bounds__(DRAW_NT)
+sample_draw_kernel(const SampleArgs a, const SampleAhead ahead) {
+  constexpr int N = Word<T>::N;
+  __shared__ u64 gt2[DRAW_NT / 64];
+  __shared__ int ties2[DRAW_NT / 64];
+  const int row = blockIdx.x;
+  const RowSettings s = row_settings(a, row);
+  const RowTop r      = row_top(ahead, row);
+  if (r.bad) return;   // (the whole workgroup; the row has its results)
+  const SampleBound b = ahead.bounds[row];
+  const Weights weight{r.top, s.rate, __builtin_ldexp(1.0, a.fix)};
+  const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
+  draw_token<T, DRAW_NT>(a, s, weight, r.top, b.v, b.ties, ahead.left + row * ahead.count, ahead.count, ahead.chunk, (a.vocab + N - 1) / N,
+                         [&](int k) { return row_word(x, k, a.vocab, -INFINITY); }, gt2, ties2);
+}
+
+template <class T, int NT, bool HELD, bool AHEAD>
 __global__ void __launch_bounds__(NT)
-sample_kernel(const SampleArgs a) {
+sample_kernel(const SampleArgs a, const SampleAhead ahead) {
   using Shared = SampleShared<NT>;
   constexpr int WAVES = Shared::WAVES, BINS = Shared::BINS, N = Word<T>::N;
   extern __shared__ uint4 row_lds[];
@@ -341,69 +737,72 @@ sample_kernel(const SampleArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, vocab = a.vocab;
   const RowWords<T, NT, HELD> words(a, row_lds);
 
-  // the row's settings
-  const tdh_sample_desc p = a.settings ? a.settings[row] : a.p;
-  const bool greedy = !(p.temperature > 0.0f);
-  const double temperature = greedy ? 1.0 : static_cast<double>(p.temperature), rate = LOG2E_64 / temperature;
-  const int top_k = greedy ? 1 : p.top_k;
-  const double share_p = fmaxf(p.top_p, 0.0f);
-  const bool with_k = top_k > 0 && top_k < vocab, with_p = !greedy && p.top_p < 1.0f, with_q = !greedy && p.min_p > 0.0f;
+  const RowSettings set = row_settings(a, row);
+  const tdh_sample_desc &p = set.p;
+  const bool with_k = set.with_k, with_p = set.with_p, with_q = set.with_q;
+  const int top_k = set.top_k;
+  const double temperature = set.temperature, share_p = set.share_p;
 
   // maximum, and how far others lie from it on average: those of every thread's first word will do
-  float top = -INFINITY, far = 0.0f;
-  int n = 0;
-  bool strange = false;
-  RowWords<T, NT, false>(a, nullptr).each_word([&](const Word<T> &w, int i) {
-    if (HELD && words.first + 64 * i < words.words) row_lds[words.first + 64 * i] = w.raw;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      top     = fmaxf(top, w[e]);
-      strange = strange || !(w[e] < INFINITY);
-    }
-    if (i == 0)
+  RowTop all_top;
+  if constexpr (AHEAD) {
+    all_top = row_top(ahead, row);
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+  } else {
+    float top = -INFINITY, far = 0.0f;
+    int n = 0;
+    bool strange = false;
+    RowWords<T, NT, false>(a, nullptr).each_word([&](const Word<T> &w, int i) {
+      if (HELD && words.first + 64 * i < words.words) row_lds[words.first + 64 * i] = w.raw;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        far += w[e] > -INFINITY ? w[e] : 0.0f;
-        n += w[e] > -INFINITY;
+        top     = fmaxf(top, w[e]);
+        strange = strange || !(w[e] < INFINITY);
       }
-  });
-  top = wave_top(top);
-  far = wave_total(far);
-  n   = wave_total(n);
-  int bad = __any(strange);
-  if (lane == 0) {
-    sh.top[wave] = top;
-    sh.far[wave] = far;
-    sh.bad[wave] = bad;
-    sh.n[wave]   = n;
-  }
-  if (tid == 0) sh.listed = 0;
-  __syncthreads();
-  far = 0.0f;
-  n = bad = 0;
+      if (i == 0)
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    top = fmaxf(top, sh.top[w]);
-    far += sh.far[w];
-    n += sh.n[w];
-    bad |= sh.bad[w];
+        for (int e = 0; e < N; ++e) {
+          far += w[e] > -INFINITY ? w[e] : 0.0f;
+          n += w[e] > -INFINITY;
+        }
+    });
+    top = wave_top(top);
+    far = wave_total(far);
+    n   = wave_total(n);
+    int bad = __any(strange);
+    if (lane == 0) {
+      sh.top[wave] = top;
+      sh.far[wave] = far;
+      sh.bad[wave] = bad;
+      sh.n[wave]   = n;
+    }
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    far = 0.0f;
+    n = bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      top = fmaxf(top, sh.top[w]);
+      far += sh.far[w];
+      n += sh.n[w];
+      bad |= sh.bad[w];
+    }
+    all_top = row_top(top, far, n, bad);
   }
-  if (bad || top == -INFINITY) {   // (the whole workgroup)
+  const float top = all_top.top, mean = all_top.mean;
+  if (all_top.bad) {   // (the whole workgroup)
     if (tid == 0) no_token(a, row);
     return;
   }
-  const double top64 = top, unit = __builtin_ldexp(1.0, a.fix);
-  // (of 2^-1000 nothing is left, nor where t is 0 times an infinity)
-  auto weight = [&](float v) { return exp2_64(__builtin_fmax((static_cast<double>(v) - top64) * rate, -1000.0)); };
-  constexpr double SHIFT = 4503599627370496.0;   // 2^52: the sum's low bits are the rounded product
-  auto whole = [&](double w) { return __builtin_bit_cast(u64, __builtin_fma(w, unit, SHIFT)) - __builtin_bit_cast(u64, SHIFT); };
+  const double top64 = top;
+  const Weights weight{top64, set.rate, __builtin_ldexp(1.0, a.fix)};
+  auto whole = [&](double w) { return weight.whole(w); };
 
   // What is left: logits above V, and the first `ties` of those that are V
   float V  = -INFINITY;
   u64 ties = 0;
   bool in_list = false;   // all that is left is in the list
-
-  const float mean = n ? top - far / static_cast<float>(n) : 16.0f;
 
   // The logit at which the sum over what is left, from the largest logit on, reaches a target: top_k (counts) or the share top_p of
   // all (weights). V becomes that logit and ties what is missing there. The first round is over the row, those behind it over the logits that the first
@@ -412,11 +811,7 @@ sample_kernel(const SampleArgs a) {
     using M = decltype(zero);
     constexpr bool MASS = sizeof(M) == 8;
     M *hist = reinterpret_cast<M *>(sh.hist);
-    // The first round's ranges: equal ones of the distance from the maximum, the last for what is beyond. That one's sum takes no atomics, so it
-    // begins behind the average where a target is likely to be nearer: 131072 logits, top_p 0.9 ... us, up to four times the average ... .
-    const bool near    = MASS ? p.top_p <= 0.95f : top_k <= vocab / 8;
-    const float reach  = (near ? 1.2f : 4.0f) * mean, scale = reach > 0.0f ? BINS / reach : 0.0f;
-    auto bin_of = [&](float v) { return static_cast<int>(fminf((top - v) * scale, static_cast<float>(BINS - 1))); };
+    const FirstBins<BINS> bin_of(top, mean, MASS ? near_p(set) : top_k <= vocab / 8);
     // the smallest logit, as a key, in range b or one before it; by all the lanes of every wave
     auto first_in = [&](const int b) {
       uint32_t from = key_of(-FLT_MAX), to = key_of(top);
@@ -601,6 +996,12 @@ sample_kernel(const SampleArgs a) {
       if (listed) {
         const int m = sh.listed;
         for (int i = tid; i < m; i += NT) one(sh.list[i]);
+      } else if (AHEAD && MASS && round == 0 && !with_k) {
+        if constexpr (AHEAD && MASS) {
+          const u64 *from = ahead.hist + static_cast<size_t>(row) * BINS;
+          hist[tid]      = from[tid];
+          hist[tid + NT] = from[tid + NT];
+        }
       } else {
         words.each(one);
       }
@@ -679,169 +1080,68 @@ sample_kernel(const SampleArgs a) {
     }
   }
 
-  // the weights that are left, wave by wave
-  const double v_weight64 = weight(V);
-  const u64 v_weight = whole(v_weight64);
-  {
-    u64 gt = 0;
-    int gt_n = 0, at = 0, tops = 0;
-    double rest = 0.0, raw = 0.0;
-    const bool same = !(with_k || with_p || with_q) && temperature == 1.0, with_raw = a.logp && !same;
-    // What is left is put behind each other in a queue of the wave's own (where the histogram was), and weighed 64 at a time.
-    float *queue = reinterpret_cast<float *>(sh.hist) + wave * 256;
-    int queued = 0;
-    auto weigh = [&](const int m) {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      queued -= m;
-      if (lane < m) {
-        const float v  = queue[queued + lane];
-        const double x = weight(v);
-        gt += whole(x);
-        rest += v < top ? x : 0.0;
-        tops += v == top;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    };
+  if constexpr (AHEAD) {   // the rest is other launches'
+    if (tid == 0) ahead.bounds[row] = SampleBound{V, ties};
+  } else {
     __syncthreads();   // (the histogram has been read)
-    words.each_word([&](const Word<T> &w, int) {
-      float m = w[0];
-#pragma unroll
-      for (int e = 1; e < N; ++e) m = fmaxf(m, w[e]);
-      if (__any(m >= V))
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float v  = w[e];
-          const u64 keep = __ballot(v > V);
-          at += __builtin_popcountll(__ballot(v == V));
-          if (v > V) queue[queued + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(keep >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(keep), 0))] = v;
-          queued += __builtin_popcountll(keep);
-          gt_n += __builtin_popcountll(keep);
-          if (e & 1)
-            while (queued >= 64) weigh(64);
-        }
-      if (with_raw) {
-        float r = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) r += w[e] < top ? exp_32(w[e] - top) : 0.0f;
-        raw += static_cast<double>(r);
-      }
-    });
-    weigh(queued);
-    gt   = wave_total(gt);
-    tops = V == top ? at : wave_total(tops);
-    rest = wave_total(rest);
-    raw  = same ? rest : wave_total(raw);
-    if (lane == 0) {
-      sh.gt[wave]   = gt;
-      sh.gt_n[wave] = gt_n;
-      sh.ties[wave] = at;
-      sh.tops[wave] = tops;
-      sh.rest[wave] = rest;
-      sh.raw[wave]  = raw;
-    }
+    const Left mine = weigh_left([&](auto f) { words.each_word([&](const Word<T> &w, int) { f(w); }); }, V, top, weight, a.logp && !set.same,
+                                 reinterpret_cast<float *>(sh.hist) + wave * LEFT_QUEUE);
+    if (lane == 0) sh.left[wave] = mine;
+    __syncthreads();
+    draw_token<T, NT>(a, set, weight, top, V, ties, sh.left, WAVES, words.per * 64, words.words, [&](int k) { return words.at(k); }, sh.gt2, sh.ties2);
   }
-  __syncthreads();
-  u64 gt_all = 0, ties_all = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    gt_all += sh.gt[w];
-    ties_all += sh.ties[w];
-  }
-  const u64 ties_left = min(ties, ties_all), all = gt_all + v_weight * ties_left;
-  const double u = a.u[row];
-  u64 r = static_cast<u64>((u > 0.0 ? fmin(u, 1.0) : 0.0) * static_cast<double>(all));
-  r = min(r, all - 1);
-  // the weights left up to a place with `g` above V and `t` with V in front of it
-  auto upto = [&](u64 g, u64 t) { return g + v_weight * min(t, ties_left); };
-  u64 g0 = 0, t0 = 0;
-  int where = 0;
-#pragma unroll 1
-  for (; where < WAVES - 1; ++where) {
-    const u64 g1 = g0 + sh.gt[where], t1 = t0 + sh.ties[where];
-    if (upto(g1, t1) > r) break;
-    g0 = g1;
-    t0 = t1;
-  }
-  // that wave's words, a share for every thread
-  const int span = words.per * 64, share = (span + NT - 1) / NT, beg = where * span + tid * share;
-  const int end = min(min(beg + share, (where + 1) * span), words.words);
-  u64 gt = 0;
-  int at = 0;
-  for (int k = beg; k < end; ++k) {
-    const Word<T> w = words.at(k);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (w[e] > V) gt += whole(weight(w[e]));
-      at += w[e] == V;
-    }
-  }
-  const u64 gt_scan = wave_scan(gt);
-  const int at_scan = wave_scan(at);
-  if (lane == 63) {
-    sh.gt2[wave]   = gt_scan;
-    sh.ties2[wave] = at_scan;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w)
-    if (w < wave) {
-      g0 += sh.gt2[w];
-      t0 += sh.ties2[w];
-    }
-  g0 += gt_scan - gt;
-  t0 += at_scan - at;
-  if (upto(g0, t0) > r || upto(g0 + gt, t0 + at) <= r) return;
-  // one thread is left
-  int token = -1;
-  float chosen = V;
-  for (int i = beg * N; i < min(end * N, vocab) && token < 0; ++i) {
-    const float v = to_f32(words.x[i]);
-    if (v < V) continue;
-    if (v > V) g0 += whole(weight(v)); else ++t0;
-    if (upto(g0, t0) > r) {
-      token  = i;
-      chosen = v;
-    }
-  }
-  a.token[row] = token;
-  u64 gt_count = 0;
-  int tops = 0;
-  double rest = 0.0, raw = 0.0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    gt_count += sh.gt_n[w];
-    tops += sh.tops[w];
-    rest += sh.rest[w];
-    raw += sh.raw[w];
-  }
-  if (a.kept) a.kept[row] = static_cast<int>(gt_count + ties_left);
-  const double d = static_cast<double>(chosen) - top64;
-  if (a.logq) a.logq[row] = static_cast<float>(V == top ? -log(static_cast<double>(ties_left))
-                                                        : d / temperature - log_of_sum(tops, rest + v_weight64 * static_cast<double>(ties_left)));
-  if (a.logp) a.logp[row] = static_cast<float>(d - log_of_sum(tops, raw));
 }
 
+// Logits of a row, and a share of the compute units in rows, from and up to which several workgroups have a row where top-p looks at all of it; twice
+// as many logits where the settings are the rows' own and may not ask for that. bf16, top_p 0.9, one workgroup and several, us: 64 rows of
+// 66000 76.4 and 66.4, of 131072 106.6 and 72.7, of 33000 48.7 and 53.1; 128 rows of 66000 77.4 and 75.4. Rows that have top_k 50 in settings of
+// their own: 64 of 131072 49.8 and 51.1, of 66000 36.8 and 42.9.
+constexpr int SAMPLE_AHEAD_VOCAB = 1 << 16, SAMPLE_AHEAD_SHARE = 4;
 constexpr size_t SAMPLE_HELD = 128 << 10;   // bytes of a row that stay in LDS
 template <class T>
 int launch_sample(const SampleArgs &a, int rows) {
-  const int words = static_cast<int>((static_cast<long>(a.vocab) + Word<T>::N - 1) / Word<T>::N);
+  const int words = static_cast<int>((static_cast<long>(a.vocab) + Word<T>::N - 1) / Word<T>::N), cus = std::max(1, ctx().compute_units);
   const size_t bytes = 16 * static_cast<size_t>(words);
-  auto go = [&](auto kernel, int nt, size_t lds) {
+  const bool with_k = a.p.top_k > 0 && a.p.top_k < a.vocab, with_p = a.p.top_p < 1.0f;
+  auto go = [&](auto kernel, int nt, size_t lds, auto... more) {
     if (lds > (32 << 10))
       TDH_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SAMPLE_HELD)));
-    TDH_LAUNCH(kernel, dim3(rows), dim3(nt), lds, ctx().stream, a);
+    TDH_LAUNCH(kernel, dim3(rows), dim3(nt), lds, ctx().stream, a, more...);
     TDH_LAUNCH_CHECK();
     return static_cast<int>(TDH_OK);
   };
-  if (words <= 128) return go(sample_kernel<T, 64, true>, 64, bytes);
-  if (words <= 1024) return go(sample_kernel<T, 256, true>, 256, bytes);
-  const bool filters = a.settings || !(a.p.temperature > 0.0f) || (a.p.top_k > 0 && a.p.top_k < a.vocab) || a.p.top_p < 1.0f || a.p.min_p > 0.0f;
-  if (!filters) return rows > 2 * ctx().compute_units ? go(sample_all_kernel<T, 512>, 512, 0) : go(sample_all_kernel<T, 1024>, 1024, 0);
-  if (bytes <= SAMPLE_HELD) return go(sample_kernel<T, 1024, true>, 1024, bytes);
-  return go(sample_kernel<T, 1024, false>, 1024, 0);
+  SampleAhead ahead{};
+  if (words <= 128) return go(sample_kernel<T, 64, true, false>, 64, bytes, ahead);
+  if (words <= 1024) return go(sample_kernel<T, 256, true, false>, 256, bytes, ahead);
+  const bool filters = a.settings || !(a.p.temperature > 0.0f) || with_k || with_p || a.p.min_p > 0.0f;
+  if (!filters) return rows > 2 * cus ? go(sample_all_kernel<T, 512>, 512, 0) : go(sample_all_kernel<T, 1024>, 1024, 0);
+  if (rows <= cus / SAMPLE_AHEAD_SHARE && (a.settings ? a.vocab >= 2 * SAMPLE_AHEAD_VOCAB : with_p && !with_k && a.vocab >= SAMPLE_AHEAD_VOCAB)) {
+    ahead.count = std::min({2 * cus / rows, ceil_div(words, AHEAD_NT), 32});
+    ahead.chunk = ceil_div(words, ahead.count);
+    const size_t parts = static_cast<size_t>(rows) * ahead.count;
+    const size_t sizes[5] = {sizeof(SamplePart) * parts, sizeof(double) * parts, sizeof(u64) * SAMPLE_BINS * rows, sizeof(SampleBound) * rows, sizeof(Left) * parts};
+    size_t total = 0;
+    for (size_t bytes : sizes) total += ws_align(bytes);
+    TDH_TRY(ws_begin(total));
+    void *mem[5] = {};
+    for (int i = 0; i < 5; ++i) TDH_TRY(ws_take(sizes[i], &mem[i]));
+    ahead.parts  = static_cast<SamplePart *>(mem[0]);
+    ahead.raw    = static_cast<double *>(mem[1]);
+    ahead.hist   = static_cast<u64 *>(mem[2]);
+    ahead.bounds = static_cast<SampleBound *>(mem[3]);
+    ahead.left   = static_cast<Left *>(mem[4]);
+    const dim3 grid(ahead.count, rows);
+    TDH_LAUNCH((sample_top_kernel<T>), grid, dim3(AHEAD_NT), 0, ctx().stream, a, ahead);
+    TDH_LAUNCH_CHECK();
+    TDH_LAUNCH((sample_sums_kernel<T>), grid, dim3(AHEAD_NT), 0, ctx().stream, a, ahead);
+    TDH_LAUNCH_CHECK();
+    TDH_TRY(go(sample_kernel<T, 1024, false, true>, 1024, 0, ahead));
+    TDH_LAUNCH((sample_left_kernel<T>), grid, dim3(AHEAD_NT), 0, ctx().stream, a, ahead);
+    TDH_LAUNCH_CHECK();
+    return go(sample_draw_kernel<T>, DRAW_NT, 0, ahead);
+  }
+  if (bytes <= SAMPLE_HELD) return go(sample_kernel<T, 1024, true, false>, 1024, bytes, ahead);
+  return go(sample_kernel<T, 1024, false, false>, 1024, 0, ahead);
 }
 
 }  // namespace
