@@ -362,8 +362,8 @@ int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, co
  * over all of them. temperature 0 takes the likeliest. logp[r] is the token's log-probability under softmax(logits), which
  * tdh_policy_loss takes as old_logp; logq[r] the one that it was drawn with; kept[r] how many were left; any of the three may be NULL. A u below 0
  * or NaN counts as 0, of 1 or more as the last number below 1. A row with NaN or +inf, or nothing but -inf, gives token -1, kept 0 and NaN.
- * Probabilities are summed as whole multiples of 2^-45 of the likeliest's (vocab up to 2^17; 2^-50 up to 2^12, 2^(b - 62) from vocab 2^b on), so the
- * same inputs give the same token.
+ * Probabilities are summed as whole multiples of 2^-45 of the likeliest's or finer (vocab up to 2^17; of 2^(b - 62) from vocab 2^b on), so a
+ * call with the same inputs gives the same tokens.
  * settings (device, [rows]): each row's own descriptor in the place of p, or NULL. Values out of range there: top_k below 1
  * and top_p of 1 or more, and NaN, leave all; top_p of 0 or less the likeliest; min_p of 0 or less, and NaN, all, above 1 what has the likeliest's
  * logit; a temperature that is 0 or less or NaN takes the likeliest, an infinite one leaves all equal. vocab up to 2^30, fewer than 2^22 rows,

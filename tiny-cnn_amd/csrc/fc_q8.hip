@@ -7,7 +7,10 @@
 //
 //   up to Q8_FEW samples   one launch: every workgroup brings the samples to 8 bits for itself and streams its rows of weights through the vector
 //                          units' four-fold products; bound by reading the weights
-//   more                   a pass that writes q and the scales, and the products of gemm16.h, pairs of bytes in the place of 16-bit elements
+//   more                   a pass that writes q and the scales, and the products of gemm16.h, pairs of bytes in the place of 16-bit elements; bound by the
+//                          matrix units
+//
+// bf16: 1 sample, 4096 -> 12288, 10.4 us, 4.8 TB/s of weights; 4096 samples 13.8 us and 201 us, 2050 TOPS (tiles of 256 x 256; of 128 x 128 225 us).
 #include "gemm16.h"
 
 #include <cfloat>
@@ -18,7 +21,7 @@ namespace {
 
 // q of eight values and a scale, as packed bytes. The quotient is fp32's, rounded to nearest, ties to even, as the product's definition has it; a product with
 // the reciprocal is within 2^-15 of it and rounds to the same number, unless it lies beside a half (one in some thousands), where it is
-// divided. 4096 x 4096 in bf16: ... us, all of them divided 15.
+// divided. 4096 x 4096 in bf16: 13.8 us, all of them divided 15.3.
 __device__ __forceinline__ uint2 quantized(const float (&v)[8], const float scale, const float inverse) {
   uint2 o = make_uint2(0, 0);
   if (!(scale > 0.0f)) return o;   // (all zero, or NaN)

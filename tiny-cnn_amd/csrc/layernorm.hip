@@ -355,6 +355,9 @@ layernorm_sum_kernel(const float *__restrict__ partial, const int parts, const i
 // ------------------------------------------------------------------ launches
 // Results that the L2 caches do not hold go past them: 8192 x 4096 in bf16 forward 37.7 us through them, 30.6 past them; 4096 x 4096 in fp32 34.5
 // and 25.9.
+// So 8192 x 4096 in bf16 goes forward at 4.4 TB/s and back, 40 us and 4.1 for the sums of its partial gradients, at 5.0: bound by memory. Not kept, us: the
+// backward pass of two workgroups a compute unit without rows ahead 54.6 (one with the next row ahead 40), with two rows ahead 44.8, reads past
+// the caches 34.5 forward, 256 lanes a row 39.6 forward.
 constexpr double NORM_ONCE_BYTES = 32 << 20;
 constexpr int NORM_HELD = 8192;   // elements of a row that a workgroup of the backward pass holds
 

@@ -25,8 +25,10 @@ constexpr int MU_NT = 256;
 // ------------------------------------------------------------------ products
 
 // C = A B of operands in two fp16 parts, p and p + plane, as hi hi + hi lo + lo hi. Tiles of 32 reduction indices of all four, two of
-// them in turns; a tile's products are summed from zero and then added in fp32, since the matrix instruction drops what falls off the end of a
-// long sum.
+// them in turns; the products of TOGETHER tiles are summed from zero and then added in fp32, since the matrix instruction drops what falls off the end
+// of a long sum. 4096^3, us, and the result's error against 64 bits after one step and after five: added after every tile 425; every 8
+// 392, 5.6e-7 and 1.1e-6; every 32 384, 9.4e-7 and 1.5e-6; at the end 377, 2.1e-6 and 4.7e-6. Products in fp32 are off by 4e-6 to 7e-6. Bound by the matrix
+// units: 4.1e11 multiplications and additions in 384 us, 1.07 PFLOP/s of fp16; tiles of 256 x 128 on eight waves take the same time.
 template <int WM, int WN, int TM, int TN, bool A_KC, bool B_KC, class Tiles, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const Epi epi, const int tiles_m, const int tiles_n,
@@ -321,7 +323,8 @@ struct LastFinish {
 
 // Tiles, by the size of the product: a side, the workgroups that a compute unit holds, us of 64 reduction indices and beside them. Whole rounds
 // of workgroups take whole tiles; the tiles of a last round that is not half full are split along k, which takes two more launches (4096 x 4096 of
-// two parts, symmetric: 528 tiles of 128 on 512 places ... us, unsplit ...).
+// two parts, symmetric: 528 tiles of 128 on 512 places 235 us, unsplit 314). Of the tiles and splits at eleven sizes from 160^2 to 1024 x 4096 the
+// rule's choices take 4.6% longer than the best of each.
 struct MuTile {
   int side, per_cu;
   double us, round_us;
@@ -567,7 +570,8 @@ bool mu_scalars(const tdh_muon &o, int m, MuPlan *p) {
 
 // ------------------------------------------------------------- small matrices
 // All of it by one workgroup, in one launch: X in its two parts twice in LDS, along either index, and the Gram matrix, whose place the polynomial takes. A
-// wave has 32 x 32 of X, in fp32, from the first step to the last. Three products in either kind. 120 x 84: ... us, as launches of their own 117.
+// wave has 32 x 32 of X, in fp32, from the first step to the last. Three products in either kind. Bound by a chain of barriers and of LDS reads;
+// 120 x 84: 45 us, as launches of their own 117.
 constexpr int MS_NT = 1024, MS_PAD = 8;   // (rows of LDS of 16 bytes more: 32 of them are read at a time)
 struct MuSmall {
   int m, n, mp, np, steps;   // mp, np: in whole blocks of 32
