@@ -558,7 +558,7 @@ struct SampleAhead {
   Left *left;          // [rows][count]
   int count, chunk;    // workgroups of a row, words of each
 };
-constexpr int SAMPLE_BINS = 2048, AHEAD_NT = 512;
+constexpr int SAMPLE_BINS = 2048, AHEAD_NT = 512, AHEAD_MOST = 32;
 struct RowTop {
   float top, mean;
   bool bad;
@@ -566,17 +566,12 @@ struct RowTop {
 __device__ __forceinline__ RowTop row_top(const float top, const float far, const int n, const bool bad) {
   return RowTop{top, n ? top - far / static_cast<float>(n) : 16.0f, bad || top == -INFINITY};
 }
+// (a lane a part: one after the other they take their way from memory each, 8 parts 4 us)
 __device__ __forceinline__ RowTop row_top(const SampleAhead &ahead, const int row) {
-  float top = -INFINITY, far = 0.0f;
-  int n = 0, bad = 0;
-  for (int i = 0; i < ahead.count; ++i) {
-    const SamplePart p = ahead.parts[row * ahead.count + i];
-    top = fmaxf(top, p.top);
-    far += p.far;
-    n += p.n;
-    bad |= p.bad;
-  }
-  return row_top(top, far, n, bad);
+  const int lane = threadIdx.x & 63;
+  SamplePart p{-INFINITY, 0.0f, 0, 0};
+  if (lane < ahead.count) p = ahead.parts[row * ahead.count + lane];
+  return row_top(wave_top(p.top), wave_total(p.far), wave_total(p.n), __any(p.bad));
 }
 template <class T>
 __global__ void __launch_bounds__(AHEAD_NT)
@@ -717,14 +712,17 @@ sample_draw_kernel(const SampleArgs a, const SampleAhead ahead) {
   constexpr int N = Word<T>::N;
   __shared__ u64 gt2[DRAW_NT / 64];
   __shared__ int ties2[DRAW_NT / 64];
+  __shared__ Left left[AHEAD_MOST];
   const int row = blockIdx.x;
+  if (threadIdx.x < ahead.count) left[threadIdx.x] = ahead.left[row * ahead.count + threadIdx.x];
+  __syncthreads();
   const RowSettings s = row_settings(a, row);
   const RowTop r      = row_top(ahead, row);
   if (r.bad) return;   // (the whole workgroup; the row has its results)
   const SampleBound b = ahead.bounds[row];
   const Weights weight{r.top, s.rate, __builtin_ldexp(1.0, a.fix)};
   const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * a.ld;
-  draw_token<T, DRAW_NT>(a, s, weight, r.top, b.v, b.ties, ahead.left + row * ahead.count, ahead.count, ahead.chunk, (a.vocab + N - 1) / N,
+  draw_token<T, DRAW_NT>(a, s, weight, r.top, b.v, b.ties, left, ahead.count, ahead.chunk, (a.vocab + N - 1) / N,
                          [&](int k) { return row_word(x, k, a.vocab, -INFINITY); }, gt2, ties2);
 }
 
@@ -1117,7 +1115,7 @@ int launch_sample(const SampleArgs &a, int rows) {
   const bool filters = a.settings || !(a.p.temperature > 0.0f) || with_k || with_p || a.p.min_p > 0.0f;
   if (!filters) return rows > 2 * cus ? go(sample_all_kernel<T, 512>, 512, 0) : go(sample_all_kernel<T, 1024>, 1024, 0);
   if (rows <= cus / SAMPLE_AHEAD_SHARE && (a.settings ? a.vocab >= 2 * SAMPLE_AHEAD_VOCAB : with_p && !with_k && a.vocab >= SAMPLE_AHEAD_VOCAB)) {
-    ahead.count = std::min({2 * cus / rows, ceil_div(words, AHEAD_NT), 32});
+    ahead.count = std::min({2 * cus / rows, ceil_div(words, AHEAD_NT), AHEAD_MOST});
     ahead.chunk = ceil_div(words, ahead.count);
     const size_t parts = static_cast<size_t>(rows) * ahead.count;
     const size_t sizes[5] = {sizeof(SamplePart) * parts, sizeof(double) * parts, sizeof(u64) * SAMPLE_BINS * rows, sizeof(SampleBound) * rows,
