@@ -1039,7 +1039,8 @@ sample_kernel(const SampleArgs a, const SampleAhead ahead) {
           }
           break;
         }
-        lo = max(lo, hi - ((1u << shift) - 1));
+        const uint32_t width = (1u << shift) - 1;   // (128 ranges of nearly all keys are wider than the lowest numbers' keys are large)
+        lo = max(lo, hi > width ? hi - width : 0u);
       }
       finer();
     }
