@@ -193,7 +193,11 @@ sample_all_kernel(const SampleArgs a) {
     int n = 0, tn = 0;
     bool bad = false;
     float t = -INFINITY;
-    const float large = ref + static_cast<float>(4.0 * temperature);   // (e^4 of the reference's weight)
+    // e^4 of the reference's weight, or the next smaller number: rounded up by half a place of the reference's it may weigh e^8, for whose whole number
+    // 52 bits are too few
+    const double border = static_cast<double>(ref) + 4.0 * temperature;
+    float large = static_cast<float>(border);
+    if (static_cast<double>(large) > border) large = of_key(key_of(large) - 1);
     words.each_word([&](const Word<T> &w, int) {
       float m = w[0];
 #pragma unroll
