@@ -361,7 +361,7 @@ int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, co
  * always the first one. token[r] is the first one left, by index, at which the sum of the probabilities of those left exceeds u times the sum
  * over all of them. temperature 0 takes the likeliest. logp[r] is the token's log-probability under softmax(logits), which
  * tdh_policy_loss takes as old_logp; logq[r] the one that it was drawn with; kept[r] how many were left; any of the three may be NULL. A u below 0
- * or NaN counts as 0, of 1 or more as the last number below 1. A row with NaN or +inf, or nothing but -inf, gives token -1, kept 0 and NaN.
+ * or NaN counts as 0, of 1 or more as the last number below 1, 1 - 2^-24. A row with NaN or +inf, or nothing but -inf, gives token -1, kept 0 and NaN.
  * Probabilities are summed as whole multiples of 2^-45 of the likeliest's or finer (vocab up to 2^17; of 2^(b - 62) from vocab 2^b on), so a
  * call with the same inputs gives the same tokens.
  * settings (device, [rows]): each row's own descriptor in the place of p, or NULL. Values out of range there: top_k below 1

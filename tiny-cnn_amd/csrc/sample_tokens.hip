@@ -140,6 +140,11 @@ struct RowWords {
   }
 };
 
+// u times all, which the weights up to and with the drawn token's exceed. A u below 0 or NaN is 0, of 1 or more fp32's last number below 1, so that
+// less than all comes out (the maximum alone weighs 2^32 or more).
+__device__ __forceinline__ u64 place_of(const float u, const u64 all) {
+  return static_cast<u64>(static_cast<double>(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f) * static_cast<double>(all));
+}
 // (a single maximum: the logarithm of 1 + rest has rest's precision)
 __device__ __forceinline__ double log_of_sum(const double tops, const double rest) { return tops == 1.0 ? log1p(rest) : log(tops + rest); }
 
@@ -278,9 +283,7 @@ sample_all_kernel(const SampleArgs a) {
   u64 all = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) all += wholes[w];
-  const double u = a.u[row];
-  u64 r = static_cast<u64>((u > 0.0 ? fmin(u, 1.0) : 0.0) * static_cast<double>(all));
-  r = min(r, all - 1);
+  const u64 r = place_of(a.u[row], all);
   u64 before = 0;
   int where = 0;
 #pragma unroll 1
@@ -442,9 +445,7 @@ __device__ __forceinline__ void draw_token(const SampleArgs &a, const RowSetting
     ties_all += left[i].ties;
   }
   const u64 ties_left = min(ties, ties_all), all = gt_all + v_weight * ties_left;
-  const double u = a.u[row];
-  u64 r = static_cast<u64>((u > 0.0 ? fmin(u, 1.0) : 0.0) * static_cast<double>(all));
-  r = min(r, all - 1);
+  const u64 r = place_of(a.u[row], all);
   // the weights left up to a place with `g` above V and `t` with V in front of it
   auto upto = [&](u64 g, u64 t) { return g + v_weight * min(t, ties_left); };
   u64 g0 = 0, t0 = 0;
