@@ -98,7 +98,7 @@ layernorm_fwd_kernel(const NormFwdArgs a) {
       for (int e = 0; e < N; ++e) s[0] += w[e];
     });
     sum(s, turn++);
-    const float mean = s[0] * a.inv_len;
+    float mean = s[0] * a.inv_len;
     s[0] = s[1] = 0.0f;
     each(0.0f, [&](int k, const Word<T> &w) {
 #pragma unroll
@@ -109,7 +109,35 @@ layernorm_fwd_kernel(const NormFwdArgs a) {
       }
     });
     sum(s, turn++);
-    const float off = s[0] * a.inv_len, var = s[1] * a.inv_len - off * off;
+    float off = s[0] * a.inv_len, var = s[1] * a.inv_len - off * off;
+    // Beyond fp32: the sum of the values, or the squares of what the mean's rounding makes of the deviations. Then every element's share of the mean is added up, and
+    // the mean taken nearer (a sum of 2^24 terms is off by 1e-3 of them at most, so four times do from any start); the squares are those of d - e. By all
+    // lanes of a row or none of them, from memory, so that nothing of it takes registers from the others.
+    if (__builtin_expect(!(var <= FLT_MAX), 0)) {
+      mean = __builtin_fabsf(mean) <= FLT_MAX ? mean : 0.0f;
+      off  = 0.0f;
+#pragma unroll 1
+      for (int pass = 0; pass < 6; ++pass) {   // four times the mean, once what it is still off by, the squares
+        s[0] = s[1] = 0.0f;
+#pragma unroll 1
+        for (int k = lane; k < words; k += LANES) {
+          const Word<T> w = row_word(x, k, a.len, 0.0f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float d = k * N + e < a.len ? (w[e] - mean) - off : 0.0f;
+            s[0] += d * (0.5f * a.inv_len);
+            s[1] = __builtin_fmaf(d, d, s[1]);
+          }
+        }
+        sum(s, turn++);
+        if (pass < 4)
+          mean = __builtin_amdgcn_fmed3f(mean + 2.0f * s[0], -FLT_MAX, FLT_MAX);
+        else if (pass < 5)
+          off = 2.0f * s[0];
+        else
+          var = s[1] * a.inv_len;
+      }
+    }
     const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
     if (!live) continue;
     if (a.stats && lane == 0) {
