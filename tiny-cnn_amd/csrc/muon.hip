@@ -539,18 +539,15 @@ bool mu_scalars(const tdh_muon &o, int m, MuPlan *p) {
       next = std::max(next, std::fabs(std::sqrt(t) * (a + q)));
       poly = std::max(poly, std::fabs(q - beta));
     };
-    // the ends, and where a slope is none: a + 3 b t + 5 c t^2 = 0, or b + 2 c t = 0
+    // the ends, and where a slope is none: a + 3 b t + 5 c t^2 = 0, or b + 2 c t = 0 (a quotient by 0 is beyond `top` or NaN, which at() leaves out)
     const double root = 9.0 * b * b - 20.0 * a * c;
     at(0.0);
     at(top);
-    if (c != 0.0) {
-      at(-b / (2.0 * c));
-      if (root >= 0.0) {
-        at((-3.0 * b + std::sqrt(root)) / (10.0 * c));
-        at((-3.0 * b - std::sqrt(root)) / (10.0 * c));
-      }
-    } else if (b != 0.0) {
-      at(-a / (3.0 * b));
+    at(-b / (2.0 * c));
+    if (root >= 0.0) {   // (a sum of two numbers of one sign: their difference has no figures left where c is small)
+      const double q = -0.5 * (3.0 * b + std::copysign(std::sqrt(root), b));
+      at(q / (5.0 * c));
+      at(a / q);
     }
     if (!(next <= 4.0)) return false;
     gram = std::max(gram, most * most + alpha);
