@@ -406,8 +406,10 @@ void tdh_opt_default(tdh_opt *o, int kind);
  *   A = X X^T, X <- a X + (b A + c A A) X       (A = X^T X on the right-hand side where there are more rows than columns)
  * which takes every singular value s to s (a + b s^2 + c s^4) and leaves the singular vectors: the result O is near the orthogonal factor of U.
  * products: TDH_F32 or TDH_F16, what the products' operands are held in. TDH_F32: in two fp16 parts, 22 bits, as precise as products in fp32. TDH_F16:
- * rounded to fp16 around known magnitudes, and O is off by 1e-3 of its size for a, b, c as they are by default. X itself is held in 22 bits
- * of either kind, and sums in fp32.
+ * rounded to fp16 around known magnitudes. O is off by 3e-4 to 1.3e-3 of its size after five steps with a, b, c as they are by default; where a few singular
+ * values are a thousand times the others, by 4e-3 to 8e-3 (of TDH_F32 by 4e-5), and three times that with every step more, since what is off beside the large
+ * ones grows as the small ones do. X itself is held in 22 bits of either kind, and sums in fp32. Small matrices (up to 96 x 128, 64 x 256,
+ * 32 x 512 and less, or turned round) go as TDH_F32 does.
  * Coefficients that take a singular value of at most 1 beyond 4 in any step are refused. Up to 16384 on the shorter side, 2^20 on the longer and
  * 2^30 elements in all. */
 typedef struct tdh_muon {
