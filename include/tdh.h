@@ -349,7 +349,8 @@ int tdh_layernorm_fwd(int dtype, int rows, int len, float eps, const void *x, si
                       void *y, size_t ld_y, float *stats);
 /* With xhat = (x - mean) * rstd and g = dy * gamma: dx = rstd * (g - mean(g) - xhat * mean(g * xhat)), means over the row; dgamma = the sum
  * over the rows of dy * xhat, dbeta = that of dy. dx is overwritten, and may be dy (with ld_dx == ld_dy); dgamma and dbeta are
- * overwritten, or added to with accumulate != 0. Any of dx, dgamma and dbeta may be NULL. */
+ * overwritten, or added to with accumulate != 0. Any of dx, dgamma and dbeta may be NULL. Sums are fp32 here too: those of |g|, |g (x - mean)| and |dy xhat|
+ * have to stay in its range. */
 int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, const void *gamma, const float *stats,
                       const void *dy, size_t ld_dy, void *dx, size_t ld_dx, void *dgamma, void *dbeta, int accumulate);
 
@@ -362,8 +363,8 @@ int tdh_layernorm_bwd(int dtype, int rows, int len, const void *x, size_t ld, co
  * over all of them. temperature 0 takes the likeliest. logp[r] is the token's log-probability under softmax(logits), which
  * tdh_policy_loss takes as old_logp; logq[r] the one that it was drawn with; kept[r] how many were left; any of the three may be NULL. A u below 0
  * or NaN counts as 0, of 1 or more as the last number below 1, 1 - 2^-24. A row with NaN or +inf, or nothing but -inf, gives token -1, kept 0 and NaN.
- * Probabilities are summed as whole multiples of 2^-45 of the likeliest's or finer (vocab up to 2^17; of 2^(b - 62) from vocab 2^b on), so a
- * call with the same inputs gives the same tokens.
+ * Probabilities are computed to 2e-12 of themselves and summed as whole multiples of 2^-41 of the likeliest's or finer (vocab up to 2^17; of 2^(b - 58) up to
+ * 2^b), so a call with the same inputs gives the same tokens.
  * settings (device, [rows]): each row's own descriptor in the place of p, or NULL. Values out of range there: top_k below 1
  * and top_p of 1 or more, and NaN, leave all; top_p of 0 or less the likeliest; min_p of 0 or less, and NaN, all, above 1 what has the likeliest's
  * logit; a temperature that is 0 or less or NaN takes the likeliest, an infinite one leaves all equal. vocab up to 2^30, fewer than 2^22 rows,

@@ -6,11 +6,13 @@
 // The sum is one of whole numbers and exact (in up to 2^17: below 2^31), so it may be split and joined in any order.
 //
 //   up to Q8_FEW samples   one launch: every workgroup brings the samples to 8 bits for itself and streams its rows of weights through the vector
-//                          units' four-fold products; bound by reading the weights
-//   more                   a pass that writes q and the scales, and the products of gemm16.h, pairs of bytes in the place of 16-bit elements; bound by the
-//                          matrix units
+//                          units' four-fold products; bound by reading the weights with one sample; eight take three times as long
+//   more                   a pass that writes q and the scales, and the products of gemm16.h, pairs of bytes in the place of 16-bit elements; the matrix
+//                          units are busy for 53% of a long prompt's
 //
-// bf16: 1 sample, 4096 -> 12288, 10.4 us, 4.8 TB/s of weights; 4096 samples 13.8 us and 201 us, 2050 TOPS (tiles of 256 x 256; of 128 x 128 225 us).
+// bf16, 4096 -> 12288: 1 sample 9.8 us with the same 50 MB of weights again and again, which the memory-side cache holds, 12.3 with eight such matrices in turns, 4.1 TB/s. In
+// the same order 2 samples 13.1 and 15.7, 4 19.4 and 21.8, 8 30.9 and 33.0; the other way 9 samples 18.1 and 20.3, 16 17.3 and 19.7, 64 20.5 and 25.1, so the border is too far up
+// for this layer. 4096 samples 13.8 us and 201 us, 2050 TOPS (tiles of 256 x 256; of 128 x 128 225 us). Packing, which reads w twice: 129 and 169 of bf16, 127 and 170 of fp32.
 #include "gemm16.h"
 
 #include <cfloat>

@@ -27,8 +27,9 @@ constexpr int MU_NT = 256;
 // C = A B of operands in two fp16 parts, p and p + plane, as hi hi + hi lo + lo hi. Tiles of 32 reduction indices of all four, two of
 // them in turns; the products of TOGETHER tiles are summed from zero and then added in fp32, since the matrix instruction drops what falls off the end
 // of a long sum. 4096^3, us, and the result's error against 64 bits after one step and after five: added after every tile 425; every 8
-// 392, 5.6e-7 and 1.1e-6; every 32 384, 9.4e-7 and 1.5e-6; at the end 377, 2.1e-6 and 4.7e-6. Products in fp32 are off by 4e-6 to 7e-6. Bound by the matrix
-// units: 4.1e11 multiplications and additions in 384 us, 1.07 PFLOP/s of fp16; tiles of 256 x 128 on eight waves take the same time.
+// 392, 5.6e-7 and 1.1e-6; every 32 384, 9.4e-7 and 1.5e-6; at the end 377, 2.1e-6 and 4.7e-6. Products in fp32 are off by 4e-6 to 7e-6. 4.1e11
+// multiplications and additions in 384 us, 1.07 PFLOP/s of fp16, where the library's product of this size reaches 1.12; the counters have the matrix units busy for 62 to 66% of
+// the time, and nothing shows what the rest waits for. Tiles of 256 x 128 on eight waves take the same time.
 template <int WM, int WN, int TM, int TN, bool A_KC, bool B_KC, class Tiles, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 gemm16x2_kernel(const G16Matrix A, const G16Matrix B, const long a_plane, const long b_plane, const Epi epi, const int tiles_m, const int tiles_n,

@@ -533,7 +533,9 @@ struct SampleShared {
 
 // The ranges of a first round: equal ones of the distance from the maximum, the last for what is beyond. That one's sum takes no atomics, so it
 // begins behind the average where a target is likely to be nearer. bf16, top_p 0.9, us, by 1.2 and by 4 times the average: 64 rows of 131072 75 and 81, 256 of
-// 32000 47 and 53, 2048 of 65536 545 and 515.
+// 32000 47 and 53, but 2048 of 65536 545 and 515: it pays where few rows wait for it. Finite masks count in the average and leave all that matters in the first few ranges: the
+// results are the same, but 2048 rows of 65536, half of them masked, take with top_p 0.9 780 where the mask is -1e4, 880 of -1e9 and 1170 of the lowest number, of -inf 500; with top_k 50
+// 490, 730, 1120 and 270.
 template <int BINS>
 struct FirstBins {
   float top, scale;
@@ -1098,9 +1100,16 @@ sample_kernel(const SampleArgs a, const SampleAhead ahead) {
 }
 
 // Logits of a row, and a share of the compute units in rows, from and up to which several workgroups have a row where top-p looks at all of it; twice
-// as many logits where the settings are the rows' own and may not ask for that. bf16, top_p 0.9, one workgroup and several, us: 64 rows of
-// 66000 76.4 and 66.4, of 131072 106.6 and 72.7, of 33000 48.7 and 53.1; 128 rows of 66000 77.4 and 75.4. Rows that have top_k 50 in settings of
-// their own: 64 of 131072 49.8 and 51.1, of 66000 36.8 and 42.9.
+// as many logits where the settings are the rows' own and may not ask for that. bf16, one workgroup and several, us:
+//   top_p 0.9          33000           66000           100000           131072           200000 logits
+//   1 row              48 and 43       76 and 52        96 and 55       101 and  49      110 and  43
+//   32 rows            50 and 48       79 and 63        99 and 67       115 and  71      152 and  74
+//   64                 51 and 53       79 and 66       100 and 75       115 and  81      152 and  91
+//   65                 51 and 53       80 and 67       100 and 75       116 and  85      152 and  94
+//   128                51 and 58       80 and 77       100 and 93       116 and 105      154 and 128
+//   192                50 and 69       80 and 101      102 and 129      119 and 151      156 and 205
+//   top_k 50 in settings of their own, 64 rows         39 and 43 (66000)  46 and 47       51 and  50       68 and  62
+// So the rows could be twice as many, and rows with settings of their own as many logits less as top-k is rare among them.
 constexpr int SAMPLE_AHEAD_VOCAB = 1 << 16, SAMPLE_AHEAD_SHARE = 4;
 constexpr size_t SAMPLE_HELD = 128 << 10;   // bytes of a row that stay in LDS
 template <class T>
