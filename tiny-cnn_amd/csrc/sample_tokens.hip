@@ -1046,8 +1046,9 @@ sample_kernel(const SampleArgs a, const SampleAhead ahead) {
           }
           break;
         }
-        const uint32_t width = (1u << shift) - 1;   // (128 ranges of nearly all keys are wider than the lowest numbers' keys are large)
-        lo = max(lo, hi > width ? hi - width : 0u);
+        // (keys of numbers are 2^23 and more, and 512 ranges 2^23 wide at most; of 128 one may be wider than the lowest numbers' keys are large)
+        const uint32_t width = (1u << shift) - 1;
+        lo = max(lo, BINS >= 512 || hi > width ? hi - width : 0u);
       }
       finer();
     }
